@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define TPA_ABI_VERSION 11
+#define TPA_ABI_VERSION 12
 
 /* element types of the factor / output arrays */
 enum { TPA_DTYPE_F32 = 0, TPA_DTYPE_BF16 = 1 };
@@ -288,6 +288,94 @@ int tpa_cache_append(const TpaAppendArgs* args, void* stream);
    tokens, dtype or d_model not eligible).  Kept for callers that size their scratch memory by it; nothing uses it now. */
 size_t tpa_cache_append_workspace_bytes(int32_t B, int32_t n, int32_t d_model, int32_t H, int32_t D, int32_t rq, int32_t rk, int32_t dtype);
 
+/*
+ * tpa_page_tables arguments: the page tables, slots and positions of a step's new tokens, from the requests' lengths.  No
+ * counterpart in the reference (whose caches are contiguous); it makes what tpa_decode, tpa_cache_append and
+ * tpa_norm_rope_write read.  Request b has kv_lengths[b] cached tokens and brings n_b = new_tokens[b] more:
+ *   starts[b] = min(n_0 + .. + n_(b-1), num_tokens): its tokens are rows starts[b] .. starts[b+1] - 1 of the packed step
+ *   its pages: ceil(kv_lengths[b] / page_size) are in its row of page_table; the next ones, as many as its new tokens open (no more
+ *   than the row has room for), come from free_pages[free_start ..], the requests served in order, and are written into the row;
+ *   new_kv_lengths[b] = kv_lengths[b] + its new tokens that have a page: tokens past the table's row or the last free page have none
+ *   positions[row] = kv_lengths[b] + (row - starts[b]);  slots[row] = page * page_size + position % page_size, or -1 without a page
+ *   rows from starts[B] on: slot -1, position 0.   new_free_start = free_start + pages taken.
+ * Lengths and counts below zero count as zero, lengths past the table's row as its end.  Nothing else of page_table is written.
+ */
+typedef struct TpaPageTablesArgs {
+  const int32_t* kv_lengths;  /* [B] */
+  const int32_t* new_tokens;  /* [B] */
+  int32_t* page_table;        /* [B, pages_per_seq], in place */
+  const int32_t* free_pages;  /* [num_free], or NULL with num_free == 0 */
+  const int32_t* free_start;  /* [1]: index of the first page that is still free, or NULL (0) */
+  int32_t* slots;             /* [num_tokens] */
+  int32_t* positions;         /* [num_tokens] */
+  int32_t* starts;            /* [B + 1] */
+  int32_t* new_kv_lengths;    /* [B]; must not overlap kv_lengths */
+  int32_t* new_free_start;    /* [1]; must not be free_start */
+  int32_t B;                  /* at most TPA_PAGE_TABLES_MAX_REQUESTS */
+  int32_t pages_per_seq, page_size, num_free, num_tokens; /* pages_per_seq * page_size below 2^31 */
+} TpaPageTablesArgs;
+#define TPA_PAGE_TABLES_MAX_REQUESTS 8192
+
+/*
+ * tpa_norm_rope arguments: the norms of queries and keys for each head and the rotation by position, on the rank factors.  No
+ * counterpart in the reference, which takes the factors as given (tpa/tpa.py:74-77).  For X in {Q, K}, with R ranks:
+ *   X_h = (1/R) sum_r a_r[h] b_r (tpa/tpa.py:317,364);  s_h = 1 / sqrt(|X_h|^2 / D + eps)
+ *   a'_r[h] = s_h a_r[h];  b'_r = rotation of (weight * b_r), pairwise as in tpa_cache_append:
+ *   y'[2j] = y[2j] c - y[2j+1] s,  y'[2j+1] = y[2j+1] c + y[2j] s,  c, s = rope_cos, rope_sin[positions[b, i, axis of j], j]
+ * so that (1/R) sum_r a'_r[h] b'_r is the rotated, weighted, normalised X_h and the rank stays what it was.  Pairs 0 .. sections[0] - 1
+ * belong to axis 0, the next sections[1] to axis 1, ..; pairs past the last section are not rotated.
+ * The outputs may be the inputs' own memory (same addresses and strides), not overlap them otherwise.
+ */
+typedef struct TpaNormRopeArgs {
+  TpaFactor qa, qb, ka, kb;         /* [B, l, rq|rk, H|D] */
+  TpaFactor qa_out, qb_out;         /* [B, l, rq, H|D] (ptr is written through) */
+  TpaFactor ka_out, kb_out;         /* the same, or with slots page pools [page, token_in_page, rk, H|D] */
+  TpaFactor va, vb, va_out, vb_out; /* with slots: [B, l, rk, H|D], copied into page pools; otherwise not looked at */
+  const int32_t* slots;             /* [B, l] or NULL: token i's K and V factors go to page slots[b, i] / page_size, place slots[b, i] %
+                                       page_size; slots outside 0 .. num_slots - 1 are dropped; no slot may be there twice */
+  int32_t page_size, num_slots;     /* num_slots = pages of the pools * page_size */
+  const int32_t* positions;         /* [B, l, n_axes] or NULL (i on every axis); clamped to 0 .. rope_len - 1 */
+  const float* rope_cos;            /* [rope_len, D/2] */
+  const float* rope_sin;
+  const void* q_weight;             /* [D] of weight_dtype, or NULL (ones) */
+  const void* k_weight;
+  int32_t n_axes, sections[4];      /* 1 .. 4 axes; sections not negative, their sum at most D/2 */
+  int32_t B, l, H, D, rq, rk;       /* D even, at most 256 */
+  int32_t rope_len, dtype, weight_dtype;
+  int32_t kernel;                   /* TPA_KERNEL_*: the MFMA kernel takes D in {64, 128}, H % 8 == 0, ranks up to 16, sections % 4 == 0 and
+                                       16-byte aligned rows */
+  int32_t normalize;                /* 0: s_h = 1 */
+  float eps;
+} TpaNormRopeArgs;
+
+/*
+ * tpa_norm_rope_bwd arguments.  With e_r = the rotation of db'_r by the opposite angle, G = the R x R products of the b_r:
+ *   u_h = sum_r da'_r[h] a_r[h];  w_h = - s_h^3 u_h / (D R^2) (0 with normalize == 0)
+ *   da_r[h] = s_h da'_r[h] + w_h sum_s G_rs a_s[h];   db_r = weight * e_r + sum_s (sum_h w_h a_r[h] a_s[h]) b_s
+ *   d weight = sum over tokens and ranks of e_r * b_r
+ * Every element of the gradients is written.  A side (q or k) whose d_a_out pointer is NULL has no gradient and none of its fields is read.
+ */
+typedef struct TpaNormRopeBwdArgs {
+  TpaFactor qa, qb, ka, kb;                 /* the forward's inputs */
+  TpaFactor dqa_out, dqb_out, dka_out, dkb_out; /* gradients of its outputs, element type = dtype */
+  TpaFactor dqa, dqb, dka, dkb;             /* gradients of its inputs, element type = dtype (ptr is written through) */
+  void* dq_weight;                          /* [D] of weight_dtype, or NULL */
+  void* dk_weight;
+  const int32_t* positions;                 /* from here on as in the forward call */
+  const float* rope_cos;
+  const float* rope_sin;
+  const void* q_weight;
+  const void* k_weight;
+  int32_t n_axes, sections[4];
+  int32_t B, l, H, D, rq, rk;
+  int32_t rope_len, dtype, weight_dtype;
+  int32_t kernel;
+  int32_t normalize;
+  float eps;
+  void* workspace;                          /* with a weight gradient: tpa_norm_rope_bwd_workspace_bytes(...), 16-byte aligned */
+  size_t workspace_bytes;
+} TpaNormRopeBwdArgs;
+
 /* ABI version of the loaded library (TPA_ABI_VERSION it was built with). */
 int tpa_abi_version(void);
 
@@ -406,6 +494,34 @@ int mha_bwd(const MhaBwdArgs* args, void* stream);
 
 /* Bytes of workspace mha_bwd needs (delta; plus fp32 copies of q, k, v when dtype is not fp32). */
 size_t mha_bwd_workspace_bytes(int32_t B, int32_t lq, int32_t lk, int32_t H, int32_t dk, int32_t dv, int32_t dtype);
+
+/* Page tables, slots and positions of a step's new tokens (see TpaPageTablesArgs): one launch. */
+int tpa_page_tables(const TpaPageTablesArgs* args, void* stream);
+
+/* Norms of queries and keys for each head and rotation by position, on the rank factors; with `slots` the K factors and the V
+   factors go into a paged cache (see TpaNormRopeArgs).  One launch. */
+int tpa_norm_rope(const TpaNormRopeArgs* args, void* stream);
+
+/* Gradients of tpa_norm_rope without slots (see TpaNormRopeBwdArgs). */
+int tpa_norm_rope_bwd(const TpaNormRopeBwdArgs* args, void* stream);
+
+/* Bytes of workspace that tpa_norm_rope_bwd needs where a weight's gradient is asked for (partial sums of it). */
+size_t tpa_norm_rope_bwd_workspace_bytes(int32_t B, int32_t l, int32_t D);
+
+/*
+ * Decode of a batch whose sequences share their first `prefix_length` tokens (a system prompt, a document that many ask about).  No
+ * counterpart in the reference.  Arguments and results are those of tpa_decode: the first prefix_length tokens of every batch entry
+ * are taken to be those of entry 0, whose cache (or pages) alone is read for them, once for all entries; every entry's other
+ * tokens are its own.  kv_lengths count both; an entry shorter than the prefix sees as much of it as its length says.
+ * num_splits must be 0.  Needs `workspace` of at least tpa_decode_shared_workspace_bytes(...) bytes, 256-byte aligned.  Matrix-core kernels take
+ * bf16 and fp32 with dk == dv in {64, 128}, H % 8 == 0, rk in {1, 2, 4, 8} and rows as tpa_decode has them; any other problem,
+ * paged ones too, runs on the vector units.
+ */
+int tpa_decode_shared(const TpaFwdArgs* args, int32_t prefix_length, void* stream);
+
+/* Bytes of workspace that tpa_decode_shared needs for this call; 0 if it would refuse it.  `workspace`, `workspace_bytes` and the
+   outputs are not looked at. */
+size_t tpa_decode_shared_workspace_bytes(const TpaFwdArgs* args, int32_t prefix_length);
 
 #ifdef __cplusplus
 }

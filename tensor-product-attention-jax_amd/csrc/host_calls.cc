@@ -18,9 +18,12 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
+#include <cmath>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "tpa_abi.h"
 
@@ -31,7 +34,9 @@ using at::Tensor;
 // ------------------------------------------------------------------------------------------------ the C ABI, by name
 #define TPA_CALLS(X)                                                                                             \
   X(tpa_fwd) X(tpa_decode) X(tpa_cache_append) X(tpa_bwd) X(tpa_strerror) X(tpa_fwd_call_workspace_bytes) \
-  X(tpa_decode_call_workspace_bytes) X(tpa_cache_append_workspace_bytes) X(tpa_bwd_workspace_bytes)
+  X(tpa_decode_call_workspace_bytes) X(tpa_cache_append_workspace_bytes) X(tpa_bwd_workspace_bytes)             \
+  X(tpa_page_tables) X(tpa_norm_rope) X(tpa_norm_rope_bwd) X(tpa_norm_rope_bwd_workspace_bytes) X(tpa_decode_shared) \
+  X(tpa_decode_shared_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
   TPA_CALLS(X)
@@ -153,6 +158,33 @@ void* aligned(const Tensor& t, size_t to) {
   return reinterpret_cast<void*>((p + to - 1) / to * to);
 }
 void* stream_of(const at::Device& device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
+
+// every operand on one device: a pointer of another would be read there, or not at all
+void one_device(std::initializer_list<Tensor> tensors) {
+  const Tensor* first = nullptr;
+  for (const Tensor& t : tensors) {
+    if (!t.defined()) continue;
+    if (!first) first = &t;
+    else if (t.device() != first->device())
+      throw Raise{PyExc_ValueError, "operands on two devices: " + first->device().str() + " and " + t.device().str()};
+  }
+}
+// a dual tensor need not ask for gradients, so an autograd node, which refuses a tangent, may never see it
+void no_tangents(std::initializer_list<Tensor> tensors, const char* name) {
+  for (const Tensor& t : tensors)
+    if (t.defined() && t._fw_grad(/*level=*/0).defined())
+      throw Raise{PyExc_NotImplementedError, std::string(name) + " has no forward-mode derivative: an input carries a tangent"};
+}
+// a call wrote into `t`: a node that saved it notices
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+template <typename Args>
+void take_workspace(const Tensor& ws, size_t alignment, Args& a) {
+  const size_t bytes = ws.numel() * ws.element_size(), skip = static_cast<char*>(aligned(ws, alignment)) - static_cast<char*>(ws.data_ptr());
+  a.workspace = aligned(ws, alignment);
+  a.workspace_bytes = bytes > skip ? bytes - skip : 0;
+}
 
 // ------------------------------------------------------------------------------------------------ forward
 struct FwdCall {
@@ -281,15 +313,8 @@ PyObject* factors(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------------------------ decode
-// decode(qa, qb, ka, kb, va, vb, kv_lengths, page_table, workspace, sm_scale, num_splits, kernel, causal, causal_offset)
-PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  BEGIN_CALL
-  count("decode", n, 14);
-  if (!gpu_tensors(args, 6) || !none_or_gpu(args[6]) || !none_or_gpu(args[7]) || !none_or_gpu(args[8])) Py_RETURN_NOTIMPLEMENTED;
-  Tensor t[6];
-  unpack_six(args, t);
-  TpaFwdArgs a{};
-  Tensor pages = tensor_or_none(args[7]), ws = tensor_or_none(args[8]);
+// the six factors and the sizes of a problem whose keys are a contiguous cache or, with `pages`, page pools; returns the table to hold on to
+Tensor describe_cache(const Tensor* t, Tensor pages, TpaFwdArgs& a) {
   if (!pages.defined()) {
     describe(t, a);
   } else {
@@ -312,6 +337,19 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.ka = factor_of<TpaFactor>(t[2]); a.kb = factor_of<TpaFactor>(t[3]);
     a.va = factor_of<TpaFactor>(t[4]); a.vb = factor_of<TpaFactor>(t[5]);
   }
+  return pages;
+}
+
+// decode(qa, qb, ka, kb, va, vb, kv_lengths, page_table, workspace, sm_scale, num_splits, kernel, causal, causal_offset)
+PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("decode", n, 14);
+  if (!gpu_tensors(args, 6) || !none_or_gpu(args[6]) || !none_or_gpu(args[7]) || !none_or_gpu(args[8])) Py_RETURN_NOTIMPLEMENTED;
+  Tensor t[6];
+  unpack_six(args, t);
+  TpaFwdArgs a{};
+  Tensor ws = tensor_or_none(args[8]);
+  const Tensor pages = describe_cache(t, tensor_or_none(args[7]), a);
   a.dtype = dtype_code(t[0].scalar_type());
   a.sm_scale = (float)real(args[9]);
   a.num_splits = (int)integer(args[10]);
@@ -572,6 +610,401 @@ PyObject* tpa(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_CALL
 }
 
+// ------------------------------------------------------------------------------------------------ decode over a shared prefix
+// decode_shared(qa, qb, ka, kb, va, vb, kv_lengths, page_table, workspace, prefix_length, sm_scale, kernel, causal, causal_offset)
+PyObject* decode_shared(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("decode_shared", n, 14);
+  if (!gpu_tensors(args, 6) || !none_or_gpu(args[6]) || !none_or_gpu(args[7]) || !none_or_gpu(args[8])) Py_RETURN_NOTIMPLEMENTED;
+  Tensor t[6];
+  unpack_six(args, t);
+  TpaFwdArgs a{};
+  Tensor ws = tensor_or_none(args[8]);
+  one_device({t[0], t[1], t[2], t[3], t[4], t[5], tensor_or_none(args[6]), tensor_or_none(args[7]), ws});
+  const int64_t prefix = integer(args[9]);
+  a.sm_scale = (float)real(args[10]);
+  a.kernel = (int)integer(args[11]);
+  a.causal = (int)integer(args[12]);
+  a.causal_offset = (int)integer(args[13]);
+  std::pair<Tensor, Tensor> r;
+  {
+    WithoutGil free;
+    const at::Device device = t[0].device();
+    const c10::DeviceGuard guard(device);
+    const Tensor pages = describe_cache(t, tensor_or_none(args[7]), a);
+    a.dtype = dtype_code(t[0].scalar_type());
+    if (prefix < 0 || prefix > a.lk)
+      throw Raise{PyExc_ValueError, "prefix_length must be between 0 and the cache's " + std::to_string(a.lk) + " tokens, got " + std::to_string(prefix)};
+    const Tensor kvlen = lengths(tensor_or_none(args[6]), a.B);
+    a.kv_lengths = ids_ptr(kvlen);
+    const auto options = at::TensorOptions().device(device);
+    r.first = at::empty({a.B, a.lq, a.H, a.dv}, options.dtype(t[0].scalar_type()));
+    r.second = at::empty({a.B, a.H, a.lq}, options.dtype(at::kFloat));
+    if (r.first.numel() && a.lk) {  // nothing to launch for no rows
+      if (!ws.defined()) ws = bytes_on(device, lib.tpa_decode_shared_workspace_bytes(&a, (int)prefix) + 256);
+      take_workspace(ws, 256, a);
+      a.o = r.first.data_ptr();
+      a.lse = f32_ptr(r.second);
+      check("tpa_decode_shared", lib.tpa_decode_shared(&a, (int)prefix, stream_of(device)));
+    } else {
+      r.first.fill_(NAN);
+      r.second.fill_(-INFINITY);
+    }
+  }
+  return pair(std::move(r));
+  END_CALL
+}
+
+// ------------------------------------------------------------------------------------------------ page tables
+PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
+  PyObject* out = PyTuple_New((Py_ssize_t)tensors.size());
+  if (!out) throw python_error();
+  Py_ssize_t i = 0;
+  for (const Tensor& t : tensors) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+  return out;
+}
+Tensor ints(const Tensor& t) { return (t.scalar_type() == at::kInt ? t : t.to(at::kInt)).contiguous(); }
+
+// page_tables(kv_lengths, new_tokens, free_pages, free_start, page_table, page_size, num_tokens)
+PyObject* page_tables(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("page_tables", n, 7);
+  if (!gpu_tensors(args, 3) || !none_or_gpu(args[3])) Py_RETURN_NOTIMPLEMENTED;
+  if (!gpu_tensors(args + 4, 1)) throw Raise{PyExc_TypeError, "page_table is written in place: it must be a GPU tensor"};
+  const Tensor table = THPVariable_Unpack(args[4]);
+  Tensor len = THPVariable_Unpack(args[0]), fresh = THPVariable_Unpack(args[1]), pool = THPVariable_Unpack(args[2]), start = tensor_or_none(args[3]);
+  one_device({len, fresh, pool, start, table});
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous())
+    throw Raise{PyExc_ValueError, "page_table is written in place: it must be a contiguous int32 [b, pages_per_seq] tensor"};
+  const int64_t b = table.size(0), page = integer(args[5]), rows = integer(args[6]);
+  if (!is_shape(len, {b})) throw Raise{PyExc_ValueError, "kv_lengths must have shape (" + std::to_string(b) + ",), got " + sizes_of(len)};
+  if (!is_shape(fresh, {b})) throw Raise{PyExc_ValueError, "new_tokens must have shape (" + std::to_string(b) + ",), got " + sizes_of(fresh)};
+  if (pool.dim() != 1) throw Raise{PyExc_ValueError, "free_pages is a list of pages, got shape " + sizes_of(pool)};
+  if (start.defined() && start.numel() != 1) throw Raise{PyExc_ValueError, "free_start is one number, got shape " + sizes_of(start)};
+  if (page < 1 || page > INT32_MAX) throw Raise{PyExc_ValueError, "page_size must be positive, got " + std::to_string(page)};
+  if (rows < 0 || rows > INT32_MAX) throw Raise{PyExc_ValueError, "num_tokens must not be negative, got " + std::to_string(rows)};
+  if (pool.numel() > INT32_MAX || b > INT32_MAX || table.size(1) > INT32_MAX) throw CallFailed{"tpa_page_tables", TPA_ERR_SHAPE};
+  Tensor out[5];
+  {
+    WithoutGil free;
+    const at::Device device = table.device();
+    const c10::DeviceGuard guard(device);
+    len = ints(len);
+    fresh = ints(fresh);
+    pool = ints(pool);
+    if (start.defined()) start = ints(start);
+    const auto options = at::TensorOptions().device(device).dtype(at::kInt);
+    // one allocation: slots, positions and lengths of a step are read on this device, and each is a few kilobytes
+    const int64_t sizes[5] = {rows, rows, b + 1, b, 1};
+    int64_t at = 0, total = 0;
+    for (int64_t s : sizes) total += (s + 63) / 64 * 64;
+    const Tensor all = at::empty({total}, options);
+    for (int i = 0; i < 5; ++i) {
+      out[i] = all.narrow(0, at, sizes[i]);
+      at += (sizes[i] + 63) / 64 * 64;
+    }
+    TpaPageTablesArgs a{};
+    a.kv_lengths = ids_ptr(len); a.new_tokens = ids_ptr(fresh);
+    a.page_table = static_cast<int32_t*>(table.data_ptr());
+    a.free_pages = ids_ptr(pool); a.free_start = ids_ptr(start);
+    int32_t* to[5];
+    for (int i = 0; i < 5; ++i) to[i] = static_cast<int32_t*>(out[i].data_ptr());
+    a.slots = to[0]; a.positions = to[1]; a.starts = to[2]; a.new_kv_lengths = to[3]; a.new_free_start = to[4];
+    a.B = (int)b; a.pages_per_seq = (int)table.size(1); a.page_size = (int)page; a.num_free = (int)pool.numel(); a.num_tokens = (int)rows;
+    check("tpa_page_tables", lib.tpa_page_tables(&a, stream_of(device)));
+    written(table);
+  }
+  return tuple_of({out[0], out[1], out[2], out[3], out[4]});
+  END_CALL
+}
+
+// ------------------------------------------------------------------------------------------------ norms and rotation
+struct NormRope {  // what a call has beside q and k
+  Tensor q_weight, k_weight, positions, cos, sin;
+  int64_t heads = 0;
+  std::vector<int64_t> sections;
+  bool normalize = true;
+  double eps = 0;
+  int kernel = TPA_KERNEL_AUTO;
+};
+
+void check_norm_rope(const Tensor& q, const Tensor& k, NormRope& c) {
+  if (q.dim() != 4 || k.dim() != 4) throw Raise{PyExc_ValueError, "q, k must be [b, l, r, h + d]"};
+  expect(k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3), k);
+  if (!(0 < c.heads && c.heads < q.size(3))) throw Raise{PyExc_AssertionError, "num_heads = " + std::to_string(c.heads) + ", " + sizes_of(q)};
+  const Tensor two[2] = {q, k};
+  static const char* const names[2] = {"q", "k"};
+  check_dtypes(two, names, 2);
+  (void)dtype_code(q.scalar_type());
+  const int64_t d = q.size(3) - c.heads;
+  expect(c.cos.sizes() == c.sin.sizes() && c.cos.dim() == 2 && c.cos.size(1) == d / 2 && c.cos.size(0) <= INT32_MAX, c.cos);
+  for (const Tensor* w : {&c.q_weight, &c.k_weight})
+    if (w->defined()) {
+      expect(is_shape(*w, {d}), *w);
+      (void)dtype_code(w->scalar_type());
+    }
+  if (c.q_weight.defined() && c.k_weight.defined() && c.q_weight.scalar_type() != c.k_weight.scalar_type())
+    throw Raise{PyExc_TypeError, std::string("k_weight has dtype ") + c10::toString(c.k_weight.scalar_type()) + ", expected " + c10::toString(c.q_weight.scalar_type())};
+  if (c.sections.empty()) c.sections = {d / 2};
+  int64_t sum = 0;
+  for (int64_t s : c.sections) {
+    if (s < 0) throw Raise{PyExc_ValueError, "sections must not be negative"};
+    sum += s;
+    if (sum > d / 2) throw Raise{PyExc_ValueError, "sections add up to more than the " + std::to_string(d / 2) + " pairs of a head"};
+  }
+  const int64_t axes = (int64_t)c.sections.size();
+  if (axes > 4) throw Raise{PyExc_ValueError, "at most 4 axes, got " + std::to_string(axes)};
+  if (c.positions.defined()) {
+    const bool flat = axes == 1 && is_shape(c.positions, {q.size(0), q.size(1)});
+    if (!flat && !is_shape(c.positions, {q.size(0), q.size(1), axes}))
+      throw Raise{PyExc_ValueError, "positions must have shape (" + std::to_string(q.size(0)) + ", " + std::to_string(q.size(1)) +
+                                        (axes == 1 ? ")" : ", " + std::to_string(axes) + ")") + ", got " + sizes_of(c.positions)};
+  }
+}
+// contiguous arrays of the types that the kernels read
+void settle(NormRope& c) {
+  if (c.positions.defined()) c.positions = ints(c.positions);
+  c.cos = c.cos.to(at::kFloat).contiguous();
+  c.sin = c.sin.to(at::kFloat).contiguous();
+  if (c.q_weight.defined()) c.q_weight = c.q_weight.contiguous();
+  if (c.k_weight.defined()) c.k_weight = c.k_weight.contiguous();
+}
+template <typename Args>
+void describe_norm_rope(const Tensor& q, const Tensor& k, const NormRope& c, Args& a) {
+  const int64_t h = c.heads;
+  a.qa = factor_of<TpaFactor>(q); a.qb = factor_of<TpaFactor>(q, h);
+  a.ka = factor_of<TpaFactor>(k); a.kb = factor_of<TpaFactor>(k, h);
+  a.positions = ids_ptr(c.positions); a.rope_cos = f32_ptr(c.cos); a.rope_sin = f32_ptr(c.sin);
+  a.q_weight = c.q_weight.defined() ? c.q_weight.data_ptr() : nullptr;
+  a.k_weight = c.k_weight.defined() ? c.k_weight.data_ptr() : nullptr;
+  const Tensor& w = c.q_weight.defined() ? c.q_weight : c.k_weight;
+  a.weight_dtype = w.defined() ? dtype_code(w.scalar_type()) : TPA_DTYPE_F32;
+  a.n_axes = (int)c.sections.size();
+  for (size_t i = 0; i < c.sections.size(); ++i) a.sections[i] = (int)c.sections[i];
+  a.B = (int)q.size(0); a.l = (int)q.size(1); a.H = (int)h; a.D = (int)(q.size(3) - h); a.rq = (int)q.size(2); a.rk = (int)k.size(2);
+  a.rope_len = (int)c.cos.size(0); a.dtype = dtype_code(q.scalar_type()); a.kernel = c.kernel;
+  a.normalize = c.normalize; a.eps = (float)c.eps;
+}
+std::pair<Tensor, Tensor> run_norm_rope(const Tensor& q, const Tensor& k, const NormRope& c) {
+  const c10::DeviceGuard guard(q.device());
+  std::pair<Tensor, Tensor> r;
+  r.first = at::empty(q.sizes(), q.options());
+  r.second = at::empty(k.sizes(), k.options());
+  if (!q.size(0) || !q.size(1)) return r;  // no tokens
+  TpaNormRopeArgs a{};
+  describe_norm_rope(q, k, c, a);
+  a.qa_out = factor_of<TpaFactor>(r.first); a.qb_out = factor_of<TpaFactor>(r.first, c.heads);
+  a.ka_out = factor_of<TpaFactor>(r.second); a.kb_out = factor_of<TpaFactor>(r.second, c.heads);
+  check("tpa_norm_rope", lib.tpa_norm_rope(&a, stream_of(q.device())));
+  return r;
+}
+// gradients of q, k, q_weight, k_weight; an output without a gradient gives its side none
+void run_norm_rope_bwd(const Tensor& q, const Tensor& k, const NormRope& c, const Tensor& dq_out, const Tensor& dk_out, const bool (&weights)[2], Tensor* grads) {
+  const c10::DeviceGuard guard(q.device());
+  const Tensor in[2] = {q, k};
+  Tensor d_out[2] = {dq_out, dk_out};
+  const Tensor weight[2] = {c.q_weight, c.k_weight};
+  for (int i = 0; i < 2; ++i) {
+    if (!d_out[i].defined()) continue;
+    expect(d_out[i].sizes() == in[i].sizes(), d_out[i]);
+    d_out[i] = d_out[i].to(q.scalar_type()).contiguous();
+    grads[i] = at::empty(in[i].sizes(), in[i].options());
+    if (weights[i] && weight[i].defined()) grads[2 + i] = at::empty(weight[i].sizes(), weight[i].options());
+  }
+  if (!d_out[0].defined() && !d_out[1].defined()) return;
+  if (!q.size(0) || !q.size(1)) {
+    for (int i = 2; i < 4; ++i)
+      if (grads[i].defined()) grads[i].zero_();
+    return;
+  }
+  TpaNormRopeBwdArgs a{};
+  describe_norm_rope(q, k, c, a);
+  const int64_t h = c.heads;
+  if (d_out[0].defined()) {
+    a.dqa_out = factor_of<TpaFactor>(d_out[0]); a.dqb_out = factor_of<TpaFactor>(d_out[0], h);
+    a.dqa = factor_of<TpaFactor>(grads[0]); a.dqb = factor_of<TpaFactor>(grads[0], h);
+  }
+  if (d_out[1].defined()) {
+    a.dka_out = factor_of<TpaFactor>(d_out[1]); a.dkb_out = factor_of<TpaFactor>(d_out[1], h);
+    a.dka = factor_of<TpaFactor>(grads[1]); a.dkb = factor_of<TpaFactor>(grads[1], h);
+  }
+  Tensor ws;
+  if (grads[2].defined() || grads[3].defined()) {
+    a.dq_weight = grads[2].defined() ? grads[2].data_ptr() : nullptr;
+    a.dk_weight = grads[3].defined() ? grads[3].data_ptr() : nullptr;
+    ws = bytes_on(q.device(), lib.tpa_norm_rope_bwd_workspace_bytes(a.B, a.l, a.D) + 256);
+    take_workspace(ws, 256, a);
+  }
+  check("tpa_norm_rope_bwd", lib.tpa_norm_rope_bwd(&a, stream_of(q.device())));
+}
+
+struct NormRopeOperator : torch::autograd::Function<NormRopeOperator> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& q_weight,
+                                                const Tensor& k_weight, const NormRope& c) {
+    auto [yq, yk] = run_norm_rope(q, k, c);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, q_weight, k_weight});
+    ctx->saved_data["call"] = c10::IValue(std::make_tuple(c.positions, c.cos, c.sin, c.heads, c.sections, c.normalize, c.eps, (int64_t)c.kernel));
+    return {yq, yk};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d_out) {
+    torch::autograd::variable_list out(5);
+    const auto saved = ctx->get_saved_variables();
+    const auto call = ctx->saved_data["call"].toTuple();
+    const auto& e = call->elements();
+    NormRope c;
+    c.q_weight = saved[2]; c.k_weight = saved[3];
+    c.positions = e[0].toTensor(); c.cos = e[1].toTensor(); c.sin = e[2].toTensor();
+    c.heads = e[3].toInt(); c.sections = e[4].toIntVector(); c.normalize = e[5].toBool(); c.eps = e[6].toDouble(); c.kernel = (int)e[7].toInt();
+    const bool weights[2] = {ctx->needs_input_grad(2), ctx->needs_input_grad(3)};
+    try {
+      run_norm_rope_bwd(saved[0], saved[1], c, d_out[0], d_out[1], weights, out.data());
+    } catch (const CallFailed& f) {  // an engine thread: hand the Python exception to the thread that asked
+      PyGILState_STATE gil = PyGILState_Ensure();
+      set_python_error(f);
+      python_error e2;
+      e2.persist();
+      PyGILState_Release(gil);
+      throw e2;
+    } catch (const Raise& f) {
+      TORCH_CHECK(false, f.text);
+    }
+    return out;
+  }
+};
+
+std::vector<int64_t> numbers(PyObject* arg) {  // None or a sequence of integers
+  std::vector<int64_t> out;
+  if (arg == Py_None) return out;
+  PyObject* seq = PySequence_Fast(arg, "sections must be a sequence of integers");
+  if (!seq) throw python_error();
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) {
+    const long long v = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i));
+    if (v == -1 && PyErr_Occurred()) {
+      Py_DECREF(seq);
+      throw python_error();
+    }
+    out.push_back(v);
+  }
+  Py_DECREF(seq);
+  if (out.empty()) throw Raise{PyExc_ValueError, "sections must have an entry for each axis"};
+  return out;
+}
+// the arguments behind the factors: rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel
+NormRope norm_rope_call(PyObject* const* args) {
+  NormRope c;
+  c.cos = THPVariable_Unpack(args[0]); c.sin = THPVariable_Unpack(args[1]);
+  c.q_weight = tensor_or_none(args[2]); c.k_weight = tensor_or_none(args[3]); c.positions = tensor_or_none(args[4]);
+  c.heads = integer(args[5]);
+  c.sections = numbers(args[6]);
+  c.normalize = integer(args[7]);
+  c.eps = real(args[8]);
+  c.kernel = (int)integer(args[9]);
+  return c;
+}
+
+// norm_rope(q, k, rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel)
+PyObject* norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("norm_rope", n, 12);
+  if (!gpu_tensors(args, 4) || !none_or_gpu(args[4]) || !none_or_gpu(args[5]) || !none_or_gpu(args[6])) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor q = THPVariable_Unpack(args[0]), k = THPVariable_Unpack(args[1]);
+  NormRope c = norm_rope_call(args + 2);
+  check_norm_rope(q, k, c);
+  one_device({q, k, c.cos, c.sin, c.q_weight, c.k_weight, c.positions});
+  no_tangents({q, k, c.q_weight, c.k_weight}, "tpa_norm_rope");
+  std::pair<Tensor, Tensor> r;
+  {
+    WithoutGil free;
+    const c10::DeviceGuard guard(q.device());
+    settle(c);
+    auto asks = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    if (at::GradMode::is_enabled() && (asks(q) || asks(k) || asks(c.q_weight) || asks(c.k_weight))) {
+      auto out = NormRopeOperator::apply(q, k, c.q_weight, c.k_weight, c);
+      r = {out[0], out[1]};
+    } else {
+      r = run_norm_rope(q, k, c);
+    }
+  }
+  return pair(std::move(r));
+  END_CALL
+}
+
+// norm_rope_backward(q, k, rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel, dq_out, dk_out)
+PyObject* norm_rope_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("norm_rope_backward", n, 14);
+  if (!gpu_tensors(args, 4) || !none_or_gpu(args[4]) || !none_or_gpu(args[5]) || !none_or_gpu(args[6]) || !gpu_tensors(args + 12, 2)) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor q = THPVariable_Unpack(args[0]), k = THPVariable_Unpack(args[1]);
+  NormRope c = norm_rope_call(args + 2);
+  check_norm_rope(q, k, c);
+  one_device({q, k, c.cos, c.sin, c.q_weight, c.k_weight, c.positions, THPVariable_Unpack(args[12]), THPVariable_Unpack(args[13])});
+  Tensor grads[4];
+  {
+    WithoutGil free;
+    const at::AutoGradMode no_grad(false);
+    const c10::DeviceGuard guard(q.device());
+    settle(c);
+    run_norm_rope_bwd(q, k, c, THPVariable_Unpack(args[12]), THPVariable_Unpack(args[13]), {true, true}, grads);
+  }
+  PyObject* out = PyTuple_New(4);
+  if (!out) throw python_error();
+  for (int i = 0; i < 4; ++i) {
+    if (!grads[i].defined()) Py_INCREF(Py_None);
+    PyTuple_SET_ITEM(out, i, grads[i].defined() ? THPVariable_Wrap(std::move(grads[i])) : Py_None);
+  }
+  return out;
+  END_CALL
+}
+
+// norm_rope_write(q, k, rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel, v, slots, ka, kb, va, vb)
+PyObject* norm_rope_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("norm_rope_write", n, 18);
+  if (!gpu_tensors(args, 4) || !none_or_gpu(args[4]) || !none_or_gpu(args[5]) || !none_or_gpu(args[6]) || !gpu_tensors(args + 12, 2)) Py_RETURN_NOTIMPLEMENTED;
+  if (!gpu_tensors(args + 14, 4)) throw Raise{PyExc_TypeError, "the cache is written in place: ka, kb, va, vb must be GPU tensors"};
+  const Tensor q = THPVariable_Unpack(args[0]), k = THPVariable_Unpack(args[1]), v = THPVariable_Unpack(args[12]);
+  Tensor slots = THPVariable_Unpack(args[13]);
+  NormRope c = norm_rope_call(args + 2);
+  check_norm_rope(q, k, c);
+  const int64_t h = c.heads, d = q.size(3) - h, rk = k.size(2);
+  expect(v.sizes() == k.sizes(), v);
+  if (!is_shape(slots, {q.size(0), q.size(1)}))
+    throw Raise{PyExc_ValueError, "slots must have shape (" + std::to_string(q.size(0)) + ", " + std::to_string(q.size(1)) + "), got " + sizes_of(slots)};
+  static const char* const names[6] = {"q", "ka", "kb", "va", "vb", "v"};
+  const Tensor t[6] = {q, THPVariable_Unpack(args[14]), THPVariable_Unpack(args[15]), THPVariable_Unpack(args[16]), THPVariable_Unpack(args[17]), v};
+  check_dtypes(t, names, 6);
+  one_device({q, k, v, c.cos, c.sin, c.q_weight, c.k_weight, c.positions, slots, t[1], t[2], t[3], t[4]});
+  const Tensor& ka = t[1];
+  if (ka.dim() != 4) throw Raise{PyExc_ValueError, "the cache's arrays are [pages, page_size, rank, x], got shape " + sizes_of(ka)};
+  for (int i = 1; i < 5; ++i) expect(is_shape(t[i], {ka.size(0), ka.size(1), rk, i % 2 ? h : d}), t[i]);
+  if (ka.size(0) * ka.size(1) > INT32_MAX) throw CallFailed{"tpa_norm_rope", TPA_ERR_SHAPE};
+  Tensor yq;
+  {
+    WithoutGil free;
+    const at::AutoGradMode no_grad(false);  // a cache is state: no gradient flows into it
+    const c10::DeviceGuard guard(q.device());
+    settle(c);
+    slots = ints(slots);
+    yq = at::empty(q.sizes(), q.options());
+    if (q.size(0) && q.size(1)) {
+      TpaNormRopeArgs a{};
+      describe_norm_rope(q, k, c, a);
+      a.qa_out = factor_of<TpaFactor>(yq); a.qb_out = factor_of<TpaFactor>(yq, h);
+      a.va = factor_of<TpaFactor>(v); a.vb = factor_of<TpaFactor>(v, h);
+      a.ka_out = factor_of<TpaFactor>(t[1]); a.kb_out = factor_of<TpaFactor>(t[2]);
+      a.va_out = factor_of<TpaFactor>(t[3]); a.vb_out = factor_of<TpaFactor>(t[4]);
+      a.slots = ids_ptr(slots);
+      a.page_size = (int)ka.size(1);
+      a.num_slots = (int)(ka.size(0) * ka.size(1));
+      check("tpa_norm_rope", lib.tpa_norm_rope(&a, stream_of(q.device())));
+      for (int i = 1; i < 5; ++i) written(t[i]);
+    }
+  }
+  return THPVariable_Wrap(std::move(yq));
+  END_CALL
+}
+
 // ------------------------------------------------------------------------------------------------ module
 // bind(path of libtpa_gfx950.so, TpaError)
 PyObject* bind(PyObject*, PyObject* args) {
@@ -597,7 +1030,8 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(factors), FAST(decode), FAST(append), FAST(backward), FAST(tpa), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(factors), FAST(decode), FAST(append), FAST(backward), FAST(tpa), FAST(decode_shared), FAST(page_tables),
+                         FAST(norm_rope), FAST(norm_rope_backward), FAST(norm_rope_write), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tpa_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

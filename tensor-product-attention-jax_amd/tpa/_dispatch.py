@@ -24,7 +24,7 @@ KERNEL_AUTO = 0
 KERNEL_GENERIC = 1
 KERNEL_MFMA = 2
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 class TpaFactor(ctypes.Structure):
@@ -199,6 +199,105 @@ class TpaAppendArgs(ctypes.Structure):
     ]
 
 
+class TpaPageTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv_lengths", ctypes.c_void_p),
+        ("new_tokens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_start", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("new_kv_lengths", ctypes.c_void_p),
+        ("new_free_start", ctypes.c_void_p),
+        ("B", ctypes.c_int32),
+        ("pages_per_seq", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_free", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+    ]
+
+
+class TpaNormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("qa", TpaFactor),
+        ("qb", TpaFactor),
+        ("ka", TpaFactor),
+        ("kb", TpaFactor),
+        ("qa_out", TpaFactor),
+        ("qb_out", TpaFactor),
+        ("ka_out", TpaFactor),
+        ("kb_out", TpaFactor),
+        ("va", TpaFactor),
+        ("vb", TpaFactor),
+        ("va_out", TpaFactor),
+        ("vb_out", TpaFactor),
+        ("slots", ctypes.c_void_p),
+        ("page_size", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32),
+        ("positions", ctypes.c_void_p),
+        ("rope_cos", ctypes.c_void_p),
+        ("rope_sin", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("n_axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("B", ctypes.c_int32),
+        ("l", ctypes.c_int32),
+        ("H", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("rq", ctypes.c_int32),
+        ("rk", ctypes.c_int32),
+        ("rope_len", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("kernel", ctypes.c_int32),
+        ("normalize", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class TpaNormRopeBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("qa", TpaFactor),
+        ("qb", TpaFactor),
+        ("ka", TpaFactor),
+        ("kb", TpaFactor),
+        ("dqa_out", TpaFactor),
+        ("dqb_out", TpaFactor),
+        ("dka_out", TpaFactor),
+        ("dkb_out", TpaFactor),
+        ("dqa", TpaFactor),
+        ("dqb", TpaFactor),
+        ("dka", TpaFactor),
+        ("dkb", TpaFactor),
+        ("dq_weight", ctypes.c_void_p),
+        ("dk_weight", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("rope_cos", ctypes.c_void_p),
+        ("rope_sin", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("n_axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("B", ctypes.c_int32),
+        ("l", ctypes.c_int32),
+        ("H", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("rq", ctypes.c_int32),
+        ("rk", ctypes.c_int32),
+        ("rope_len", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("kernel", ctypes.c_int32),
+        ("normalize", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class TpaError(RuntimeError):
     """A non-zero return code of the C ABI."""
 
@@ -265,6 +364,16 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.tpa_bwd_workspace_bytes.argtypes = [ctypes.c_int32] * 6
         lib.mha_bwd_workspace_bytes.restype = ctypes.c_size_t
         lib.mha_bwd_workspace_bytes.argtypes = [ctypes.c_int32] * 7
+        for name, args in (("tpa_page_tables", TpaPageTablesArgs), ("tpa_norm_rope", TpaNormRopeArgs), ("tpa_norm_rope_bwd", TpaNormRopeBwdArgs)):
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        lib.tpa_norm_rope_bwd_workspace_bytes.restype = ctypes.c_size_t
+        lib.tpa_norm_rope_bwd_workspace_bytes.argtypes = [ctypes.c_int32] * 3
+        lib.tpa_decode_shared.restype = ctypes.c_int
+        lib.tpa_decode_shared.argtypes = [ctypes.POINTER(TpaFwdArgs), ctypes.c_int32, ctypes.c_void_p]
+        lib.tpa_decode_shared_workspace_bytes.restype = ctypes.c_size_t
+        lib.tpa_decode_shared_workspace_bytes.argtypes = [ctypes.POINTER(TpaFwdArgs), ctypes.c_int32]
         if lib.tpa_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{p}: ABI version {lib.tpa_abi_version()} != {ABI_VERSION}")
         if path is None:

@@ -28,6 +28,7 @@ reference, all on purpose:
 
 from __future__ import annotations
 
+import ctypes
 import dataclasses
 
 import numpy as np
@@ -37,7 +38,7 @@ from . import _dispatch as _d
 
 __all__ = [
     "BlockSizes", "tpa", "tpa_factors", "tpa_decode", "tpa_cache_append", "tpa_factors_bwd", "_tpa_fwd", "_tpa_bwd", "_fwd", "_bwd",
-    "_precompute_delta", "_lse", "_lse_accum",
+    "_precompute_delta", "_lse", "_lse_accum", "tpa_decode_shared", "tpa_page_tables", "tpa_norm_rope", "tpa_norm_rope_bwd", "tpa_norm_rope_write",
 ]
 
 
@@ -210,6 +211,129 @@ def tpa_decode(
     )
 
 
+def tpa_decode_shared(
+    qa, qb, ka, kb, va, vb,
+    *,
+    prefix_length: int,
+    sm_scale: float = 1.0,
+    workspace: torch.Tensor | None = None,
+    kernel: int = _d.KERNEL_AUTO,
+    kv_lengths=None,
+    page_table=None,
+    causal: bool = False,
+    causal_offset: int = 0,
+):
+    """`tpa_decode` for a batch whose sequences share their first `prefix_length` tokens (an addition): a system prompt, or a
+    document that many ask about.  Operands and results are `tpa_decode`'s; the first `prefix_length` tokens of every
+    sequence are taken to be those of entry 0, whose cache (or whose pages, by row 0 of `page_table`) alone is read for them,
+    once for the whole batch.  In a paged cache the rows of `page_table` may name the same pages there; a page that the prefix
+    only begins belongs to one sequence, since its rest does.  `kv_lengths` count the prefix too; a sequence shorter than the prefix
+    sees as much of it as its length says.  `workspace` (uint8, at least
+    `decode_shared_workspace_bytes(...)`) may be passed to avoid the allocation; a workspace serves one call at a time.
+    Returns (o[b,lq,h,dv], lse[b,h,lq]).
+    """
+    return _call(
+        _d.host_calls().decode_shared, (qa, qb, ka, kb, va, vb, kv_lengths, page_table, workspace),
+        int(prefix_length), sm_scale, int(kernel), _causal_code(causal), int(causal_offset),
+    )
+
+
+def tpa_page_tables(kv_lengths, new_tokens, page_table, free_pages, *, page_size: int, num_tokens: int, free_start=None):
+    """Page tables, slots and positions of a serving step's new tokens, built on the GPU from the requests' lengths (an addition).
+
+    Request i has `kv_lengths[i]` cached tokens, whose pages stand in row i of `page_table` (int32 [b, pages_per_seq], a contiguous GPU tensor
+    that is updated in place), and brings `new_tokens[i]` more.  The tokens of a step are packed request after request into
+    `num_tokens` rows (padding behind them).  Pages that the new tokens open are taken from `free_pages` from index `free_start` on (int32 [1], 0 if
+    not given), the requests served in order.  Tokens past the end of the table's row, or past the last free page, get
+    no slot.  All results stay on the GPU (no synchronisation):
+
+        slots[num_tokens]      page * page_size + place in it, for `tpa_norm_rope_write`; -1 for padding and tokens without a page
+        positions[num_tokens]  position of every row's token in its sequence; 0 for padding
+        starts[b + 1]          first row of every request
+        new_kv_lengths[b]      lengths with the new tokens that have a slot, for `tpa_decode` and the next step
+        new_free_start[1]      `free_start` and the pages taken
+    """
+    return _call(
+        _d.host_calls().page_tables, (kv_lengths, new_tokens, free_pages, free_start), page_table, int(page_size), int(num_tokens)
+    )
+
+
+def tpa_norm_rope(
+    q, k,
+    num_heads: int,
+    rope_cos, rope_sin,
+    q_weight=None, k_weight=None,
+    positions=None,
+    sections=None,
+    eps: float = 1e-6,
+    normalize: bool = True,
+    kernel: int = _d.KERNEL_AUTO,
+):
+    """Norms of queries and keys for each head and the rotation by position, on the rank factors (an addition, differentiable with
+    respect to q, k and the weights).
+
+    q[b,l,rq,h+d], k[b,l,rk,h+d] as `tpa` takes them.  With X_h = (1/R) sum_r a_r[h] b_r the head vectors that the factors stand for,
+    the results' head vectors are rotation(weight * X_h / sqrt(mean(X_h^2) + eps)): the norm of a head scales the head factors,
+    weight and rotation act on the b factors, so rank and layout stay and the results go straight into `tpa` or a cache.
+    rope_cos, rope_sin[rope_len, d/2] fp32 and the rotated pairs are those of `tpa_cache_append`.  `positions`: int [b, l] (default: 0 .. l-1), or
+    [b, l, axes] with `sections`, the number of pairs that belong to each axis (time, height, width; up to four): pair j
+    turns by its own axis' position, pairs past the last section do not turn.  `q_weight`, `k_weight` [d] (fp32 or bf16; default
+    ones).  `normalize=False` leaves the norms out.  Returns (q', k') in the inputs' shapes and type.
+    """
+    return _call(
+        _d.host_calls().norm_rope, (q, k, rope_cos, rope_sin, q_weight, k_weight, positions),
+        int(num_heads), sections, bool(normalize), float(eps), int(kernel),
+    )
+
+
+def tpa_norm_rope_bwd(
+    q, k,
+    num_heads: int,
+    rope_cos, rope_sin,
+    dq_out, dk_out,
+    q_weight=None, k_weight=None,
+    positions=None,
+    sections=None,
+    eps: float = 1e-6,
+    normalize: bool = True,
+    kernel: int = _d.KERNEL_AUTO,
+):
+    """Gradients of `tpa_norm_rope` from those of its results: (dq, dk, dq_weight, dk_weight), None for a weight that is not
+    given.  torch.autograd reaches the same through `tpa_norm_rope`."""
+    device = _pick_device(q, k)
+    arrays = [None if x is None else _as_device_tensor(x, device) for x in (q, k, rope_cos, rope_sin, q_weight, k_weight, positions)]
+    return _d.host_calls().norm_rope_backward(
+        *arrays, int(num_heads), sections, bool(normalize), float(eps), int(kernel), *(_as_device_tensor(x, device) for x in (dq_out, dk_out))
+    )
+
+
+def tpa_norm_rope_write(
+    q, k, v,
+    num_heads: int,
+    rope_cos, rope_sin,
+    ka, kb, va, vb,
+    slots,
+    q_weight=None, k_weight=None,
+    positions=None,
+    sections=None,
+    eps: float = 1e-6,
+    normalize: bool = True,
+    kernel: int = _d.KERNEL_AUTO,
+):
+    """`tpa_norm_rope` for serving: the K factors and the V factors (copied) go into a paged cache.
+
+    q[b,l,rq,h+d], k[b,l,rk,h+d], v[b,l,rk,h+d] of the new tokens, packed (b = 1) or not; `slots` int [b, l] of
+    `tpa_page_tables`: token i's factors go to place slots[i] % page_size of page slots[i] // page_size of the pools ka, kb, va, vb
+    [pages, page_size, rk, h|d], which `tpa_decode` reads; slots outside the pools (-1) are dropped, and no slot may be there twice.  A contiguous
+    cache [b, cache_len, rk, h|d] is a pool whose pages are the batch entries.  Returns q' like q.  No gradient flows through this call.
+    """
+    device = _pick_device(q, k, v)
+    arrays = [None if x is None else _as_device_tensor(x, device) for x in (q, k, rope_cos, rope_sin, q_weight, k_weight, positions)]
+    return _d.host_calls().norm_rope_write(
+        *arrays, int(num_heads), sections, bool(normalize), float(eps), int(kernel), *(_as_device_tensor(x, device) for x in (v, slots)), ka, kb, va, vb
+    )
+
+
 def tpa_cache_append(
     x, w, rope_cos, rope_sin, ka, kb, va, vb,
     kv_lengths=None,
@@ -332,6 +456,20 @@ def tpa_factors_bwd(
     with torch.cuda.device(device):
         _d.check("tpa_bwd", lib.tpa_bwd(args, _d.current_stream_ptr(device)))
     return tuple(grads)
+
+
+def decode_shared_workspace_bytes(qa, qb, ka, kb, va, vb, *, prefix_length: int, page_table=None, kernel: int = _d.KERNEL_AUTO) -> int:
+    """What `tpa_decode_shared` needs for operands of these shapes and layouts (room to align it among it)."""
+    b, lq, rq, h = qa.shape
+    rows, per, rk, dv = vb.shape
+    lk = per if page_table is None else page_table.shape[1] * per
+    args = _d.TpaFwdArgs(
+        qa=_d.factor(qa), qb=_d.factor(qb), ka=_d.factor(ka), kb=_d.factor(kb), va=_d.factor(va), vb=_d.factor(vb),
+        B=b, lq=lq, lk=lk, H=h, dk=qb.shape[-1], dv=dv, rq=rq, rk=rk, dtype=_d.dtype_code(qa.dtype), sm_scale=1.0, kernel=int(kernel),
+        page_table=None if page_table is None else page_table.data_ptr(), page_size=0 if page_table is None else per,
+        pages_per_seq=0 if page_table is None else page_table.shape[1],
+    )
+    return int(_d.load_library().tpa_decode_shared_workspace_bytes(ctypes.byref(args), int(prefix_length))) + 256
 
 
 def bwd_workspace_bytes(b: int, lq: int, lk: int, h: int, dk: int, dv: int) -> int:

@@ -1,0 +1,134 @@
+"""tpa_page_tables (page tables, slots and positions of a step's new tokens) against a plain walk over the requests, and its refusals.
+All results are whole numbers and have to be equal."""
+
+import numpy as np
+import pytest
+import torch
+
+from tpa import tpa
+
+pytestmark = pytest.mark.gpu
+
+
+def walk(lengths, news, table, free, page, rows, start):
+    """The definition, request by request and token by token."""
+    table = table.copy()
+    cap = table.shape[1] * page
+    slots, positions = np.full(rows, -1, np.int32), np.zeros(rows, np.int32)
+    starts, after, row, at = [0], [], 0, max(0, min(start, len(free)))
+    for b, (length, new) in enumerate(zip(lengths, news)):
+        length, new = max(0, min(length, cap)), min(max(new, 0), rows - row)
+        have = -(-length // page)
+        want = -(-min(length + new, cap) // page) - have
+        got = min(want, len(free) - at)
+        table[b, have : have + got] = free[at : at + got]
+        end = min(length + new, cap) if got == want else (have + got) * page
+        for i in range(new):
+            positions[row + i] = length + i
+            if length + i < end:
+                slots[row + i] = table[b, (length + i) // page] * page + (length + i) % page
+        at += got
+        row += new
+        starts.append(row)
+        after.append(end)
+    return slots, positions, np.array(starts), np.array(after), np.array([at]), table
+
+
+def check(gpu, lengths, news, pages, page, rows, n_free, start, seed=0):
+    rng = np.random.default_rng(seed)
+    ids = rng.permutation(len(lengths) * pages + n_free).astype(np.int32)
+    table, free = ids[: len(lengths) * pages].reshape(len(lengths), pages).copy(), ids[len(lengths) * pages :].copy()
+    want = walk(lengths, news, table, free, page, rows, start or 0)
+    dev = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=gpu)
+    t = dev(table)
+    got = tpa.tpa_page_tables(dev(lengths), dev(news), t, dev(free), page_size=page, num_tokens=rows, free_start=None if start is None else dev([start]))
+    for name, g, w in zip(("slots", "positions", "starts", "new_kv_lengths", "new_free_start", "page_table"), (*got, t), want):
+        assert g.dtype == torch.int32 and g.cpu().tolist() == w.tolist(), name
+
+
+@pytest.mark.parametrize(
+    "lengths,news,pages,page,rows,n_free,start",
+    [
+        ([0], [1], 1, 1, 1, 1, None),                        # the smallest step
+        ([5], [0], 2, 4, 0, 3, 0),                           # no new token, no row
+        ([0, 3, 4, 7], [1, 1, 1, 1], 2, 4, 4, 9, 2),         # first page, inside a page, at a page's end
+        ([0, 0, 0], [0, 9, 0], 4, 4, 16, 4, 1),              # requests without tokens beside one with three pages, padding
+        ([6, 2], [5, 9], 2, 4, 14, 9, 0),                    # past the end of the table's row
+        ([3, 3, 3], [6, 6, 6], 4, 4, 18, 4, 1),              # the free list runs out inside the second request
+        ([4, 4], [4, 4], 4, 4, 8, 0, None),                  # no free page at all
+        ([1, 1], [3, 3], 4, 4, 8, 5, 99),                    # start behind the list's end; no page is needed
+        ([-2, 50, 2], [-1, 3, 2], 3, 8, 6, 5, -4),           # lengths, counts and a start outside their ranges
+        ([0, 0], [7, 7], 4, 4, 10, 9, 0),                    # more tokens than rows: the rest has none
+        ([2147483647, 0], [2147483647, 2147483647], 4, 4, 20, 9, 0),
+    ],
+)
+def test_steps(gpu, lengths, news, pages, page, rows, n_free, start):
+    check(gpu, lengths, news, pages, page, rows, n_free, start)
+
+
+@pytest.mark.parametrize("b,most,page,pages", [(64, 1, 64, 8), (255, 40, 16, 9), (256, 3, 1, 12), (257, 700, 16, 60), (1031, 5, 7, 11), (8192, 2, 32, 3)])
+@pytest.mark.parametrize("scarce", [False, True])
+def test_many_requests(gpu, b, most, page, pages, scarce):
+    rng = np.random.default_rng(b)
+    lengths, news = rng.integers(0, pages * page, b).tolist(), rng.integers(0, most + 1, b).tolist()
+    rows = sum(news) + (0 if scarce else 77)
+    check(gpu, lengths, news, pages, page, rows, b * pages // (8 if scarce else 1) + 3, 3, seed=b)
+
+
+def test_numpy_lengths_and_int64(gpu):
+    t = torch.zeros((2, 4), dtype=torch.int32, device=gpu)
+    got = tpa.tpa_page_tables(np.array([0, 5]), torch.tensor([2, 1], device=gpu), t, torch.arange(10, 20, device=gpu), page_size=4, num_tokens=3)
+    assert got[0].tolist() == [40, 41, 1] and t.tolist() == [[10, 0, 0, 0], [0, 0, 0, 0]]
+
+
+def test_replays_from_a_graph_and_on_another_stream(gpu):
+    """Three decode steps captured once: the lengths, the table and the free list's start go from step to step on the GPU."""
+    b, page, pages = 5, 4, 6
+    lengths0 = torch.tensor([0, 3, 4, 9, 15], dtype=torch.int32, device=gpu)
+    news, free = torch.ones(b, dtype=torch.int32, device=gpu), torch.arange(40, 70, dtype=torch.int32, device=gpu)
+    table0 = torch.arange(b * pages, dtype=torch.int32, device=gpu).view(b, pages)
+    lengths, table, start = lengths0.clone(), table0.clone(), torch.zeros(1, dtype=torch.int32, device=gpu)
+
+    def step():
+        slots, _, _, after, at = tpa.tpa_page_tables(lengths, news, table, free, page_size=page, num_tokens=b, free_start=start)
+        lengths.copy_(after)
+        start.copy_(at)
+        return slots
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            captured = step()
+    torch.cuda.synchronize()
+    lengths.copy_(lengths0)
+    table.copy_(table0)
+    start.zero_()
+    at, t, n = 0, table0.cpu().numpy(), lengths0.tolist()
+    for _ in range(6):
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = walk(n, [1] * b, t, free.cpu().numpy(), page, b, at)
+        t, n, at = want[5], want[3].tolist(), int(want[4][0])
+        assert captured.tolist() == want[0].tolist() and table.cpu().tolist() == t.tolist() and lengths.tolist() == n and start.tolist() == [at]
+
+
+def test_refusals(gpu):
+    t = torch.zeros((2, 4), dtype=torch.int32, device=gpu)
+    n = torch.zeros(2, dtype=torch.int32, device=gpu)
+    with pytest.raises(TypeError):
+        tpa.tpa_page_tables(n, n, t.cpu(), n, page_size=4, num_tokens=2)
+    for bad in (t.long(), t.T, t[0]):
+        with pytest.raises(ValueError):
+            tpa.tpa_page_tables(n, n, bad, n, page_size=4, num_tokens=2)
+    with pytest.raises(ValueError):
+        tpa.tpa_page_tables(n[:1], n, t, n, page_size=4, num_tokens=2)
+    with pytest.raises(ValueError):
+        tpa.tpa_page_tables(n, n, t, n, page_size=0, num_tokens=2)
+    with pytest.raises(ValueError):
+        tpa.tpa_page_tables(n, n, t, n, page_size=4, num_tokens=-1)
+    with pytest.raises(ValueError):
+        tpa.tpa_page_tables(n, n, t, n, page_size=4, num_tokens=1, free_start=n)
