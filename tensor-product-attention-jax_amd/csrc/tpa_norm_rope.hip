@@ -7,6 +7,7 @@
 //
 // G has signs, so |X_h|^2 may be far below the sum of its terms' sizes where ranks cancel.  It is summed in fp32 for bf16 factors,
 // whose products are exact there, and in 64 bits for fp32 factors.
+#include <algorithm>
 #include <type_traits>
 
 #include "tpa_common.h"
@@ -245,7 +246,583 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumParams p) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------- matrix cores
+// A wave takes the rank rows of as many tokens of one side as fit the 16 rows of a matrix instruction, RM to a token: lane (i, g) holds
+// row i's elements 32 s + 8 g + 0..7 of every chunk s, 16 bytes a load.  That is at once the layout of both operands of G = B B^T
+// (no exchange between lanes) and whole pairs for the rotation.  A head's norm is a lane's: G through LDS, R^2 products.
+// HBM bounds it: a token's factors come once and go once.
+typedef __attribute__((ext_vector_type(4))) double f64x4;
+constexpr int kNormWaves = 4;
+
+template <typename T>
+struct Chunk {  // eight elements as loaded
+  u32x4 x[sizeof(T) / 2];
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(T) == 2) return e & 1 ? bf16hi_to_f32(x[0][e / 2]) : bf16lo_to_f32(x[0][e / 2]);
+    else return __uint_as_float(x[e / 4][e % 4]);
+  }
+};
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* from) {
+  Chunk<T> c;
+#pragma unroll
+  for (int n = 0; n < (int)sizeof(T) / 2; ++n) c.x[n] = reinterpret_cast<const u32x4*>(from)[n];
+  return c;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* to, const float (&y)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<u32x4*>(to) = u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])};
+  } else {
+    *reinterpret_cast<f32x4*>(to) = f32x4{y[0], y[1], y[2], y[3]};
+    *reinterpret_cast<f32x4*>(to + 4) = f32x4{y[4], y[5], y[6], y[7]};
+  }
+}
+// VH neighbouring head factors
+template <typename T, int VH>
+__device__ __forceinline__ void load_heads(const T* from, float (&a)[VH]) {
+  if constexpr (VH == 1) {
+    a[0] = load_as_f32(from);
+  } else if constexpr (sizeof(T) == 2) {
+    const uint32_t x = *reinterpret_cast<const uint32_t*>(from);
+    a[0] = bf16lo_to_f32(x); a[1] = bf16hi_to_f32(x);
+  } else {
+    const float2 x = *reinterpret_cast<const float2*>(from);
+    a[0] = x.x; a[1] = x.y;
+  }
+}
+template <typename T, int VH>
+__device__ __forceinline__ void store_heads(T* to, const float (&a)[VH]) {
+  if constexpr (VH == 1) store_from_f32(to, a[0]);
+  else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16(a[0], a[1]);
+  else *reinterpret_cast<float2*>(to) = make_float2(a[0], a[1]);
+}
+
+// what a wave's tokens are: 16 / RM of them, lane i's row is rank i % RM of token i / RM
+template <int RM>
+struct Rows {
+  static constexpr int P = 16 / RM;
+  int token, bi, i;  // of this lane's row (clamped)
+  int r;
+  bool there;        // the row is a rank of a token
+  int first;         // token of row 0
+  __device__ __forceinline__ Rows(int group, int tokens, int l, int R, int lane) {
+    const int row = lane & 15, tt = row / RM;
+    first = group * P;
+    r = row - tt * RM;
+    there = tt < P && r < R && first + tt < tokens;
+    token = min(first + min(tt, P - 1), tokens - 1);
+    r = min(r, R - 1);
+    bi = token / l;
+    i = token - bi * l;
+  }
+};
+// the sums of G and what is made from them: 32 bits for bf16 factors, 64 for fp32
+template <typename T>
+using Sum = std::conditional_t<sizeof(T) == 2, float, double>;
+
+// G of the wave's tokens, token by token in LDS: row r of token tt at (tt RM + r) RMP
+template <int RM>
+constexpr int kGramStride = (RM + 3) / 4 * 4;
+template <typename T, int D, int RM>
+__device__ __forceinline__ bool gram_to_lds(const Chunk<T> (&x)[D / 32], Sum<T>* G, int lane) {
+  const int i = lane & 15, g = lane >> 4;
+  bool finite = true;
+  auto put = [&](int row, Sum<T> v) __attribute__((always_inline)) {
+    finite = finite && __builtin_fabs(v) <= 3.4028235e38;
+    if (row / RM == i / RM && i / RM < 16 / RM) G[(i / RM * RM + row % RM) * kGramStride<RM> + i % RM] = v;
+  };
+  if constexpr (sizeof(T) == 2) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      const bf16x8 f = __builtin_bit_cast(bf16x8, x[s].x[0]);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, f, acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) put(4 * g + e, acc[e]);
+  } else {
+    f64x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double f = x[s][e];
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(f, f, acc, 0, 0, 0);
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) put(4 * e + g, acc[e]);
+  }
+  return !__any(!finite);
+}
+// G a of a lane's heads; a^T G a comes back
+template <typename T, int RM, int VH>
+__device__ __forceinline__ void times_gram(const Sum<T>* G, int tt, const float (&a)[RM][VH], Sum<T> (&y)[RM][VH], Sum<T> (&square)[VH]) {
+#pragma unroll
+  for (int v = 0; v < VH; ++v) square[v] = 0;
+#pragma unroll
+  for (int r = 0; r < RM; ++r) {
+    const Sum<T>* const row = G + (tt * RM + r) * kGramStride<RM>;
+#pragma unroll
+    for (int v = 0; v < VH; ++v) y[r][v] = 0;
+#pragma unroll
+    for (int t = 0; t < RM; ++t) {
+      const Sum<T> x = row[t];
+#pragma unroll
+      for (int v = 0; v < VH; ++v) y[r][v] += x * (Sum<T>)a[t][v];
+    }
+#pragma unroll
+    for (int v = 0; v < VH; ++v) square[v] += (Sum<T>)a[r][v] * y[r][v];
+  }
+}
+template <typename S>
+__device__ __forceinline__ float inverse_norm_of(S square, int R, int D, float eps) {
+  const float mean = (float)(square / (S)(R * R * D));
+  return rsqrtf((mean < 0 ? 0 : mean) + eps);  // NaN stays NaN
+}
+
+// cos and sin of a lane's four pairs of chunk s
+template <int D, bool AXES>
+struct Turns {
+  f32x4 c[D / 32], s[D / 32];
+  __device__ __forceinline__ Turns(const Rotation& rot, int token, int i, int g) {
+    int64_t row = 0;
+    if constexpr (!AXES) row = row_of(rot, token, i, 0) * (D / 2);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+      const int j = 16 * x + 4 * g;
+      if constexpr (AXES) {
+        int axis = 0;
+#pragma unroll
+        for (int a = 0; a < 3; ++a) axis += j >= rot.last_of[a];
+        row = row_of(rot, token, i, min(axis, rot.n_axes - 1)) * (D / 2);
+      }
+      c[x] = *reinterpret_cast<const f32x4*>(rot.cos + row + j);
+      s[x] = *reinterpret_cast<const f32x4*>(rot.sin + row + j);
+      if constexpr (AXES)
+        if (j >= rot.last_of[3]) {
+          c[x] = f32x4{1.f, 1.f, 1.f, 1.f};
+          s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+  }
+};
+__device__ __forceinline__ void weights_at(const void* w, int bf16, int d, float (&out)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out[e] = 1.f;
+  if (!w) return;
+  if (bf16) {
+    const Chunk<uint16_t> c = load_chunk(static_cast<const uint16_t*>(w) + d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = c[e];
+  } else {
+    const Chunk<float> c = load_chunk(static_cast<const float*>(w) + d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = c[e];
+  }
+}
+__device__ __forceinline__ void wave_lds_fence() {  // the wave's own writes have landed
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_wave_barrier();
+}
+
+// calls f with the rows to a token that a rank of R takes
+template <typename F>
+__device__ __forceinline__ void with_rows(int R, F f) {
+  if (R == 1) f(std::integral_constant<int, 1>{});
+  else if (R == 2) f(std::integral_constant<int, 2>{});
+  else if (R <= 4) f(std::integral_constant<int, 4>{});
+  else if (R <= 6) f(std::integral_constant<int, 6>{});
+  else if (R <= 8) f(std::integral_constant<int, 8>{});
+  else f(std::integral_constant<int, 16>{});
+}
+__host__ __device__ inline int tokens_per_wave(int R) { return R == 1 ? 16 : R == 2 ? 8 : R <= 4 ? 4 : R <= 8 ? 2 : 1; }
+
+constexpr int kGramElements = 16 * 16;  // of G of a wave's tokens, at most
+
+// the place that a token's K and V factors go to: page and token in it, or the token's own
+__device__ __forceinline__ bool place_of(const NormRopeParams& p, bool cached, int token, int bi, int i, int64_t& page, int64_t& at) {
+  page = bi;
+  at = i;
+  if (!cached) return true;
+  const int slot = p.slots[token];
+  if (slot < 0 || slot >= p.num_slots) return false;
+  page = slot / p.page_size;
+  at = slot - page * p.page_size;
+  return true;
+}
+
+template <typename T, int D, bool AXES, int RM>
+__device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Side& side, bool cached, int group, int tokens, Sum<T>* G) {
+  constexpr int P = 16 / RM, NS = D / 32;
+  const int lane = threadIdx.x & 63, g = lane >> 4, R = side.R, H = p.H;
+  const Rows<RM> me(group, tokens, p.l, R, lane);
+  const T* const b = static_cast<const T*>(side.b.ptr) + me.bi * side.b.stride_b + me.i * side.b.stride_l + me.r * side.b.stride_r + 8 * g;
+  Chunk<T> x[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) x[s] = me.there ? load_chunk(b + 32 * s) : Chunk<T>{};
+  const Turns<D, AXES> turn(p.rot, me.token, me.i, g);
+  int64_t page, at;
+  const bool stored = place_of(p, cached, me.token, me.bi, me.i, page, at) && me.there;
+  if (p.normalize) {
+    gram_to_lds<T, D, RM>(x, G, lane);
+    wave_lds_fence();
+  }
+  // the b rows: weight, rotation
+  T* const bo = static_cast<T*>(const_cast<void*>(side.b_out.ptr)) + page * side.b_out.stride_b + at * side.b_out.stride_l + me.r * side.b_out.stride_r + 8 * g;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    float wt[8], y[8];
+    weights_at(side.weight, p.weight_bf16, 32 * s + 8 * g, wt);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y0 = x[s][2 * e] * wt[2 * e], y1 = x[s][2 * e + 1] * wt[2 * e + 1];
+      y[2 * e] = y0 * turn.c[s][e] - y1 * turn.s[s][e];
+      y[2 * e + 1] = y1 * turn.c[s][e] + y0 * turn.s[s][e];
+    }
+    if (stored) store_chunk(bo + 32 * s, y);
+  }
+  // the head factors
+  auto heads = [&](auto vh_c) __attribute__((always_inline)) {
+    constexpr int VH = decltype(vh_c)::value;
+    for (int at_head = VH * lane; at_head < P * H; at_head += VH * 64) {
+      const int tt = at_head / H, h = at_head - tt * H, token = me.first + tt;
+      if (token >= tokens) continue;
+      const int bi = token / p.l, i = token - bi * p.l;
+      int64_t page, at;
+      if (!place_of(p, cached, token, bi, i, page, at)) continue;
+      const T* const from = static_cast<const T*>(side.a.ptr) + bi * side.a.stride_b + i * side.a.stride_l + h;
+      T* const to = static_cast<T*>(const_cast<void*>(side.a_out.ptr)) + page * side.a_out.stride_b + at * side.a_out.stride_l + h;
+      float a[RM][VH];
+#pragma unroll
+      for (int r = 0; r < RM; ++r) {
+        if (r < R) load_heads<T, VH>(from + r * side.a.stride_r, a[r]);
+        else
+#pragma unroll
+          for (int v = 0; v < VH; ++v) a[r][v] = 0.f;
+      }
+      float scale[VH];
+#pragma unroll
+      for (int v = 0; v < VH; ++v) scale[v] = 1.f;
+      if (p.normalize) {
+        Sum<T> y[RM][VH], square[VH];
+        times_gram<T, RM, VH>(G, tt, a, y, square);
+#pragma unroll
+        for (int v = 0; v < VH; ++v) scale[v] = inverse_norm_of(square[v], R, D, p.eps);
+      }
+#pragma unroll
+      for (int r = 0; r < RM; ++r) {
+        float out[VH];
+#pragma unroll
+        for (int v = 0; v < VH; ++v) out[v] = a[r][v] * scale[v];
+        if (r < R) store_heads<T, VH>(to + r * side.a_out.stride_r, out);
+      }
+    }
+  };
+  if (P * H <= 64) heads(std::integral_constant<int, 1>{});
+  else heads(std::integral_constant<int, 2>{});
+}
+
+template <typename T, int D, bool AXES>
+__global__ __launch_bounds__(kNormWaves * 64) void norm_rope_kernel(NormRopeParams p, int groups_q, int groups_k, int groups_v) {
+  __shared__ Sum<T> gram[kNormWaves][kGramElements];
+  const int w = scalar(threadIdx.x >> 6), tokens = p.B * p.l;
+  int task = blockIdx.x * kNormWaves + w;
+  if (task < groups_q + groups_k) {
+    const bool keys = task >= groups_q;
+    const Side& side = p.side[keys];
+    with_rows(side.R, [&](auto rm) __attribute__((always_inline)) {
+      norm_rope_rows<T, D, AXES, decltype(rm)::value>(p, side, keys && p.slots, keys ? task - groups_q : task, tokens, gram[w]);
+    });
+    return;
+  }
+  task -= groups_q + groups_k;
+  if (task >= groups_v) return;
+  // V factors into their slots, 16 bytes a lane: chunks of a row of ranks, head factors first
+  constexpr int E = 16 / sizeof(T);
+  const int R = p.side[1].R, lane = threadIdx.x & 63, per_rank = (p.H + D) / E, per_token = R * per_rank, P = tokens_per_wave(R);
+  for (int x = lane; x < P * per_token; x += 64) {
+    const int tt = x / per_token, token = task * P + tt, rest = x - tt * per_token, r = rest / per_rank, c = (rest - r * per_rank) * E;
+    if (token >= tokens) break;
+    const int bi = token / p.l, i = token - bi * p.l;
+    int64_t page, at;
+    if (!place_of(p, true, token, bi, i, page, at)) continue;
+    const bool head = c < p.H;
+    const TpaFactor &in = head ? p.va : p.vb, &out = head ? p.va_out : p.vb_out;
+    const int col = head ? c : c - p.H;
+    *reinterpret_cast<u32x4*>(static_cast<T*>(const_cast<void*>(out.ptr)) + page * out.stride_b + at * out.stride_l + r * out.stride_r + col) =
+        *reinterpret_cast<const u32x4*>(static_cast<const T*>(in.ptr) + bi * in.stride_b + i * in.stride_l + r * in.stride_r + col);
+  }
+}
+
+// ---- gradients.  The R x R sums M = A diag(w) A^T over the heads and the mixture M B of the b rows are products of the matrix cores
+// too: M's result layout is that of the second product's operand, whose other one are the b rows read back transposed.  For bf16
+// factors w a and M are kept as two bf16 numbers each.  The rows of a wave's tokens stand in one product, so the rows of the other
+// tokens meet zeros: where a b row is not finite, 0 * inf would spread, and the tokens take turns instead.
+template <typename T, int D>
+struct BwdLds {
+  static constexpr int kStride = sizeof(T) == 2 ? D : D + 4;              // of a b row (elements)
+  static constexpr size_t kRows = 16 * kStride * sizeof(T), kGram = kGramElements * sizeof(Sum<T>);
+  static size_t bytes(int most_pairs) { return kNormWaves * (kRows + kGram + (size_t)(most_pairs + 3) / 4 * 16); }
+};
+
+template <typename T, int D, bool AXES, int RM>
+__device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, const BwdSide& side, int group, int tokens, unsigned char* lds, float (&d_weight)[D / 4]) {
+  constexpr int P = 16 / RM, NS = D / 32;
+  using Lds = BwdLds<T, D>;
+  T* const rows = reinterpret_cast<T*>(lds);
+  Sum<T>* const G = reinterpret_cast<Sum<T>*>(lds + Lds::kRows);
+  float* const W = reinterpret_cast<float*>(lds + Lds::kRows + Lds::kGram);  // [P][H]
+  const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, R = side.R, H = p.H;
+  const Rows<RM> me(group, tokens, p.l, R, lane);
+  const T* const b = static_cast<const T*>(side.b.ptr) + me.bi * side.b.stride_b + me.i * side.b.stride_l + me.r * side.b.stride_r + 8 * g;
+  const T* const db = static_cast<const T*>(side.db_out.ptr) + me.bi * side.db_out.stride_b + me.i * side.db_out.stride_l + me.r * side.db_out.stride_r + 8 * g;
+  Chunk<T> x[NS], dy[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    x[s] = me.there ? load_chunk(b + 32 * s) : Chunk<T>{};
+    dy[s] = me.there ? load_chunk(db + 32 * s) : Chunk<T>{};
+  }
+  const Turns<D, AXES> turn(p.rot, me.token, me.i, g);
+  bool finite = true;
+  if (p.normalize) {
+    finite = gram_to_lds<T, D, RM>(x, G, lane);
+    if (finite)
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int n = 0; n < (int)sizeof(T) / 2; ++n) reinterpret_cast<u32x4*>(rows + row * Lds::kStride + 32 * s + 8 * g)[n] = x[s].x[n];
+    wave_lds_fence();
+  }
+  // head factors: a lane's heads
+  auto heads = [&](auto vh_c) __attribute__((always_inline)) {
+    constexpr int VH = decltype(vh_c)::value;
+    for (int at_head = VH * lane; at_head < P * H; at_head += VH * 64) {
+      const int tt = at_head / H, h = at_head - tt * H, token = me.first + tt;
+      float w[VH];
+      if (token < tokens) {
+        const int bi = token / p.l, i = token - bi * p.l;
+        const T* const from = static_cast<const T*>(side.a.ptr) + bi * side.a.stride_b + i * side.a.stride_l + h;
+        const T* const d_from = static_cast<const T*>(side.da_out.ptr) + bi * side.da_out.stride_b + i * side.da_out.stride_l + h;
+        T* const to = static_cast<T*>(const_cast<void*>(side.da.ptr)) + bi * side.da.stride_b + i * side.da.stride_l + h;
+        float a[RM][VH], da[RM][VH];
+#pragma unroll
+        for (int r = 0; r < RM; ++r) {
+          if (r < R) {
+            load_heads<T, VH>(from + r * side.a.stride_r, a[r]);
+            load_heads<T, VH>(d_from + r * side.da_out.stride_r, da[r]);
+          } else {
+#pragma unroll
+            for (int v = 0; v < VH; ++v) a[r][v] = da[r][v] = 0.f;
+          }
+        }
+        if (p.normalize) {
+          Sum<T> y[RM][VH], square[VH];
+          times_gram<T, RM, VH>(G, tt, a, y, square);
+#pragma unroll
+          for (int v = 0; v < VH; ++v) {
+            const float scale = inverse_norm_of(square[v], R, D, p.eps);
+            float u = 0.f;
+#pragma unroll
+            for (int r = 0; r < RM; ++r) u = fmaf(da[r][v], a[r][v], u);
+            w[v] = -scale * scale * scale * u / (float)(D * R * R);
+#pragma unroll
+            for (int r = 0; r < RM; ++r) da[r][v] = da[r][v] * scale + w[v] * (float)y[r][v];
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RM; ++r)
+          if (r < R) store_heads<T, VH>(to + r * side.da.stride_r, da[r]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < VH; ++v) w[v] = 0.f;
+      }
+      if (p.normalize)
+#pragma unroll
+        for (int v = 0; v < VH; ++v) W[at_head + v] = w[v];
+    }
+  };
+  if (P * H <= 64) heads(std::integral_constant<int, 1>{});
+  else heads(std::integral_constant<int, 2>{});
+  // M[4 g + e][row] of the token's rows
+  f32x4 M = {0.f, 0.f, 0.f, 0.f};
+  if (p.normalize) {
+    wave_lds_fence();
+    const T* const a = static_cast<const T*>(side.a.ptr) + me.bi * side.a.stride_b + me.i * side.a.stride_l + me.r * side.a.stride_r;
+    const float* const w_of = W + min(row / RM, P - 1) * H;
+    if constexpr (sizeof(T) == 2) {
+      for (int h = 8 * g; h - 8 * g < H; h += 32) {
+        const bool there = me.there && h < H;
+        const Chunk<T> ac = there ? load_chunk(a + h) : Chunk<T>{};
+        u32x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float w0 = there ? ac[2 * e] * w_of[h + 2 * e] : 0.f, w1 = there ? ac[2 * e + 1] * w_of[h + 2 * e + 1] : 0.f;
+          hi[e] = pack_bf16(w0, w1);
+          lo[e] = pack_bf16(w0 - bf16lo_to_f32(hi[e]), w1 - bf16hi_to_f32(hi[e]));
+        }
+        const bf16x8 f = __builtin_bit_cast(bf16x8, ac.x[0]);
+        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, lo), M, 0, 0, 0);
+        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, hi), M, 0, 0, 0);
+      }
+    } else {
+      for (int h = 8 * g; h - 8 * g < H; h += 32) {
+        const bool there = me.there && h < H;
+        const Chunk<T> ac = there ? load_chunk(a + h) : Chunk<T>{};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) M = __builtin_amdgcn_mfma_f32_16x16x4f32(ac[e], there ? ac[e] * w_of[h + e] : 0.f, M, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((4 * g + e) / RM != row / RM || row / RM >= P) M[e] = 0.f;
+  }
+  // mixture of the b rows: out[n][e] of this lane's row at d = 32 (n / 2) + 8 g + 4 (n % 2) + e
+  f32x4 mixed[2 * NS];
+#pragma unroll
+  for (int n = 0; n < 2 * NS; ++n) mixed[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto mix = [&](f32x4 (&out)[2 * NS]) __attribute__((always_inline)) {
+    if constexpr (sizeof(T) == 2) {
+      const u32x2 hi = {pack_bf16(M[0], M[1]), pack_bf16(M[2], M[3])};
+      const u32x2 lo = {pack_bf16(M[0] - bf16lo_to_f32(hi[0]), M[1] - bf16hi_to_f32(hi[0])), pack_bf16(M[2] - bf16lo_to_f32(hi[1]), M[3] - bf16hi_to_f32(hi[1]))};
+#pragma unroll
+      for (int n = 0; n < 2 * NS; ++n) {
+        // rows 4 g + 0..3 of the column that this lane stands for: 16 lanes bring 4 rows x 16 columns and get them transposed
+        const T* const from = rows + (4 * g + (row >> 2)) * Lds::kStride + 32 * (n / 2) + 8 * (row & 3) + 4 * (n % 2);
+        const s16x4 f = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)from);
+        out[n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, lo), out[n], 0, 0, 0);
+        out[n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, hi), out[n], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2 * NS; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          out[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows[(4 * g + e) * Lds::kStride + 32 * (n / 2) + 8 * (row >> 2) + 4 * (n % 2) + (row & 3)], M[e], out[n], 0, 0, 0);
+    }
+  };
+  if (p.normalize) {
+    if (finite) {
+      mix(mixed);
+    } else {
+      for (int tt = 0; tt < P; ++tt) {
+        wave_lds_fence();
+        const bool mine = row / RM == tt;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int n = 0; n < (int)sizeof(T) / 2; ++n)
+            reinterpret_cast<u32x4*>(rows + row * Lds::kStride + 32 * s + 8 * g)[n] = mine ? x[s].x[n] : u32x4{0, 0, 0, 0};
+        wave_lds_fence();
+        f32x4 one[2 * NS];
+#pragma unroll
+        for (int n = 0; n < 2 * NS; ++n) one[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        mix(one);
+#pragma unroll
+        for (int n = 0; n < 2 * NS; ++n) mixed[n] = mine ? one[n] : mixed[n];
+      }
+    }
+  }
+  T* const bo = static_cast<T*>(const_cast<void*>(side.db.ptr)) + me.bi * side.db.stride_b + me.i * side.db.stride_l + me.r * side.db.stride_r + 8 * g;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    float wt[8], y[8];
+    weights_at(side.weight, p.weight_bf16, 32 * s + 8 * g, wt);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y0 = dy[s][2 * e], y1 = dy[s][2 * e + 1];
+      const float e0 = y0 * turn.c[s][e] + y1 * turn.s[s][e], e1 = y1 * turn.c[s][e] - y0 * turn.s[s][e];
+      d_weight[8 * s + 2 * e] = fmaf(e0, x[s][2 * e], d_weight[8 * s + 2 * e]);
+      d_weight[8 * s + 2 * e + 1] = fmaf(e1, x[s][2 * e + 1], d_weight[8 * s + 2 * e + 1]);
+      y[2 * e] = fmaf(e0, wt[2 * e], mixed[2 * s + e / 2][2 * e % 4]);
+      y[2 * e + 1] = fmaf(e1, wt[2 * e + 1], mixed[2 * s + e / 2][(2 * e + 1) % 4]);
+    }
+    if (me.there) store_chunk(bo + 32 * s, y);
+  }
+  wave_lds_fence();  // the next tokens' rows go where these are
+}
+
+// Workgroups 0 .. parts_q - 1 share out the queries' tokens, the others the keys'
+template <typename T, int D, bool AXES>
+__global__ __launch_bounds__(kNormWaves * 64) void norm_rope_bwd_kernel(NormRopeBwdParams p, int parts_q, int parts_k, int wave_bytes) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bwd_mem[];
+  const int w = scalar(threadIdx.x >> 6), lane = threadIdx.x & 63, tokens = p.B * p.l;
+  const bool keys = (int)blockIdx.x >= parts_q;
+  const BwdSide& side = p.side[keys];
+  const int part = keys ? blockIdx.x - parts_q : blockIdx.x, parts = keys ? parts_k : parts_q;
+  float d_weight[D / 4];  // of this lane's row: element 8 s + e is d = 32 s + 8 g + e
+#pragma unroll
+  for (int x = 0; x < D / 4; ++x) d_weight[x] = 0.f;
+  with_rows(side.R, [&](auto rm) __attribute__((always_inline)) {
+    constexpr int RM = decltype(rm)::value, P = 16 / RM;
+    for (int group = part * kNormWaves + w; group < (tokens + P - 1) / P; group += parts * kNormWaves)
+      norm_rope_bwd_rows<T, D, AXES, RM>(p, side, group, tokens, bwd_mem + w * wave_bytes, d_weight);
+  });
+  if (!side.d_weight) return;
+  // over the rows of the wave, then over the waves
+#pragma unroll
+  for (int x = 0; x < D / 4; ++x) {
+    float v = d_weight[x];
+    v += __int_as_float(lanes_of<0xB1>(__float_as_int(v)));
+    v += __int_as_float(lanes_of<0x4E>(__float_as_int(v)));
+    v += __int_as_float(lanes_of<0x141>(__float_as_int(v)));
+    v += __int_as_float(lanes_of<0x140>(__float_as_int(v)));
+    d_weight[x] = v;
+  }
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(bwd_mem);
+  if ((lane & 15) == 0)
+#pragma unroll
+    for (int x = 0; x < D / 4; ++x) sums[w * D + 32 * (x / 8) + 8 * (lane >> 4) + x % 8] = d_weight[x];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float v = 0.f;
+    for (int x = 0; x < kNormWaves; ++x) v += sums[x * D + threadIdx.x];
+    p.partial[((int64_t)keys * kPartials + part) * D + threadIdx.x] = v;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- checks
+template <typename Args>
+bool fast_takes(const Args* a, const TpaFactor* const* fs, int n) {
+  if (a->kernel == TPA_KERNEL_GENERIC || (a->D != 64 && a->D != 128) || a->H % 8 || a->rq > 16 || a->rk > 16) return false;
+  if ((int64_t)a->B * a->l > (1 << 30)) return false;
+  for (int i = 0; i < a->n_axes; ++i)
+    if (a->sections[i] % 4) return false;
+  const int chunk = a->dtype == TPA_DTYPE_BF16 ? 8 : 4;
+  for (int i = 0; i < n; ++i) {
+    const TpaFactor& f = *fs[i];
+    if ((reinterpret_cast<uintptr_t>(f.ptr) & 15) || f.stride_b % chunk || f.stride_l % chunk || f.stride_r % chunk) return false;
+  }
+  return !((reinterpret_cast<uintptr_t>(a->rope_cos) | reinterpret_cast<uintptr_t>(a->rope_sin) | reinterpret_cast<uintptr_t>(a->q_weight) | reinterpret_cast<uintptr_t>(a->k_weight)) & 15);
+}
+template <typename T, int D>
+int launch_fast(const NormRopeParams& p, hipStream_t s) {
+  const int64_t tokens = (int64_t)p.B * p.l;
+  auto groups = [&](int R) { return (int)((tokens + tokens_per_wave(R) - 1) / tokens_per_wave(R)); };
+  const int q = groups(p.side[0].R), k = groups(p.side[1].R), v = p.slots ? k : 0;
+  const dim3 grid((unsigned)(((int64_t)q + k + v + kNormWaves - 1) / kNormWaves));
+  const bool axes = p.rot.n_axes > 1 || p.rot.last_of[3] < D / 2;
+  if (axes) hipLaunchKernelGGL((norm_rope_kernel<T, D, true>), grid, dim3(kNormWaves * 64), 0, s, p, q, k, v);
+  else hipLaunchKernelGGL((norm_rope_kernel<T, D, false>), grid, dim3(kNormWaves * 64), 0, s, p, q, k, v);
+  return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
+}
+inline int most_pairs(int rq, int rk, int H) { return (tokens_per_wave(rq) > tokens_per_wave(rk) ? tokens_per_wave(rq) : tokens_per_wave(rk)) * H; }
+template <typename T, int D>
+int launch_fast_bwd(const NormRopeBwdParams& p, int (&parts)[2], hipStream_t s) {
+  const int64_t tokens = (int64_t)p.B * p.l;
+  for (int x = 0; x < 2; ++x) {
+    const int64_t groups = (tokens + tokens_per_wave(p.side[x].R) - 1) / tokens_per_wave(p.side[x].R);
+    parts[x] = p.side[x].da_out.ptr ? (int)std::min<int64_t>((groups + kNormWaves - 1) / kNormWaves, kPartials) : 0;
+  }
+  const size_t lds = BwdLds<T, D>::bytes(most_pairs(p.side[0].R, p.side[1].R, p.H));
+  const bool axes = p.rot.n_axes > 1 || p.rot.last_of[3] < D / 2;
+  const dim3 grid(parts[0] + parts[1]);
+  if (axes) hipLaunchKernelGGL((norm_rope_bwd_kernel<T, D, true>), grid, dim3(kNormWaves * 64), lds, s, p, parts[0], parts[1], (int)(lds / kNormWaves));
+  else hipLaunchKernelGGL((norm_rope_bwd_kernel<T, D, false>), grid, dim3(kNormWaves * 64), lds, s, p, parts[0], parts[1], (int)(lds / kNormWaves));
+  return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
+}
+
 constexpr size_t kMostLds = 160 * 1024;
 int check_sizes(int B, int l, int H, int D, int rq, int rk, int rope_len, int dtype, int weight_dtype, int kernel, int n_axes, const int32_t* sections) {
   if (dtype != TPA_DTYPE_F32 && dtype != TPA_DTYPE_BF16) return TPA_ERR_DTYPE;
@@ -298,6 +875,10 @@ extern "C" int tpa_norm_rope(const TpaNormRopeArgs* a, void* stream) {
   p.B = a->B; p.l = a->l; p.H = a->H; p.D = a->D;
   p.weight_bf16 = a->weight_dtype == TPA_DTYPE_BF16; p.normalize = a->normalize != 0; p.eps = a->eps;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (fast_takes(a, fs, a->slots ? 12 : 8)) {
+    if (a->dtype == TPA_DTYPE_BF16) return a->D == 128 ? launch_fast<uint16_t, 128>(p, s) : launch_fast<uint16_t, 64>(p, s);
+    return a->D == 128 ? launch_fast<float, 128>(p, s) : launch_fast<float, 64>(p, s);
+  }
   if (a->kernel == TPA_KERNEL_MFMA) return TPA_ERR_UNSUPPORTED;
   const size_t lds = any_lds(a->rq > a->rk ? a->rq : a->rk, a->H, a->D, false);
   if (lds > kMostLds) return TPA_ERR_SHAPE;
@@ -333,15 +914,22 @@ extern "C" int tpa_norm_rope_bwd(const TpaNormRopeBwdArgs* a, void* stream) {
   p.weight_bf16 = a->weight_dtype == TPA_DTYPE_BF16; p.normalize = a->normalize != 0; p.eps = a->eps;
   p.partial = static_cast<float*>(a->workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->kernel == TPA_KERNEL_MFMA) return TPA_ERR_UNSUPPORTED;
-  const size_t lds = any_lds(a->rq > a->rk ? a->rq : a->rk, a->H, a->D, true);
-  if (lds > kMostLds) return TPA_ERR_SHAPE;
-  const int64_t tokens = (int64_t)a->B * a->l;
-  const int groups = (int)(tokens < kPartials ? tokens : kPartials);
-  SumParams sum{p.partial, {p.side[0].d_weight, p.side[1].d_weight}, {groups, groups}, a->D, p.weight_bf16};
-  static bool done[2][kMaxDevices] = {};
-  const int rc = a->dtype == TPA_DTYPE_BF16 ? launch_any(norm_rope_bwd_any_kernel<uint16_t>, dim3(groups, 2), lds, done[0], s, p)
-                                            : launch_any(norm_rope_bwd_any_kernel<float>, dim3(groups, 2), lds, done[1], s, p);
+  SumParams sum{p.partial, {p.side[0].d_weight, p.side[1].d_weight}, {0, 0}, a->D, p.weight_bf16};
+  int rc;
+  if (fast_takes(a, &fs[0][0], 12) && (a->dtype == TPA_DTYPE_BF16 ? BwdLds<uint16_t, 128>::bytes(most_pairs(a->rq, a->rk, a->H))
+                                                                  : BwdLds<float, 128>::bytes(most_pairs(a->rq, a->rk, a->H))) <= 64 * 1024) {
+    if (a->dtype == TPA_DTYPE_BF16) rc = a->D == 128 ? launch_fast_bwd<uint16_t, 128>(p, sum.count, s) : launch_fast_bwd<uint16_t, 64>(p, sum.count, s);
+    else rc = a->D == 128 ? launch_fast_bwd<float, 128>(p, sum.count, s) : launch_fast_bwd<float, 64>(p, sum.count, s);
+  } else {
+    if (a->kernel == TPA_KERNEL_MFMA) return TPA_ERR_UNSUPPORTED;
+    const size_t lds = any_lds(a->rq > a->rk ? a->rq : a->rk, a->H, a->D, true);
+    if (lds > kMostLds) return TPA_ERR_SHAPE;
+    const int64_t tokens = (int64_t)a->B * a->l;
+    const int groups = sum.count[0] = sum.count[1] = (int)(tokens < kPartials ? tokens : kPartials);
+    static bool done[2][kMaxDevices] = {};
+    rc = a->dtype == TPA_DTYPE_BF16 ? launch_any(norm_rope_bwd_any_kernel<uint16_t>, dim3(groups, 2), lds, done[0], s, p)
+                                    : launch_any(norm_rope_bwd_any_kernel<float>, dim3(groups, 2), lds, done[1], s, p);
+  }
   if (rc != TPA_OK || !sums) return rc;
   hipLaunchKernelGGL(sum_partials_kernel, dim3((a->D + 31) / 32, 2), dim3(1024), 0, s, sum);
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
