@@ -122,12 +122,12 @@ __global__ __launch_bounds__(kAnyThreads) void shared_any_kernel(SharedParams p)
 // head) the logits are s[c, t] = sum_r ka[t, r, h] (Qm[c, :] . kb[t, r, :]), the output (1 / R) sum_t sum_r (p[c, t] va[t, r, h]) vb[t, r, :], two
 // products of the rows (t, r) with the columns.  The rows serve every column, so a workgroup takes a tile of 4 blocks of 32 rows
 // once for up to 256 columns: the columns of the prefix are those of all sequences, 32 to a wave; where there are fewer (a sequence's
-// own keys, few sequences) groups of waves share the tile's blocks and are joined at the end.  Tiles go from memory straight to LDS,
-// two buffers, one barrier a tile.
+// own keys, few sequences) waves share the tile's blocks and are joined at the end.  Tiles go from memory straight to LDS, two
+// buffers.
 // Qm is kept as two bf16 numbers, 2^-17 of it off: with one the logits carry the rounding of Qm, 2^-9 each, and the output's error
 // grows by half; the second costs 8 of 24 matrix instructions a block.  The weights p va are rounded to bf16 once, sums are fp32.
 constexpr int kRows = 32;           // rows (token, rank) of a block
-constexpr int kBlocks = 4;          // blocks of a tile
+constexpr int kBlocks = 4;          // blocks of a tile, each of them brought by two waves
 constexpr int kWaves = 8;
 constexpr int kRsrcFlags = 0x00020000;  // raw 32-bit data format
 constexpr int64_t kFarthestRow = 1 << 25;  // elements between neighbouring rows, at most: 31 of them in 32-bit byte offsets
@@ -136,17 +136,22 @@ template <int D>
 struct SharedLds {
   static constexpr int kB = kRows * D * 2, kA = kRows * 32 * 2;              // bytes of a block's b rows, a rows (32 heads)
   static constexpr int kBuffer = kBlocks * 2 * (kB + kA);                     // kb, vb, ka, va of a tile
-  static constexpr int kPart = 32 * D * 4 + 2 * 64 * 4;                       // a wave's sums on their way to another
-  static constexpr size_t kBytes = 2 * kBuffer > 4 * kPart ? 2 * kBuffer : 4 * kPart;
+  static constexpr int kPart = 32 * D * 4 + 2 * 64 * 4;                       // a wave's sums of a set of columns on their way to another
+  static constexpr size_t kBytes = 2 * kBuffer;
+  static_assert(4 * kPart <= 2 * kBuffer, "the sums that four waves hand over at a time fit the buffers");
 };
 
+// Columns come in sets of 32: the heads of a block of heads (8, 16, 24 or 32) for as many query rows as fit, so that all sets have the same head
+// factors.
+struct SharedPart {        // the prefix, or the sequences' own keys
+  int waves;               // waves side by side over the columns
+  int groups;              // workgroups for all columns of a block of heads
+  int ranges, tiles;       // key ranges, tiles of a range
+  int grid;                // workgroups
+};
 struct SharedPlan {
   int hb, nhb;             // heads of a block of heads, blocks of heads
-  int waves_p, waves_s;    // waves side by side over the columns, of the prefix and of a sequence's own keys
-  int groups_p, groups_s;  // groups of as many columns
-  int ranges_p, ranges_s;  // key ranges
-  int tiles_p, tiles_s;    // tiles of a range
-  int grid_p, grid_s;      // workgroups
+  SharedPart prefix, own;
   int64_t rows;            // B lq
 };
 struct SharedMfmaParams {
@@ -157,19 +162,21 @@ struct SharedMfmaParams {
   int page_shift;  // log2 of the rows of a page, or -1
 };
 
-// Where a lane's pieces of a block of rows of D lie in LDS (elements): 16-byte chunk c of row r at chunk c ^ (r mod chunks)
+// Where a lane's pieces of a block of rows of D lie in LDS (elements): 16-byte chunk c of row r at chunk c ^ f(r), so that neither the reads of
+// one chunk of 16 rows nor the transposed ones of 4 chunks of 4 rows meet a bank twice
 template <int D>
 struct BlockAt {
   static constexpr int CPR = D / 8;
+  __device__ __forceinline__ static int f(int r) { return CPR == 16 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3); }
   int row, tr;
   __device__ __forceinline__ explicit BlockAt(int l) {
     const int i = l & 31, g = l >> 5, lp = l & 15, dhalf = (l >> 4) & 1, r = 4 * g + (lp >> 2);
-    row = i * D + 8 * (g ^ (i & (CPR - 1)));
-    tr = r * D + 8 * ((2 * dhalf + ((lp & 3) >> 1)) ^ r) + 4 * (lp & 1);
+    row = i * D + 8 * (g ^ f(i));
+    tr = r * D + 8 * ((2 * dhalf + ((lp & 3) >> 1)) ^ f(r)) + 4 * (lp & 1);
   }
   __device__ __forceinline__ int read(int ks) const { return row ^ (16 * ks); }  // row i, chunk 2 ks + g
   // transposed: rows 16 kk + 8 hi + 4 g + 0..3, columns 32 db + 0..31
-  __device__ __forceinline__ int read_tr(int kk, int hi, int db) const { return (tr ^ (32 * db) ^ (hi && CPR == 16 ? 64 : 0)) + (16 * kk + 8 * hi) * D; }
+  __device__ __forceinline__ int read_tr(int kk, int hi, int db) const { return (tr ^ (32 * db) ^ (16 * hi)) + (16 * kk + 8 * hi) * D; }
 };
 typedef s16x4 __attribute__((address_space(3))) lds_s16x4;
 template <int D>
@@ -180,54 +187,66 @@ __device__ __forceinline__ bf16x8 block_tr(const uint16_t* block, const BlockAt<
 }
 
 template <int D, int RK, bool PAGED>
-__global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaParams p) {
+__device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const SharedPart& part, bool own, int id, unsigned char* mem) {
   using Lds = SharedLds<D>;
-  constexpr int NKS = D / 16, NDB = D / 32, CPR = D / 8, RPI = 64 / CPR, NI = 16 / RPI;  // NI: load instructions of a wave for its 16 b rows
-  constexpr int TPB = kRows / RK;                                                          // tokens of a block
+  constexpr int NKS = D / 16, NDB = D / 32, CPR = D / 8, RPI = 64 / CPR, NI = 16 / RPI;  // NI: load instructions of a wave's 16 b rows
+  constexpr int TPB = kRows / RK;                                                           // tokens of a block
   constexpr int NTOK = RK <= 4 ? 16 / RK : 32 / RK;  // tokens whose rows this lane holds, per block
   constexpr int NV = RK <= 4 ? RK : RK / 2;          // rows of one token held by this half of the wave
-  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_mem[];
   const SharedParams& c = p.c;
   const SharedPlan& plan = p.plan;
   const int tid = threadIdx.x, w = scalar(tid >> 6), l = tid & 63, i = l & 31, g = l >> 5, lp = l & 15, dhalf = (l >> 4) & 1;
 
   // ---- which keys and columns: workgroups that read the same keys sit on one XCD (ids are dealt to the eight in turn)
-  const bool own = (int)blockIdx.x >= plan.grid_p;
-  const int id = (int)blockIdx.x - (own ? plan.grid_p : 0);
-  const int cwaves = own ? plan.waves_s : plan.waves_p, sharing = plan.nhb * (own ? plan.groups_s : plan.groups_p);
+  const int sharing = plan.nhb * part.groups;
   const int unit = id / (8 * sharing) * 8 + (id & 7), member = id / 8 % sharing;
-  if (unit >= (own ? c.B * plan.ranges_s : plan.ranges_p)) return;
-  const int b_own = own ? unit / plan.ranges_s : 0, range = own ? unit - b_own * plan.ranges_s : unit;
-  const int h0 = member % plan.nhb * plan.hb;
-  const int kwaves = min(kWaves / cwaves, kBlocks), cw = w % cwaves, kw = w / cwaves;
-  const int col0 = (member / plan.nhb * cwaves + cw) * 32;  // this wave's first column
-  const int64_t row_base = own ? (int64_t)b_own * c.lq : 0;
-  const int n_cols = (int)(own ? c.lq : plan.rows) * plan.hb;
-  const int col = min(col0 + i, n_cols - 1);
-  const int64_t row = row_base + col / plan.hb;  // this lane's query row among all, and its head
-  const int head = h0 + col % plan.hb;
-  const int b = (int)(row / c.lq), row_in_b = (int)(row - (int64_t)b * c.lq);
-  const bool works = kw < kwaves && col0 < n_cols;
+  if (unit >= (own ? c.B * part.ranges : part.ranges)) return;
+  const int b_own = own ? unit / part.ranges : 0, range = own ? unit - b_own * part.ranges : unit;
+  const int h0 = member % plan.nhb * plan.hb, rps = 32 / plan.hb;  // rows of a set
+  const int cwaves = part.waves, kwaves = min(kWaves / cwaves, kBlocks), cw = w % cwaves, kw = w / cwaves;
+  const int n_rows = own ? c.lq : (int)plan.rows, wave_row = (member / plan.nhb * cwaves + cw) * rps;  // this wave's first row
+  const bool works = kw < kwaves && wave_row < n_rows;
+  const int in_set = min(i / plan.hb, rps - 1), head = h0 + i % plan.hb;  // lanes behind the last whole row of a set repeat it
+  const bool stored = wave_row + in_set < n_rows && i < rps * plan.hb;
+  const int row = (own ? b_own * c.lq : 0) + min(wave_row + in_set, n_rows - 1);  // this lane's query row among all
+  const int b = c.lq == 1 ? row : row / c.lq, row_in_b = row - b * c.lq;
 
-  // ---- the range's rows (token, rank): first .. end - 1 of those, in blocks from a block's border on
-  const int tiles = own ? plan.tiles_s : plan.tiles_p;
-  const int origin = own ? c.prefix / TPB * TPB : 0;
-  const int seen = keys_seen(c, b, row_in_b);
-  const int mine = own ? seen : min(seen, c.prefix);  // keys of this part that this lane's column sees: those below
+  // ---- Qm^T[d, c] = sum_r qb[r, d] qa[r, c] by the matrix cores, 16 ranks a time, a set's rows one after the other with the other rows' columns
+  // zero: asked for here, finished while the first tile is on its way
+  uint16_t qa_in[8], qb_in[NDB][8];
+  auto request_q = [&](int in_row, int r0) __attribute__((always_inline)) {
+    const int of = (own ? b_own * c.lq : 0) + min(wave_row + in_row, n_rows - 1), ob = c.lq == 1 ? of : of / c.lq;
+    const uint16_t* const qa = static_cast<const uint16_t*>(c.qa.ptr) + ob * c.qa.stride_b + (of - ob * c.lq) * c.qa.stride_l + head;
+    const uint16_t* const qb = static_cast<const uint16_t*>(c.qb.ptr) + ob * c.qb.stride_b + (of - ob * c.lq) * c.qb.stride_l + i;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = min(r0 + 8 * g + j, c.rq - 1);
+      qa_in[j] = qa[r * c.qa.stride_r];
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) qb_in[db][j] = qb[r * c.qb.stride_r + 32 * db];
+    }
+  };
+  request_q(0, 0);
+
+  // ---- keys of this part that a column sees: those below `mine`
+  const int seen = keys_seen(c, b, row_in_b), mine = own ? seen : min(seen, c.prefix);
   const int most = scalar(wave_max(mine)), least = scalar(wave_min(mine));
-  int* const red = reinterpret_cast<int*>(shared_mem);
+  int* const red = reinterpret_cast<int*>(mem);
   if (l == 0) red[w] = most;
-  __syncthreads();
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   int end = 0;
 #pragma unroll
   for (int x = 0; x < kWaves; ++x) end = max(end, red[x]);
-  __syncthreads();
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   end = scalar(end);
-  const int begin = origin + range * tiles * kBlocks * TPB;
-  const int stop = min(end, begin + tiles * kBlocks * TPB);
-  const int64_t slot = ((own ? plan.ranges_p : 0) + range) * plan.rows;
+
+  // ---- the range's rows (token, rank), in blocks from a block's border on
+  const int origin = own ? c.prefix / TPB * TPB : 0;
+  const int begin = origin + range * part.tiles * kBlocks * TPB;
+  const int stop = min(end, begin + part.tiles * kBlocks * TPB);
+  const int64_t slot = ((own ? plan.prefix.ranges : 0) + range) * plan.rows;
   if (stop <= begin || stop <= (own ? c.prefix : 0)) {  // no key of this range is seen
-    if (works && kw == 0 && g == 0 && col0 + i < n_cols) p.part_m[(slot + row) * c.H + head] = -INFINITY;
+    if (works && kw == 0 && g == 0 && stored) p.part_m[(slot + row) * c.H + head] = -INFINITY;
     return;
   }
   const int n_tiles = (stop - begin + kBlocks * TPB - 1) / (kBlocks * TPB);
@@ -240,10 +259,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
                                    static_cast<const uint16_t*>(c.ka.ptr) + boff * c.ka.stride_b + h0, static_cast<const uint16_t*>(c.va.ptr) + boff * c.va.stride_b + h0};
   const int64_t page_stride[4] = {c.kb.stride_b, c.vb.stride_b, c.ka.stride_b, c.va.stride_b};
   const int sr[4] = {2 * (int)c.kb.stride_r, 2 * (int)c.vb.stride_r, 2 * (int)c.ka.stride_r, 2 * (int)c.va.stride_r};
-  const int a_chunk = min(l & 3, plan.hb / 8 - 1);
-  const int chunk = 16 * ((l % CPR) ^ (l / CPR));
-  const int b_row = 16 * (w & 1) + l / CPR, a_row = 16 * (w & 1) + (l >> 2);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)shared_mem;
+  const int a_chunk = 16 * min(l & 3, plan.hb / 8 - 1), b_chunk = 16 * ((l % CPR) ^ BlockAt<D>::f(l / CPR));  // and of row n RPI + l / CPR: f differs by f(n RPI)
+  const int a_row = 16 * (w & 1) + (l >> 2), b_row = 16 * (w & 1) + l / CPR;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)mem;
   const int rpp = PAGED ? c.page_size * RK : 1;
   auto block_row = [&](int tile) __attribute__((always_inline)) { return begin * RK + (tile * kBlocks + (w >> 1)) * kRows; };
   auto page_of = [&](int row0) __attribute__((always_inline)) { return p.page_shift >= 0 ? row0 >> p.page_shift : row0 / rpp; };
@@ -269,76 +287,85 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
       if (x < 2) {
 #pragma unroll
         for (int n = 0; n < NI; ++n)
-          load((uint32_t)scalar(to + x * kBlocks * Lds::kB + (w >> 1) * Lds::kB + (16 * (w & 1) + n * RPI) * 2 * D),
-               (b_row + n * RPI - skip) * sr[x] + (chunk ^ (CPR == 16 ? 64 * n : 0)), rs);
+          load((uint32_t)scalar(to + (x * kBlocks + (w >> 1)) * Lds::kB + (NI * (w & 1) + n) * 1024), (b_row + n * RPI - skip) * sr[x] + (b_chunk ^ (16 * BlockAt<D>::f(n * RPI))), rs);
       } else {
-        load((uint32_t)scalar(to + 2 * kBlocks * Lds::kB + (x - 2) * kBlocks * Lds::kA + (w >> 1) * Lds::kA + 16 * (w & 1) * 64), (a_row - skip) * sr[x] + 16 * a_chunk, rs);
+        load((uint32_t)scalar(to + 2 * kBlocks * Lds::kB + ((x - 2) * kBlocks + (w >> 1)) * Lds::kA + (w & 1) * 1024), (a_row - skip) * sr[x] + a_chunk, rs);
       }
     }
   };
   issue(0, 0, scalar(lookup(0)));
   int page_ahead = lookup(1);
 
-  // ---- Qm of this lane's column, d = 16 ks + 8 g + 0..7, in two parts
+  // ---- Qm of this lane's column as the operand of its products, d = 16 ks + 8 g + 0..7, in two parts
   bf16x8 q_hi[NKS], q_lo[NKS];
-  {
-    const uint16_t* const qa = static_cast<const uint16_t*>(c.qa.ptr) + b * c.qa.stride_b + row_in_b * c.qa.stride_l + head;
-    const uint16_t* const qb = static_cast<const uint16_t*>(c.qb.ptr) + b * c.qb.stride_b + row_in_b * c.qb.stride_l + 8 * g;
-    float q[NKS][8];
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[ks][e] = 0.f;
-    for (int r = 0; r < c.rq; ++r) {
-      const float a = bf16bits_to_f32(qa[r * c.qa.stride_r]) * p.qscale;
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(qb + r * c.qb.stride_r + 16 * ks);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          q[ks][2 * e] = fmaf(a, bf16lo_to_f32(x[e]), q[ks][2 * e]);
-          q[ks][2 * e + 1] = fmaf(a, bf16hi_to_f32(x[e]), q[ks][2 * e + 1]);
-        }
-      }
-    }
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      u32x4 hi, lo;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        hi[e] = pack_bf16(q[ks][2 * e], q[ks][2 * e + 1]);
-        lo[e] = pack_bf16(q[ks][2 * e] - bf16lo_to_f32(hi[e]), q[ks][2 * e + 1] - bf16hi_to_f32(hi[e]));
-      }
-      q_hi[ks] = __builtin_bit_cast(bf16x8, hi);
-      q_lo[ks] = __builtin_bit_cast(bf16x8, lo);
-    }
-  }
-
   f32x16 o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+  for (int in_row = 0; in_row < rps; ++in_row)
+    for (int r0 = 0; r0 < c.rq; r0 += 16) {
+      if (in_row || r0) request_q(in_row, r0);
+      u32x4 a, x[NDB];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + 8 * g + 2 * j;
+        const uint32_t lo = r < c.rq ? 0xffffu : 0u, hi = r + 1 < c.rq ? 0xffff0000u : 0u;
+        a[j] = in_set == in_row ? (((uint32_t)qa_in[2 * j + 1] << 16 | qa_in[2 * j]) & (lo | hi)) : 0u;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) x[db][j] = ((uint32_t)qb_in[db][2 * j + 1] << 16 | qb_in[db][2 * j]) & (lo | hi);
+      }
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        f32x16 one;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) one[v] = 0.f;
+        one = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x[db]), __builtin_bit_cast(bf16x8, a), one, 0, 0, 0);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] += in_set == in_row ? one[v] : 0.f;  // another row's infinities stay with it
+      }
+    }
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float q0 = o[ks / 2][8 * (ks & 1) + 2 * j] * p.qscale, q1 = o[ks / 2][8 * (ks & 1) + 2 * j + 1] * p.qscale;
+      hi[j] = pack_bf16(q0, q1);
+      lo[j] = pack_bf16(q0 - bf16lo_to_f32(hi[j]), q1 - bf16hi_to_f32(hi[j]));
+    }
+    // a result column has d = 8 q + 4 g + e of its block: the halves exchange for the operand's order
+    auto order = [&](const uint32_t (&x)[4]) __attribute__((always_inline)) {
+      const auto even = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), odd = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+      return __builtin_bit_cast(bf16x8, u32x4{even[0], odd[0], even[1], odd[1]});
+    };
+    q_hi[ks] = order(hi);
+    q_lo[ks] = order(lo);
+  }
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   float m = -INFINITY, lsum = 0.f;
   const BlockAt<D> at(l);
-  const int a_head = ((col0 + 16 * dhalf + 4 * (lp & 3)) % plan.hb);  // of the four columns whose a's this lane helps to transpose
-  const int row_last = mine * RK - 1, row_first = own ? c.prefix * RK : 0;
+  const int a_head = (16 * dhalf + 4 * (lp & 3)) % plan.hb;  // of the four columns whose a's this lane helps to transpose
+  const int row_first = own ? c.prefix * RK : 0;
 
-  auto compute = [&](int tile, int buffer, int blk) __attribute__((always_inline)) {
-    const int row0 = begin * RK + (tile * kBlocks + blk) * kRows;
-    if (row0 >= row_end) return;
-    const unsigned char* const buf = shared_mem + buffer * Lds::kBuffer;
-    const uint16_t* const kb = reinterpret_cast<const uint16_t*>(buf + blk * Lds::kB);
-    const uint16_t* const vb = reinterpret_cast<const uint16_t*>(buf + (kBlocks + blk) * Lds::kB);
+  struct Block { const uint16_t *kb, *vb, *ka, *va; int row0; };
+  auto block_of = [&](int tile, int blk) __attribute__((always_inline)) {
+    const unsigned char* const buf = mem + (tile & 1) * Lds::kBuffer;
     const uint16_t* const ka = reinterpret_cast<const uint16_t*>(buf + 2 * kBlocks * Lds::kB + blk * Lds::kA);
-    const uint16_t* const va = ka + kBlocks * Lds::kA / 2;
+    return Block{reinterpret_cast<const uint16_t*>(buf + blk * Lds::kB), reinterpret_cast<const uint16_t*>(buf + (kBlocks + blk) * Lds::kB), ka, ka + kBlocks * Lds::kA / 2,
+                 begin * RK + (tile * kBlocks + blk) * kRows};
+  };
+  auto step = [&](const Block& x) __attribute__((always_inline)) {
     // S'^T[row, c] = kb[row, :] . Qm[c, :]
     f32x16 sp;
 #pragma unroll
     for (int v = 0; v < 16; ++v) sp[v] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) {
-      const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kb + at.read(ks));
+      const bf16x8 kf = *reinterpret_cast<const bf16x8*>(x.kb + at.read(ks));
       sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q_lo[ks], sp, 0, 0, 0);
       sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q_hi[ks], sp, 0, 0, 0);
     }
@@ -346,8 +373,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int a_at = (8 * q + 4 * g + (lp >> 2)) * 32 + a_head;
-      const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(ka + a_at));
-      const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + a_at));
+      const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x.ka + a_at));
+      const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x.va + a_at));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
@@ -364,11 +391,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
       if constexpr (RK >= 8) acc = halves_sum(acc);
       st[t] = acc;
     }
-    if (row0 + kRows > least * RK || row0 < row_first) {
+    if (x.row0 + kRows > least * RK || x.row0 < row_first) {
 #pragma unroll
       for (int t = 0; t < NTOK; ++t) {
-        const int at_row = RK >= 8 ? row0 + RK * t : row0 + 8 * (t * NV >> 2) + 4 * g + (t * NV & 3);  // the token's first row
-        if (at_row > row_last || at_row < row_first) st[t] = -INFINITY;
+        const int at_row = RK >= 8 ? x.row0 + RK * t : x.row0 + 8 * (t * NV >> 2) + 4 * g + (t * NV & 3);  // the token's first row
+        if (at_row >= mine * RK || at_row < row_first) st[t] = -INFINITY;
       }
     }
     float tmax = st[0];
@@ -404,7 +431,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
       for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(pp[8 * kk + 2 * j], pp[8 * kk + 2 * j + 1]);
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(block_tr<D>(vb, at, kk, db), __builtin_bit_cast(bf16x8, pk), o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(block_tr<D>(x.vb, at, kk, db), __builtin_bit_cast(bf16x8, pk), o[db], 0, 0, 0);
     }
   };
 
@@ -416,13 +443,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
       page_ahead = lookup(t + 2);
     }
     if (works)
-      for (int blk = kw; blk < kBlocks; blk += kwaves) compute(t, t & 1, blk);
+      for (int blk = kw; blk < kBlocks; blk += kwaves) {
+        const Block x = block_of(t, blk);
+        if (x.row0 < row_end) step(x);
+      }
   }
 
-  // ---- the groups of waves that shared the blocks are joined, half of them handing their sums to the other half at a time
+  // ---- the waves that shared the blocks are joined, half of them handing their sums to the other half at a time
   lsum = halves_sum(lsum);
   for (int half = kwaves / 2; half; half /= 2) {
-    float* const part = reinterpret_cast<float*>(shared_mem + (cw + cwaves * (kw % half)) * Lds::kPart);
+    float* const part = reinterpret_cast<float*>(mem + (cw + cwaves * (kw % half)) * Lds::kPart);
     __syncthreads();  // the tiles, or what was handed over before, have been read
     if (works && kw >= half && kw < 2 * half) {
 #pragma unroll
@@ -445,7 +475,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
       }
     }
   }
-  if (!works || kw || col0 + i >= n_cols) return;
+  if (!works || kw || !stored) return;
   const int64_t to = (slot + row) * c.H + head;
 #pragma unroll
   for (int x = 0; x < NDB * 4; ++x)
@@ -456,35 +486,65 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
   }
 }
 
-// Joins the ranges' parts of a row and head: a thread per four columns of the output
+template <int D, int RK, bool PAGED>
+__global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaParams p) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_mem[];
+  const bool own = (int)blockIdx.x >= p.plan.prefix.grid;
+  const SharedPart& part = own ? p.plan.own : p.plan.prefix;
+  const int id = (int)blockIdx.x - (own ? p.plan.prefix.grid : 0);
+  shared_part<D, RK, PAGED>(p, part, own, id, shared_mem);
+}
+
+// Joins the ranges' parts: a wave per query row and head.  Its lanes take a range each for the weights; then groups of D / 4 lanes, 16
+// bytes a lane, walk the ranges side by side with several loads on their way, and are added up.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMfmaParams p) {
-  constexpr int TPR = D / 4;
+  constexpr int TPR = D / 4, GROUPS = 64 / TPR, AHEAD = 4;
   const SharedParams& c = p.c;
-  const int64_t n = p.plan.rows * c.H, at = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int lane = threadIdx.x & 63, grp = lane / TPR, d = 4 * (lane % TPR), ranges = p.plan.prefix.ranges + p.plan.own.ranges;
+  const int64_t n = p.plan.rows * c.H, at = (int64_t)blockIdx.x * 4 + scalar(threadIdx.x >> 6);
   if (at >= n) return;
-  const int d = 4 * (threadIdx.x % TPR), ranges = p.plan.ranges_p + p.plan.ranges_s;
-  float most = -INFINITY;
-  for (int x = 0; x < ranges; ++x) most = fmaxf(most, p.part_m[x * n + at]);
-  float total = 0.f;
+  float most = -INFINITY, total = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int x = 0; x < ranges; ++x) {
-    const float m = p.part_m[x * n + at];
-    if (m == -INFINITY) continue;  // nothing else was written
-    const float f = __builtin_amdgcn_exp2f(m - most);
-    total += f * p.part_l[x * n + at];
-    sum += f * *reinterpret_cast<const f32x4*>(p.part_o + (x * n + at) * D + d);
+  for (int x0 = 0; x0 < ranges; x0 += 64) {
+    const bool there = x0 + lane < ranges;
+    const float m = there ? p.part_m[(x0 + lane) * n + at] : -INFINITY, l = there ? p.part_l[(x0 + lane) * n + at] : 0.f;
+    float m_new = m;
+#pragma unroll
+    for (int s = 32; s; s >>= 1) m_new = fmaxf(m_new, __shfl_xor(m_new, s));
+    m_new = fmaxf(m_new, most);
+    const float base = m_new == -INFINITY ? 0.f : m_new, keep = __builtin_amdgcn_exp2f(most - base);
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    total = total * keep + (m == -INFINITY ? 0.f : f * l);  // a range without keys has written nothing but its maximum
+    sum *= keep;
+    most = m_new;
+    const int count = min(64, ranges - x0);
+    for (int x = 0; x < count; x += GROUPS * AHEAD) {
+      f32x4 part[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) part[u] = *reinterpret_cast<const f32x4*>(p.part_o + ((x0 + min(x + u * GROUPS + grp, count - 1)) * n + at) * D + d);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int mine = x + u * GROUPS + grp;
+        const float g = __shfl(f, min(mine, 63)), gm = __shfl(m, min(mine, 63));
+        if (mine < count && gm != -INFINITY) sum += g * part[u];
+      }
+    }
   }
+#pragma unroll
+  for (int s = 32; s; s >>= 1) total += __shfl_xor(total, s);
+#pragma unroll
+  for (int s = 32; s >= TPR; s >>= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], s);
   const bool empty = most == -INFINITY;
   const float inv = empty ? NAN : 1.f / (total * c.rk);
   T* const out = static_cast<T*>(c.o) + at * D + d;
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv)};
-  } else {
-    *reinterpret_cast<f32x4*>(out) = f32x4{sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
+  if (grp == 0) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv)};
+    else *reinterpret_cast<f32x4*>(out) = f32x4{sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
   }
-  if (d == 0 && c.lse) {
+  if (lane == 0 && c.lse) {
     const int64_t row = at / c.H;
     const int h = (int)(at - row * c.H), b = (int)(row / c.lq);
     c.lse[((int64_t)b * c.H + h) * c.lq + (row - (int64_t)b * c.lq)] = empty ? -INFINITY : (most + __log2f(total)) * kLn2;
@@ -510,46 +570,62 @@ bool mfma_takes(const TpaFwdArgs* a) {
   return (int64_t)a->lk * a->rk < (1 << 30);
 }
 
+// What the plan reckons with, ns: a block of a wave, at head size 128 and 64 (5.8 and 3.5 us for a tile of four by eight waves); a tile of a
+// sequence's own keys at head size 128, which memory brings; a workgroup's way to its first tile and behind its last one; a number of a
+// range's results, written and read again.
+constexpr double kBlockNs128 = 1450, kBlockNs64 = 875, kOwnTileNs = 3000, kFixedNs = 12000, kPartNs = 8. / 5e3;
 SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   SharedPlan s{};
   s.hb = a->H % 32 == 0 ? 32 : a->H % 24 == 0 ? 24 : a->H % 16 == 0 ? 16 : 8;
   s.nhb = a->H / s.hb;
   s.rows = (int64_t)a->B * a->lq;
-  auto waves = [&](int64_t cols) { int n = 1; while (n < kWaves && 32 * n < cols) n *= 2; return n; };
-  s.waves_p = waves(s.rows * s.hb);
-  s.waves_s = waves((int64_t)a->lq * s.hb);
-  s.groups_p = ceil_div(s.rows * s.hb, 32 * s.waves_p);
-  s.groups_s = ceil_div((int64_t)a->lq * s.hb, 32 * s.waves_s);
-  const int tpb = kRows / a->rk, tpt = tpb * kBlocks;
+  const int tpb = kRows / a->rk, tpt = tpb * kBlocks, rps = 32 / s.hb;
+  auto columns = [&](SharedPart& x, int64_t rows) {
+    const int sets = ceil_div(rows, rps);
+    x.waves = 1;
+    while (x.waves < kWaves && x.waves < sets) x.waves *= 2;
+    x.groups = ceil_div(sets, x.waves);
+  };
+  columns(s.prefix, s.rows);
+  columns(s.own, a->lq);
   const int all_p = ceil_div(prefix, tpt), all_s = ceil_div(a->lk - prefix / tpb * tpb, tpt);
-  const int share_p = s.nhb * s.groups_p, share_s = s.nhb * s.groups_s;
-  // as many tiles to a workgroup as give every compute unit one
-  const int64_t work = (int64_t)all_p * share_p + (prefix < a->lk ? (int64_t)all_s * share_s * a->B : 0);
-  const int each = std::max(1, ceil_div(work, 256));
-  if (prefix) {
-    s.ranges_p = std::max(1, ceil_div(all_p, each));
-    s.tiles_p = ceil_div(all_p, s.ranges_p);
-    s.ranges_p = ceil_div(all_p, s.tiles_p);
+  const int share_p = s.nhb * s.prefix.groups, share_s = s.nhb * s.own.groups;
+  // One workgroup is resident on a compute unit, so the launch lasts as long as the longest of 256, or longer by what more of them do.  Every
+  // length of time up to that of one workgroup for all is tried for what the ranges would be; the shortest launch wins.
+  const bool has_p = prefix > 0, has_s = prefix < a->lk;
+  auto tile_ns = [&](const SharedPart& x) { return (a->dk == 128 ? kBlockNs128 : kBlockNs64) * kBlocks / std::min(kWaves / x.waves, kBlocks); };
+  const double tile_p = tile_ns(s.prefix), tile_s = std::max(tile_ns(s.own), kOwnTileNs * a->dk / 128);
+  double best = 0;
+  for (double time = std::min(tile_p, tile_s); ; time *= 1.07) {
+    const int tiles_p = has_p ? std::min(all_p, std::max(1, (int)(time / tile_p))) : 0, tiles_s = has_s ? std::min(all_s, std::max(1, (int)(time / tile_s))) : 0;
+    const int ranges_p = has_p ? ceil_div(all_p, tiles_p) : 0, ranges_s = has_s ? ceil_div(all_s, tiles_s) : 0;
+    // an XCD takes whole ranges: what counts is the one that has most of them, as if all had
+    const double groups_p = (double)ceil_div(ranges_p, 8) * 8 * share_p, groups_s = (double)ceil_div((int64_t)ranges_s * a->B, 8) * 8 * share_s;
+    const double each_p = kFixedNs + tiles_p * tile_p, each_s = kFixedNs + tiles_s * tile_s;
+    double cost = std::max(has_p ? each_p : 0., has_s ? each_s : 0.);
+    if (groups_p + groups_s > 256) cost += (groups_p * each_p + groups_s * each_s) / 256;  // the last ones start where others end
+    cost += kPartNs * (ranges_p + ranges_s) * (double)s.rows * a->H * a->dv;
+    if (best == 0 || cost < best) {
+      best = cost;
+      s.prefix.tiles = tiles_p; s.own.tiles = tiles_s; s.prefix.ranges = ranges_p; s.own.ranges = ranges_s;
+    }
+    if (tiles_p == (has_p ? all_p : 0) && tiles_s == (has_s ? all_s : 0)) break;
   }
-  if (prefix < a->lk) {
-    s.ranges_s = std::max(1, ceil_div(all_s, each));
-    s.tiles_s = ceil_div(all_s, s.ranges_s);
-    s.ranges_s = ceil_div(all_s, s.tiles_s);
-  }
-  s.grid_p = ceil_div(s.ranges_p, 8) * 8 * share_p;
-  s.grid_s = ceil_div((int64_t)s.ranges_s * a->B, 8) * 8 * share_s;
+  s.prefix.grid = ceil_div(s.prefix.ranges, 8) * 8 * share_p;
+  s.own.grid = ceil_div((int64_t)s.own.ranges * a->B, 8) * 8 * share_s;
   return s;
 }
-size_t plan_bytes(const SharedPlan& s, int H, int D) { return (size_t)(s.ranges_p + s.ranges_s) * s.rows * H * (D + 2) * sizeof(float); }
+int ranges_of(const SharedPlan& s) { return s.prefix.ranges + s.own.ranges; }
+size_t plan_bytes(const SharedPlan& s, int H, int D) { return (size_t)ranges_of(s) * s.rows * H * (D + 2) * sizeof(float); }
 
 template <int D, int RK, bool PAGED>
 int launch_mfma_t(const SharedMfmaParams& p, hipStream_t s) {
   auto kern = shared_mfma_kernel<D, RK, PAGED>;
   static bool done[kMaxDevices] = {};
   if (const int rc = raise_lds_limit(done, reinterpret_cast<const void*>(kern), SharedLds<D>::kBytes); rc != TPA_OK) return rc;
-  hipLaunchKernelGGL(kern, dim3(p.plan.grid_p + p.plan.grid_s), dim3(kWaves * 64), SharedLds<D>::kBytes, s, p);
+  hipLaunchKernelGGL(kern, dim3(p.plan.prefix.grid + p.plan.own.grid), dim3(kWaves * 64), SharedLds<D>::kBytes, s, p);
   if (hipGetLastError() != hipSuccess) return TPA_ERR_LAUNCH;
-  hipLaunchKernelGGL((shared_merge_kernel<uint16_t, D>), dim3(ceil_div(p.plan.rows * p.c.H, 256 / (D / 4))), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((shared_merge_kernel<uint16_t, D>), dim3(ceil_div(p.plan.rows * p.c.H, 4)), dim3(256), 0, s, p);
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
 template <int D, int RK>
@@ -609,7 +685,7 @@ extern "C" int tpa_decode_shared(const TpaFwdArgs* a, int32_t prefix, void* stre
     SharedMfmaParams m{p, plan_of(a, prefix)};
     if (!a->workspace || a->workspace_bytes < plan_bytes(m.plan, a->H, a->dv)) return TPA_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return TPA_ERR_ALIGN;
-    const size_t parts = (size_t)(m.plan.ranges_p + m.plan.ranges_s) * m.plan.rows * a->H;
+    const size_t parts = (size_t)ranges_of(m.plan) * m.plan.rows * a->H;
     m.part_o = static_cast<float*>(a->workspace);
     m.part_m = m.part_o + parts * a->dv;
     m.part_l = m.part_m + parts;
