@@ -235,8 +235,13 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumParams p) {
   const int which = blockIdx.y, col = threadIdx.x & 31, part = threadIdx.x >> 5, d = blockIdx.x * 32 + col;
   if (!p.out[which]) return;
   float sum = 0.f;
-  if (d < p.D)
-    for (int i = part; i < p.count[which]; i += 32) sum += p.partial[((int64_t)which * kPartials + i) * p.D + d];
+  if (d < p.D) {
+    float v[kPartials / 32];  // all of them on their way at once
+#pragma unroll
+    for (int x = 0; x < kPartials / 32; ++x) v[x] = part + 32 * x < p.count[which] ? p.partial[((int64_t)which * kPartials + part + 32 * x) * p.D + d] : 0.f;
+#pragma unroll
+    for (int x = 0; x < kPartials / 32; ++x) sum += v[x];
+  }
   red[part][col] = sum;
   __syncthreads();
   if (part == 0 && d < p.D) {
@@ -247,12 +252,24 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumParams p) {
 }
 
 // ---------------------------------------------------------------------------------------------- matrix cores
-// A wave takes the rank rows of as many tokens of one side as fit the 16 rows of a matrix instruction, RM to a token: lane (i, g) holds
-// row i's elements 32 s + 8 g + 0..7 of every chunk s, 16 bytes a load.  That is at once the layout of both operands of G = B B^T
-// (no exchange between lanes) and whole pairs for the rotation.  A head's norm is a lane's: G through LDS, R^2 products.
-// HBM bounds it: a token's factors come once and go once.
+// A wave takes the rank rows of as many tokens of one side as fit the 16 rows of a matrix instruction, a power of two to a token.  Lane (i, g)
+// holds row i's elements 32 s + 8 g + 0..7 of every chunk s, 16 bytes a load: at once the layout of both operands of G = B B^T and whole
+// pairs for the rotation.  G's result layout - column i, four rows - is, G being symmetric, that of an operand of the next product Y = G A, 16
+// heads a time; there lane (n, g) holds four rows of head n of Y and, as the other operand, the same four of A, so that |X_h|^2 = a_h . y_h is
+// a sum over a lane's registers and a few lanes.  Nothing goes through LDS.  For bf16 factors G goes into that product as three bf16
+// numbers, 2^-27 of it off; for fp32 factors both are products in 64 bits.
+// The rows of a wave's tokens stand in one product, so a token's rows meet zeros for the other tokens'; where those are not finite, 0 * inf
+// would spread, and the tokens take turns.
+// HBM bounds it: a token's factors come once and go once, at 2.6 to 3.5 TB/s in the cases below, where a plain copy of their size has about 4.5.  (With
+// G through LDS and R^2 products a head on the vector units, 310 registers and 1300 vector instructions per 16 rows, their backward
+// took 66 and 256 us.)
 typedef __attribute__((ext_vector_type(4))) double f64x4;
 constexpr int kNormWaves = 4;
+// Waves of a SIMD that the registers are kept to.  What these kernels need is loads on their way, so waves; one more of them costs scratch memory:
+// us at (4, 3, 2) / (5, 4, 3), forward and backward of 4 x 4096 tokens, 16 heads of 128 23 / 41 and 38 / 38, of 8 x 2048, 64 heads of 64, ranks 16
+// and 8 58 / 77 and 118 / 184.  (The factors of the next tokens asked for ahead take the registers of a wave: 24 and 50, 56 and 183.)
+constexpr int fwd_waves(int size, int d) { return size == 2 ? 4 : d == 64 ? 3 : 2; }
+constexpr int bwd_waves(int size, int d) { return size == 2 && d == 64 ? 3 : 2; }
 
 template <typename T>
 struct Chunk {  // eight elements as loaded
@@ -283,102 +300,99 @@ template <typename T, int VH>
 __device__ __forceinline__ void load_heads(const T* from, float (&a)[VH]) {
   if constexpr (VH == 1) {
     a[0] = load_as_f32(from);
-  } else if constexpr (sizeof(T) == 2) {
+  } else if constexpr (sizeof(T) * VH == 4) {
     const uint32_t x = *reinterpret_cast<const uint32_t*>(from);
     a[0] = bf16lo_to_f32(x); a[1] = bf16hi_to_f32(x);
+  } else if constexpr (sizeof(T) * VH == 8) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(from);
+#pragma unroll
+    for (int v = 0; v < VH; ++v) a[v] = VH == 2 ? __uint_as_float(x[v]) : v & 1 ? bf16hi_to_f32(x[v / 2]) : bf16lo_to_f32(x[v / 2]);
   } else {
-    const float2 x = *reinterpret_cast<const float2*>(from);
-    a[0] = x.x; a[1] = x.y;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(from);
+#pragma unroll
+    for (int v = 0; v < VH; ++v) a[v] = x[v];
   }
 }
 template <typename T, int VH>
 __device__ __forceinline__ void store_heads(T* to, const float (&a)[VH]) {
   if constexpr (VH == 1) store_from_f32(to, a[0]);
-  else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16(a[0], a[1]);
-  else *reinterpret_cast<float2*>(to) = make_float2(a[0], a[1]);
+  else if constexpr (sizeof(T) * VH == 4) *reinterpret_cast<uint32_t*>(to) = pack_bf16(a[0], a[1]);
+  else if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3])};
+  else if constexpr (VH == 2) *reinterpret_cast<float2*>(to) = make_float2(a[0], a[1]);
+  else *reinterpret_cast<f32x4*>(to) = f32x4{a[0], a[1], a[2], a[3]};
 }
+// two where 16 lanes still take whole rows of them (four of 64 heads: backward of the second case below 157 us, two 117)
+template <typename F>
+void with_heads(int H, F f) {
+  if (H > 16) f(std::integral_constant<int, 2>{});
+  else f(std::integral_constant<int, 1>{});
+}
+// log2 of the rows that a token of rank R takes
+__host__ __device__ inline int rows_log2(int R) { return R <= 1 ? 0 : R <= 2 ? 1 : R <= 4 ? 2 : R <= 8 ? 3 : 4; }
+__host__ __device__ inline int tokens_per_wave(int R) { return 16 >> rows_log2(R); }
 
-// what a wave's tokens are: 16 / RM of them, lane i's row is rank i % RM of token i / RM
-template <int RM>
-struct Rows {
-  static constexpr int P = 16 / RM;
-  int token, bi, i;  // of this lane's row (clamped)
-  int r;
-  bool there;        // the row is a rank of a token
-  int first;         // token of row 0
-  __device__ __forceinline__ Rows(int group, int tokens, int l, int R, int lane) {
-    const int row = lane & 15, tt = row / RM;
-    first = group * P;
-    r = row - tt * RM;
-    there = tt < P && r < R && first + tt < tokens;
-    token = min(first + min(tt, P - 1), tokens - 1);
-    r = min(r, R - 1);
-    bi = token / l;
-    i = token - bi * l;
-  }
-};
-// the sums of G and what is made from them: 32 bits for bf16 factors, 64 for fp32
+// sums in 32 bits for bf16 factors, in 64 for fp32
 template <typename T>
-using Sum = std::conditional_t<sizeof(T) == 2, float, double>;
+struct Sums {
+  using S = float;
+  using V = f32x4;
+  __device__ __forceinline__ static int row(int g, int j) { return 4 * g + j; }  // of a lane's result register j
+};
+template <>
+struct Sums<float> {
+  using S = double;
+  using V = f64x4;
+  __device__ __forceinline__ static int row(int g, int j) { return 4 * j + g; }
+};
 
-// G of the wave's tokens, token by token in LDS: row r of token tt at (tt RM + r) RMP
-template <int RM>
-constexpr int kGramStride = (RM + 3) / 4 * 4;
-template <typename T, int D, int RM>
-__device__ __forceinline__ bool gram_to_lds(const Chunk<T> (&x)[D / 32], Sum<T>* G, int lane) {
-  const int i = lane & 15, g = lane >> 4;
-  bool finite = true;
-  auto put = [&](int row, Sum<T> v) __attribute__((always_inline)) {
-    finite = finite && __builtin_fabs(v) <= 3.4028235e38;
-    if (row / RM == i / RM && i / RM < 16 / RM) G[(i / RM * RM + row % RM) * kGramStride<RM> + i % RM] = v;
-  };
-  if constexpr (sizeof(T) == 2) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      const bf16x8 f = __builtin_bit_cast(bf16x8, x[s].x[0]);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, f, acc, 0, 0, 0);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) put(4 * g + e, acc[e]);
-  } else {
-    f64x4 acc = {0, 0, 0, 0};
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double f = x[s][e];
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(f, f, acc, 0, 0, 0);
-      }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) put(4 * e + g, acc[e]);
-  }
-  return !__any(!finite);
+__device__ __forceinline__ float with_lane(float x, int apart) {  // x + that of the lane 16 (32) apart
+  const uint32_t u = __float_as_uint(x);
+  const auto r = apart == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// G a of a lane's heads; a^T G a comes back
-template <typename T, int RM, int VH>
-__device__ __forceinline__ void times_gram(const Sum<T>* G, int tt, const float (&a)[RM][VH], Sum<T> (&y)[RM][VH], Sum<T> (&square)[VH]) {
+__device__ __forceinline__ double with_lane(double x, int apart) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+  const auto rl = apart == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+  const auto rh = apart == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+  return __longlong_as_double((long long)((uint64_t)rh[0] << 32 | rl[0])) + __longlong_as_double((long long)((uint64_t)rh[1] << 32 | rl[1]));
+}
+// four rows' terms -> for each the sum over the 2^lg rows of its token
+template <typename T, typename S>
+__device__ __forceinline__ void over_token(S (&v)[4], int lg) {
+  auto pairs = [&] { v[0] = v[1] = v[0] + v[1]; v[2] = v[3] = v[2] + v[3]; };
+  auto all = [&] { v[0] = v[1] = v[2] = v[3] = v[0] + v[2]; };
+  auto lanes = [&](int apart) {
 #pragma unroll
-  for (int v = 0; v < VH; ++v) square[v] = 0;
-#pragma unroll
-  for (int r = 0; r < RM; ++r) {
-    const Sum<T>* const row = G + (tt * RM + r) * kGramStride<RM>;
-#pragma unroll
-    for (int v = 0; v < VH; ++v) y[r][v] = 0;
-#pragma unroll
-    for (int t = 0; t < RM; ++t) {
-      const Sum<T> x = row[t];
-#pragma unroll
-      for (int v = 0; v < VH; ++v) y[r][v] += x * (Sum<T>)a[t][v];
-    }
-#pragma unroll
-    for (int v = 0; v < VH; ++v) square[v] += (Sum<T>)a[r][v] * y[r][v];
+    for (int j = 0; j < 4; ++j) v[j] = with_lane(v[j], apart);
+  };
+  if constexpr (sizeof(T) == 2) {  // rows 4 g + j
+    if (lg >= 1) pairs();
+    if (lg >= 2) all();
+    if (lg >= 3) v[0] = v[1] = v[2] = v[3] = with_lane(v[0], 16);
+    if (lg >= 4) v[0] = v[1] = v[2] = v[3] = with_lane(v[0], 32);
+  } else {  // rows 4 j + g
+    if (lg >= 1) lanes(16);
+    if (lg >= 2) lanes(32);
+    if (lg >= 3) pairs();
+    if (lg >= 4) all();
   }
 }
 template <typename S>
-__device__ __forceinline__ float inverse_norm_of(S square, int R, int D, float eps) {
-  const float mean = (float)(square / (S)(R * R * D));
-  return rsqrtf((mean < 0 ? 0 : mean) + eps);  // NaN stays NaN
+__device__ __forceinline__ float inverse_norm_of(S square, S inv, float eps) {  // inv = 1 / (R R D)
+  const float mean = (float)(square * inv);
+  return __builtin_amdgcn_rsqf((mean < 0 ? 0 : mean) + eps);  // one unit in the last place; NaN stays NaN
+}
+// for four rows; rows of one token have one
+template <typename T, typename S>
+__device__ __forceinline__ void inverse_norms(const S (&square)[4], S inv, float eps, int lg, float (&scale)[4]) {
+  scale[0] = inverse_norm_of(square[0], inv, eps);
+  if (lg >= (sizeof(T) == 2 ? 2 : 4)) {
+    scale[1] = scale[2] = scale[3] = scale[0];
+  } else {
+#pragma unroll
+    for (int j = 1; j < 4; ++j) scale[j] = inverse_norm_of(square[j], inv, eps);
+  }
 }
 
 // cos and sin of a lane's four pairs of chunk s
@@ -407,335 +421,440 @@ struct Turns {
     }
   }
 };
-__device__ __forceinline__ void weights_at(const void* w, int bf16, int d, float (&out)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) out[e] = 1.f;
-  if (!w) return;
-  if (bf16) {
-    const Chunk<uint16_t> c = load_chunk(static_cast<const uint16_t*>(w) + d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = c[e];
-  } else {
-    const Chunk<float> c = load_chunk(static_cast<const float*>(w) + d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = c[e];
-  }
+// a side's weights as fp32 in LDS, by the whole workgroup
+template <int D>
+__device__ __forceinline__ void weights_to_lds(const void* from, int bf16, float* to) {
+  if (threadIdx.x < D) to[threadIdx.x] = weight_at(from, bf16, threadIdx.x);
+  __syncthreads();
 }
 __device__ __forceinline__ void wave_lds_fence() {  // the wave's own writes have landed
   __builtin_amdgcn_s_waitcnt(0xc07f);
   __builtin_amdgcn_wave_barrier();
 }
 
-// calls f with the rows to a token that a rank of R takes
-template <typename F>
-__device__ __forceinline__ void with_rows(int R, F f) {
-  if (R == 1) f(std::integral_constant<int, 1>{});
-  else if (R == 2) f(std::integral_constant<int, 2>{});
-  else if (R <= 4) f(std::integral_constant<int, 4>{});
-  else if (R <= 6) f(std::integral_constant<int, 6>{});
-  else if (R <= 8) f(std::integral_constant<int, 8>{});
-  else f(std::integral_constant<int, 16>{});
+// A wave's tokens are of one batch entry: what its lanes add to the entry's base fits 32 bits
+template <typename T>
+__device__ __forceinline__ T* base_of(const TpaFactor& f, int bi, int first) {
+  return static_cast<T*>(const_cast<void*>(f.ptr)) + bi * f.stride_b + first * f.stride_l;
 }
-__host__ __device__ inline int tokens_per_wave(int R) { return R == 1 ? 16 : R == 2 ? 8 : R <= 4 ? 4 : R <= 8 ? 2 : 1; }
-
-constexpr int kGramElements = 16 * 16;  // of G of a wave's tokens, at most
-
-// the place that a token's K and V factors go to: page and token in it, or the token's own
-__device__ __forceinline__ bool place_of(const NormRopeParams& p, bool cached, int token, int bi, int i, int64_t& page, int64_t& at) {
-  page = bi;
-  at = i;
-  if (!cached) return true;
-  const int slot = p.slots[token];
-  if (slot < 0 || slot >= p.num_slots) return false;
+__device__ __forceinline__ uint32_t offset_of(const TpaFactor& f, int tt, int r) { return (uint32_t)(tt * (int)f.stride_l + r * (int)f.stride_r); }
+// page and place of a token's slot
+__device__ __forceinline__ bool slot_of(const NormRopeParams& p, int bi, int i, int64_t& page, int64_t& at) {
+  const int slot = p.slots[bi * p.l + i];
   page = slot / p.page_size;
   at = slot - page * p.page_size;
-  return true;
+  return slot >= 0 && slot < p.num_slots;
 }
 
-template <typename T, int D, bool AXES, int RM>
-__device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Side& side, bool cached, int group, int tokens, Sum<T>* G) {
-  constexpr int P = 16 / RM, NS = D / 32;
-  const int lane = threadIdx.x & 63, g = lane >> 4, R = side.R, H = p.H;
-  const Rows<RM> me(group, tokens, p.l, R, lane);
-  const T* const b = static_cast<const T*>(side.b.ptr) + me.bi * side.b.stride_b + me.i * side.b.stride_l + me.r * side.b.stride_r + 8 * g;
+// G of the wave's rows, the other tokens' columns zero; `finite`: whether all of its numbers are
+template <typename T, int D>
+__device__ __forceinline__ typename Sums<T>::V gram(const Chunk<T> (&x)[D / 32], int row, int g, int lg, bool& finite) {
+  typename Sums<T>::V G = {0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x8 f = __builtin_bit_cast(bf16x8, x[s].x[0]);
+      G = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, f, G, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) G = __builtin_amdgcn_mfma_f64_16x16x4f64((double)x[s][e], (double)x[s][e], G, 0, 0, 0);
+    }
+  }
+  bool fine = true;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    fine = fine && __builtin_fabsf((float)G[j]) <= 3.4028235e38f;
+    if (Sums<T>::row(g, j) >> lg != row >> lg) G[j] = 0;
+  }
+  finite = !__any(!fine);
+  return G;
+}
+// G as the operand of Y = G A
+template <typename T>
+struct GramOperand;
+template <>
+struct GramOperand<uint16_t> {
+  s16x4 part[3];
+  __device__ __forceinline__ explicit GramOperand(f32x4 G) {
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      const u32x2 p = {pack_bf16(G[0], G[1]), pack_bf16(G[2], G[3])};
+      part[n] = __builtin_bit_cast(s16x4, p);
+      G = f32x4{G[0] - bf16lo_to_f32(p[0]), G[1] - bf16hi_to_f32(p[0]), G[2] - bf16lo_to_f32(p[1]), G[3] - bf16hi_to_f32(p[1])};
+    }
+  }
+  __device__ __forceinline__ f32x4 times(const float (&a)[4]) const {  // a: numbers of bf16
+    const u32x2 p = {__builtin_amdgcn_perm(__float_as_uint(a[1]), __float_as_uint(a[0]), 0x07060302), __builtin_amdgcn_perm(__float_as_uint(a[3]), __float_as_uint(a[2]), 0x07060302)};
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 2; n >= 0; --n) y = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(part[n], __builtin_bit_cast(s16x4, p), y, 0, 0, 0);
+    return y;
+  }
+};
+template <>
+struct GramOperand<float> {
+  f64x4 G;
+  __device__ __forceinline__ explicit GramOperand(f64x4 from) : G(from) {}
+  __device__ __forceinline__ f64x4 times(const float (&a)[4]) const {
+    f64x4 y = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y = __builtin_amdgcn_mfma_f64_16x16x4f64(G[j], (double)a[j], y, 0, 0, 0);
+    return y;
+  }
+};
+// Y of 16 heads; where a number is not finite the tokens take turns
+template <typename T>
+__device__ __forceinline__ typename Sums<T>::V times_gram(const GramOperand<T>& G, const float (&a)[4], bool finite, int g, int lg) {
+  bool fine = finite;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) fine = fine && __builtin_fabsf(a[j]) <= 3.4028235e38f;
+  if (lg == 4 || !__any(!fine)) return G.times(a);
+  typename Sums<T>::V y = {0, 0, 0, 0};
+  for (int tt = 0; tt < 16 >> lg; ++tt) {
+    float one[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) one[j] = Sums<T>::row(g, j) >> lg == tt ? a[j] : 0.f;
+    const typename Sums<T>::V yt = G.times(one);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (Sums<T>::row(g, j) >> lg == tt) y[j] = yt[j];
+  }
+  return y;
+}
+
+// a wave's tokens, and this lane's row of theirs
+struct Rows {
+  int bi, first;  // batch entry, its first token
+  int tt, r, i;   // this lane's token among the wave's, its rank, the token in the entry (clamped)
+  bool there;
+  __device__ __forceinline__ Rows(int group, int l, int R, int lg, int lane) {
+    const int P = 16 >> lg, per_entry = (l + P - 1) / P, row = lane & 15;
+    bi = group / per_entry;
+    first = (group - bi * per_entry) * P;
+    tt = min(row >> lg, l - 1 - first);
+    there = (row & ((1 << lg) - 1)) < R && row >> lg == tt;
+    r = min(row & ((1 << lg) - 1), R - 1);
+    i = first + tt;
+  }
+};
+
+template <typename T, int D, bool AXES, int VH, bool CACHED>
+__device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Side& side, int group, const float* wt) {
+  constexpr int NS = D / 32;
+  const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, R = side.R, H = p.H, lg = rows_log2(R);
+  const Rows me(group, p.l, R, lg, lane);
+  const T* const b = base_of<const T>(side.b, me.bi, me.first) + (offset_of(side.b, me.tt, me.r) + 8 * g);
   Chunk<T> x[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) x[s] = me.there ? load_chunk(b + 32 * s) : Chunk<T>{};
-  const Turns<D, AXES> turn(p.rot, me.token, me.i, g);
-  int64_t page, at;
-  const bool stored = place_of(p, cached, me.token, me.bi, me.i, page, at) && me.there;
-  if (p.normalize) {
-    gram_to_lds<T, D, RM>(x, G, lane);
-    wave_lds_fence();
+  // head factors: of four rows this lane has VH heads of every 16 VH
+  const T* const a_base = base_of<const T>(side.a, me.bi, me.first);
+  uint32_t a_in[4];
+  T* a_out[4];  // CACHED: by slot
+  uint32_t a_to[4];
+  T* const a_out_base = CACHED ? nullptr : base_of<T>(side.a_out, me.bi, me.first);
+  bool a_there[4], a_stored[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int rj = Sums<T>::row(g, j), tt = min(rj >> lg, p.l - 1 - me.first), r = min(rj & ((1 << lg) - 1), R - 1);
+    a_there[j] = rj >> lg == tt && (rj & ((1 << lg) - 1)) < R;
+    a_in[j] = offset_of(side.a, tt, r);
+    a_stored[j] = a_there[j];
+    if constexpr (CACHED) {
+      int64_t page, at;
+      a_stored[j] = slot_of(p, me.bi, me.first + tt, page, at) && a_there[j];
+      a_out[j] = static_cast<T*>(const_cast<void*>(side.a_out.ptr)) + page * side.a_out.stride_b + at * side.a_out.stride_l + r * side.a_out.stride_r;
+    } else {
+      a_to[j] = offset_of(side.a_out, tt, r);
+    }
   }
-  // the b rows: weight, rotation
-  T* const bo = static_cast<T*>(const_cast<void*>(side.b_out.ptr)) + page * side.b_out.stride_b + at * side.b_out.stride_l + me.r * side.b_out.stride_r + 8 * g;
+  auto heads = [&](int h, float (&a)[4][VH]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int v = 0; v < VH; ++v) a[j][v] = 0.f;
+      if (a_there[j] && h < H) load_heads<T, VH>(a_base + (a_in[j] + h), a[j]);
+    }
+  };
+  float a[4][VH];
+  heads(VH * row, a);
+  const Turns<D, AXES> turn(p.rot, me.bi * p.l + me.i, me.i, g);
+  bool stored = me.there;
+  T* bo;
+  if constexpr (CACHED) {
+    int64_t page, at;
+    stored = slot_of(p, me.bi, me.i, page, at) && me.there;
+    bo = static_cast<T*>(const_cast<void*>(side.b_out.ptr)) + page * side.b_out.stride_b + at * side.b_out.stride_l + me.r * side.b_out.stride_r + 8 * g;
+  } else {
+    bo = base_of<T>(side.b_out, me.bi, me.first) + (offset_of(side.b_out, me.tt, me.r) + 8 * g);
+  }
+  bool finite = true;
+  typename Sums<T>::V G0 = {0, 0, 0, 0};
+  if (p.normalize) G0 = gram<T, D>(x, row, g, lg, finite);
+  const GramOperand<T> G(G0);
+  const typename Sums<T>::S inv = (typename Sums<T>::S)1 / (typename Sums<T>::S)(R * R * D);
+  for (int h = VH * row; h - VH * row < H; h += 16 * VH) {
+    float next[4][VH];
+    heads(h + 16 * VH, next);
+    if (p.normalize) {
+#pragma unroll
+      for (int v = 0; v < VH; ++v) {
+        const float av[4] = {a[0][v], a[1][v], a[2][v], a[3][v]};
+        const typename Sums<T>::V y = times_gram<T>(G, av, finite, g, lg);
+        typename Sums<T>::S square[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) square[j] = av[j] * y[j];
+        over_token<T>(square, lg);
+        float scale[4];
+        inverse_norms<T>(square, inv, p.eps, lg, scale);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j][v] *= scale[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (a_stored[j] && h < H) store_heads<T, VH>(CACHED ? a_out[j] + h : a_out_base + (a_to[j] + h), a[j]);
+#pragma unroll
+      for (int v = 0; v < VH; ++v) a[j][v] = next[j][v];
+    }
+  }
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    float wt[8], y[8];
-    weights_at(side.weight, p.weight_bf16, 32 * s + 8 * g, wt);
+    float y[8];
+    const Chunk<float> w = load_chunk(wt + 32 * s + 8 * g);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float y0 = x[s][2 * e] * wt[2 * e], y1 = x[s][2 * e + 1] * wt[2 * e + 1];
+      const float y0 = x[s][2 * e] * w[2 * e], y1 = x[s][2 * e + 1] * w[2 * e + 1];
       y[2 * e] = y0 * turn.c[s][e] - y1 * turn.s[s][e];
       y[2 * e + 1] = y1 * turn.c[s][e] + y0 * turn.s[s][e];
     }
     if (stored) store_chunk(bo + 32 * s, y);
   }
-  // the head factors
-  auto heads = [&](auto vh_c) __attribute__((always_inline)) {
-    constexpr int VH = decltype(vh_c)::value;
-    for (int at_head = VH * lane; at_head < P * H; at_head += VH * 64) {
-      const int tt = at_head / H, h = at_head - tt * H, token = me.first + tt;
-      if (token >= tokens) continue;
-      const int bi = token / p.l, i = token - bi * p.l;
-      int64_t page, at;
-      if (!place_of(p, cached, token, bi, i, page, at)) continue;
-      const T* const from = static_cast<const T*>(side.a.ptr) + bi * side.a.stride_b + i * side.a.stride_l + h;
-      T* const to = static_cast<T*>(const_cast<void*>(side.a_out.ptr)) + page * side.a_out.stride_b + at * side.a_out.stride_l + h;
-      float a[RM][VH];
-#pragma unroll
-      for (int r = 0; r < RM; ++r) {
-        if (r < R) load_heads<T, VH>(from + r * side.a.stride_r, a[r]);
-        else
-#pragma unroll
-          for (int v = 0; v < VH; ++v) a[r][v] = 0.f;
-      }
-      float scale[VH];
-#pragma unroll
-      for (int v = 0; v < VH; ++v) scale[v] = 1.f;
-      if (p.normalize) {
-        Sum<T> y[RM][VH], square[VH];
-        times_gram<T, RM, VH>(G, tt, a, y, square);
-#pragma unroll
-        for (int v = 0; v < VH; ++v) scale[v] = inverse_norm_of(square[v], R, D, p.eps);
-      }
-#pragma unroll
-      for (int r = 0; r < RM; ++r) {
-        float out[VH];
-#pragma unroll
-        for (int v = 0; v < VH; ++v) out[v] = a[r][v] * scale[v];
-        if (r < R) store_heads<T, VH>(to + r * side.a_out.stride_r, out);
-      }
-    }
-  };
-  if (P * H <= 64) heads(std::integral_constant<int, 1>{});
-  else heads(std::integral_constant<int, 2>{});
 }
 
-template <typename T, int D, bool AXES>
-__global__ __launch_bounds__(kNormWaves * 64) void norm_rope_kernel(NormRopeParams p, int groups_q, int groups_k, int groups_v) {
-  __shared__ Sum<T> gram[kNormWaves][kGramElements];
-  const int w = scalar(threadIdx.x >> 6), tokens = p.B * p.l;
-  int task = blockIdx.x * kNormWaves + w;
-  if (task < groups_q + groups_k) {
-    const bool keys = task >= groups_q;
-    const Side& side = p.side[keys];
-    with_rows(side.R, [&](auto rm) __attribute__((always_inline)) {
-      norm_rope_rows<T, D, AXES, decltype(rm)::value>(p, side, keys && p.slots, keys ? task - groups_q : task, tokens, gram[w]);
-    });
-    return;
-  }
-  task -= groups_q + groups_k;
-  if (task >= groups_v) return;
-  // V factors into their slots, 16 bytes a lane: chunks of a row of ranks, head factors first
+// V factors into their slots, 16 bytes a lane: chunks of a row of ranks, head factors first
+template <typename T, int D>
+__device__ __forceinline__ void copy_values(const NormRopeParams& p, int group) {
   constexpr int E = 16 / sizeof(T);
   const int R = p.side[1].R, lane = threadIdx.x & 63, per_rank = (p.H + D) / E, per_token = R * per_rank, P = tokens_per_wave(R);
+  const int per_entry = (p.l + P - 1) / P, bi = group / per_entry, first = (group - bi * per_entry) * P;
   for (int x = lane; x < P * per_token; x += 64) {
-    const int tt = x / per_token, token = task * P + tt, rest = x - tt * per_token, r = rest / per_rank, c = (rest - r * per_rank) * E;
-    if (token >= tokens) break;
-    const int bi = token / p.l, i = token - bi * p.l;
+    const int tt = x / per_token, i = first + tt, rest = x - tt * per_token, r = rest / per_rank, c = (rest - r * per_rank) * E;
+    if (i >= p.l) break;
     int64_t page, at;
-    if (!place_of(p, true, token, bi, i, page, at)) continue;
+    if (!slot_of(p, bi, i, page, at)) continue;
     const bool head = c < p.H;
     const TpaFactor &in = head ? p.va : p.vb, &out = head ? p.va_out : p.vb_out;
     const int col = head ? c : c - p.H;
     *reinterpret_cast<u32x4*>(static_cast<T*>(const_cast<void*>(out.ptr)) + page * out.stride_b + at * out.stride_l + r * out.stride_r + col) =
-        *reinterpret_cast<const u32x4*>(static_cast<const T*>(in.ptr) + bi * in.stride_b + i * in.stride_l + r * in.stride_r + col);
+        *reinterpret_cast<const u32x4*>(base_of<const T>(in, bi, first) + (offset_of(in, tt, r) + col));
+  }
+}
+
+// Workgroups 0 .. parts_q - 1 share out the queries' tokens, the next parts_k the keys', the others the values'
+template <typename T, int D, bool AXES, int VH, bool CACHED>
+__global__ __launch_bounds__(kNormWaves * 64, fwd_waves(sizeof(T), D)) void norm_rope_kernel(NormRopeParams p, int parts_q, int parts_k, int parts_v) {
+  __shared__ __attribute__((aligned(16))) float wt[D];
+  const int w = scalar(threadIdx.x >> 6), part = blockIdx.x;
+  auto groups = [&](int R) { return (p.l + tokens_per_wave(R) - 1) / tokens_per_wave(R) * p.B; };
+  if (part < parts_q) {
+    weights_to_lds<D>(p.side[0].weight, p.weight_bf16, wt);
+    for (int group = part * kNormWaves + w; group < groups(p.side[0].R); group += parts_q * kNormWaves) norm_rope_rows<T, D, AXES, VH, false>(p, p.side[0], group, wt);
+  } else if (part < parts_q + parts_k) {
+    weights_to_lds<D>(p.side[1].weight, p.weight_bf16, wt);
+    for (int group = (part - parts_q) * kNormWaves + w; group < groups(p.side[1].R); group += parts_k * kNormWaves) norm_rope_rows<T, D, AXES, VH, CACHED>(p, p.side[1], group, wt);
+  } else if constexpr (CACHED) {
+    for (int group = (part - parts_q - parts_k) * kNormWaves + w; group < groups(p.side[1].R); group += parts_v * kNormWaves) copy_values<T, D>(p, group);
   }
 }
 
 // ---- gradients.  The R x R sums M = A diag(w) A^T over the heads and the mixture M B of the b rows are products of the matrix cores
-// too: M's result layout is that of the second product's operand, whose other one are the b rows read back transposed.  For bf16
-// factors w a and M are kept as two bf16 numbers each.  The rows of a wave's tokens stand in one product, so the rows of the other
-// tokens meet zeros: where a b row is not finite, 0 * inf would spread, and the tokens take turns instead.
+// too: M's result layout is that of the second product's operand, whose other one are the b rows read back transposed from LDS.  For bf16
+// factors w a and M are kept as two bf16 numbers each.
 template <typename T, int D>
 struct BwdLds {
-  static constexpr int kStride = sizeof(T) == 2 ? D : D + 4;              // of a b row (elements)
-  static constexpr size_t kRows = 16 * kStride * sizeof(T), kGram = kGramElements * sizeof(Sum<T>);
-  static size_t bytes(int most_pairs) { return kNormWaves * (kRows + kGram + (size_t)(most_pairs + 3) / 4 * 16); }
+  static constexpr int kStride = sizeof(T) == 2 ? D : D + 4;  // of a b row (elements)
+  static constexpr size_t kRows = 16 * kStride * sizeof(T);
+  static size_t wave_bytes(int most_pairs) { return kRows + (size_t)(most_pairs + 3) / 4 * 16; }
+  static size_t bytes(int most_pairs) { return kNormWaves * wave_bytes(most_pairs) + D * sizeof(float); }
 };
 
-template <typename T, int D, bool AXES, int RM>
-__device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, const BwdSide& side, int group, int tokens, unsigned char* lds, float (&d_weight)[D / 4]) {
-  constexpr int P = 16 / RM, NS = D / 32;
+template <typename T, int D, bool AXES, int VH>
+__device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, const BwdSide& side, int group, unsigned char* lds, const float* wt, float (&d_weight)[D / 4]) {
+  constexpr int NS = D / 32;
   using Lds = BwdLds<T, D>;
   T* const rows = reinterpret_cast<T*>(lds);
-  Sum<T>* const G = reinterpret_cast<Sum<T>*>(lds + Lds::kRows);
-  float* const W = reinterpret_cast<float*>(lds + Lds::kRows + Lds::kGram);  // [P][H]
-  const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, R = side.R, H = p.H;
-  const Rows<RM> me(group, tokens, p.l, R, lane);
-  const T* const b = static_cast<const T*>(side.b.ptr) + me.bi * side.b.stride_b + me.i * side.b.stride_l + me.r * side.b.stride_r + 8 * g;
-  const T* const db = static_cast<const T*>(side.db_out.ptr) + me.bi * side.db_out.stride_b + me.i * side.db_out.stride_l + me.r * side.db_out.stride_r + 8 * g;
+  float* const W = reinterpret_cast<float*>(lds + Lds::kRows);  // [token][H]
+  const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, R = side.R, H = p.H, lg = rows_log2(R);
+  const Rows me(group, p.l, R, lg, lane);
+  const T* const b = base_of<const T>(side.b, me.bi, me.first) + (offset_of(side.b, me.tt, me.r) + 8 * g);
+  const T* const db = base_of<const T>(side.db_out, me.bi, me.first) + (offset_of(side.db_out, me.tt, me.r) + 8 * g);
   Chunk<T> x[NS], dy[NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    x[s] = me.there ? load_chunk(b + 32 * s) : Chunk<T>{};
-    dy[s] = me.there ? load_chunk(db + 32 * s) : Chunk<T>{};
+  for (int s = 0; s < NS; ++s) x[s] = me.there ? load_chunk(b + 32 * s) : Chunk<T>{};
+#pragma unroll
+  for (int s = 0; s < NS; ++s) dy[s] = me.there ? load_chunk(db + 32 * s) : Chunk<T>{};
+  const T *const a_base = base_of<const T>(side.a, me.bi, me.first), *const da_base = base_of<const T>(side.da_out, me.bi, me.first);
+  T* const out_base = base_of<T>(side.da, me.bi, me.first);
+  uint32_t a_in[4], da_in[4], da_out[4];
+  bool a_there[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int rj = Sums<T>::row(g, j), tt = min(rj >> lg, p.l - 1 - me.first), r = min(rj & ((1 << lg) - 1), R - 1);
+    a_there[j] = rj >> lg == tt && (rj & ((1 << lg) - 1)) < R;
+    a_in[j] = offset_of(side.a, tt, r);
+    da_in[j] = offset_of(side.da_out, tt, r);
+    da_out[j] = offset_of(side.da, tt, r);
   }
-  const Turns<D, AXES> turn(p.rot, me.token, me.i, g);
+  auto heads = [&](int h, float (&a)[4][VH], float (&da)[4][VH]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int v = 0; v < VH; ++v) a[j][v] = da[j][v] = 0.f;
+      if (a_there[j] && h < H) {
+        load_heads<T, VH>(a_base + (a_in[j] + h), a[j]);
+        load_heads<T, VH>(da_base + (da_in[j] + h), da[j]);
+      }
+    }
+  };
+  float a[4][VH], da[4][VH];
+  heads(VH * row, a, da);
   bool finite = true;
+  typename Sums<T>::V G0 = {0, 0, 0, 0};
   if (p.normalize) {
-    finite = gram_to_lds<T, D, RM>(x, G, lane);
+    G0 = gram<T, D>(x, row, g, lg, finite);
     if (finite)
 #pragma unroll
       for (int s = 0; s < NS; ++s)
 #pragma unroll
         for (int n = 0; n < (int)sizeof(T) / 2; ++n) reinterpret_cast<u32x4*>(rows + row * Lds::kStride + 32 * s + 8 * g)[n] = x[s].x[n];
-    wave_lds_fence();
   }
-  // head factors: a lane's heads
-  auto heads = [&](auto vh_c) __attribute__((always_inline)) {
-    constexpr int VH = decltype(vh_c)::value;
-    for (int at_head = VH * lane; at_head < P * H; at_head += VH * 64) {
-      const int tt = at_head / H, h = at_head - tt * H, token = me.first + tt;
-      float w[VH];
-      if (token < tokens) {
-        const int bi = token / p.l, i = token - bi * p.l;
-        const T* const from = static_cast<const T*>(side.a.ptr) + bi * side.a.stride_b + i * side.a.stride_l + h;
-        const T* const d_from = static_cast<const T*>(side.da_out.ptr) + bi * side.da_out.stride_b + i * side.da_out.stride_l + h;
-        T* const to = static_cast<T*>(const_cast<void*>(side.da.ptr)) + bi * side.da.stride_b + i * side.da.stride_l + h;
-        float a[RM][VH], da[RM][VH];
+  const GramOperand<T> G(G0);
+  const typename Sums<T>::S inv = (typename Sums<T>::S)1 / (typename Sums<T>::S)(R * R * D);
+  for (int h = VH * row; h - VH * row < H; h += 16 * VH) {
+    float next[4][VH], d_next[4][VH];
+    heads(h + 16 * VH, next, d_next);
+    if (p.normalize) {
 #pragma unroll
-        for (int r = 0; r < RM; ++r) {
-          if (r < R) {
-            load_heads<T, VH>(from + r * side.a.stride_r, a[r]);
-            load_heads<T, VH>(d_from + r * side.da_out.stride_r, da[r]);
-          } else {
+      for (int v = 0; v < VH; ++v) {
+        const float av[4] = {a[0][v], a[1][v], a[2][v], a[3][v]};
+        const typename Sums<T>::V y = times_gram<T>(G, av, finite, g, lg);
+        typename Sums<T>::S square[4];
+        float u[4];
 #pragma unroll
-            for (int v = 0; v < VH; ++v) a[r][v] = da[r][v] = 0.f;
-          }
+        for (int j = 0; j < 4; ++j) {
+          square[j] = av[j] * y[j];
+          u[j] = da[j][v] * av[j];
         }
-        if (p.normalize) {
-          Sum<T> y[RM][VH], square[VH];
-          times_gram<T, RM, VH>(G, tt, a, y, square);
+        over_token<T>(square, lg);
+        over_token<T>(u, lg);
+        float scale[4];
+        inverse_norms<T>(square, inv, p.eps, lg, scale);
 #pragma unroll
-          for (int v = 0; v < VH; ++v) {
-            const float scale = inverse_norm_of(square[v], R, D, p.eps);
-            float u = 0.f;
-#pragma unroll
-            for (int r = 0; r < RM; ++r) u = fmaf(da[r][v], a[r][v], u);
-            w[v] = -scale * scale * scale * u / (float)(D * R * R);
-#pragma unroll
-            for (int r = 0; r < RM; ++r) da[r][v] = da[r][v] * scale + w[v] * (float)y[r][v];
-          }
+        for (int j = 0; j < 4; ++j) {
+          const float w = -scale[j] * scale[j] * scale[j] * u[j] * (float)inv;
+          da[j][v] = da[j][v] * scale[j] + w * (float)y[j];
+          const int rj = Sums<T>::row(g, j);
+          if ((rj & ((1 << lg) - 1)) == 0 && h < H) W[(rj >> lg) * H + h + v] = w;
         }
-#pragma unroll
-        for (int r = 0; r < RM; ++r)
-          if (r < R) store_heads<T, VH>(to + r * side.da.stride_r, da[r]);
-      } else {
-#pragma unroll
-        for (int v = 0; v < VH; ++v) w[v] = 0.f;
       }
-      if (p.normalize)
-#pragma unroll
-        for (int v = 0; v < VH; ++v) W[at_head + v] = w[v];
     }
-  };
-  if (P * H <= 64) heads(std::integral_constant<int, 1>{});
-  else heads(std::integral_constant<int, 2>{});
-  // M[4 g + e][row] of the token's rows
-  f32x4 M = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (a_there[j] && h < H) store_heads<T, VH>(out_base + (da_out[j] + h), da[j]);
+#pragma unroll
+      for (int v = 0; v < VH; ++v) {
+        a[j][v] = next[j][v];
+        da[j][v] = d_next[j][v];
+      }
+    }
+  }
+  const Turns<D, AXES> turn(p.rot, me.bi * p.l + me.i, me.i, g);
+  f32x4 M = {0.f, 0.f, 0.f, 0.f};  // M[4 g + e][row] of the token's rows
+  u32x2 hi = {0, 0}, lo = {0, 0};  // in two bf16 numbers
   if (p.normalize) {
     wave_lds_fence();
-    const T* const a = static_cast<const T*>(side.a.ptr) + me.bi * side.a.stride_b + me.i * side.a.stride_l + me.r * side.a.stride_r;
-    const float* const w_of = W + min(row / RM, P - 1) * H;
-    if constexpr (sizeof(T) == 2) {
-      for (int h = 8 * g; h - 8 * g < H; h += 32) {
-        const bool there = me.there && h < H;
-        const Chunk<T> ac = there ? load_chunk(a + h) : Chunk<T>{};
-        u32x4 hi, lo;
+    const T* const a_row = a_base + offset_of(side.a, me.tt, me.r);
+    const float* const w_of = W + (row >> lg) * H;
+    for (int h = 8 * g; h - 8 * g < H; h += 32) {
+      const bool there = me.there && h < H;
+      const Chunk<T> ac = there ? load_chunk(a_row + h) : Chunk<T>{};
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = there ? ac[e] * w_of[h + e] : 0.f;
+      if constexpr (sizeof(T) == 2) {
+        u32x4 wh, wl;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float w0 = there ? ac[2 * e] * w_of[h + 2 * e] : 0.f, w1 = there ? ac[2 * e + 1] * w_of[h + 2 * e + 1] : 0.f;
-          hi[e] = pack_bf16(w0, w1);
-          lo[e] = pack_bf16(w0 - bf16lo_to_f32(hi[e]), w1 - bf16hi_to_f32(hi[e]));
+          wh[e] = pack_bf16(w[2 * e], w[2 * e + 1]);
+          wl[e] = pack_bf16(w[2 * e] - bf16lo_to_f32(wh[e]), w[2 * e + 1] - bf16hi_to_f32(wh[e]));
         }
         const bf16x8 f = __builtin_bit_cast(bf16x8, ac.x[0]);
-        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, lo), M, 0, 0, 0);
-        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, hi), M, 0, 0, 0);
-      }
-    } else {
-      for (int h = 8 * g; h - 8 * g < H; h += 32) {
-        const bool there = me.there && h < H;
-        const Chunk<T> ac = there ? load_chunk(a + h) : Chunk<T>{};
+        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, wl), M, 0, 0, 0);
+        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, wh), M, 0, 0, 0);
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) M = __builtin_amdgcn_mfma_f32_16x16x4f32(ac[e], there ? ac[e] * w_of[h + e] : 0.f, M, 0, 0, 0);
+        for (int e = 0; e < 8; ++e) M = __builtin_amdgcn_mfma_f32_16x16x4f32(ac[e], w[e], M, 0, 0, 0);
       }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if ((4 * g + e) / RM != row / RM || row / RM >= P) M[e] = 0.f;
-  }
-  // mixture of the b rows: out[n][e] of this lane's row at d = 32 (n / 2) + 8 g + 4 (n % 2) + e
-  f32x4 mixed[2 * NS];
-#pragma unroll
-  for (int n = 0; n < 2 * NS; ++n) mixed[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto mix = [&](f32x4 (&out)[2 * NS]) __attribute__((always_inline)) {
+      if ((4 * g + e) >> lg != row >> lg) M[e] = 0.f;
     if constexpr (sizeof(T) == 2) {
-      const u32x2 hi = {pack_bf16(M[0], M[1]), pack_bf16(M[2], M[3])};
-      const u32x2 lo = {pack_bf16(M[0] - bf16lo_to_f32(hi[0]), M[1] - bf16hi_to_f32(hi[0])), pack_bf16(M[2] - bf16lo_to_f32(hi[1]), M[3] - bf16hi_to_f32(hi[1]))};
-#pragma unroll
-      for (int n = 0; n < 2 * NS; ++n) {
-        // rows 4 g + 0..3 of the column that this lane stands for: 16 lanes bring 4 rows x 16 columns and get them transposed
-        const T* const from = rows + (4 * g + (row >> 2)) * Lds::kStride + 32 * (n / 2) + 8 * (row & 3) + 4 * (n % 2);
-        const s16x4 f = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)from);
-        out[n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, lo), out[n], 0, 0, 0);
-        out[n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, hi), out[n], 0, 0, 0);
-      }
+      hi = u32x2{pack_bf16(M[0], M[1]), pack_bf16(M[2], M[3])};
+      lo = u32x2{pack_bf16(M[0] - bf16lo_to_f32(hi[0]), M[1] - bf16hi_to_f32(hi[0])), pack_bf16(M[2] - bf16lo_to_f32(hi[1]), M[3] - bf16hi_to_f32(hi[1]))};
+    }
+  }
+  // the mixture of the b rows for this lane's row: element e of piece n is d = 32 (n / 2) + 8 g + 4 (n % 2) + e
+  auto mix = [&](int n) __attribute__((always_inline)) {
+    f32x4 out = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (sizeof(T) == 2) {
+      // rows 4 g + 0..3 of the column that this lane stands for: 16 lanes bring 4 rows x 16 columns and get them transposed
+      const T* const from = rows + (4 * g + (row >> 2)) * Lds::kStride + 32 * (n / 2) + 8 * (row & 3) + 4 * (n % 2);
+      const s16x4 f = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)from);
+      out = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, lo), out, 0, 0, 0);
+      return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, hi), out, 0, 0, 0);
     } else {
 #pragma unroll
-      for (int n = 0; n < 2 * NS; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          out[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows[(4 * g + e) * Lds::kStride + 32 * (n / 2) + 8 * (row >> 2) + 4 * (n % 2) + (row & 3)], M[e], out[n], 0, 0, 0);
+      for (int e = 0; e < 4; ++e)
+        out = __builtin_amdgcn_mfma_f32_16x16x4f32(rows[(4 * g + e) * Lds::kStride + 32 * (n / 2) + 8 * (row >> 2) + 4 * (n % 2) + (row & 3)], M[e], out, 0, 0, 0);
+      return out;
     }
   };
-  if (p.normalize) {
-    if (finite) {
-      mix(mixed);
-    } else {
-      for (int tt = 0; tt < P; ++tt) {
-        wave_lds_fence();
-        const bool mine = row / RM == tt;
+  T* const bo = base_of<T>(side.db, me.bi, me.first) + (offset_of(side.db, me.tt, me.r) + 8 * g);
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+  for (int s = 0; s < NS; ++s) {
+    f32x4 mixed[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (p.normalize) {
+      if (finite) {
+        mixed[0] = mix(2 * s);
+        mixed[1] = mix(2 * s + 1);
+      } else {
+        for (int tt = 0; tt < 16 >> lg; ++tt) {
+          wave_lds_fence();
+          const bool mine = row >> lg == tt;
 #pragma unroll
           for (int n = 0; n < (int)sizeof(T) / 2; ++n)
             reinterpret_cast<u32x4*>(rows + row * Lds::kStride + 32 * s + 8 * g)[n] = mine ? x[s].x[n] : u32x4{0, 0, 0, 0};
-        wave_lds_fence();
-        f32x4 one[2 * NS];
+          wave_lds_fence();
 #pragma unroll
-        for (int n = 0; n < 2 * NS; ++n) one[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        mix(one);
-#pragma unroll
-        for (int n = 0; n < 2 * NS; ++n) mixed[n] = mine ? one[n] : mixed[n];
+          for (int n = 0; n < 2; ++n) {
+            const f32x4 one = mix(2 * s + n);
+            mixed[n] = mine ? one : mixed[n];
+          }
+        }
       }
     }
-  }
-  T* const bo = static_cast<T*>(const_cast<void*>(side.db.ptr)) + me.bi * side.db.stride_b + me.i * side.db.stride_l + me.r * side.db.stride_r + 8 * g;
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    float wt[8], y[8];
-    weights_at(side.weight, p.weight_bf16, 32 * s + 8 * g, wt);
+    float y[8];
+    const Chunk<float> w = load_chunk(wt + 32 * s + 8 * g);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float y0 = dy[s][2 * e], y1 = dy[s][2 * e + 1];
       const float e0 = y0 * turn.c[s][e] + y1 * turn.s[s][e], e1 = y1 * turn.c[s][e] - y0 * turn.s[s][e];
       d_weight[8 * s + 2 * e] = fmaf(e0, x[s][2 * e], d_weight[8 * s + 2 * e]);
       d_weight[8 * s + 2 * e + 1] = fmaf(e1, x[s][2 * e + 1], d_weight[8 * s + 2 * e + 1]);
-      y[2 * e] = fmaf(e0, wt[2 * e], mixed[2 * s + e / 2][2 * e % 4]);
-      y[2 * e + 1] = fmaf(e1, wt[2 * e + 1], mixed[2 * s + e / 2][(2 * e + 1) % 4]);
+      y[2 * e] = fmaf(e0, w[2 * e], mixed[e / 2][2 * e % 4]);
+      y[2 * e + 1] = fmaf(e1, w[2 * e + 1], mixed[e / 2][(2 * e + 1) % 4]);
     }
     if (me.there) store_chunk(bo + 32 * s, y);
   }
@@ -743,22 +862,25 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
 }
 
 // Workgroups 0 .. parts_q - 1 share out the queries' tokens, the others the keys'
-template <typename T, int D, bool AXES>
-__global__ __launch_bounds__(kNormWaves * 64) void norm_rope_bwd_kernel(NormRopeBwdParams p, int parts_q, int parts_k, int wave_bytes) {
+template <typename T, int D, bool AXES, int VH>
+__global__ __launch_bounds__(kNormWaves * 64, bwd_waves(sizeof(T), D)) void norm_rope_bwd_kernel(NormRopeBwdParams p, int parts_q, int parts_k, int wave_bytes) {
   extern __shared__ __attribute__((aligned(16))) unsigned char bwd_mem[];
-  const int w = scalar(threadIdx.x >> 6), lane = threadIdx.x & 63, tokens = p.B * p.l;
+  const int w = scalar(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const bool keys = (int)blockIdx.x >= parts_q;
-  const BwdSide& side = p.side[keys];
-  const int part = keys ? blockIdx.x - parts_q : blockIdx.x, parts = keys ? parts_k : parts_q;
+  const int part = keys ? blockIdx.x - parts_q : blockIdx.x;
   float d_weight[D / 4];  // of this lane's row: element 8 s + e is d = 32 s + 8 g + e
 #pragma unroll
   for (int x = 0; x < D / 4; ++x) d_weight[x] = 0.f;
-  with_rows(side.R, [&](auto rm) __attribute__((always_inline)) {
-    constexpr int RM = decltype(rm)::value, P = 16 / RM;
-    for (int group = part * kNormWaves + w; group < (tokens + P - 1) / P; group += parts * kNormWaves)
-      norm_rope_bwd_rows<T, D, AXES, RM>(p, side, group, tokens, bwd_mem + w * wave_bytes, d_weight);
-  });
-  if (!side.d_weight) return;
+  float* const wt = reinterpret_cast<float*>(bwd_mem + kNormWaves * wave_bytes);
+  auto rows_of = [&](const BwdSide& side, int parts) __attribute__((always_inline)) {
+    const int P = tokens_per_wave(side.R), groups = (p.l + P - 1) / P * p.B;
+    weights_to_lds<D>(side.weight, p.weight_bf16, wt);
+    for (int group = part * kNormWaves + w; group < groups; group += parts * kNormWaves)
+      norm_rope_bwd_rows<T, D, AXES, VH>(p, side, group, bwd_mem + w * wave_bytes, wt, d_weight);
+  };
+  if (keys) rows_of(p.side[1], parts_k);
+  else rows_of(p.side[0], parts_q);
+  if (!(keys ? p.side[1].d_weight : p.side[0].d_weight)) return;
   // over the rows of the wave, then over the waves
 #pragma unroll
   for (int x = 0; x < D / 4; ++x) {
@@ -786,40 +908,68 @@ __global__ __launch_bounds__(kNormWaves * 64) void norm_rope_bwd_kernel(NormRope
 template <typename Args>
 bool fast_takes(const Args* a, const TpaFactor* const* fs, int n) {
   if (a->kernel == TPA_KERNEL_GENERIC || (a->D != 64 && a->D != 128) || a->H % 8 || a->rq > 16 || a->rk > 16) return false;
-  if ((int64_t)a->B * a->l > (1 << 30)) return false;
+  if ((int64_t)a->B * a->l > (1 << 26)) return false;  // groups of tokens of every entry in 32 bits
   for (int i = 0; i < a->n_axes; ++i)
     if (a->sections[i] % 4) return false;
   const int chunk = a->dtype == TPA_DTYPE_BF16 ? 8 : 4;
   for (int i = 0; i < n; ++i) {
     const TpaFactor& f = *fs[i];
     if ((reinterpret_cast<uintptr_t>(f.ptr) & 15) || f.stride_b % chunk || f.stride_l % chunk || f.stride_r % chunk) return false;
+    if (f.stride_l < 0 || f.stride_r < 0 || f.stride_l > (1 << 25) || f.stride_r > (1 << 25)) return false;  // 16 tokens' offsets in 32 bits
   }
   return !((reinterpret_cast<uintptr_t>(a->rope_cos) | reinterpret_cast<uintptr_t>(a->rope_sin) | reinterpret_cast<uintptr_t>(a->q_weight) | reinterpret_cast<uintptr_t>(a->k_weight)) & 15);
 }
+// entries that follow one another in every array are one: what positions count from then has to be given
+bool follows(const TpaFactor& f, int l) { return f.stride_b == f.stride_l * l; }
+// workgroups for a side's tokens
+int parts_of(int B, int l, int R, int most) {
+  const int64_t groups = (int64_t)B * ((l + tokens_per_wave(R) - 1) / tokens_per_wave(R));
+  return (int)std::min<int64_t>((groups + kNormWaves - 1) / kNormWaves, most);
+}
 template <typename T, int D>
-int launch_fast(const NormRopeParams& p, hipStream_t s) {
+int launch_fast(NormRopeParams p, hipStream_t s) {
   const int64_t tokens = (int64_t)p.B * p.l;
-  auto groups = [&](int R) { return (int)((tokens + tokens_per_wave(R) - 1) / tokens_per_wave(R)); };
-  const int q = groups(p.side[0].R), k = groups(p.side[1].R), v = p.slots ? k : 0;
-  const dim3 grid((unsigned)(((int64_t)q + k + v + kNormWaves - 1) / kNormWaves));
+  bool one = p.rot.positions != nullptr;
+  for (const Side& x : p.side) one = one && follows(x.a, p.l) && follows(x.b, p.l);
+  for (int x = 0; x < (p.slots ? 1 : 2); ++x) one = one && follows(p.side[x].a_out, p.l) && follows(p.side[x].b_out, p.l);
+  if (p.slots) one = one && follows(p.va, p.l) && follows(p.vb, p.l);
+  if (one) {
+    p.l = (int)tokens;
+    p.B = 1;
+  }
+  const int q = parts_of(p.B, p.l, p.side[0].R, 4096), k = parts_of(p.B, p.l, p.side[1].R, 4096), v = p.slots ? k : 0;
   const bool axes = p.rot.n_axes > 1 || p.rot.last_of[3] < D / 2;
-  if (axes) hipLaunchKernelGGL((norm_rope_kernel<T, D, true>), grid, dim3(kNormWaves * 64), 0, s, p, q, k, v);
-  else hipLaunchKernelGGL((norm_rope_kernel<T, D, false>), grid, dim3(kNormWaves * 64), 0, s, p, q, k, v);
+  with_heads(p.H, [&](auto vh) {
+    constexpr int VH = decltype(vh)::value;
+    auto kern = axes ? (p.slots ? norm_rope_kernel<T, D, true, VH, true> : norm_rope_kernel<T, D, true, VH, false>)
+                     : (p.slots ? norm_rope_kernel<T, D, false, VH, true> : norm_rope_kernel<T, D, false, VH, false>);
+    hipLaunchKernelGGL(kern, dim3(q + k + v), dim3(kNormWaves * 64), 0, s, p, q, k, v);
+  });
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
 inline int most_pairs(int rq, int rk, int H) { return (tokens_per_wave(rq) > tokens_per_wave(rk) ? tokens_per_wave(rq) : tokens_per_wave(rk)) * H; }
 template <typename T, int D>
-int launch_fast_bwd(const NormRopeBwdParams& p, int (&parts)[2], hipStream_t s) {
+int launch_fast_bwd(NormRopeBwdParams p, int (&parts)[2], hipStream_t s) {
   const int64_t tokens = (int64_t)p.B * p.l;
+  bool one = p.rot.positions != nullptr;
   for (int x = 0; x < 2; ++x) {
-    const int64_t groups = (tokens + tokens_per_wave(p.side[x].R) - 1) / tokens_per_wave(p.side[x].R);
-    parts[x] = p.side[x].da_out.ptr ? (int)std::min<int64_t>((groups + kNormWaves - 1) / kNormWaves, kPartials) : 0;
+    const BwdSide& side = p.side[x];
+    if (side.da_out.ptr)
+      for (const TpaFactor* f : {&side.a, &side.b, &side.da_out, &side.db_out, &side.da, &side.db}) one = one && follows(*f, p.l);
   }
-  const size_t lds = BwdLds<T, D>::bytes(most_pairs(p.side[0].R, p.side[1].R, p.H));
+  if (one) {
+    p.l = (int)tokens;
+    p.B = 1;
+  }
+  for (int x = 0; x < 2; ++x) parts[x] = p.side[x].da_out.ptr ? parts_of(p.B, p.l, p.side[x].R, kPartials) : 0;
+  const int pairs = most_pairs(p.side[0].R, p.side[1].R, p.H), wave = (int)BwdLds<T, D>::wave_bytes(pairs);
+  const size_t lds = BwdLds<T, D>::bytes(pairs);
   const bool axes = p.rot.n_axes > 1 || p.rot.last_of[3] < D / 2;
   const dim3 grid(parts[0] + parts[1]);
-  if (axes) hipLaunchKernelGGL((norm_rope_bwd_kernel<T, D, true>), grid, dim3(kNormWaves * 64), lds, s, p, parts[0], parts[1], (int)(lds / kNormWaves));
-  else hipLaunchKernelGGL((norm_rope_bwd_kernel<T, D, false>), grid, dim3(kNormWaves * 64), lds, s, p, parts[0], parts[1], (int)(lds / kNormWaves));
+  with_heads(p.H, [&](auto vh) {
+    constexpr int VH = decltype(vh)::value;
+    hipLaunchKernelGGL((axes ? norm_rope_bwd_kernel<T, D, true, VH> : norm_rope_bwd_kernel<T, D, false, VH>), grid, dim3(kNormWaves * 64), lds, s, p, parts[0], parts[1], wave);
+  });
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
 
