@@ -699,8 +699,10 @@ PyObject* page_tables(PyObject*, PyObject* const* args, Py_ssize_t n) {
     int64_t at = 0, total = 0;
     for (int64_t s : sizes) total += (s + 63) / 64 * 64;
     const Tensor all = at::empty({total}, options);
-    for (int i = 0; i < 5; ++i) {
-      out[i] = all.narrow(0, at, sizes[i]);
+    for (int i = 0; i < 5; ++i) {  // (narrow() takes longer than the kernel for five of them)
+      out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+      out[i].unsafeGetTensorImpl()->set_storage_offset(at);
+      out[i].unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
       at += (sizes[i] + 63) / 64 * 64;
     }
     TpaPageTablesArgs a{};
@@ -930,22 +932,22 @@ PyObject* norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_CALL
 }
 
-// norm_rope_backward(q, k, rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel, dq_out, dk_out)
+// norm_rope_backward(q, k, dq_out, dk_out, rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel)
 PyObject* norm_rope_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   BEGIN_CALL
   count("norm_rope_backward", n, 14);
-  if (!gpu_tensors(args, 4) || !none_or_gpu(args[4]) || !none_or_gpu(args[5]) || !none_or_gpu(args[6]) || !gpu_tensors(args + 12, 2)) Py_RETURN_NOTIMPLEMENTED;
-  const Tensor q = THPVariable_Unpack(args[0]), k = THPVariable_Unpack(args[1]);
-  NormRope c = norm_rope_call(args + 2);
+  if (!gpu_tensors(args, 6) || !none_or_gpu(args[6]) || !none_or_gpu(args[7]) || !none_or_gpu(args[8])) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor q = THPVariable_Unpack(args[0]), k = THPVariable_Unpack(args[1]), dq_out = THPVariable_Unpack(args[2]), dk_out = THPVariable_Unpack(args[3]);
+  NormRope c = norm_rope_call(args + 4);
   check_norm_rope(q, k, c);
-  one_device({q, k, c.cos, c.sin, c.q_weight, c.k_weight, c.positions, THPVariable_Unpack(args[12]), THPVariable_Unpack(args[13])});
+  one_device({q, k, c.cos, c.sin, c.q_weight, c.k_weight, c.positions, dq_out, dk_out});
   Tensor grads[4];
   {
     WithoutGil free;
     const at::AutoGradMode no_grad(false);
     const c10::DeviceGuard guard(q.device());
     settle(c);
-    run_norm_rope_bwd(q, k, c, THPVariable_Unpack(args[12]), THPVariable_Unpack(args[13]), {true, true}, grads);
+    run_norm_rope_bwd(q, k, c, dq_out, dk_out, {true, true}, grads);
   }
   PyObject* out = PyTuple_New(4);
   if (!out) throw python_error();
@@ -957,15 +959,15 @@ PyObject* norm_rope_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_CALL
 }
 
-// norm_rope_write(q, k, rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel, v, slots, ka, kb, va, vb)
+// norm_rope_write(q, k, v, slots, rope_cos, rope_sin, q_weight, k_weight, positions, num_heads, sections, normalize, eps, kernel, ka, kb, va, vb)
 PyObject* norm_rope_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   BEGIN_CALL
   count("norm_rope_write", n, 18);
-  if (!gpu_tensors(args, 4) || !none_or_gpu(args[4]) || !none_or_gpu(args[5]) || !none_or_gpu(args[6]) || !gpu_tensors(args + 12, 2)) Py_RETURN_NOTIMPLEMENTED;
+  if (!gpu_tensors(args, 6) || !none_or_gpu(args[6]) || !none_or_gpu(args[7]) || !none_or_gpu(args[8])) Py_RETURN_NOTIMPLEMENTED;
   if (!gpu_tensors(args + 14, 4)) throw Raise{PyExc_TypeError, "the cache is written in place: ka, kb, va, vb must be GPU tensors"};
-  const Tensor q = THPVariable_Unpack(args[0]), k = THPVariable_Unpack(args[1]), v = THPVariable_Unpack(args[12]);
-  Tensor slots = THPVariable_Unpack(args[13]);
-  NormRope c = norm_rope_call(args + 2);
+  const Tensor q = THPVariable_Unpack(args[0]), k = THPVariable_Unpack(args[1]), v = THPVariable_Unpack(args[2]);
+  Tensor slots = THPVariable_Unpack(args[3]);
+  NormRope c = norm_rope_call(args + 4);
   check_norm_rope(q, k, c);
   const int64_t h = c.heads, d = q.size(3) - h, rk = k.size(2);
   expect(v.sizes() == k.sizes(), v);

@@ -595,8 +595,10 @@ SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   const bool has_p = prefix > 0, has_s = prefix < a->lk;
   auto tile_ns = [&](const SharedPart& x) { return (a->dk == 128 ? kBlockNs128 : kBlockNs64) * kBlocks / std::min(kWaves / x.waves, kBlocks); };
   const double tile_p = tile_ns(s.prefix), tile_s = std::max(tile_ns(s.own), kOwnTileNs * a->dk / 128);
+  // (not those that would make several rounds of workgroups, and none far behind the best)
+  const double all_ns = (double)all_p * share_p * tile_p * has_p + (double)all_s * share_s * a->B * tile_s * has_s;
   double best = 0;
-  for (double time = std::min(tile_p, tile_s); ; time *= 1.07) {
+  for (double time = std::max(std::min(tile_p, tile_s), all_ns / 800); ; time *= 1.07) {
     const int tiles_p = has_p ? std::min(all_p, std::max(1, (int)(time / tile_p))) : 0, tiles_s = has_s ? std::min(all_s, std::max(1, (int)(time / tile_s))) : 0;
     const int ranges_p = has_p ? ceil_div(all_p, tiles_p) : 0, ranges_s = has_s ? ceil_div(all_s, tiles_s) : 0;
     // an XCD takes whole ranges: what counts is the one that has most of them, as if all had
@@ -609,7 +611,7 @@ SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
       best = cost;
       s.prefix.tiles = tiles_p; s.own.tiles = tiles_s; s.prefix.ranges = ranges_p; s.own.ranges = ranges_s;
     }
-    if (tiles_p == (has_p ? all_p : 0) && tiles_s == (has_s ? all_s : 0)) break;
+    if (cost > 2 * best || (tiles_p == (has_p ? all_p : 0) && tiles_s == (has_s ? all_s : 0))) break;
   }
   s.prefix.grid = ceil_div(s.prefix.ranges, 8) * 8 * share_p;
   s.own.grid = ceil_div((int64_t)s.own.ranges * a->B, 8) * 8 * share_s;

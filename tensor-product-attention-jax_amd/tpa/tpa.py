@@ -300,10 +300,9 @@ def tpa_norm_rope_bwd(
 ):
     """Gradients of `tpa_norm_rope` from those of its results: (dq, dk, dq_weight, dk_weight), None for a weight that is not
     given.  torch.autograd reaches the same through `tpa_norm_rope`."""
-    device = _pick_device(q, k)
-    arrays = [None if x is None else _as_device_tensor(x, device) for x in (q, k, rope_cos, rope_sin, q_weight, k_weight, positions)]
-    return _d.host_calls().norm_rope_backward(
-        *arrays, int(num_heads), sections, bool(normalize), float(eps), int(kernel), *(_as_device_tensor(x, device) for x in (dq_out, dk_out))
+    return _call(
+        _d.host_calls().norm_rope_backward, (q, k, dq_out, dk_out, rope_cos, rope_sin, q_weight, k_weight, positions),
+        int(num_heads), sections, bool(normalize), float(eps), int(kernel),
     )
 
 
@@ -327,10 +326,9 @@ def tpa_norm_rope_write(
     [pages, page_size, rk, h|d], which `tpa_decode` reads; slots outside the pools (-1) are dropped, and no slot may be there twice.  A contiguous
     cache [b, cache_len, rk, h|d] is a pool whose pages are the batch entries.  Returns q' like q.  No gradient flows through this call.
     """
-    device = _pick_device(q, k, v)
-    arrays = [None if x is None else _as_device_tensor(x, device) for x in (q, k, rope_cos, rope_sin, q_weight, k_weight, positions)]
-    return _d.host_calls().norm_rope_write(
-        *arrays, int(num_heads), sections, bool(normalize), float(eps), int(kernel), *(_as_device_tensor(x, device) for x in (v, slots)), ka, kb, va, vb
+    return _call(
+        _d.host_calls().norm_rope_write, (q, k, v, slots, rope_cos, rope_sin, q_weight, k_weight, positions),
+        int(num_heads), sections, bool(normalize), float(eps), int(kernel), ka, kb, va, vb,
     )
 
 
