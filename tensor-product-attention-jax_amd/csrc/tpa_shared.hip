@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kAnyThreads) void shared_any_kernel(SharedParams p)
   if (tid == 0 && p.lse) p.lse[((int64_t)b * p.H + h) * p.lq + row] = empty ? -INFINITY : (most + log2f(total)) * kLn2;
 }
 
-// ---------------------------------------------------------------------------------------------- bf16, matrix cores
+// ---------------------------------------------------------------------------------------------- matrix cores
 // As in the split-key decode nothing is expanded to dense keys or values: with Qm[c, :] = (scale / (Rq R)) sum_i qa_i qb_i of column c = (row,
 // head) the logits are s[c, t] = sum_r ka[t, r, h] (Qm[c, :] . kb[t, r, :]), the output (1 / R) sum_t sum_r (p[c, t] va[t, r, h]) vb[t, r, :], two
 // products of the rows (t, r) with the columns.  The rows serve every column, so a workgroup takes a tile of 4 blocks of 32 rows
@@ -126,15 +126,19 @@ __global__ __launch_bounds__(kAnyThreads) void shared_any_kernel(SharedParams p)
 // buffers.
 // Qm is kept as two bf16 numbers, 2^-17 of it off: with one the logits carry the rounding of Qm, 2^-9 each, and the output's error
 // grows by half; the second costs 8 of 24 matrix instructions a block.  The weights p va are rounded to bf16 once, sums are fp32.
+// In fp32 nothing is rounded, a tile has 2 blocks, and what a product takes is read as it lies: over d the halves of a wave take d = 8 m + 4 g + e
+// in turn (16 bytes of a row feed four products), over a block's rows the row that their logits' register belongs to, and row i of
+// block db of the output is d = (D / 32) i + db, so that one read of a v row serves all blocks.
 constexpr int kRows = 32;           // rows (token, rank) of a block
-constexpr int kBlocks = 4;          // blocks of a tile, each of them brought by two waves
 constexpr int kWaves = 8;
 constexpr int kRsrcFlags = 0x00020000;  // raw 32-bit data format
-constexpr int64_t kFarthestRow = 1 << 25;  // elements between neighbouring rows, at most: 31 of them in 32-bit byte offsets
+constexpr int64_t kFarthestRow = 1 << 26;  // bytes between neighbouring rows, at most: 31 of them in 32-bit byte offsets
+constexpr int blocks_of_tile(int bytes) { return bytes == 2 ? 4 : 2; }  // of numbers of so many bytes
 
-template <int D>
+template <typename T, int D>
 struct SharedLds {
-  static constexpr int kB = kRows * D * 2, kA = kRows * 32 * 2;              // bytes of a block's b rows, a rows (32 heads)
+  static constexpr int kBlocks = blocks_of_tile(sizeof(T));
+  static constexpr int kB = kRows * D * sizeof(T), kA = kRows * 32 * sizeof(T);  // bytes of a block's b rows, a rows (32 heads)
   static constexpr int kBuffer = kBlocks * 2 * (kB + kA);                     // kb, vb, ka, va of a tile
   static constexpr int kPart = 32 * D * 4 + 2 * 64 * 4;                       // a wave's sums of a set of columns on their way to another
   static constexpr size_t kBytes = 2 * kBuffer;
@@ -164,8 +168,10 @@ struct SharedMfmaParams {
 
 // Where a lane's pieces of a block of rows of D lie in LDS (elements): 16-byte chunk c of row r at chunk c ^ f(r), so that neither the reads of
 // one chunk of 16 rows nor the transposed ones of 4 chunks of 4 rows meet a bank twice
+template <typename T, int D>
+struct BlockAt;
 template <int D>
-struct BlockAt {
+struct BlockAt<uint16_t, D> {
   static constexpr int CPR = D / 8;
   __device__ __forceinline__ static int f(int r) { return CPR == 16 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3); }
   int row, tr;
@@ -178,18 +184,34 @@ struct BlockAt {
   // transposed: rows 16 kk + 8 hi + 4 g + 0..3, columns 32 db + 0..31
   __device__ __forceinline__ int read_tr(int kk, int hi, int db) const { return (tr ^ (32 * db) ^ (16 * hi)) + (16 * kk + 8 * hi) * D; }
 };
+template <int D>
+struct BlockAt<float, D> {
+  __device__ __forceinline__ static int f(int r) { return r & 15; }
+  int l, row;
+  __device__ __forceinline__ explicit BlockAt(int lane) : l(lane), row((lane & 31) * D + 4 * ((lane >> 5) ^ f(lane & 31))) {}
+  __device__ __forceinline__ int read(int m) const { return row ^ (8 * m); }  // row i, chunk 2 m + g
+  // columns D / 32 i and following of the row of register v
+  __device__ __forceinline__ int read_v(int v) const {
+    const int i = l & 31, r = 8 * (v >> 2) + 4 * (l >> 5) + (v & 3), at = D / 32 * i;
+    return r * D + (at ^ (4 * f(r)));
+  }
+};
 typedef s16x4 __attribute__((address_space(3))) lds_s16x4;
 template <int D>
-__device__ __forceinline__ bf16x8 block_tr(const uint16_t* block, const BlockAt<D>& at, int kk, int db) {
+__device__ __forceinline__ bf16x8 block_tr(const uint16_t* block, const BlockAt<uint16_t, D>& at, int kk, int db) {
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(block + at.read_tr(kk, 0, db)));
   const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(block + at.read_tr(kk, 1, db)));
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-template <int D, int RK, bool PAGED>
+template <typename T, int D, int RK, bool PAGED>
 __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const SharedPart& part, bool own, int id, unsigned char* mem) {
-  using Lds = SharedLds<D>;
-  constexpr int NKS = D / 16, NDB = D / 32, CPR = D / 8, RPI = 64 / CPR, NI = 16 / RPI;  // NI: load instructions of a wave's 16 b rows
+  using Lds = SharedLds<T, D>;
+  using At = BlockAt<T, D>;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int kBlocks = Lds::kBlocks, kSize = sizeof(T), kPer = 16 / kSize;  // kPer: numbers of a load of 16 bytes
+  constexpr int WPB = kWaves / kBlocks, RPW = kRows / WPB;                     // waves that bring a block, rows of each
+  constexpr int NKS = D / 16, NDB = D / 32, CPR = D / kPer, RPI = 64 / CPR, NI = RPW / RPI;  // NI: load instructions of a wave's b rows
   constexpr int TPB = kRows / RK;                                                           // tokens of a block
   constexpr int NTOK = RK <= 4 ? 16 / RK : 32 / RK;  // tokens whose rows this lane holds, per block
   constexpr int NV = RK <= 4 ? RK : RK / 2;          // rows of one token held by this half of the wave
@@ -211,10 +233,10 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   const int row = (own ? b_own * c.lq : 0) + min(wave_row + in_set, n_rows - 1);  // this lane's query row among all
   const int b = c.lq == 1 ? row : row / c.lq, row_in_b = row - b * c.lq;
 
-  // ---- Qm^T[d, c] = sum_r qb[r, d] qa[r, c] by the matrix cores, 16 ranks a time, a set's rows one after the other with the other rows' columns
+  // ---- Qm^T[d, c] = sum_r qb[r, d] qa[r, c] by the matrix cores in bf16, 16 ranks a time, a set's rows one after the other with the other rows' columns
   // zero: asked for here, finished while the first tile is on its way
-  uint16_t qa_in[8], qb_in[NDB][8];
-  auto request_q = [&](int in_row, int r0) __attribute__((always_inline)) {
+  [[maybe_unused]] uint16_t qa_in[8], qb_in[NDB][8];
+  [[maybe_unused]] auto request_q = [&](int in_row, int r0) __attribute__((always_inline)) {
     const int of = (own ? b_own * c.lq : 0) + min(wave_row + in_row, n_rows - 1), ob = c.lq == 1 ? of : of / c.lq;
     const uint16_t* const qa = static_cast<const uint16_t*>(c.qa.ptr) + ob * c.qa.stride_b + (of - ob * c.lq) * c.qa.stride_l + head;
     const uint16_t* const qb = static_cast<const uint16_t*>(c.qb.ptr) + ob * c.qb.stride_b + (of - ob * c.lq) * c.qb.stride_l + i;
@@ -226,7 +248,7 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
       for (int db = 0; db < NDB; ++db) qb_in[db][j] = qb[r * c.qb.stride_r + 32 * db];
     }
   };
-  request_q(0, 0);
+  if constexpr (!F32) request_q(0, 0);
 
   // ---- keys of this part that a column sees: those below `mine`
   const int seen = keys_seen(c, b, row_in_b), mine = own ? seen : min(seen, c.prefix);
@@ -252,18 +274,19 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   const int n_tiles = (stop - begin + kBlocks * TPB - 1) / (kBlocks * TPB);
   const int row_end = stop * RK;  // rows from here on read as zeros
 
-  // ---- loads: wave w brings rows 16 (w & 1) .. + 15 of block w / 2 of a tile; a lane's chunk is the one that belongs where it lands
+  // ---- loads: wave w brings RPW rows of block w / WPB of a tile; a lane's chunk is the one that belongs where it lands
   typedef uint32_t Resource __attribute__((ext_vector_type(4)));
   const int64_t boff = PAGED ? 0 : b_own;
-  const uint16_t* const base[4] = {static_cast<const uint16_t*>(c.kb.ptr) + boff * c.kb.stride_b, static_cast<const uint16_t*>(c.vb.ptr) + boff * c.vb.stride_b,
-                                   static_cast<const uint16_t*>(c.ka.ptr) + boff * c.ka.stride_b + h0, static_cast<const uint16_t*>(c.va.ptr) + boff * c.va.stride_b + h0};
+  const T* const base[4] = {static_cast<const T*>(c.kb.ptr) + boff * c.kb.stride_b, static_cast<const T*>(c.vb.ptr) + boff * c.vb.stride_b,
+                            static_cast<const T*>(c.ka.ptr) + boff * c.ka.stride_b + h0, static_cast<const T*>(c.va.ptr) + boff * c.va.stride_b + h0};
   const int64_t page_stride[4] = {c.kb.stride_b, c.vb.stride_b, c.ka.stride_b, c.va.stride_b};
-  const int sr[4] = {2 * (int)c.kb.stride_r, 2 * (int)c.vb.stride_r, 2 * (int)c.ka.stride_r, 2 * (int)c.va.stride_r};
-  const int a_chunk = 16 * min(l & 3, plan.hb / 8 - 1), b_chunk = 16 * ((l % CPR) ^ BlockAt<D>::f(l / CPR));  // and of row n RPI + l / CPR: f differs by f(n RPI)
-  const int a_row = 16 * (w & 1) + (l >> 2), b_row = 16 * (w & 1) + l / CPR;
+  const int sr[4] = {kSize * (int)c.kb.stride_r, kSize * (int)c.vb.stride_r, kSize * (int)c.ka.stride_r, kSize * (int)c.va.stride_r};
+  constexpr int ACH = 32 / kPer;  // 16-byte chunks of a row of 32 heads
+  const int a_row = RPW * (w % WPB) + l / ACH, b_row = RPW * (w % WPB) + l / CPR;
+  const int a_chunk = 16 * min(l % ACH, plan.hb / kPer - 1), b_chunk = 16 * ((l % CPR) ^ At::f(b_row));  // and of row b_row + n RPI: f differs by f(n RPI)
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)mem;
   const int rpp = PAGED ? c.page_size * RK : 1;
-  auto block_row = [&](int tile) __attribute__((always_inline)) { return begin * RK + (tile * kBlocks + (w >> 1)) * kRows; };
+  auto block_row = [&](int tile) __attribute__((always_inline)) { return begin * RK + (tile * kBlocks + w / WPB) * kRows; };
   auto page_of = [&](int row0) __attribute__((always_inline)) { return p.page_shift >= 0 ? row0 >> p.page_shift : row0 / rpp; };
   auto lookup = [&](int tile) __attribute__((always_inline)) -> int {
     if constexpr (!PAGED) return 0;
@@ -280,82 +303,101 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
     const uint32_t to = lds0 + buffer * Lds::kBuffer;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const uintptr_t at = reinterpret_cast<uintptr_t>(base[x] + (PAGED ? (int64_t)page * page_stride[x] : 0) + first * (sr[x] / 2));
-      const int width = x < 2 ? 2 * D : 2 * plan.hb;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(base[x] + (PAGED ? (int64_t)page * page_stride[x] : 0) + first * (sr[x] / kSize));
+      const int width = kSize * (x < 2 ? D : plan.hb);
       const Resource rs = {(uint32_t)scalar((int)(uint32_t)at), (uint32_t)scalar((int)((uint32_t)(at >> 32) & 0xffff)), (uint32_t)scalar(rows > 0 ? (rows - 1) * sr[x] + width : 0),
                            (uint32_t)kRsrcFlags};
       if (x < 2) {
 #pragma unroll
         for (int n = 0; n < NI; ++n)
-          load((uint32_t)scalar(to + (x * kBlocks + (w >> 1)) * Lds::kB + (NI * (w & 1) + n) * 1024), (b_row + n * RPI - skip) * sr[x] + (b_chunk ^ (16 * BlockAt<D>::f(n * RPI))), rs);
+          load((uint32_t)scalar(to + (x * kBlocks + w / WPB) * Lds::kB + (NI * (w % WPB) + n) * 1024), (b_row + n * RPI - skip) * sr[x] + (b_chunk ^ (16 * At::f(n * RPI))), rs);
       } else {
-        load((uint32_t)scalar(to + 2 * kBlocks * Lds::kB + ((x - 2) * kBlocks + (w >> 1)) * Lds::kA + (w & 1) * 1024), (a_row - skip) * sr[x] + a_chunk, rs);
+        load((uint32_t)scalar(to + 2 * kBlocks * Lds::kB + ((x - 2) * kBlocks + w / WPB) * Lds::kA + (w % WPB) * 1024), (a_row - skip) * sr[x] + a_chunk, rs);
       }
     }
   };
   issue(0, 0, scalar(lookup(0)));
   int page_ahead = lookup(1);
 
-  // ---- Qm of this lane's column as the operand of its products, d = 16 ks + 8 g + 0..7, in two parts
-  bf16x8 q_hi[NKS], q_lo[NKS];
+  // ---- Qm of this lane's column as the operand of its products: in bf16 d = 16 ks + 8 g + 0..7, in two parts, in fp32 d = 8 m + 4 g + e
+  [[maybe_unused]] bf16x8 q_hi[NKS], q_lo[NKS];
+  [[maybe_unused]] float qf[D / 2];
   f32x16 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
-  for (int in_row = 0; in_row < rps; ++in_row)
-    for (int r0 = 0; r0 < c.rq; r0 += 16) {
-      if (in_row || r0) request_q(in_row, r0);
-      u32x4 a, x[NDB];
+  if constexpr (F32) {
+    const T* const qa = static_cast<const T*>(c.qa.ptr) + b * c.qa.stride_b + row_in_b * c.qa.stride_l + head;
+    const T* const qb = static_cast<const T*>(c.qb.ptr) + b * c.qb.stride_b + row_in_b * c.qb.stride_l + 4 * g;
+#pragma unroll
+    for (int x = 0; x < D / 2; ++x) qf[x] = 0.f;
+    for (int r = 0; r < c.rq; ++r) {
+      const float a = qa[r * c.qa.stride_r];
+#pragma unroll
+      for (int mm = 0; mm < D / 8; ++mm) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(qb + r * c.qb.stride_r + 8 * mm);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[4 * mm + e] = fmaf(a, x[e], qf[4 * mm + e]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < D / 2; ++x) qf[x] *= p.qscale;
+  } else {
+    for (int in_row = 0; in_row < rps; ++in_row)
+      for (int r0 = 0; r0 < c.rq; r0 += 16) {
+        if (in_row || r0) request_q(in_row, r0);
+        u32x4 a, x[NDB];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = r0 + 8 * g + 2 * j;
+          const uint32_t lo = r < c.rq ? 0xffffu : 0u, hi = r + 1 < c.rq ? 0xffff0000u : 0u;
+          a[j] = in_set == in_row ? (((uint32_t)qa_in[2 * j + 1] << 16 | qa_in[2 * j]) & (lo | hi)) : 0u;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) x[db][j] = ((uint32_t)qb_in[db][2 * j + 1] << 16 | qb_in[db][2 * j]) & (lo | hi);
+        }
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          f32x16 one;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) one[v] = 0.f;
+          one = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x[db]), __builtin_bit_cast(bf16x8, a), one, 0, 0, 0);
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[db][v] += in_set == in_row ? one[v] : 0.f;  // another row's infinities stay with it
+        }
+      }
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int r = r0 + 8 * g + 2 * j;
-        const uint32_t lo = r < c.rq ? 0xffffu : 0u, hi = r + 1 < c.rq ? 0xffff0000u : 0u;
-        a[j] = in_set == in_row ? (((uint32_t)qa_in[2 * j + 1] << 16 | qa_in[2 * j]) & (lo | hi)) : 0u;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) x[db][j] = ((uint32_t)qb_in[db][2 * j + 1] << 16 | qb_in[db][2 * j]) & (lo | hi);
+        const float q0 = o[ks / 2][8 * (ks & 1) + 2 * j] * p.qscale, q1 = o[ks / 2][8 * (ks & 1) + 2 * j + 1] * p.qscale;
+        hi[j] = pack_bf16(q0, q1);
+        lo[j] = pack_bf16(q0 - bf16lo_to_f32(hi[j]), q1 - bf16hi_to_f32(hi[j]));
       }
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        f32x16 one;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) one[v] = 0.f;
-        one = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x[db]), __builtin_bit_cast(bf16x8, a), one, 0, 0, 0);
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[db][v] += in_set == in_row ? one[v] : 0.f;  // another row's infinities stay with it
-      }
+      // a result column has d = 8 q + 4 g + e of its block: the halves exchange for the operand's order
+      auto order = [&](const uint32_t (&x)[4]) __attribute__((always_inline)) {
+        const auto even = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), odd = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+        return __builtin_bit_cast(bf16x8, u32x4{even[0], odd[0], even[1], odd[1]});
+      };
+      q_hi[ks] = order(hi);
+      q_lo[ks] = order(lo);
     }
-#pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float q0 = o[ks / 2][8 * (ks & 1) + 2 * j] * p.qscale, q1 = o[ks / 2][8 * (ks & 1) + 2 * j + 1] * p.qscale;
-      hi[j] = pack_bf16(q0, q1);
-      lo[j] = pack_bf16(q0 - bf16lo_to_f32(hi[j]), q1 - bf16hi_to_f32(hi[j]));
-    }
-    // a result column has d = 8 q + 4 g + e of its block: the halves exchange for the operand's order
-    auto order = [&](const uint32_t (&x)[4]) __attribute__((always_inline)) {
-      const auto even = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), odd = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
-      return __builtin_bit_cast(bf16x8, u32x4{even[0], odd[0], even[1], odd[1]});
-    };
-    q_hi[ks] = order(hi);
-    q_lo[ks] = order(lo);
   }
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   float m = -INFINITY, lsum = 0.f;
-  const BlockAt<D> at(l);
-  const int a_head = (16 * dhalf + 4 * (lp & 3)) % plan.hb;  // of the four columns whose a's this lane helps to transpose
+  const At at(l);
+  [[maybe_unused]] const int a_head = (16 * dhalf + 4 * (lp & 3)) % plan.hb;  // of the four columns whose a's this lane helps to transpose
   const int row_first = own ? c.prefix * RK : 0;
 
-  struct Block { const uint16_t *kb, *vb, *ka, *va; int row0; };
+  struct Block { const T *kb, *vb, *ka, *va; int row0; };
   auto block_of = [&](int tile, int blk) __attribute__((always_inline)) {
     const unsigned char* const buf = mem + (tile & 1) * Lds::kBuffer;
-    const uint16_t* const ka = reinterpret_cast<const uint16_t*>(buf + 2 * kBlocks * Lds::kB + blk * Lds::kA);
-    return Block{reinterpret_cast<const uint16_t*>(buf + blk * Lds::kB), reinterpret_cast<const uint16_t*>(buf + (kBlocks + blk) * Lds::kB), ka, ka + kBlocks * Lds::kA / 2,
+    const T* const ka = reinterpret_cast<const T*>(buf + 2 * kBlocks * Lds::kB + blk * Lds::kA);
+    return Block{reinterpret_cast<const T*>(buf + blk * Lds::kB), reinterpret_cast<const T*>(buf + (kBlocks + blk) * Lds::kB), ka, ka + kBlocks * Lds::kA / kSize,
                  begin * RK + (tile * kBlocks + blk) * kRows};
   };
   auto step = [&](const Block& x) __attribute__((always_inline)) {
@@ -363,22 +405,44 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
     f32x16 sp;
 #pragma unroll
     for (int v = 0; v < 16; ++v) sp[v] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      const bf16x8 kf = *reinterpret_cast<const bf16x8*>(x.kb + at.read(ks));
-      sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q_lo[ks], sp, 0, 0, 0);
-      sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q_hi[ks], sp, 0, 0, 0);
-    }
     float ak[16], av[16];
+    if constexpr (F32) {
+      f32x16 odd;  // a second chain of sums
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int a_at = (8 * q + 4 * g + (lp >> 2)) * 32 + a_head;
-      const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x.ka + a_at));
-      const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x.va + a_at));
+      for (int v = 0; v < 16; ++v) odd[v] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
-        av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
+      for (int mm = 0; mm < D / 8; ++mm) {
+        const f32x4 kf = *reinterpret_cast<const f32x4*>(x.kb + at.read(mm));
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          sp = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[4 * mm + e], sp, 0, 0, 0);
+          odd = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e + 1], qf[4 * mm + e + 1], odd, 0, 0, 0);
+        }
+      }
+      const int a_at = 4 * g * 32 + head - h0;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        sp[v] += odd[v];
+        ak[v] = x.ka[a_at + (8 * (v >> 2) + (v & 3)) * 32];
+        av[v] = x.va[a_at + (8 * (v >> 2) + (v & 3)) * 32];
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(x.kb + at.read(ks));
+        sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q_lo[ks], sp, 0, 0, 0);
+        sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q_hi[ks], sp, 0, 0, 0);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int a_at = (8 * q + 4 * g + (lp >> 2)) * 32 + a_head;
+        const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x.ka + a_at));
+        const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x.va + a_at));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
+          av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
+        }
       }
     }
     // logits per token (log2 domain); a token's rows are registers v0 .. v0 + NV - 1, at rank 8 in both halves of the wave
@@ -423,15 +487,25 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
 #pragma unroll
       for (int j = 0; j < NV; ++j) pp[t * NV + j] = pt * av[t * NV + j];
     }
-    // O^T[d, c] += sum_row vb[row, d] P'[row, c]; slot (g, j) = row 16 kk + 8 (j / 4) + 4 g + j % 4
+    // O^T[d, c] += sum_row vb[row, d] P'[row, c]; in bf16 slot (g, j) = row 16 kk + 8 (j / 4) + 4 g + j % 4
+    if constexpr (F32) {
+      typedef float Values __attribute__((ext_vector_type(NDB)));
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      u32x4 pk;
+      for (int v = 0; v < 16; ++v) {
+        const Values vf = *reinterpret_cast<const Values*>(x.vb + at.read_v(v));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(pp[8 * kk + 2 * j], pp[8 * kk + 2 * j + 1]);
+        for (int db = 0; db < NDB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[db], pp[v], o[db], 0, 0, 0);
+      }
+    } else {
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(block_tr<D>(x.vb, at, kk, db), __builtin_bit_cast(bf16x8, pk), o[db], 0, 0, 0);
+      for (int kk = 0; kk < 2; ++kk) {
+        u32x4 pk;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(pp[8 * kk + 2 * j], pp[8 * kk + 2 * j + 1]);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(block_tr<D>(x.vb, at, kk, db), __builtin_bit_cast(bf16x8, pk), o[db], 0, 0, 0);
+      }
     }
   };
 
@@ -478,21 +552,34 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   if (!works || kw || !stored) return;
   const int64_t to = (slot + row) * c.H + head;
 #pragma unroll
-  for (int x = 0; x < NDB * 4; ++x)
-    *reinterpret_cast<f32x4*>(p.part_o + to * D + 32 * (x / 4) + 8 * (x % 4) + 4 * g) = f32x4{o[x / 4][4 * (x % 4)], o[x / 4][4 * (x % 4) + 1], o[x / 4][4 * (x % 4) + 2], o[x / 4][4 * (x % 4) + 3]};
+  for (int x = 0; x < NDB * 4; ++x) {
+    f32x4 part;  // of four neighbouring d
+    int d;
+    if constexpr (F32) {
+      const int v = x * 4 / NDB;  // the first row of a block's
+      d = NDB * (8 * (v >> 2) + 4 * g + (v & 3));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[e] = o[e % NDB][v + e / NDB];
+    } else {
+      d = 32 * (x / 4) + 8 * (x % 4) + 4 * g;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[e] = o[x / 4][4 * (x % 4) + e];
+    }
+    *reinterpret_cast<f32x4*>(p.part_o + to * D + d) = part;
+  }
   if (g == 0) {
     p.part_m[to] = m;
     p.part_l[to] = lsum;
   }
 }
 
-template <int D, int RK, bool PAGED>
+template <typename T, int D, int RK, bool PAGED>
 __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaParams p) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_mem[];
   const bool own = (int)blockIdx.x >= p.plan.prefix.grid;
   const SharedPart& part = own ? p.plan.own : p.plan.prefix;
   const int id = (int)blockIdx.x - (own ? p.plan.prefix.grid : 0);
-  shared_part<D, RK, PAGED>(p, part, own, id, shared_mem);
+  shared_part<T, D, RK, PAGED>(p, part, own, id, shared_mem);
 }
 
 // Joins the ranges' parts: a wave per query row and head.  Its lanes take a range each for the weights; then groups of D / 4 lanes, 16
@@ -555,17 +642,18 @@ bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15)
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 bool mfma_takes(const TpaFwdArgs* a) {
-  if (a->dtype != TPA_DTYPE_BF16 || a->kernel == TPA_KERNEL_GENERIC) return false;
+  if (a->kernel == TPA_KERNEL_GENERIC) return false;
+  const int size = a->dtype == TPA_DTYPE_BF16 ? 2 : 4, per = 16 / size;
   if (a->dk != a->dv || (a->dk != 64 && a->dk != 128)) return false;
   if (a->rk != 1 && a->rk != 2 && a->rk != 4 && a->rk != 8) return false;
   if (a->H % 8) return false;
   // rows (token, rank) are uniformly strided and lie where 32-bit offsets reach; 16-byte loads
   const TpaFactor* fs[4] = {&a->ka, &a->kb, &a->va, &a->vb};
   for (const TpaFactor* f : fs) {
-    if (f->stride_l != (int64_t)a->rk * f->stride_r || f->stride_r < 0 || f->stride_r > kFarthestRow) return false;
-    if (!aligned16(f->ptr) || f->stride_r % 8 || f->stride_b % 8) return false;
+    if (f->stride_l != (int64_t)a->rk * f->stride_r || f->stride_r < 0 || f->stride_r > kFarthestRow / size) return false;
+    if (!aligned16(f->ptr) || f->stride_r % per || f->stride_b % per) return false;
   }
-  if (!aligned16(a->qb.ptr) || a->qb.stride_r % 8 || a->qb.stride_l % 8 || a->qb.stride_b % 8) return false;
+  if (!aligned16(a->qb.ptr) || a->qb.stride_r % per || a->qb.stride_l % per || a->qb.stride_b % per) return false;
   if (a->page_table && a->page_size * (int64_t)a->rk % kRows) return false;
   return (int64_t)a->lk * a->rk < (1 << 30);
 }
@@ -573,13 +661,15 @@ bool mfma_takes(const TpaFwdArgs* a) {
 // What the plan reckons with, ns: a block of a wave, at head size 128 and 64 (5.8 and 3.5 us for a tile of four by eight waves); a tile of a
 // sequence's own keys at head size 128, which memory brings; a workgroup's way to its first tile and behind its last one; a number of a
 // range's results, written and read again.
-constexpr double kBlockNs128 = 1450, kBlockNs64 = 875, kOwnTileNs = 3000, kFixedNs = 12000, kPartNs = 8. / 5e3;
+// In fp32 (kBlockF32Ns) the matrix cores are what a block takes, less by half where only one wave works on each.
+constexpr double kBlockNs128 = 1450, kBlockNs64 = 875, kOwnTileNs = 3000, kFixedNs = 12000, kPartNs = 8. / 5e3, kBlockF32Ns = 7000;
 SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   SharedPlan s{};
   s.hb = a->H % 32 == 0 ? 32 : a->H % 24 == 0 ? 24 : a->H % 16 == 0 ? 16 : 8;
   s.nhb = a->H / s.hb;
   s.rows = (int64_t)a->B * a->lq;
-  const int tpb = kRows / a->rk, tpt = tpb * kBlocks, rps = 32 / s.hb;
+  const bool bf16 = a->dtype == TPA_DTYPE_BF16;
+  const int blocks = blocks_of_tile(bf16 ? 2 : 4), tpb = kRows / a->rk, tpt = tpb * blocks, rps = 32 / s.hb;
   auto columns = [&](SharedPart& x, int64_t rows) {
     const int sets = ceil_div(rows, rps);
     x.waves = 1;
@@ -593,7 +683,11 @@ SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   // One workgroup is resident on a compute unit, so the launch lasts as long as the longest of 256, or longer by what more of them do.  Every
   // length of time up to that of one workgroup for all is tried for what the ranges would be; the shortest launch wins.
   const bool has_p = prefix > 0, has_s = prefix < a->lk;
-  auto tile_ns = [&](const SharedPart& x) { return (a->dk == 128 ? kBlockNs128 : kBlockNs64) * kBlocks / std::min(kWaves / x.waves, kBlocks); };
+  auto tile_ns = [&](const SharedPart& x) {
+    const int side = std::min(kWaves / x.waves, blocks);  // waves that share a set's blocks
+    if (!bf16) return kBlockF32Ns * a->dk / 128 * blocks / side * std::max(.5, side * x.waves / (double)kWaves);
+    return (a->dk == 128 ? kBlockNs128 : kBlockNs64) * blocks / side;
+  };
   const double tile_p = tile_ns(s.prefix), tile_s = std::max(tile_ns(s.own), kOwnTileNs * a->dk / 128);
   // (not those that would make several rounds of workgroups, and none far behind the best)
   const double all_ns = (double)all_p * share_p * tile_p * has_p + (double)all_s * share_s * a->B * tile_s * has_s;
@@ -620,27 +714,28 @@ SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
 int ranges_of(const SharedPlan& s) { return s.prefix.ranges + s.own.ranges; }
 size_t plan_bytes(const SharedPlan& s, int H, int D) { return (size_t)ranges_of(s) * s.rows * H * (D + 2) * sizeof(float); }
 
-template <int D, int RK, bool PAGED>
+template <typename T, int D, int RK, bool PAGED>
 int launch_mfma_t(const SharedMfmaParams& p, hipStream_t s) {
-  auto kern = shared_mfma_kernel<D, RK, PAGED>;
+  auto kern = shared_mfma_kernel<T, D, RK, PAGED>;
+  constexpr size_t bytes = SharedLds<T, D>::kBytes;
   static bool done[kMaxDevices] = {};
-  if (const int rc = raise_lds_limit(done, reinterpret_cast<const void*>(kern), SharedLds<D>::kBytes); rc != TPA_OK) return rc;
-  hipLaunchKernelGGL(kern, dim3(p.plan.prefix.grid + p.plan.own.grid), dim3(kWaves * 64), SharedLds<D>::kBytes, s, p);
+  if (const int rc = raise_lds_limit(done, reinterpret_cast<const void*>(kern), bytes); rc != TPA_OK) return rc;
+  hipLaunchKernelGGL(kern, dim3(p.plan.prefix.grid + p.plan.own.grid), dim3(kWaves * 64), bytes, s, p);
   if (hipGetLastError() != hipSuccess) return TPA_ERR_LAUNCH;
-  hipLaunchKernelGGL((shared_merge_kernel<uint16_t, D>), dim3(ceil_div(p.plan.rows * p.c.H, 4)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((shared_merge_kernel<T, D>), dim3(ceil_div(p.plan.rows * p.c.H, 4)), dim3(256), 0, s, p);
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
-template <int D, int RK>
+template <typename T, int D, int RK>
 int launch_mfma_p(const SharedMfmaParams& p, hipStream_t s) {
-  return p.c.page_table ? launch_mfma_t<D, RK, true>(p, s) : launch_mfma_t<D, RK, false>(p, s);
+  return p.c.page_table ? launch_mfma_t<T, D, RK, true>(p, s) : launch_mfma_t<T, D, RK, false>(p, s);
 }
-template <int D>
+template <typename T, int D>
 int launch_mfma(const SharedMfmaParams& p, hipStream_t s) {
   switch (p.c.rk) {
-    case 1: return launch_mfma_p<D, 1>(p, s);
-    case 2: return launch_mfma_p<D, 2>(p, s);
-    case 4: return launch_mfma_p<D, 4>(p, s);
-    default: return launch_mfma_p<D, 8>(p, s);
+    case 1: return launch_mfma_p<T, D, 1>(p, s);
+    case 2: return launch_mfma_p<T, D, 2>(p, s);
+    case 4: return launch_mfma_p<T, D, 4>(p, s);
+    default: return launch_mfma_p<T, D, 8>(p, s);
   }
 }
 
@@ -697,7 +792,8 @@ extern "C" int tpa_decode_shared(const TpaFwdArgs* a, int32_t prefix, void* stre
       const int rows = a->page_size * a->rk;
       if (!(rows & (rows - 1))) m.page_shift = __builtin_ctz(rows);
     }
-    return a->dk == 128 ? launch_mfma<128>(m, s) : launch_mfma<64>(m, s);
+    if (a->dtype == TPA_DTYPE_BF16) return a->dk == 128 ? launch_mfma<uint16_t, 128>(m, s) : launch_mfma<uint16_t, 64>(m, s);
+    return a->dk == 128 ? launch_mfma<float, 128>(m, s) : launch_mfma<float, 64>(m, s);
   }
   if (a->kernel == TPA_KERNEL_MFMA) return TPA_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)(a->B * a->lq * a->H));
