@@ -140,17 +140,17 @@ struct SharedLds {
   static constexpr int kBlocks = blocks_of_tile(sizeof(T));
   static constexpr int kB = kRows * D * sizeof(T), kA = kRows * 32 * sizeof(T);  // bytes of a block's b rows, a rows (32 heads)
   static constexpr int kBuffer = kBlocks * 2 * (kB + kA);                     // kb, vb, ka, va of a tile
-  static constexpr int kPart = 32 * D * 4 + 2 * 64 * 4;                       // a wave's sums of a set of columns on their way to another
+  static constexpr int kPart = 32 * D * 4 + 2 * 64 * 4;                       // a wave's sums of a set of columns on their way to others
   static constexpr size_t kBytes = 2 * kBuffer;
-  static_assert(4 * kPart <= 2 * kBuffer, "the sums that four waves hand over at a time fit the buffers");
+  static_assert(kWaves * kPart <= 2 * kBuffer, "what all waves hand over fits the buffers");
 };
 
 // Columns come in sets of 32: the heads of a block of heads (8, 16, 24 or 32) for as many query rows as fit, so that all sets have the same head
 // factors.
 struct SharedPart {        // the prefix, or the sequences' own keys
-  int waves;               // waves side by side over the columns
+  int waves, side;         // waves side by side over the columns, waves that share the blocks of each
   int groups;              // workgroups for all columns of a block of heads
-  int ranges, tiles;       // key ranges, tiles of a range
+  int ranges, blocks;      // key ranges, blocks of a range
   int grid;                // workgroups
 };
 struct SharedPlan {
@@ -225,7 +225,7 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   if (unit >= (own ? c.B * part.ranges : part.ranges)) return;
   const int b_own = own ? unit / part.ranges : 0, range = own ? unit - b_own * part.ranges : unit;
   const int h0 = member % plan.nhb * plan.hb, rps = 32 / plan.hb;  // rows of a set
-  const int cwaves = part.waves, kwaves = min(kWaves / cwaves, kBlocks), cw = w % cwaves, kw = w / cwaves;
+  const int cwaves = part.waves, kwaves = part.side, cw = w % cwaves, kw = w / cwaves;
   const int n_rows = own ? c.lq : (int)plan.rows, wave_row = (member / plan.nhb * cwaves + cw) * rps;  // this wave's first row
   const bool works = kw < kwaves && wave_row < n_rows;
   const int in_set = min(i / plan.hb, rps - 1), head = h0 + i % plan.hb;  // lanes behind the last whole row of a set repeat it
@@ -233,39 +233,45 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   const int row = (own ? b_own * c.lq : 0) + min(wave_row + in_set, n_rows - 1);  // this lane's query row among all
   const int b = c.lq == 1 ? row : row / c.lq, row_in_b = row - b * c.lq;
 
-  // ---- Qm^T[d, c] = sum_r qb[r, d] qa[r, c] by the matrix cores in bf16, 16 ranks a time, a set's rows one after the other with the other rows' columns
-  // zero: asked for here, finished while the first tile is on its way
-  [[maybe_unused]] uint16_t qa_in[8], qb_in[NDB][8];
-  [[maybe_unused]] auto request_q = [&](int in_row, int r0) __attribute__((always_inline)) {
-    const int of = (own ? b_own * c.lq : 0) + min(wave_row + in_row, n_rows - 1), ob = c.lq == 1 ? of : of / c.lq;
-    const uint16_t* const qa = static_cast<const uint16_t*>(c.qa.ptr) + ob * c.qa.stride_b + (of - ob * c.lq) * c.qa.stride_l + head;
-    const uint16_t* const qb = static_cast<const uint16_t*>(c.qb.ptr) + ob * c.qb.stride_b + (of - ob * c.lq) * c.qb.stride_l + i;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int r = min(r0 + 8 * g + j, c.rq - 1);
-      qa_in[j] = qa[r * c.qa.stride_r];
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) qb_in[db][j] = qb[r * c.qb.stride_r + 32 * db];
-    }
+  // ---- keys of this part that a column sees: those below `mine`; the workgroup's range ends with the last that any of them sees
+  auto keys_of = [&](int of) __attribute__((always_inline)) {  // row `of` of this part's
+    const int all = (own ? b_own * c.lq : 0) + min(of, n_rows - 1), entry = c.lq == 1 ? all : all / c.lq, seen = keys_seen(c, entry, all - entry * c.lq);
+    return own ? seen : min(seen, c.prefix);
   };
-  if constexpr (!F32) request_q(0, 0);
-
-  // ---- keys of this part that a column sees: those below `mine`
-  const int seen = keys_seen(c, b, row_in_b), mine = own ? seen : min(seen, c.prefix);
-  const int most = scalar(wave_max(mine)), least = scalar(wave_min(mine));
-  int* const red = reinterpret_cast<int*>(mem);
-  if (l == 0) red[w] = most;
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  int end = 0;
-#pragma unroll
-  for (int x = 0; x < kWaves; ++x) end = max(end, red[x]);
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  end = scalar(end);
-
+  const int mine = keys_of(wave_row + in_set), theirs = keys_of(member / plan.nhb * cwaves * rps + min(l, cwaves * rps - 1));
   // ---- the range's rows (token, rank), in blocks from a block's border on
   const int origin = own ? c.prefix / TPB * TPB : 0;
-  const int begin = origin + range * part.tiles * kBlocks * TPB;
-  const int stop = min(end, begin + part.tiles * kBlocks * TPB);
+  const int begin = origin + range * part.blocks * TPB;
+  const int rpp = PAGED ? c.page_size * RK : 1;
+  auto block_row = [&](int tile) __attribute__((always_inline)) { return begin * RK + (tile * kBlocks + w / WPB) * kRows; };
+  auto page_of = [&](int row0) __attribute__((always_inline)) { return p.page_shift >= 0 ? row0 >> p.page_shift : row0 / rpp; };
+  auto lookup = [&](int tile, int rows) __attribute__((always_inline)) -> int {  // of a cache of so many rows
+    if constexpr (!PAGED) return 0;
+    return c.page_table[(int64_t)b_own * c.pages_per_seq + page_of(min(block_row(tile), rows - 1) / kRows * kRows)];
+  };
+  const int first_page = lookup(0, c.lk * RK);  // asked for before it is known whether there are keys
+
+  // ---- Qm^T[d, c] = sum_r qb[r, d] qa[r, c] by the matrix cores in bf16, 16 ranks a step, a set's rows one after the other with the other rows'
+  // columns zero; qb's rows go by LDS (the second buffer, a part for each wave), which transposes them.  Asked for here, two steps in flight, finished while
+  // the first tile is on its way.
+  constexpr int QRPI = F32 ? 1 : 64 / (D / 8), QL = 16 / QRPI;  // rows of a load instruction, loads of 16 rows
+  struct QIn { uint16_t a[8]; u32x4 b[QL]; };
+  [[maybe_unused]] QIn q_in[2];
+  const int q_chunks = (c.rq + 15) / 16, q_steps = rps * q_chunks;
+  [[maybe_unused]] auto request_q = [&](QIn& in, int n) __attribute__((always_inline)) {
+    const int in_row = n / q_chunks, r0 = n % q_chunks * 16;
+    const int of = (own ? b_own * c.lq : 0) + min(wave_row + in_row, n_rows - 1), ob = c.lq == 1 ? of : of / c.lq;
+    const uint16_t* const qa = static_cast<const uint16_t*>(c.qa.ptr) + ob * c.qa.stride_b + (of - ob * c.lq) * c.qa.stride_l + head;
+    const uint16_t* const qb = static_cast<const uint16_t*>(c.qb.ptr) + ob * c.qb.stride_b + (of - ob * c.lq) * c.qb.stride_l + 8 * (l % (D / 8));
+#pragma unroll
+    for (int x = 0; x < QL; ++x) in.b[x] = *reinterpret_cast<const u32x4*>(qb + min(r0 + x * QRPI + l / (D / 8), c.rq - 1) * c.qb.stride_r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) in.a[j] = qa[min(r0 + 8 * (j / 4) + 4 * g + j % 4, c.rq - 1) * c.qa.stride_r];
+  };
+  if constexpr (!F32) request_q(q_in[0], 0);  // (in no branch, behind which the keys would be waited for together with it)
+
+  const int least = scalar(wave_min(mine)), end = scalar(wave_max(theirs));
+  const int stop = min(end, begin + part.blocks * TPB);
   const int64_t slot = ((own ? plan.prefix.ranges : 0) + range) * plan.rows;
   if (stop <= begin || stop <= (own ? c.prefix : 0)) {  // no key of this range is seen
     if (works && kw == 0 && g == 0 && stored) p.part_m[(slot + row) * c.H + head] = -INFINITY;
@@ -285,13 +291,6 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   const int a_row = RPW * (w % WPB) + l / ACH, b_row = RPW * (w % WPB) + l / CPR;
   const int a_chunk = 16 * min(l % ACH, plan.hb / kPer - 1), b_chunk = 16 * ((l % CPR) ^ At::f(b_row));  // and of row b_row + n RPI: f differs by f(n RPI)
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)mem;
-  const int rpp = PAGED ? c.page_size * RK : 1;
-  auto block_row = [&](int tile) __attribute__((always_inline)) { return begin * RK + (tile * kBlocks + w / WPB) * kRows; };
-  auto page_of = [&](int row0) __attribute__((always_inline)) { return p.page_shift >= 0 ? row0 >> p.page_shift : row0 / rpp; };
-  auto lookup = [&](int tile) __attribute__((always_inline)) -> int {
-    if constexpr (!PAGED) return 0;
-    return c.page_table[(int64_t)b_own * c.pages_per_seq + page_of(min(block_row(tile), row_end - 1) / kRows * kRows)];
-  };
   auto load = [&](uint32_t to, int at, const Resource& rs) __attribute__((always_inline)) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(rs) : "memory");
   };
@@ -316,8 +315,8 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
       }
     }
   };
-  issue(0, 0, scalar(lookup(0)));
-  int page_ahead = lookup(1);
+  issue(0, 0, block_row(0) < row_end ? scalar(first_page) : 0);
+  int page_ahead = lookup(1, row_end);
 
   // ---- Qm of this lane's column as the operand of its products: in bf16 d = 16 ks + 8 g + 0..7, in two parts, in fp32 d = 8 m + 4 g + e
   [[maybe_unused]] bf16x8 q_hi[NKS], q_lo[NKS];
@@ -328,60 +327,81 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   if constexpr (F32) {
-    const T* const qa = static_cast<const T*>(c.qa.ptr) + b * c.qa.stride_b + row_in_b * c.qa.stride_l + head;
-    const T* const qb = static_cast<const T*>(c.qb.ptr) + b * c.qb.stride_b + row_in_b * c.qb.stride_l + 4 * g;
+    if (works) {
+      const T* const qa = static_cast<const T*>(c.qa.ptr) + b * c.qa.stride_b + row_in_b * c.qa.stride_l + head;
+      const T* const qb = static_cast<const T*>(c.qb.ptr) + b * c.qb.stride_b + row_in_b * c.qb.stride_l + 4 * g;
 #pragma unroll
-    for (int x = 0; x < D / 2; ++x) qf[x] = 0.f;
-    for (int r = 0; r < c.rq; ++r) {
-      const float a = qa[r * c.qa.stride_r];
+      for (int x = 0; x < D / 2; ++x) qf[x] = 0.f;
+      for (int r = 0; r < c.rq; ++r) {
+        const float a = qa[r * c.qa.stride_r];
 #pragma unroll
-      for (int mm = 0; mm < D / 8; ++mm) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(qb + r * c.qb.stride_r + 8 * mm);
+        for (int mm = 0; mm < D / 8; ++mm) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(qb + r * c.qb.stride_r + 8 * mm);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) qf[4 * mm + e] = fmaf(a, x[e], qf[4 * mm + e]);
+          for (int e = 0; e < 4; ++e) qf[4 * mm + e] = fmaf(a, x[e], qf[4 * mm + e]);
+        }
       }
+#pragma unroll
+      for (int x = 0; x < D / 2; ++x) qf[x] *= p.qscale;
     }
-#pragma unroll
-    for (int x = 0; x < D / 2; ++x) qf[x] *= p.qscale;
   } else {
-    for (int in_row = 0; in_row < rps; ++in_row)
-      for (int r0 = 0; r0 < c.rq; r0 += 16) {
-        if (in_row || r0) request_q(in_row, r0);
-        u32x4 a, x[NDB];
+    const BlockAt<uint16_t, D> q_at(l);
+    uint16_t* const rows_at = reinterpret_cast<uint16_t*>(mem + Lds::kBuffer + w * (16 * D * 2));
+    f32x16 sum[NDB];
+    auto use_q = [&](const QIn& in, int n) __attribute__((always_inline)) {
+      const int in_row = n / q_chunks, r0 = n % q_chunks * 16;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = r0 + 8 * g + 2 * j;
-          const uint32_t lo = r < c.rq ? 0xffffu : 0u, hi = r + 1 < c.rq ? 0xffff0000u : 0u;
-          a[j] = in_set == in_row ? (((uint32_t)qa_in[2 * j + 1] << 16 | qa_in[2 * j]) & (lo | hi)) : 0u;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) x[db][j] = ((uint32_t)qb_in[db][2 * j + 1] << 16 | qb_in[db][2 * j]) & (lo | hi);
-        }
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          f32x16 one;
-#pragma unroll
-          for (int v = 0; v < 16; ++v) one[v] = 0.f;
-          one = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x[db]), __builtin_bit_cast(bf16x8, a), one, 0, 0, 0);
-#pragma unroll
-          for (int v = 0; v < 16; ++v) o[db][v] += in_set == in_row ? one[v] : 0.f;  // another row's infinities stay with it
-        }
+      for (int x = 0; x < QL; ++x) {
+        const int r = x * QRPI + l / (D / 8);
+        *reinterpret_cast<u32x4*>(rows_at + r * D + 8 * (l % (D / 8) ^ BlockAt<uint16_t, D>::f(r))) = r0 + r < c.rq ? in.b[x] : u32x4{0, 0, 0, 0};
       }
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      uint32_t hi[4], lo[4];
+      u32x4 a;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float q0 = o[ks / 2][8 * (ks & 1) + 2 * j] * p.qscale, q1 = o[ks / 2][8 * (ks & 1) + 2 * j + 1] * p.qscale;
-        hi[j] = pack_bf16(q0, q1);
-        lo[j] = pack_bf16(q0 - bf16lo_to_f32(hi[j]), q1 - bf16hi_to_f32(hi[j]));
+        const int r = r0 + 8 * (j / 2) + 4 * g + 2 * j % 4;
+        const uint32_t lo = r < c.rq ? 0xffffu : 0u, hi = r + 1 < c.rq ? 0xffff0000u : 0u;
+        a[j] = in_set == in_row ? (((uint32_t)in.a[2 * j + 1] << 16 | in.a[2 * j]) & (lo | hi)) : 0u;
       }
-      // a result column has d = 8 q + 4 g + e of its block: the halves exchange for the operand's order
-      auto order = [&](const uint32_t (&x)[4]) __attribute__((always_inline)) {
-        const auto even = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), odd = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
-        return __builtin_bit_cast(bf16x8, u32x4{even[0], odd[0], even[1], odd[1]});
-      };
-      q_hi[ks] = order(hi);
-      q_lo[ks] = order(lo);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (r0 == 0)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sum[db][v] = 0.f;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) sum[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(block_tr<D>(rows_at, q_at, 0, db), __builtin_bit_cast(bf16x8, a), sum[db], 0, 0, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (r0 + 16 >= c.rq)  // the row's own columns: another row's infinities stay with it
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[db][v] = in_set == in_row ? sum[db][v] : o[db][v];
+    };
+    if (works) {
+      if (q_steps > 1) request_q(q_in[1], 1);
+      for (int n = 0; n < q_steps; n += 2) {
+        use_q(q_in[0], n);
+        if (n + 2 < q_steps) request_q(q_in[0], n + 2);
+        if (n + 1 < q_steps) use_q(q_in[1], n + 1);
+        if (n + 3 < q_steps) request_q(q_in[1], n + 3);
+      }
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float q0 = o[ks / 2][8 * (ks & 1) + 2 * j] * p.qscale, q1 = o[ks / 2][8 * (ks & 1) + 2 * j + 1] * p.qscale;
+          hi[j] = pack_bf16(q0, q1);
+          lo[j] = pack_bf16(q0 - bf16lo_to_f32(hi[j]), q1 - bf16hi_to_f32(hi[j]));
+        }
+        // a result column has d = 8 q + 4 g + e of its block: the halves exchange for the operand's order
+        auto order = [&](const uint32_t (&x)[4]) __attribute__((always_inline)) {
+          const auto even = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), odd = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+          return __builtin_bit_cast(bf16x8, u32x4{even[0], odd[0], even[1], odd[1]});
+        };
+        q_hi[ks] = order(hi);
+        q_lo[ks] = order(lo);
+      }
     }
   }
 #pragma unroll
@@ -514,7 +534,7 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (t + 1 < n_tiles) {
       issue(t + 1, (t + 1) & 1, scalar(page_ahead));
-      page_ahead = lookup(t + 2);
+      page_ahead = lookup(t + 2, row_end);
     }
     if (works)
       for (int blk = kw; blk < kBlocks; blk += kwaves) {
@@ -523,49 +543,61 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
       }
   }
 
-  // ---- the waves that shared the blocks are joined, half of them handing their sums to the other half at a time
-  lsum = halves_sum(lsum);
-  for (int half = kwaves / 2; half; half /= 2) {
-    float* const part = reinterpret_cast<float*>(mem + (cw + cwaves * (kw % half)) * Lds::kPart);
-    __syncthreads();  // the tiles, or what was handed over before, have been read
-    if (works && kw >= half && kw < 2 * half) {
+  // ---- results: in pieces of four neighbouring d, 16 bytes a lane
+  constexpr int NP = NDB * 4;
+  auto piece = [&](int x) __attribute__((always_inline)) {
+    f32x4 y;
 #pragma unroll
-      for (int x = 0; x < NDB * 4; ++x)
-        *reinterpret_cast<f32x4*>(part + 256 * x + 4 * l) = f32x4{o[x / 4][4 * (x % 4)], o[x / 4][4 * (x % 4) + 1], o[x / 4][4 * (x % 4) + 2], o[x / 4][4 * (x % 4) + 3]};
-      part[32 * D + l] = m;
-      part[32 * D + 64 + l] = lsum;
+    for (int e = 0; e < 4; ++e) y[e] = F32 ? o[e % NDB][x * 4 / NDB + e / NDB] : o[x / 4][4 * (x % 4) + e];
+    return y;
+  };
+  const int64_t to = (slot + row) * c.H + head;
+  // (not for this XCD's cache, where a kernel's end would have to wait for its way out: 64 sequences over 8192 tokens 51.7 -> @NT us)
+  auto store = [&](int x, const f32x4& y) __attribute__((always_inline)) {
+    const int v = x * 4 / NDB, d = F32 ? NDB * (8 * (v >> 2) + 4 * g + (v & 3)) : 32 * (x / 4) + 8 * (x % 4) + 4 * g;
+    __builtin_nontemporal_store(y, reinterpret_cast<f32x4*>(p.part_o + to * D + d));
+  };
+  lsum = halves_sum(lsum);
+  if (kwaves == 1) {
+    if (!works || !stored) return;
+#pragma unroll
+    for (int x = 0; x < NP; ++x) store(x, piece(x));
+  } else {  // the waves that shared the blocks are joined: each puts all it has into LDS and adds up its share of the pieces
+    float* const parts = reinterpret_cast<float*>(mem + cw * Lds::kPart);
+    const int next = cwaves * Lds::kPart / 4;
+    __syncthreads();  // the tiles have been read
+    if (works) {
+      float* const mine_of = parts + kw * next;
+#pragma unroll
+      for (int x = 0; x < NP; ++x) *reinterpret_cast<f32x4*>(mine_of + 256 * x + 4 * l) = piece(x);
+      mine_of[32 * D + l] = m;
+      mine_of[32 * D + 64 + l] = lsum;
     }
     __syncthreads();
-    if (works && kw < half) {
-      const float m2 = part[32 * D + l], m_new = fmaxf(m, m2), m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float f1 = __builtin_amdgcn_exp2f(m - m_use), f2 = __builtin_amdgcn_exp2f(m2 - m_use);
-      lsum = lsum * f1 + part[32 * D + 64 + l] * f2;
-      m = m_new;
+    if (!works || !stored) return;
+    float weight[kBlocks];
+    m = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < NDB * 4; ++x) {
-        const f32x4 other = *reinterpret_cast<const f32x4*>(part + 256 * x + 4 * l);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[x / 4][4 * (x % 4) + e] = o[x / 4][4 * (x % 4) + e] * f1 + other[e] * f2;
-      }
+    for (int k = 0; k < kBlocks; ++k) {
+      weight[k] = k < kwaves ? parts[k * next + 32 * D + l] : -INFINITY;
+      m = fmaxf(m, weight[k]);
     }
-  }
-  if (!works || kw || !stored) return;
-  const int64_t to = (slot + row) * c.H + head;
+    const float base_m = m == -INFINITY ? 0.f : m;
+    lsum = 0.f;
 #pragma unroll
-  for (int x = 0; x < NDB * 4; ++x) {
-    f32x4 part;  // of four neighbouring d
-    int d;
-    if constexpr (F32) {
-      const int v = x * 4 / NDB;  // the first row of a block's
-      d = NDB * (8 * (v >> 2) + 4 * g + (v & 3));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part[e] = o[e % NDB][v + e / NDB];
-    } else {
-      d = 32 * (x / 4) + 8 * (x % 4) + 4 * g;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part[e] = o[x / 4][4 * (x % 4) + e];
+    for (int k = 0; k < kBlocks; ++k) {
+      weight[k] = __builtin_amdgcn_exp2f(weight[k] - base_m);
+      if (k < kwaves) lsum += weight[k] * parts[k * next + 32 * D + 64 + l];
     }
-    *reinterpret_cast<f32x4*>(p.part_o + to * D + d) = part;
+#pragma unroll 2
+    for (int x = kw * (NP / kwaves); x < (kw + 1) * (NP / kwaves); ++x) {
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k)
+        if (k < kwaves) sum += weight[k] * *reinterpret_cast<const f32x4*>(parts + k * next + 256 * x + 4 * l);
+      store(x, sum);
+    }
+    if (kw) return;
   }
   if (g == 0) {
     p.part_m[to] = m;
@@ -582,19 +614,28 @@ __global__ __launch_bounds__(kWaves * 64, 2) void shared_mfma_kernel(SharedMfmaP
   shared_part<T, D, RK, PAGED>(p, part, own, id, shared_mem);
 }
 
-// Joins the ranges' parts: a wave per query row and head.  Its lanes take a range each for the weights; then groups of D / 4 lanes, 16
+// Joins the ranges' parts: W waves per query row and head.  A wave's lanes take a range each for the weights; then groups of D / 4 lanes, 16
 // bytes a lane, walk the ranges side by side with several loads on their way, and are added up.
-template <typename T, int D>
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMfmaParams p) {
-  constexpr int TPR = D / 4, GROUPS = 64 / TPR, AHEAD = 4;
+  constexpr int TPR = D / 4, GROUPS = 64 / TPR * W, AHEAD = 8;
+  __shared__ f32x4 from_wave[W == 1 ? 1 : W - 1][TPR];
   const SharedParams& c = p.c;
-  const int lane = threadIdx.x & 63, grp = lane / TPR, d = 4 * (lane % TPR), ranges = p.plan.prefix.ranges + p.plan.own.ranges;
-  const int64_t n = p.plan.rows * c.H, at = (int64_t)blockIdx.x * 4 + scalar(threadIdx.x >> 6);
+  const int w = scalar(threadIdx.x >> 6), lane = threadIdx.x & 63, grp = lane / TPR + (W == 1 ? 0 : w * (64 / TPR)), d = 4 * (lane % TPR);
+  const int ranges = p.plan.prefix.ranges + p.plan.own.ranges;
+  const int64_t n = p.plan.rows * c.H, at = W == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
   if (at >= n) return;
   float most = -INFINITY, total = 0.f;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f}, part[AHEAD];
+  auto request = [&](int first, int count) __attribute__((always_inline)) {  // ranges first .. first + count - 1
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (u * GROUPS < count) part[u] = *reinterpret_cast<const f32x4*>(p.part_o + ((first + min(u * GROUPS + grp, count - 1)) * n + at) * D + d);
+  };
   for (int x0 = 0; x0 < ranges; x0 += 64) {
     const bool there = x0 + lane < ranges;
+    const int count = min(64, ranges - x0);
+    request(x0, min(count, GROUPS * AHEAD));  // beside the maxima; a range without keys has left here what was there
     const float m = there ? p.part_m[(x0 + lane) * n + at] : -INFINITY, l = there ? p.part_l[(x0 + lane) * n + at] : 0.f;
     float m_new = m;
 #pragma unroll
@@ -605,11 +646,8 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMfmaParams p) {
     total = total * keep + (m == -INFINITY ? 0.f : f * l);  // a range without keys has written nothing but its maximum
     sum *= keep;
     most = m_new;
-    const int count = min(64, ranges - x0);
     for (int x = 0; x < count; x += GROUPS * AHEAD) {
-      f32x4 part[AHEAD];
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) part[u] = *reinterpret_cast<const f32x4*>(p.part_o + ((x0 + min(x + u * GROUPS + grp, count - 1)) * n + at) * D + d);
+      if (x) request(x0 + x, min(count - x, GROUPS * AHEAD));
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int mine = x + u * GROUPS + grp;
@@ -624,10 +662,17 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMfmaParams p) {
   for (int s = 32; s >= TPR; s >>= 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], s);
+  if constexpr (W > 1) {
+    if (w && lane < TPR) from_wave[w - 1][lane] = sum;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int x = 0; x < W - 1; ++x) sum += from_wave[x][lane % TPR];
+  }
   const bool empty = most == -INFINITY;
   const float inv = empty ? NAN : 1.f / (total * c.rk);
   T* const out = static_cast<T*>(c.o) + at * D + d;
-  if (grp == 0) {
+  if (lane < TPR) {
     if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv)};
     else *reinterpret_cast<f32x4*>(out) = f32x4{sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
   }
@@ -637,6 +682,9 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMfmaParams p) {
     c.lse[((int64_t)b * c.H + h) * c.lq + (row - (int64_t)b * c.lq)] = empty ? -INFINITY : (most + __log2f(total)) * kLn2;
   }
 }
+
+// Below so many rows and heads four waves share one (the chip has 1024 SIMDs; us of the merge with one / four: @MW)
+constexpr int64_t kMergeWaves = 1024;
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -658,18 +706,19 @@ bool mfma_takes(const TpaFwdArgs* a) {
   return (int64_t)a->lk * a->rk < (1 << 30);
 }
 
-// What the plan reckons with, ns: a block of a wave, at head size 128 and 64 (5.8 and 3.5 us for a tile of four by eight waves); a tile of a
-// sequence's own keys at head size 128, which memory brings; a workgroup's way to its first tile and behind its last one; a number of a
-// range's results, written and read again.
-// In fp32 (kBlockF32Ns) the matrix cores are what a block takes, less by half where only one wave works on each.
-constexpr double kBlockNs128 = 1450, kBlockNs64 = 875, kOwnTileNs = 3000, kFixedNs = 12000, kPartNs = 8. / 5e3, kBlockF32Ns = 7000;
+// What the plan reckons with, ns.  In bf16 the columns' waves take kBlockNs for a block at head size 128 and 64 (5.8 and 3.5 us for a tile of four by
+// eight waves), or kOwnTileNs for a tile of a sequence's own keys, which memory brings; in fp32 the matrix cores decide (kBlockF32Ns).  Half the
+// waves or fewer have the unit to themselves and are faster (kFewWaves).  Data of a first tile arrives at kLandNs for a KiB: what a compute unit
+// gets by itself.  A workgroup's way to its first load and behind its last block; a number of a range's results, written and read again;
+// a range's turn in the merge.
+constexpr double kBlockNs128 = 1450, kBlockNs64 = 875, kOwnTileNs = 3000, kBlockF32Ns = 7000, kFewWaves = .7, kLandNs = 45, kFixedNs = 7500, kPartNs = 8. / 5e3, kMergeNs = 30;
 SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   SharedPlan s{};
   s.hb = a->H % 32 == 0 ? 32 : a->H % 24 == 0 ? 24 : a->H % 16 == 0 ? 16 : 8;
   s.nhb = a->H / s.hb;
   s.rows = (int64_t)a->B * a->lq;
   const bool bf16 = a->dtype == TPA_DTYPE_BF16;
-  const int blocks = blocks_of_tile(bf16 ? 2 : 4), tpb = kRows / a->rk, tpt = tpb * blocks, rps = 32 / s.hb;
+  const int in_tile = blocks_of_tile(bf16 ? 2 : 4), tpb = kRows / a->rk, rps = 32 / s.hb;
   auto columns = [&](SharedPart& x, int64_t rows) {
     const int sets = ceil_div(rows, rps);
     x.waves = 1;
@@ -678,35 +727,49 @@ SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   };
   columns(s.prefix, s.rows);
   columns(s.own, a->lq);
-  const int all_p = ceil_div(prefix, tpt), all_s = ceil_div(a->lk - prefix / tpb * tpb, tpt);
+  const int all_p = ceil_div(prefix, tpb), all_s = ceil_div(a->lk - prefix / tpb * tpb, tpb);
   const int share_p = s.nhb * s.prefix.groups, share_s = s.nhb * s.own.groups;
-  // One workgroup is resident on a compute unit, so the launch lasts as long as the longest of 256, or longer by what more of them do.  Every
-  // length of time up to that of one workgroup for all is tried for what the ranges would be; the shortest launch wins.
-  const bool has_p = prefix > 0, has_s = prefix < a->lk;
-  auto tile_ns = [&](const SharedPart& x) {
-    const int side = std::min(kWaves / x.waves, blocks);  // waves that share a set's blocks
-    if (!bf16) return kBlockF32Ns * a->dk / 128 * blocks / side * std::max(.5, side * x.waves / (double)kWaves);
-    return (a->dk == 128 ? kBlockNs128 : kBlockNs64) * blocks / side;
+  // waves that share the blocks of a range of so many
+  auto side = [&](const SharedPart& x, int blocks) {
+    int n = std::min(kWaves / x.waves, in_tile);
+    while (n / 2 >= blocks) n /= 2;
+    return n;
   };
-  const double tile_p = tile_ns(s.prefix), tile_s = std::max(tile_ns(s.own), kOwnTileNs * a->dk / 128);
-  // (not those that would make several rounds of workgroups, and none far behind the best)
-  const double all_ns = (double)all_p * share_p * tile_p * has_p + (double)all_s * share_s * a->B * tile_s * has_s;
+  const double block_ns = bf16 ? (a->dk == 128 ? kBlockNs128 : kBlockNs64) : kBlockF32Ns * a->dk / 128;
+  const double land_ns = kLandNs * kRows * 2 * (a->dk + s.hb) * (bf16 ? 2 : 4) / 1024;
+  auto each = [&](const SharedPart& x, int blocks) {  // a workgroup of a range of so many blocks
+    const int n = side(x, blocks);
+    double tile = block_ns * ceil_div(std::min(blocks, in_tile), n) * (n * x.waves <= kWaves / 2 ? kFewWaves : 1.);
+    if (bf16 && &x == &s.own && blocks >= in_tile) tile = std::max(tile, kOwnTileNs * a->dk / 128);
+    return kFixedNs + land_ns * std::min(blocks, in_tile) + tile * ceil_div(blocks, in_tile);
+  };
+  // One workgroup is resident on a compute unit, so the launch lasts as long as the longest of 256, or longer by what more of them do.  For every
+  // length of the prefix's ranges - 1, 2 blocks, whole tiles - the longest of the own keys' that do not last longer; the shortest launch wins.
+  const bool has_p = prefix > 0, has_s = prefix < a->lk;
+  auto longer = [&](int blocks) { return blocks < in_tile ? 2 * blocks : in_tile * std::max(blocks / in_tile + 1, blocks / in_tile * 17 / 16); };
   double best = 0;
-  for (double time = std::max(std::min(tile_p, tile_s), all_ns / 800); ; time *= 1.07) {
-    const int tiles_p = has_p ? std::min(all_p, std::max(1, (int)(time / tile_p))) : 0, tiles_s = has_s ? std::min(all_s, std::max(1, (int)(time / tile_s))) : 0;
-    const int ranges_p = has_p ? ceil_div(all_p, tiles_p) : 0, ranges_s = has_s ? ceil_div(all_s, tiles_s) : 0;
+  int p = 1, o = 1;
+  for (;;) {
+    const int blocks_p = std::max(1, std::min(p, all_p)), blocks_s = std::max(1, std::min(o, all_s));
+    const int ranges_p = has_p ? ceil_div(all_p, blocks_p) : 0, ranges_s = has_s ? ceil_div(all_s, blocks_s) : 0;
     // an XCD takes whole ranges: what counts is the one that has most of them, as if all had
     const double groups_p = (double)ceil_div(ranges_p, 8) * 8 * share_p, groups_s = (double)ceil_div((int64_t)ranges_s * a->B, 8) * 8 * share_s;
-    const double each_p = kFixedNs + tiles_p * tile_p, each_s = kFixedNs + tiles_s * tile_s;
-    double cost = std::max(has_p ? each_p : 0., has_s ? each_s : 0.);
+    const double each_p = has_p ? each(s.prefix, blocks_p) : 0., each_s = has_s ? each(s.own, blocks_s) : 0.;
+    double cost = std::max(each_p, each_s);
     if (groups_p + groups_s > 256) cost += (groups_p * each_p + groups_s * each_s) / 256;  // the last ones start where others end
-    cost += kPartNs * (ranges_p + ranges_s) * (double)s.rows * a->H * a->dv;
+    cost += (ranges_p + ranges_s) * (kMergeNs + kPartNs * (double)s.rows * a->H * a->dv);
     if (best == 0 || cost < best) {
       best = cost;
-      s.prefix.tiles = tiles_p; s.own.tiles = tiles_s; s.prefix.ranges = ranges_p; s.own.ranges = ranges_s;
+      s.prefix.blocks = blocks_p; s.own.blocks = blocks_s; s.prefix.ranges = ranges_p; s.own.ranges = ranges_s;
     }
-    if (cost > 2 * best || (tiles_p == (has_p ? all_p : 0) && tiles_s == (has_s ? all_s : 0))) break;
+    const bool more_p = has_p && blocks_p < all_p, more_s = has_s && blocks_s < all_s;
+    if (std::max(each_p, each_s) > 2 * best || !(more_p || more_s)) break;
+    // the part whose workgroups would still be the shorter ones gets longer ranges
+    if (more_p && (!more_s || each(s.prefix, std::min(longer(p), all_p)) <= each(s.own, std::min(longer(o), all_s)))) p = longer(p);
+    else o = longer(o);
   }
+  s.prefix.side = side(s.prefix, s.prefix.blocks);
+  s.own.side = side(s.own, s.own.blocks);
   s.prefix.grid = ceil_div(s.prefix.ranges, 8) * 8 * share_p;
   s.own.grid = ceil_div((int64_t)s.own.ranges * a->B, 8) * 8 * share_s;
   return s;
@@ -722,7 +785,9 @@ int launch_mfma_t(const SharedMfmaParams& p, hipStream_t s) {
   if (const int rc = raise_lds_limit(done, reinterpret_cast<const void*>(kern), bytes); rc != TPA_OK) return rc;
   hipLaunchKernelGGL(kern, dim3(p.plan.prefix.grid + p.plan.own.grid), dim3(kWaves * 64), bytes, s, p);
   if (hipGetLastError() != hipSuccess) return TPA_ERR_LAUNCH;
-  hipLaunchKernelGGL((shared_merge_kernel<T, D>), dim3(ceil_div(p.plan.rows * p.c.H, 4)), dim3(256), 0, s, p);
+  const int64_t n = p.plan.rows * p.c.H;
+  if (n < kMergeWaves) hipLaunchKernelGGL((shared_merge_kernel<T, D, 4>), dim3(n), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((shared_merge_kernel<T, D, 1>), dim3(ceil_div(n, 4)), dim3(256), 0, s, p);
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
 template <typename T, int D, int RK>

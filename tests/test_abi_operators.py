@@ -2,6 +2,7 @@
 C ABI and the host layer refuse is refused before any launch."""
 
 import ctypes
+import itertools
 import os
 import subprocess
 
@@ -119,6 +120,25 @@ def shared(prefix=4, **changed):
 )
 def test_decode_shared_refuses(code, changed):
     assert shared(**changed) == code
+
+
+@pytest.mark.parametrize("h,dk", [(8, 64), (24, 128), (32, 64), (64, 128)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_the_workspace_holds_whole_ranges(dtype, h, dk):
+    """For every split of a cache into prefix and own keys: parts of D + 2 numbers a row and head, no more ranges than blocks of 32 rows."""
+    from tpa import _dispatch as d
+
+    lib = d.load_library()
+    f = lambda w: d.TpaFactor(P, 1 << 20, 8 * w, w)
+    for b, lq, rk, lk in itertools.product((1, 2, 37, 300), (1, 5, 64), (1, 2, 8), (1, 31, 200, 5000, 70000)):
+        for prefix in sorted({0, 1, lk // 2, lk - 1, lk}):
+            a = d.TpaFwdArgs(qa=f(h), qb=f(dk), ka=f(h), kb=f(dk), va=f(h), vb=f(dk), B=b, lq=lq, lk=lk, H=h, dk=dk, dv=dk, rq=6, rk=rk, dtype=dtype, sm_scale=1.0)
+            for name in ("ka", "kb", "va", "vb"):
+                w = getattr(a, name).stride_r
+                getattr(a, name).stride_l = rk * w
+            size = lib.tpa_decode_shared_workspace_bytes(ctypes.byref(a), prefix)
+            of_range = 4 * b * lq * h * (dk + 2)
+            assert size % of_range == 0 and 1 <= size // of_range <= (prefix * rk + 31) // 32 + ((lk - prefix) * rk + 63) // 32 + 1, (b, lq, rk, lk, prefix, size)
 
 
 def test_the_host_layer_refuses_operands_that_do_not_fit():
