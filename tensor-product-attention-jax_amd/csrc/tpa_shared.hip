@@ -3,6 +3,7 @@
 // A query row attends to the keys of the prefix, which are entry 0's, and to the keys behind it, which are its own sequence's; the
 // parts are joined by the running maximum and sum of the softmax.
 #include <algorithm>
+#include <cmath>
 
 #include "tpa_common.h"
 
@@ -552,7 +553,7 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
     return y;
   };
   const int64_t to = (slot + row) * c.H + head;
-  // (not for this XCD's cache, where a kernel's end would have to wait for its way out: 64 sequences over 8192 tokens 51.7 -> @NT us)
+  // (not for this XCD's cache, where the kernel's end would wait for its way out: 12 sequences of 4 tokens over 4096, 64 heads of 64: 45.5 -> 44.0 us)
   auto store = [&](int x, const f32x4& y) __attribute__((always_inline)) {
     const int v = x * 4 / NDB, d = F32 ? NDB * (8 * (v >> 2) + 4 * g + (v & 3)) : 32 * (x / 4) + 8 * (x % 4) + 4 * g;
     __builtin_nontemporal_store(y, reinterpret_cast<f32x4*>(p.part_o + to * D + d));
@@ -683,7 +684,8 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMfmaParams p) {
   }
 }
 
-// Below so many rows and heads four waves share one (the chip has 1024 SIMDs; us of the merge with one / four: @MW)
+// Below so many rows and heads four waves share one: the chip has 1024 SIMDs.  (us of the call with one / four waves: 64 rows and heads 18.7 / 14.8,
+// 512 57.5 / 54.1, 1024 77.9 / 78.0, 2048 54.7 / 56.3.)
 constexpr int64_t kMergeWaves = 1024;
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
@@ -710,8 +712,9 @@ bool mfma_takes(const TpaFwdArgs* a) {
 // eight waves), or kOwnTileNs for a tile of a sequence's own keys, which memory brings; in fp32 the matrix cores decide (kBlockF32Ns).  Half the
 // waves or fewer have the unit to themselves and are faster (kFewWaves).  Data of a first tile arrives at kLandNs for a KiB: what a compute unit
 // gets by itself.  A workgroup's way to its first load and behind its last block; a number of a range's results, written and read again;
-// a range's turn in the merge.
-constexpr double kBlockNs128 = 1450, kBlockNs64 = 875, kOwnTileNs = 3000, kBlockF32Ns = 7000, kFewWaves = .7, kLandNs = 45, kFixedNs = 7500, kPartNs = 8. / 5e3, kMergeNs = 30;
+// a range's turn in the merge; a workgroup that finds no keys.
+constexpr double kBlockNs128 = 1450, kBlockNs64 = 875, kOwnTileNs = 3000, kBlockF32Ns = 7000, kFewWaves = .7, kLandNs = 45, kFixedNs = 7500, kPartNs = 8. / 5e3, kMergeNs = 30, kEmptyNs = 3000;
+constexpr double kUnits = 256;  // compute units
 SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   SharedPlan s{};
   s.hb = a->H % 32 == 0 ? 32 : a->H % 24 == 0 ? 24 : a->H % 16 == 0 ? 16 : 8;
@@ -728,7 +731,6 @@ SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
   columns(s.prefix, s.rows);
   columns(s.own, a->lq);
   const int all_p = ceil_div(prefix, tpb), all_s = ceil_div(a->lk - prefix / tpb * tpb, tpb);
-  const int share_p = s.nhb * s.prefix.groups, share_s = s.nhb * s.own.groups;
   // waves that share the blocks of a range of so many
   auto side = [&](const SharedPart& x, int blocks) {
     int n = std::min(kWaves / x.waves, in_tile);
@@ -736,42 +738,62 @@ SharedPlan plan_of(const TpaFwdArgs* a, int prefix) {
     return n;
   };
   const double block_ns = bf16 ? (a->dk == 128 ? kBlockNs128 : kBlockNs64) : kBlockF32Ns * a->dk / 128;
-  const double land_ns = kLandNs * kRows * 2 * (a->dk + s.hb) * (bf16 ? 2 : 4) / 1024;
-  auto each = [&](const SharedPart& x, int blocks) {  // a workgroup of a range of so many blocks
-    const int n = side(x, blocks);
-    double tile = block_ns * ceil_div(std::min(blocks, in_tile), n) * (n * x.waves <= kWaves / 2 ? kFewWaves : 1.);
-    if (bf16 && &x == &s.own && blocks >= in_tile) tile = std::max(tile, kOwnTileNs * a->dk / 128);
-    return kFixedNs + land_ns * std::min(blocks, in_tile) + tile * ceil_div(blocks, in_tile);
+  const double land_ns = kLandNs * kRows * 2 * (a->dk + s.hb) * (bf16 ? 2 : 4) / 1024, own_ns = bf16 ? kOwnTileNs * a->dk / 128 : 0.;
+  auto each = [&](const SharedPart& x, int blocks) {  // a workgroup of a range of so many blocks, 1, 2 or whole tiles
+    const int n = side(x, blocks), first = std::min(blocks, in_tile);
+    double tile = block_ns * ((first + n - 1) / n) * (n * x.waves <= kWaves / 2 ? kFewWaves : 1.);
+    if (&x == &s.own && blocks >= in_tile) tile = std::max(tile, own_ns);
+    return kFixedNs + land_ns * first + tile * ((blocks + in_tile - 1) / in_tile);
   };
-  // One workgroup is resident on a compute unit, so the launch lasts as long as the longest of 256, or longer by what more of them do.  For every
-  // length of the prefix's ranges - 1, 2 blocks, whole tiles - the longest of the own keys' that do not last longer; the shortest launch wins.
-  const bool has_p = prefix > 0, has_s = prefix < a->lk;
-  auto longer = [&](int blocks) { return blocks < in_tile ? 2 * blocks : in_tile * std::max(blocks / in_tile + 1, blocks / in_tile * 17 / 16); };
+  auto longer = [&](int blocks) { return blocks < in_tile ? 2 * blocks : in_tile * std::max(blocks / in_tile + 1, blocks / in_tile * 9 / 8); };
+  // One workgroup is resident on a compute unit and the prefix's start first: their rounds of 256, then the own keys' where a round leaves units
+  // free and behind them (own lengths differ: on average half of their ranges have no keys).  For every length of the prefix's ranges - 1, 2
+  // blocks, whole tiles, from those on that make two rounds - the own keys' that last as long and half as long are tried; the shortest
+  // launch wins.
+  const double share_p = (double)s.nhb * s.prefix.groups, share_s = (double)s.nhb * s.own.groups;
   double best = 0;
-  int p = 1, o = 1;
-  for (;;) {
-    const int blocks_p = std::max(1, std::min(p, all_p)), blocks_s = std::max(1, std::min(o, all_s));
-    const int ranges_p = has_p ? ceil_div(all_p, blocks_p) : 0, ranges_s = has_s ? ceil_div(all_s, blocks_s) : 0;
+  // ranges of p and o blocks (0: there are none), whose workgroups last each_p and each_s
+  auto consider = [&](int p, int o, double each_p, double each_s) {
+    const int ranges_p = p ? (all_p + p - 1) / p : 0, ranges_s = o ? (all_s + o - 1) / o : 0;
     // an XCD takes whole ranges: what counts is the one that has most of them, as if all had
-    const double groups_p = (double)ceil_div(ranges_p, 8) * 8 * share_p, groups_s = (double)ceil_div((int64_t)ranges_s * a->B, 8) * 8 * share_s;
-    const double each_p = has_p ? each(s.prefix, blocks_p) : 0., each_s = has_s ? each(s.own, blocks_s) : 0.;
-    double cost = std::max(each_p, each_s);
-    if (groups_p + groups_s > 256) cost += (groups_p * each_p + groups_s * each_s) / 256;  // the last ones start where others end
+    const double groups_p = (ranges_p + 7) / 8 * 8 * share_p, groups_s = std::ceil(ranges_s * (double)a->B / 8) * 8 * share_s;
+    const double mean_s = o ? (.5 * (ranges_s + 1) * each_s + .5 * (ranges_s - 1) * kEmptyNs) / ranges_s : 0.;
+    const double rounds = std::floor(groups_p / kUnits), last = groups_p - rounds * kUnits;
+    const double beside = last && o ? (kUnits - last) * std::max(1., std::floor(each_p / mean_s)) : 0.;
+    double cost = rounds * each_p + (last ? std::max(each_p, each_s) : 0.);
+    if (groups_s > beside) cost += std::max(std::ceil((groups_s - beside) / kUnits) * mean_s, last ? 0. : each_s);
     cost += (ranges_p + ranges_s) * (kMergeNs + kPartNs * (double)s.rows * a->H * a->dv);
-    if (best == 0 || cost < best) {
-      best = cost;
-      s.prefix.blocks = blocks_p; s.own.blocks = blocks_s; s.prefix.ranges = ranges_p; s.own.ranges = ranges_s;
+    if (best != 0 && cost >= best) return;
+    best = cost;
+    s.prefix.blocks = p; s.own.blocks = o; s.prefix.ranges = ranges_p; s.own.ranges = ranges_s;
+  };
+  int p = prefix > 0, o = prefix < a->lk;
+  while (p && p < all_p && ceil_div(all_p, p) * share_p > 2 * kUnits) p = std::min(longer(p), all_p);
+  while (o && o < all_s && ceil_div(all_s, o) * share_s * a->B > 4 * kUnits) o = std::min(longer(o), all_s);
+  double each_p = p ? each(s.prefix, p) : 0., each_s = o ? each(s.own, o) : 0.;
+  for (;;) {
+    consider(p, o, each_p, each_s);
+    if (o > in_tile) {
+      const int half = (o / 2 + in_tile - 1) / in_tile * in_tile;
+      consider(p, half, each_p, each(s.own, half));
     }
-    const bool more_p = has_p && blocks_p < all_p, more_s = has_s && blocks_s < all_s;
-    if (std::max(each_p, each_s) > 2 * best || !(more_p || more_s)) break;
+    const bool more_p = p && p < all_p, more_o = o && o < all_s;
+    if (std::max(each_p, each_s) > 2 * best || !(more_p || more_o)) break;
     // the part whose workgroups would still be the shorter ones gets longer ranges
-    if (more_p && (!more_s || each(s.prefix, std::min(longer(p), all_p)) <= each(s.own, std::min(longer(o), all_s)))) p = longer(p);
-    else o = longer(o);
+    const int next_p = std::min(longer(p), all_p), next_o = std::min(longer(o), all_s);
+    const double then_p = more_p ? each(s.prefix, next_p) : 0., then_s = more_o ? each(s.own, next_o) : 0.;
+    if (more_p && (!more_o || then_p <= then_s)) {
+      p = next_p;
+      each_p = then_p;
+    } else {
+      o = next_o;
+      each_s = then_s;
+    }
   }
-  s.prefix.side = side(s.prefix, s.prefix.blocks);
-  s.own.side = side(s.own, s.own.blocks);
-  s.prefix.grid = ceil_div(s.prefix.ranges, 8) * 8 * share_p;
-  s.own.grid = ceil_div((int64_t)s.own.ranges * a->B, 8) * 8 * share_s;
+  s.prefix.side = side(s.prefix, std::max(1, s.prefix.blocks));
+  s.own.side = side(s.own, std::max(1, s.own.blocks));
+  s.prefix.grid = (int)((s.prefix.ranges + 7) / 8 * 8 * share_p);
+  s.own.grid = (int)(ceil_div((int64_t)s.own.ranges * a->B, 8) * 8 * share_s);
   return s;
 }
 int ranges_of(const SharedPlan& s) { return s.prefix.ranges + s.own.ranges; }
