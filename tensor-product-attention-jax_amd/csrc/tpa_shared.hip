@@ -487,9 +487,9 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
 #pragma unroll
     for (int t = 1; t < NTOK; ++t) tmax = fmaxf(tmax, st[t]);
     tmax = halves_max(tmax);
-    // the reference is a whole number (the running maximum rounded up): the rounding of p va does not depend on how the keys are
-    // split, and every rescaling factor is an exact power of two
-    const float m_new = fmaxf(m, __builtin_ceilf(tmax));
+    // the reference is the largest logit when it was set, and set again where one more than twice as heavy comes: what weighs most by far then
+    // has the weight 1, whose product with va needs no rounding, and the sums are rescaled seldom
+    const float m_new = tmax > m + 1.f ? tmax : m;
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
     if (__any(m_new > m)) {
       const float alpha = __builtin_amdgcn_exp2f(m - m_use);
