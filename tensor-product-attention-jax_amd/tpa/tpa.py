@@ -228,7 +228,7 @@ def tpa_decode_shared(
     sequence are taken to be those of entry 0, whose cache (or whose pages, by row 0 of `page_table`) alone is read for them,
     once for the whole batch.  In a paged cache the rows of `page_table` may name the same pages there; a page that the prefix
     only begins belongs to one sequence, since its rest does.  `kv_lengths` count the prefix too; a sequence shorter than the prefix
-    sees as much of it as its length says.  `workspace` (uint8, at least
+    sees as much of it as its length says, and entry 0's cache holds the prefix whatever its own length is.  `workspace` (uint8, at least
     `decode_shared_workspace_bytes(...)`) may be passed to avoid the allocation; a workspace serves one call at a time.
     Returns (o[b,lq,h,dv], lse[b,h,lq]).
     """

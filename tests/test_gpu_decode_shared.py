@@ -255,6 +255,74 @@ def test_replays_from_a_graph_and_two_streams(gpu):
     assert all(torch.equal(x, y) for r in got for one in r for x, y in zip(one, want))
 
 
+def test_a_captured_serving_step(gpu):
+    """The three calls of a step in one graph that advances its own lengths: every replay gives what the eager step gives, pages opened on the way."""
+    b, h, d, rq, rk, page, prefix, pages, steps = 4, 8, 64, 6, 2, 32, 64, 5, 5
+    g = torch.Generator().manual_seed(9)
+    ang = torch.arange(256, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    cos, sin = ang.cos().float().to(gpu), ang.sin().float().to(gpu)
+    new = [[torch.randn((1, b, r, h + d), generator=g).to(BF).to(gpu) for r in (rq, rk, rk)] for _ in range(steps)]
+    pools = [torch.randn((24, page, rk, w), generator=g).to(BF) for w in (h, d, h, d)]
+    table = torch.full((b, pages), -1, dtype=torch.int32)
+    table[:, :2], table[:, 2] = torch.tensor([5, 3]), torch.tensor([7, 8, -1, 9])
+    lengths = torch.tensor([prefix + 30, prefix + 31, prefix, prefix + 5], dtype=torch.int32)
+
+    class State:
+        def __init__(self):
+            self.pools, self.table, self.lengths = [p.to(gpu) for p in pools], table.to(gpu), lengths.to(gpu)
+            self.free, self.start, self.ones = torch.arange(10, 20, dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu), torch.ones(b, dtype=torch.int32, device=gpu)
+            self.x = [t.clone() for t in new[0]]
+
+        def step(self):
+            slots, positions, starts, after, start = tpa.tpa_page_tables(self.lengths, self.ones, self.table, self.free, page_size=page, num_tokens=b, free_start=self.start)
+            q = tpa.tpa_norm_rope_write(*self.x, h, cos, sin, *self.pools, slots[None], positions=positions[None]).transpose(0, 1)
+            out = tpa.tpa_decode_shared(q[..., :h], q[..., h:], *self.pools, prefix_length=prefix, sm_scale=d**-0.5, kv_lengths=after, page_table=self.table)
+            self.lengths.copy_(after)
+            self.start.copy_(start)
+            return out
+
+    State().step()  # the kernels' first launches
+    eager, state = State(), State()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = state.step()
+    for x in new:
+        for to, t in zip(state.x + eager.x, x + x):
+            to.copy_(t)
+        want = eager.step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not want[0].isnan().any()
+        assert all(torch.equal(y, z) for y, z in zip(captured, want))
+        assert all(torch.equal(y, z) for y, z in zip([state.table, state.lengths, state.start, *state.pools], [eager.table, eager.lengths, eager.start, *eager.pools]))
+    assert eager.lengths.tolist() == [n + steps for n in lengths.tolist()] and int(eager.start) == 3
+
+
+def test_the_plan_s_borders(gpu):
+    """Ranges of one block, of two, of whole tiles that end inside a tile; waves side by side from one to eight, and sharing blocks."""
+    for b, lq, prefix, own, h, d, rk in ((1, 1, 17, 16, 8, 64, 2), (1, 2, 33, 31, 8, 128, 1), (2, 1, 2000, 700, 16, 64, 2), (16, 1, 500, 3, 8, 128, 4), (3, 4, 129, 260, 24, 64, 8), (70, 1, 257, 20, 16, 64, 1)):
+        for dtype in (BF, F32):
+            check(gpu, b, lq, prefix, own, h, d, 3, rk, dtype, 2)
+            check(gpu, b, lq, prefix // 32 * 32 + 32, own, h, d, 17, rk, dtype, 2, page=32)
+
+
+def test_a_row_that_is_not_finite_stays_with_itself(gpu):
+    """Infinite and NaN queries of one sequence, in the column sets of others, and non-finite own keys."""
+    for dtype, h in ((BF, 8), (BF, 32), (F32, 16)):
+        g = torch.Generator().manual_seed(3)
+        n = lambda *s: torch.randn(s, generator=g).to(dtype).to(gpu)
+        qa, qb, caches = n(6, 1, 5, h), n(6, 1, 5, 64), [n(6, 150, 2, w) for w in (h, 64, h, 64)]
+        call = lambda: tpa.tpa_decode_shared(qa, qb, *caches, prefix_length=100, sm_scale=0.125, kernel=2)
+        want, want_lse = call()
+        qa[1, 0, 2], qb[3, 0, 4, 7], caches[1][4, 120, 1, 3] = math.inf, math.nan, math.nan
+        got, lse = call()
+        for i in (0, 2, 5):
+            assert torch.equal(got[i], want[i]) and torch.equal(lse[i], want_lse[i])
+        assert all(got[i].isnan().any() for i in (1, 3, 4))
+
+
 def test_refusals(gpu):
     n = lambda *s: torch.zeros(s, dtype=BF, device=gpu)
     qa, qb, caches = n(2, 1, 6, 8), n(2, 1, 6, 64), [n(2, 20, 2, w) for w in (8, 64, 8, 64)]
