@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -21,6 +22,7 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
+#include <optional>
 #include <string>
 #include <utility>
 #include <vector>
@@ -175,12 +177,25 @@ void no_tangents(std::initializer_list<Tensor> tensors, const char* name) {
     if (t.defined() && t._fw_grad(/*level=*/0).defined())
       throw Raise{PyExc_NotImplementedError, std::string(name) + " has no forward-mode derivative: an input carries a tangent"};
 }
+// The gradient of a leaf is accumulated on the stream that the leaf's node was made on.  While an eager graph of the leaf lives, that is not
+// the stream that is being captured, and a backward pass in the capture would wait for the other one, which ends the process.
+void no_node_from_outside_a_capture(std::initializer_list<Tensor> tensors, const char* name) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor& t : tensors) {
+    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto of = node ? node->stream() : std::nullopt;
+    if (of && *of != c10::hip::getCurrentHIPStream(t.device().index()).unwrap())
+      throw Raise{PyExc_RuntimeError, std::string(name) + " is being captured into a graph while an eager graph of one of its inputs lives: delete what was computed from it first, or detach the input"};
+  }
+}
 // a call wrote into `t`: a node that saved it notices
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 template <typename Args>
 void take_workspace(const Tensor& ws, size_t alignment, Args& a) {
+  if (!ws.is_contiguous()) throw Raise{PyExc_ValueError, "workspace must be contiguous"};
   const size_t bytes = ws.numel() * ws.element_size(), skip = static_cast<char*>(aligned(ws, alignment)) - static_cast<char*>(ws.data_ptr());
   a.workspace = aligned(ws, alignment);
   a.workspace_bytes = bytes > skip ? bytes - skip : 0;
@@ -663,7 +678,12 @@ PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
   for (const Tensor& t : tensors) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
   return out;
 }
-Tensor ints(const Tensor& t) { return (t.scalar_type() == at::kInt ? t : t.to(at::kInt)).contiguous(); }
+// as int32; what does not fit stays out of every range
+Tensor ints(const Tensor& t) {
+  if (!at::isIntegralType(t.scalar_type(), /*includeBool=*/false))
+    throw Raise{PyExc_TypeError, std::string("lengths, pages, slots and positions are integers, got ") + c10::toString(t.scalar_type())};
+  return (t.scalar_type() == at::kInt ? t : t.scalar_type() == at::kLong ? t.clamp(INT32_MIN, INT32_MAX).to(at::kInt) : t.to(at::kInt)).contiguous();
+}
 
 // page_tables(kv_lengths, new_tokens, free_pages, free_start, page_table, page_size, num_tokens)
 PyObject* page_tables(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -841,16 +861,18 @@ void run_norm_rope_bwd(const Tensor& q, const Tensor& k, const NormRope& c, cons
 }
 
 struct NormRopeOperator : torch::autograd::Function<NormRopeOperator> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& q_weight,
-                                                const Tensor& k_weight, const NormRope& c) {
+  // (a weight that is not given is no argument of the node: an undefined tensor would be refused)
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const std::optional<Tensor>& q_weight,
+                                                const std::optional<Tensor>& k_weight, const NormRope& c) {
     auto [yq, yk] = run_norm_rope(q, k, c);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, q_weight, k_weight});
+    ctx->save_for_backward({q, k, q_weight.value_or(Tensor()), k_weight.value_or(Tensor())});
     ctx->saved_data["call"] = c10::IValue(std::make_tuple(c.positions, c.cos, c.sin, c.heads, c.sections, c.normalize, c.eps, (int64_t)c.kernel));
     return {yq, yk};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d_out) {
     torch::autograd::variable_list out(5);
+    TORCH_CHECK(!at::GradMode::is_enabled(), "tpa_norm_rope has no second derivative (create_graph)");
     const auto saved = ctx->get_saved_variables();
     const auto call = ctx->saved_data["call"].toTuple();
     const auto& e = call->elements();
@@ -858,7 +880,7 @@ struct NormRopeOperator : torch::autograd::Function<NormRopeOperator> {
     c.q_weight = saved[2]; c.k_weight = saved[3];
     c.positions = e[0].toTensor(); c.cos = e[1].toTensor(); c.sin = e[2].toTensor();
     c.heads = e[3].toInt(); c.sections = e[4].toIntVector(); c.normalize = e[5].toBool(); c.eps = e[6].toDouble(); c.kernel = (int)e[7].toInt();
-    const bool weights[2] = {ctx->needs_input_grad(2), ctx->needs_input_grad(3)};
+    const bool weights[2] = {c.q_weight.defined() && ctx->needs_input_grad(2), c.k_weight.defined() && ctx->needs_input_grad(c.q_weight.defined() ? 3 : 2)};
     try {
       run_norm_rope_bwd(saved[0], saved[1], c, d_out[0], d_out[1], weights, out.data());
     } catch (const CallFailed& f) {  // an engine thread: hand the Python exception to the thread that asked
@@ -922,7 +944,9 @@ PyObject* norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     settle(c);
     auto asks = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
     if (at::GradMode::is_enabled() && (asks(q) || asks(k) || asks(c.q_weight) || asks(c.k_weight))) {
-      auto out = NormRopeOperator::apply(q, k, c.q_weight, c.k_weight, c);
+      no_node_from_outside_a_capture({q, k, c.q_weight, c.k_weight}, "tpa_norm_rope");
+      auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+      auto out = NormRopeOperator::apply(q, k, given(c.q_weight), given(c.k_weight), c);
       r = {out[0], out[1]};
     } else {
       r = run_norm_rope(q, k, c);

@@ -709,7 +709,7 @@ bool mfma_takes(const TpaFwdArgs* a) {
     if (!aligned16(f->ptr) || f->stride_r % per || f->stride_b % per) return false;
   }
   if (!aligned16(a->qb.ptr) || a->qb.stride_r % per || a->qb.stride_l % per || a->qb.stride_b % per) return false;
-  if (a->page_table && a->page_size * (int64_t)a->rk % kRows) return false;
+  if (a->page_table && (a->page_size * (int64_t)a->rk % kRows || a->page_size * (int64_t)a->rk >= (1 << 30))) return false;
   return (int64_t)a->lk * a->rk < (1 << 30);
 }
 
@@ -851,7 +851,7 @@ int validate(const TpaFwdArgs* a, int prefix) {
   if (a->q_segment_ids || a->nomat || a->num_splits) return TPA_ERR_UNSUPPORTED;
   if (prefix < 0 || prefix > a->lk) return TPA_ERR_SHAPE;
   if (a->page_table && (a->page_size <= 0 || a->pages_per_seq <= 0 || (int64_t)a->pages_per_seq * a->page_size < a->lk)) return TPA_ERR_SHAPE;
-  if ((int64_t)a->B * a->lq * a->H > INT32_MAX) return TPA_ERR_SHAPE;
+  if ((int64_t)a->B * a->lq * a->H >= 1 << 24) return TPA_ERR_SHAPE;  // workgroups of 256 threads, 2^32 threads a launch
   return TPA_OK;
 }
 

@@ -116,7 +116,7 @@ def shared(prefix=4, **changed):
     [(SHAPE, dict(prefix=-1)), (SHAPE, dict(prefix=41)), (SHAPE, dict(B=0)), (SHAPE, dict(dk=300)), (DTYPE, dict(dtype=7)), (NULL, dict(o=None)), (NULL, dict(vb=None)),
      (UNSUPPORTED, dict(num_splits=3)), (UNSUPPORTED, dict(nomat=1)), (UNSUPPORTED, dict(q_segment_ids=P, kv_segment_ids=P)), (UNSUPPORTED, dict(causal=3)), (UNSUPPORTED, dict(kernel=5)),
      (SHAPE, dict(page_table=P, page_size=0, pages_per_seq=3)), (SHAPE, dict(page_table=P, page_size=16, pages_per_seq=2)), (UNSUPPORTED, dict(kernel=2, H=9)), (UNSUPPORTED, dict(kernel=2, rk=3)),
-     (SHAPE, dict(B=1 << 20, lq=1 << 10))],
+     (SHAPE, dict(B=1 << 20, lq=1 << 10)), (SHAPE, dict(B=1 << 18, lq=8))],
 )
 def test_decode_shared_refuses(code, changed):
     assert shared(**changed) == code

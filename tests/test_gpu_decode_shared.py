@@ -340,3 +340,5 @@ def test_refusals(gpu):
     need = tpa.decode_shared_workspace_bytes(qa, qb, *caches, prefix_length=4)
     o, _ = tpa.tpa_decode_shared(qa, qb, *caches, prefix_length=4, workspace=torch.empty(need, dtype=torch.uint8, device=gpu))
     assert not o.any()
+    with pytest.raises(ValueError):
+        tpa.tpa_decode_shared(qa, qb, *caches, prefix_length=4, workspace=torch.empty(1, dtype=torch.uint8, device=gpu).expand(need))

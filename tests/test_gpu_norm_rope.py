@@ -322,6 +322,84 @@ def test_replays_from_a_graph(gpu):
         assert all(torch.equal(g, w) for g, w in zip((*captured, *pools), eager))
 
 
+@pytest.mark.parametrize("given", [(), ("wq",), ("wk",), ("wq", "wk")])
+def test_autograd_with_and_without_weights(gpu, given):
+    """torch.autograd gives the backward call's gradients, to the weights that are there and no others."""
+    h, d = 8, 64
+    x = make(37, 2, 9, h, d, 6, 2, torch.bfloat16)
+    kw = dict(call(x, h, None, gpu), q_weight=None, k_weight=None, positions=None)
+    for n in given:
+        kw[n[1] + "_weight"] = x[n].to(gpu)
+    q, k, dq, dk = (x[n].to(gpu) for n in ("q", "k", "dq", "dk"))
+    want = [g for g in tpa.tpa_norm_rope_bwd(q, k, dq_out=dq, dk_out=dk, **kw) if g is not None]
+    leaves = [t.requires_grad_() for t in (q, k, kw["q_weight"], kw["k_weight"]) if t is not None]
+    got = torch.autograd.grad(tpa.tpa_norm_rope(q, k, **kw), leaves, (dq, dk))
+    assert len(got) == len(want) == 2 + len(given) and all(torch.equal(a, b) for a, b in zip(got, want))
+    for i in range(len(leaves)):  # one at a time
+        for j, t in enumerate(leaves):
+            t.requires_grad_(j == i)
+        assert torch.equal(torch.autograd.grad(tpa.tpa_norm_rope(q, k, **kw), leaves[i], (dq, dk), allow_unused=True)[0] if i > 1 else
+                           torch.autograd.grad(tpa.tpa_norm_rope(q, k, **kw)[i], leaves[i], (dq, dk)[i])[0], want[i])
+
+
+def test_a_backward_pass_in_a_graph(gpu):
+    """Captured with its gradients while nothing eager of the leaves lives; refused, before any of it is recorded, while something does."""
+    h, d = 16, 64
+    x = make(29, 2, 40, h, d, 6, 2, torch.bfloat16)
+    kw = call(x, h, None, gpu)
+    q, k, dq, dk = (x[n].to(gpu) for n in ("q", "k", "dq", "dk"))
+    want = tpa.tpa_norm_rope_bwd(q, k, dq_out=dq, dk_out=dk, **kw)
+    leaves = [q.requires_grad_(), k.requires_grad_()]
+    work = lambda: torch.autograd.grad(tpa.tpa_norm_rope(q, k, **kw), leaves, (dq, dk))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = work()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    alive = tpa.tpa_norm_rope(q, k, **kw)
+    torch.cuda.synchronize()
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused, stream=stream):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            tpa.tpa_norm_rope(q, k, **kw)
+        kept = tpa.tpa_norm_rope(q.detach(), k.detach(), **kw)
+    refused.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(kept[0], alive[0]) and torch.equal(kept[1], alive[1])
+
+
+def test_slots_and_positions_of_64_bits(gpu):
+    """Numbers that 32 bits do not hold are outside the pools and behind the last position, not some other place."""
+    h, d = 8, 64
+    x = make(31, 1, 4, h, d, 6, 2, torch.bfloat16)
+    kw = call(x, h, None, gpu)
+    q, k = x["q"].to(gpu), x["k"].to(gpu)
+    pools = [torch.zeros((2, 4, 2, w), dtype=torch.bfloat16, device=gpu) for w in (h, d, h, d)]
+    slots = torch.tensor([[1, 2**32 + 3, -(2**32) + 2, 6]], device=gpu)
+    write = lambda s, p: tpa.tpa_norm_rope_write(q, k, k, h, kw["rope_cos"], kw["rope_sin"], *pools, s, kw["q_weight"], kw["k_weight"], p)
+    write(slots, kw["positions"])
+    used = pools[1].flatten(0, 1).flatten(1).any(1)
+    assert used.tolist() == [i in (1, 6) for i in range(8)]
+    last = kw["rope_cos"].shape[0] - 1
+    far, end = (tpa.tpa_norm_rope(q, k, **dict(kw, positions=torch.tensor([[0, 1, p, 2]], device=gpu))) for p in (2**40, last))
+    assert torch.equal(far[0], end[0]) and torch.equal(far[1], end[1])
+    for bad in (slots.float(), slots > 0):
+        with pytest.raises(TypeError):
+            write(bad, kw["positions"])
+        with pytest.raises(TypeError):
+            write(slots, bad)
+
+
 def test_refusals(gpu):
     h, d = 8, 64
     x = make(29, 2, 6, h, d, 6, 2, torch.bfloat16)
@@ -349,3 +427,7 @@ def test_refusals(gpu):
         tpa.tpa_norm_rope_write(q, k, v, h, cos, sin, pools[1], *pools[1:], slots)
     with pytest.raises(TypeError):
         tpa.tpa_norm_rope_write(q, k, v, h, cos, sin, *(p.float() for p in pools), slots)
+    r = q.clone().requires_grad_()
+    out = tpa.tpa_norm_rope(r, k, h, cos, sin)[0]
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.float().square().sum(), r, create_graph=True)

@@ -132,3 +132,13 @@ def test_refusals(gpu):
         tpa.tpa_page_tables(n, n, t, n, page_size=4, num_tokens=-1)
     with pytest.raises(ValueError):
         tpa.tpa_page_tables(n, n, t, n, page_size=4, num_tokens=1, free_start=n)
+
+
+def test_under_inference_mode(gpu):
+    with torch.inference_mode():
+        table = torch.full((2, 4), -1, dtype=torch.int32, device=gpu)
+        free = torch.arange(5, 13, dtype=torch.int32, device=gpu)
+        slots, positions, starts, after, start = tpa.tpa_page_tables(torch.tensor([0, 0], device=gpu), torch.tensor([3, 9], device=gpu), table, free, page_size=4, num_tokens=14)
+        after = after + 1
+    assert slots.tolist() == [20, 21, 22, 24, 25, 26, 27, 28, 29, 30, 31, 32, -1, -1] and starts.tolist() == [0, 3, 12]
+    assert after.tolist() == [4, 10] and int(start) == 4 and table.tolist() == [[5, -1, -1, -1], [6, 7, 8, -1]] and positions[:3].tolist() == [0, 1, 2]
