@@ -395,22 +395,33 @@ __device__ __forceinline__ void inverse_norms(const S (&square)[4], S inv, float
   }
 }
 
+// positions by which a lane's pairs turn: asked for first, since the rows of cos and sin wait for them
+template <int D, bool AXES>
+struct TurnAt {
+  int row[AXES ? D / 32 : 1];
+  __device__ __forceinline__ TurnAt(const Rotation& rot, int token, int i, int g) {
+    if constexpr (!AXES) {
+      row[0] = (int)row_of(rot, token, i, 0);
+    } else {
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        int axis = 0;
+#pragma unroll
+        for (int a = 0; a < 3; ++a) axis += 16 * x + 4 * g >= rot.last_of[a];
+        row[x] = (int)row_of(rot, token, i, min(axis, rot.n_axes - 1));
+      }
+    }
+  }
+};
 // cos and sin of a lane's four pairs of chunk s
 template <int D, bool AXES>
 struct Turns {
   f32x4 c[D / 32], s[D / 32];
-  __device__ __forceinline__ Turns(const Rotation& rot, int token, int i, int g) {
-    int64_t row = 0;
-    if constexpr (!AXES) row = row_of(rot, token, i, 0) * (D / 2);
+  __device__ __forceinline__ Turns(const Rotation& rot, const TurnAt<D, AXES>& at, int g) {
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) {
       const int j = 16 * x + 4 * g;
-      if constexpr (AXES) {
-        int axis = 0;
-#pragma unroll
-        for (int a = 0; a < 3; ++a) axis += j >= rot.last_of[a];
-        row = row_of(rot, token, i, min(axis, rot.n_axes - 1)) * (D / 2);
-      }
+      const int64_t row = (int64_t)at.row[AXES ? x : 0] * (D / 2);
       c[x] = *reinterpret_cast<const f32x4*>(rot.cos + row + j);
       s[x] = *reinterpret_cast<const f32x4*>(rot.sin + row + j);
       if constexpr (AXES)
@@ -543,6 +554,7 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
   constexpr int NS = D / 32;
   const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, R = side.R, H = p.H, lg = rows_log2(R);
   const Rows me(group, p.l, R, lg, lane);
+  const TurnAt<D, AXES> turn_at(p.rot, me.bi * p.l + me.i, me.i, g);
   const T* const b = base_of<const T>(side.b, me.bi, me.first) + (offset_of(side.b, me.tt, me.r) + 8 * g);
   Chunk<T> x[NS];
 #pragma unroll
@@ -578,7 +590,7 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
   };
   float a[4][VH];
   heads(VH * row, a);
-  const Turns<D, AXES> turn(p.rot, me.bi * p.l + me.i, me.i, g);
+  const Turns<D, AXES> turn(p.rot, turn_at, g);
   bool stored = me.there;
   T* bo;
   if constexpr (CACHED) {
@@ -687,6 +699,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
   float* const W = reinterpret_cast<float*>(lds + Lds::kRows);  // [token][H]
   const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, R = side.R, H = p.H, lg = rows_log2(R);
   const Rows me(group, p.l, R, lg, lane);
+  const TurnAt<D, AXES> turn_at(p.rot, me.bi * p.l + me.i, me.i, g);
   const T* const b = base_of<const T>(side.b, me.bi, me.first) + (offset_of(side.b, me.tt, me.r) + 8 * g);
   const T* const db = base_of<const T>(side.db_out, me.bi, me.first) + (offset_of(side.db_out, me.tt, me.r) + 8 * g);
   Chunk<T> x[NS], dy[NS];
@@ -769,16 +782,18 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
       }
     }
   }
-  const Turns<D, AXES> turn(p.rot, me.bi * p.l + me.i, me.i, g);
+  const T* const a_row = a_base + offset_of(side.a, me.tt, me.r);
+  auto factors = [&](int h) __attribute__((always_inline)) { return me.there && h < H ? load_chunk(a_row + h) : Chunk<T>{}; };
+  Chunk<T> ac = factors(8 * g);
+  const Turns<D, AXES> turn(p.rot, turn_at, g);
   f32x4 M = {0.f, 0.f, 0.f, 0.f};  // M[4 g + e][row] of the token's rows
   u32x2 hi = {0, 0}, lo = {0, 0};  // in two bf16 numbers
   if (p.normalize) {
     wave_lds_fence();
-    const T* const a_row = a_base + offset_of(side.a, me.tt, me.r);
     const float* const w_of = W + (row >> lg) * H;
     for (int h = 8 * g; h - 8 * g < H; h += 32) {
       const bool there = me.there && h < H;
-      const Chunk<T> ac = there ? load_chunk(a_row + h) : Chunk<T>{};
+      const Chunk<T> next = factors(h + 32);
       float w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = there ? ac[e] * w_of[h + e] : 0.f;
@@ -796,6 +811,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
 #pragma unroll
         for (int e = 0; e < 8; ++e) M = __builtin_amdgcn_mfma_f32_16x16x4f32(ac[e], w[e], M, 0, 0, 0);
       }
+      ac = next;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
