@@ -274,6 +274,12 @@ constexpr int bwd_waves(int size, int d) { return size == 2 && d == 64 ? 3 : 2; 
 template <typename T>
 struct Chunk {  // eight elements as loaded
   u32x4 x[sizeof(T) / 2];
+  __device__ __forceinline__ void keep(bool there) {  // zeros otherwise
+#pragma unroll
+    for (int n = 0; n < (int)sizeof(T) / 2; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[n][j] = there ? x[n][j] : 0u;
+  }
   __device__ __forceinline__ float operator[](int e) const {
     if constexpr (sizeof(T) == 2) return e & 1 ? bf16hi_to_f32(x[0][e / 2]) : bf16lo_to_f32(x[0][e / 2]);
     else return __uint_as_float(x[e / 4][e % 4]);
@@ -295,31 +301,32 @@ __device__ __forceinline__ void store_chunk(T* to, const float (&y)[8]) {
     *reinterpret_cast<f32x4*>(to + 4) = f32x4{y[4], y[5], y[6], y[7]};
   }
 }
-// VH neighbouring head factors
+// VH neighbouring head factors as loaded
 template <typename T, int VH>
-__device__ __forceinline__ void load_heads(const T* from, float (&a)[VH]) {
-  if constexpr (VH == 1) {
-    a[0] = load_as_f32(from);
-  } else if constexpr (sizeof(T) * VH == 4) {
-    const uint32_t x = *reinterpret_cast<const uint32_t*>(from);
-    a[0] = bf16lo_to_f32(x); a[1] = bf16hi_to_f32(x);
-  } else if constexpr (sizeof(T) * VH == 8) {
-    const u32x2 x = *reinterpret_cast<const u32x2*>(from);
+struct Heads {
+  using Word = std::conditional_t<sizeof(T) * VH == 2, uint16_t, std::conditional_t<sizeof(T) * VH == 4, uint32_t, u32x2>>;
+  Word x;
+  __device__ __forceinline__ void unpack(bool there, float (&a)[VH]) const {  // zeros where they are not there
 #pragma unroll
-    for (int v = 0; v < VH; ++v) a[v] = VH == 2 ? __uint_as_float(x[v]) : v & 1 ? bf16hi_to_f32(x[v / 2]) : bf16lo_to_f32(x[v / 2]);
-  } else {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(from);
-#pragma unroll
-    for (int v = 0; v < VH; ++v) a[v] = x[v];
+    for (int v = 0; v < VH; ++v) {
+      float y;
+      if constexpr (sizeof(Word) == 2) y = bf16bits_to_f32(x);
+      else if constexpr (sizeof(T) == 2) y = v ? bf16hi_to_f32(x) : bf16lo_to_f32(x);
+      else if constexpr (VH == 1) y = __uint_as_float(x);
+      else y = __uint_as_float(x[v]);
+      a[v] = there ? y : 0.f;
+    }
   }
+};
+template <typename T, int VH>
+__device__ __forceinline__ Heads<T, VH> load_heads(const T* from) {
+  return {*reinterpret_cast<const typename Heads<T, VH>::Word*>(from)};
 }
 template <typename T, int VH>
 __device__ __forceinline__ void store_heads(T* to, const float (&a)[VH]) {
   if constexpr (VH == 1) store_from_f32(to, a[0]);
-  else if constexpr (sizeof(T) * VH == 4) *reinterpret_cast<uint32_t*>(to) = pack_bf16(a[0], a[1]);
-  else if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3])};
-  else if constexpr (VH == 2) *reinterpret_cast<float2*>(to) = make_float2(a[0], a[1]);
-  else *reinterpret_cast<f32x4*>(to) = f32x4{a[0], a[1], a[2], a[3]};
+  else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16(a[0], a[1]);
+  else *reinterpret_cast<float2*>(to) = make_float2(a[0], a[1]);
 }
 // two where 16 lanes still take whole rows of them (four of 64 heads: backward of the second case below 157 us, two 117)
 template <typename F>
@@ -357,26 +364,38 @@ __device__ __forceinline__ double with_lane(double x, int apart) {
   const auto rh = apart == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
   return __longlong_as_double((long long)((uint64_t)rh[0] << 32 | rl[0])) + __longlong_as_double((long long)((uint64_t)rh[1] << 32 | rl[1]));
 }
-// four rows' terms -> for each the sum over the 2^lg rows of its token
+// four rows' terms -> for each the sum over the 2^lg rows of its token (in scalars: arrays that a lambda or a branch writes went to scratch memory)
 template <typename T, typename S>
 __device__ __forceinline__ void over_token(S (&v)[4], int lg) {
-  auto pairs = [&] { v[0] = v[1] = v[0] + v[1]; v[2] = v[3] = v[2] + v[3]; };
-  auto all = [&] { v[0] = v[1] = v[2] = v[3] = v[0] + v[2]; };
-  auto lanes = [&](int apart) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = with_lane(v[j], apart);
-  };
+  S a = v[0], b = v[1], c = v[2], d = v[3];
   if constexpr (sizeof(T) == 2) {  // rows 4 g + j
-    if (lg >= 1) pairs();
-    if (lg >= 2) all();
-    if (lg >= 3) v[0] = v[1] = v[2] = v[3] = with_lane(v[0], 16);
-    if (lg >= 4) v[0] = v[1] = v[2] = v[3] = with_lane(v[0], 32);
+    if (lg >= 1) {
+      a += b; b = a;
+      c += d; d = c;
+    }
+    if (lg >= 2) {
+      a += c;
+      if (lg >= 3) a = with_lane(a, 16);
+      if (lg >= 4) a = with_lane(a, 32);
+      b = c = d = a;
+    }
   } else {  // rows 4 j + g
-    if (lg >= 1) lanes(16);
-    if (lg >= 2) lanes(32);
-    if (lg >= 3) pairs();
-    if (lg >= 4) all();
+    if (lg >= 1) {
+      a = with_lane(a, 16); b = with_lane(b, 16); c = with_lane(c, 16); d = with_lane(d, 16);
+    }
+    if (lg >= 2) {
+      a = with_lane(a, 32); b = with_lane(b, 32); c = with_lane(c, 32); d = with_lane(d, 32);
+    }
+    if (lg >= 3) {
+      a += b; b = a;
+      c += d; d = c;
+    }
+    if (lg >= 4) {
+      a += c;
+      b = c = d = a;
+    }
   }
+  v[0] = a; v[1] = b; v[2] = c; v[3] = d;
 }
 template <typename S>
 __device__ __forceinline__ float inverse_norm_of(S square, S inv, float eps) {  // inv = 1 / (R R D)
@@ -386,13 +405,14 @@ __device__ __forceinline__ float inverse_norm_of(S square, S inv, float eps) {  
 // for four rows; rows of one token have one
 template <typename T, typename S>
 __device__ __forceinline__ void inverse_norms(const S (&square)[4], S inv, float eps, int lg, float (&scale)[4]) {
-  scale[0] = inverse_norm_of(square[0], inv, eps);
-  if (lg >= (sizeof(T) == 2 ? 2 : 4)) {
-    scale[1] = scale[2] = scale[3] = scale[0];
-  } else {
-#pragma unroll
-    for (int j = 1; j < 4; ++j) scale[j] = inverse_norm_of(square[j], inv, eps);
+  const float a = inverse_norm_of(square[0], inv, eps);
+  float b = a, c = a, d = a;
+  if (lg < (sizeof(T) == 2 ? 2 : 4)) {
+    b = inverse_norm_of(square[1], inv, eps);
+    c = inverse_norm_of(square[2], inv, eps);
+    d = inverse_norm_of(square[3], inv, eps);
   }
+  scale[0] = a; scale[1] = b; scale[2] = c; scale[3] = d;
 }
 
 // positions by which a lane's pairs turn: asked for first, since the rows of cos and sin wait for them
@@ -558,7 +578,7 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
   const T* const b = base_of<const T>(side.b, me.bi, me.first) + (offset_of(side.b, me.tt, me.r) + 8 * g);
   Chunk<T> x[NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) x[s] = me.there ? load_chunk(b + 32 * s) : Chunk<T>{};
+  for (int s = 0; s < NS; ++s) x[s] = load_chunk(b + 32 * s);  // (rows that are not there repeat one: a load in a branch would be waited for there)
   // head factors: of four rows this lane has VH heads of every 16 VH
   const T* const a_base = base_of<const T>(side.a, me.bi, me.first);
   uint32_t a_in[4];
@@ -580,16 +600,12 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
       a_to[j] = offset_of(side.a_out, tt, r);
     }
   }
-  auto heads = [&](int h, float (&a)[4][VH]) __attribute__((always_inline)) {
+  Heads<T, VH> next[4];
+  auto heads = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int v = 0; v < VH; ++v) a[j][v] = 0.f;
-      if (a_there[j] && h < H) load_heads<T, VH>(a_base + (a_in[j] + h), a[j]);
-    }
+    for (int j = 0; j < 4; ++j) next[j] = load_heads<T, VH>(a_base + (a_in[j] + min(h, H - VH)));
   };
-  float a[4][VH];
-  heads(VH * row, a);
+  heads(VH * row);
   const Turns<D, AXES> turn(p.rot, turn_at, g);
   bool stored = me.there;
   T* bo;
@@ -600,14 +616,18 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
   } else {
     bo = base_of<T>(side.b_out, me.bi, me.first) + (offset_of(side.b_out, me.tt, me.r) + 8 * g);
   }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) x[s].keep(me.there);
   bool finite = true;
   typename Sums<T>::V G0 = {0, 0, 0, 0};
   if (p.normalize) G0 = gram<T, D>(x, row, g, lg, finite);
   const GramOperand<T> G(G0);
   const typename Sums<T>::S inv = (typename Sums<T>::S)1 / (typename Sums<T>::S)(R * R * D);
   for (int h = VH * row; h - VH * row < H; h += 16 * VH) {
-    float next[4][VH];
-    heads(h + 16 * VH, next);
+    float a[4][VH];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) next[j].unpack(a_there[j] && h < H, a[j]);
+    if (h - VH * row + 16 * VH < H) heads(h + 16 * VH);
     if (p.normalize) {
 #pragma unroll
       for (int v = 0; v < VH; ++v) {
@@ -624,11 +644,8 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 4; ++j)
       if (a_stored[j] && h < H) store_heads<T, VH>(CACHED ? a_out[j] + h : a_out_base + (a_to[j] + h), a[j]);
-#pragma unroll
-      for (int v = 0; v < VH; ++v) a[j][v] = next[j][v];
-    }
   }
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
@@ -704,9 +721,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
   const T* const db = base_of<const T>(side.db_out, me.bi, me.first) + (offset_of(side.db_out, me.tt, me.r) + 8 * g);
   Chunk<T> x[NS], dy[NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) x[s] = me.there ? load_chunk(b + 32 * s) : Chunk<T>{};
-#pragma unroll
-  for (int s = 0; s < NS; ++s) dy[s] = me.there ? load_chunk(db + 32 * s) : Chunk<T>{};
+  for (int s = 0; s < NS; ++s) x[s] = load_chunk(b + 32 * s);
   const T *const a_base = base_of<const T>(side.a, me.bi, me.first), *const da_base = base_of<const T>(side.da_out, me.bi, me.first);
   T* const out_base = base_of<T>(side.da, me.bi, me.first);
   uint32_t a_in[4], da_in[4], da_out[4];
@@ -719,19 +734,19 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
     da_in[j] = offset_of(side.da_out, tt, r);
     da_out[j] = offset_of(side.da, tt, r);
   }
-  auto heads = [&](int h, float (&a)[4][VH], float (&da)[4][VH]) __attribute__((always_inline)) {
+  Heads<T, VH> next[4], d_next[4];
+  auto heads = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int v = 0; v < VH; ++v) a[j][v] = da[j][v] = 0.f;
-      if (a_there[j] && h < H) {
-        load_heads<T, VH>(a_base + (a_in[j] + h), a[j]);
-        load_heads<T, VH>(da_base + (da_in[j] + h), da[j]);
-      }
+      next[j] = load_heads<T, VH>(a_base + (a_in[j] + min(h, H - VH)));
+      d_next[j] = load_heads<T, VH>(da_base + (da_in[j] + min(h, H - VH)));
     }
   };
-  float a[4][VH], da[4][VH];
-  heads(VH * row, a, da);
+  heads(VH * row);
+#pragma unroll
+  for (int s = 0; s < NS; ++s) dy[s] = load_chunk(db + 32 * s);
+#pragma unroll
+  for (int s = 0; s < NS; ++s) x[s].keep(me.there);
   bool finite = true;
   typename Sums<T>::V G0 = {0, 0, 0, 0};
   if (p.normalize) {
@@ -745,8 +760,13 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
   const GramOperand<T> G(G0);
   const typename Sums<T>::S inv = (typename Sums<T>::S)1 / (typename Sums<T>::S)(R * R * D);
   for (int h = VH * row; h - VH * row < H; h += 16 * VH) {
-    float next[4][VH], d_next[4][VH];
-    heads(h + 16 * VH, next, d_next);
+    float a[4][VH], da[4][VH];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      next[j].unpack(a_there[j] && h < H, a[j]);
+      d_next[j].unpack(a_there[j] && h < H, da[j]);
+    }
+    if (h - VH * row + 16 * VH < H) heads(h + 16 * VH);
     if (p.normalize) {
 #pragma unroll
       for (int v = 0; v < VH; ++v) {
@@ -773,17 +793,13 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 4; ++j)
       if (a_there[j] && h < H) store_heads<T, VH>(out_base + (da_out[j] + h), da[j]);
-#pragma unroll
-      for (int v = 0; v < VH; ++v) {
-        a[j][v] = next[j][v];
-        da[j][v] = d_next[j][v];
-      }
-    }
   }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) dy[s].keep(me.there);
   const T* const a_row = a_base + offset_of(side.a, me.tt, me.r);
-  auto factors = [&](int h) __attribute__((always_inline)) { return me.there && h < H ? load_chunk(a_row + h) : Chunk<T>{}; };
+  auto factors = [&](int h) __attribute__((always_inline)) { return load_chunk(a_row + min(h, H - 8)); };
   Chunk<T> ac = factors(8 * g);
   const Turns<D, AXES> turn(p.rot, turn_at, g);
   f32x4 M = {0.f, 0.f, 0.f, 0.f};  // M[4 g + e][row] of the token's rows
@@ -793,6 +809,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
     const float* const w_of = W + (row >> lg) * H;
     for (int h = 8 * g; h - 8 * g < H; h += 32) {
       const bool there = me.there && h < H;
+      ac.keep(there);
       const Chunk<T> next = factors(h + 32);
       float w[8];
 #pragma unroll
