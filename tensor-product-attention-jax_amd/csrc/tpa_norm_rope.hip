@@ -260,16 +260,18 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumParams p) {
 // numbers, 2^-27 of it off; for fp32 factors both are products in 64 bits.
 // The rows of a wave's tokens stand in one product, so a token's rows meet zeros for the other tokens'; where those are not finite, 0 * inf
 // would spread, and the tokens take turns.
-// HBM bounds it: a token's factors come once and go once, at 2.6 to 3.5 TB/s in the cases below, where a plain copy of their size has about 4.5.  (With
+// HBM bounds it: a token's factors come once and go once, forward at 4.1 to 4.9 TB/s in the cases below, backward, whose chain of products is longer, at
+// 3.1 to 3.7, where a plain copy of their size has about 4.5.  (With
 // G through LDS and R^2 products a head on the vector units, 310 registers and 1300 vector instructions per 16 rows, their backward
 // took 66 and 256 us.)
 typedef __attribute__((ext_vector_type(4))) double f64x4;
 constexpr int kNormWaves = 4;
-// Waves of a SIMD that the registers are kept to.  What these kernels need is loads on their way, so waves; one more of them costs scratch memory:
-// us at (4, 3, 2) / (5, 4, 3), forward and backward of 4 x 4096 tokens, 16 heads of 128 23 / 41 and 38 / 38, of 8 x 2048, 64 heads of 64, ranks 16
-// and 8 58 / 77 and 118 / 184.  (The factors of the next tokens asked for ahead take the registers of a wave: 24 and 50, 56 and 183.)
+// Waves of a SIMD that the registers are kept to.  More of them hide more of the loads until they cost much scratch memory: us of the backward of
+// 4 x 4096 tokens, 16 heads of 128, at 2 / 3 waves 42.0 / 38.6, of 4 x 2048, 24 heads 29.1 / 37.5; of 8 x 2048, 64 heads of 64, ranks 16 and 8, at 3 / 4
+// 83 / 137; forward of the last at 4 / 5 / 6 waves 41.3 / 44.9 / 105.  (The factors of the next tokens asked for ahead take the registers of
+// a wave, which costs more than it hides.)
 constexpr int fwd_waves(int size, int d) { return size == 2 ? 4 : d == 64 ? 3 : 2; }
-constexpr int bwd_waves(int size, int d) { return size == 2 && d == 64 ? 3 : 2; }
+constexpr int bwd_waves(int size, int d, int heads_of_lane) { return size == 2 && (d == 64 || heads_of_lane == 1) ? 3 : 2; }
 
 template <typename T>
 struct Chunk {  // eight elements as loaded
@@ -896,7 +898,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
 
 // Workgroups 0 .. parts_q - 1 share out the queries' tokens, the others the keys'
 template <typename T, int D, bool AXES, int VH>
-__global__ __launch_bounds__(kNormWaves * 64, bwd_waves(sizeof(T), D)) void norm_rope_bwd_kernel(NormRopeBwdParams p, int parts_q, int parts_k, int wave_bytes) {
+__global__ __launch_bounds__(kNormWaves * 64, bwd_waves(sizeof(T), D, VH)) void norm_rope_bwd_kernel(NormRopeBwdParams p, int parts_q, int parts_k, int wave_bytes) {
   extern __shared__ __attribute__((aligned(16))) unsigned char bwd_mem[];
   const int w = scalar(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const bool keys = (int)blockIdx.x >= parts_q;
@@ -994,7 +996,16 @@ int launch_fast_bwd(NormRopeBwdParams p, int (&parts)[2], hipStream_t s) {
     p.l = (int)tokens;
     p.B = 1;
   }
-  for (int x = 0; x < 2; ++x) parts[x] = p.side[x].da_out.ptr ? parts_of(p.B, p.l, p.side[x].R, kPartials) : 0;
+  // All workgroups are resident at once, and their waves take the same number of tokens' groups: what a wave has to do behind its last one - the weights'
+  // gradients - is done once.  (With up to 768 workgroups
+  // a side / so, us: 4 x 4096 tokens, 16 heads of 128, three axes 42.1 / 40.3, 4 x 2048, 24 heads 29.3 / 27.0.)
+  const int64_t resident = 256 * bwd_waves(sizeof(T), D, p.H > 16 ? 2 : 1);
+  int64_t groups[2];
+  for (int x = 0; x < 2; ++x) groups[x] = p.side[x].da_out.ptr ? (int64_t)p.B * ((p.l + tokens_per_wave(p.side[x].R) - 1) / tokens_per_wave(p.side[x].R)) : 0;
+  auto parts_for = [&](int x, int64_t each) { return (groups[x] + each * kNormWaves - 1) / (each * kNormWaves); };
+  int64_t each = std::max<int64_t>(1, (groups[0] + groups[1]) / (kNormWaves * resident));
+  while (parts_for(0, each) + parts_for(1, each) > resident) ++each;
+  for (int x = 0; x < 2; ++x) parts[x] = (int)parts_for(x, each);
   const int pairs = most_pairs(p.side[0].R, p.side[1].R, p.H), wave = (int)BwdLds<T, D>::wave_bytes(pairs);
   const size_t lds = BwdLds<T, D>::bytes(pairs);
   const bool axes = p.rot.n_axes > 1 || p.rot.last_of[3] < D / 2;
