@@ -28,9 +28,9 @@ struct SharedParams {
   float scale;               // sm_scale * log2 e
 };
 
-// keys that query row `row` of entry b sees
-__device__ __forceinline__ int keys_seen(const SharedParams& p, int b, int row) {
-  const int len = p.kvlen ? max(0, min(p.kvlen[b], p.lk)) : p.lk;
+// keys that query row `row` of an entry of `length` keys sees
+__device__ __forceinline__ int keys_seen(const SharedParams& p, int length, int row) {
+  const int len = max(0, min(length, p.lk));
   if (!p.causal) return len;
   const int64_t last = (int64_t)row + p.coff + 1 + (p.causal == TPA_CAUSAL_BOTTOM_RIGHT ? len - p.lq : 0);
   return (int)max((int64_t)0, min((int64_t)len, last));
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kAnyThreads) void shared_any_kernel(SharedParams p)
     q[tid] = sum * (p.scale / ((float)p.rq * p.rk));
   }
   __syncthreads();
-  const int keys = keys_seen(p, b, row);
+  const int keys = keys_seen(p, p.kvlen ? p.kvlen[b] : p.lk, row);
   float most = -INFINITY, total = 0.f, out = 0.f;  // the same in all threads; out: of column tid
   for (int t0 = 0; t0 < keys; t0 += kAnyThreads) {
     float x = -INFINITY;
@@ -240,11 +240,14 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   const int b = c.lq == 1 ? row : row / c.lq, row_in_b = row - b * c.lq;
 
   // ---- keys of this part that a column sees: those below `mine`; the workgroup's range ends with the last that any of them sees
-  auto keys_of = [&](int of) __attribute__((always_inline)) {  // row `of` of this part's
-    const int all = (own ? b_own * c.lq : 0) + min(of, n_rows - 1), entry = c.lq == 1 ? all : all / c.lq, seen = keys_seen(c, entry, all - entry * c.lq);
-    return own ? seen : min(seen, c.prefix);
-  };
-  const int mine = keys_of(wave_row + in_set), theirs = keys_of(member / plan.nhb * cwaves * rps + min(l, cwaves * rps - 1));
+  auto row_among_all = [&](int of) __attribute__((always_inline)) { return (own ? b_own * c.lq : 0) + min(of, n_rows - 1); };  // row `of` of this part's
+  const int row_of[2] = {row, row_among_all(member / plan.nhb * cwaves * rps + min(l, cwaves * rps - 1))};
+  const int entry_of[2] = {b, c.lq == 1 ? row_of[1] : row_of[1] / c.lq};
+  int length_of[2] = {c.lk, c.lk};
+  if (c.kvlen) {  // (nothing but the loads here, which would be waited for one by one)
+    length_of[0] = c.kvlen[entry_of[0]];
+    length_of[1] = c.kvlen[entry_of[1]];
+  }
   // ---- the range's rows (token, rank), in blocks from a block's border on
   const int origin = own ? c.prefix / TPB * TPB : 0;
   const int begin = origin + range * part.blocks * TPB;
@@ -276,7 +279,11 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   };
   if constexpr (!F32) request_q(q_in[0], 0);  // (in no branch, behind which the keys would be waited for together with it)
 
-  const int least = scalar(wave_min(mine)), end = scalar(wave_max(theirs));
+  auto keys_of = [&](int x) __attribute__((always_inline)) {
+    const int seen = keys_seen(c, length_of[x], row_of[x] - entry_of[x] * c.lq);
+    return own ? seen : min(seen, c.prefix);
+  };
+  const int mine = keys_of(0), least = scalar(wave_min(mine)), end = scalar(wave_max(keys_of(1)));
   const int stop = min(end, begin + part.blocks * TPB);
   const int64_t slot = ((own ? plan.prefix.ranges : 0) + range) * plan.rows;
   if (stop <= begin || stop <= (own ? c.prefix : 0)) {  // no key of this range is seen
