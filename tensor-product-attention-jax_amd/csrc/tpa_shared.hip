@@ -230,11 +230,12 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   const int unit = id / (8 * sharing) * 8 + (id & 7), member = id / 8 % sharing;
   if (unit >= (own ? c.B * part.ranges : part.ranges)) return;
   const int b_own = own ? unit / part.ranges : 0, range = own ? unit - b_own * part.ranges : unit;
-  const int h0 = member % plan.nhb * plan.hb, rps = 32 / plan.hb;  // rows of a set
-  const int cwaves = part.waves, kwaves = part.side, cw = w % cwaves, kw = w / cwaves;
+  const int h0 = member % plan.nhb * plan.hb, rps = plan.hb >= 24 ? 1 : plan.hb == 16 ? 2 : 4;  // rows of a set
+  const int cwaves = part.waves, kwaves = part.side, cw = w & (cwaves - 1), kw = w >> __builtin_ctz(cwaves);
   const int n_rows = own ? c.lq : (int)plan.rows, wave_row = (member / plan.nhb * cwaves + cw) * rps;  // this wave's first row
   const bool works = kw < kwaves && wave_row < n_rows;
-  const int in_set = min(i / plan.hb, rps - 1), head = h0 + i % plan.hb;  // lanes behind the last whole row of a set repeat it
+  auto in_block = [&](int x) __attribute__((always_inline)) { return plan.hb == 24 ? (x >= 24 ? x - 24 : x) : x & (plan.hb - 1); };  // x % hb, x < 32
+  const int in_set = rps == 1 ? 0 : i >> __builtin_ctz(plan.hb), head = h0 + in_block(i);  // lanes behind the last whole row of a set repeat it
   const bool stored = wave_row + in_set < n_rows && i < rps * plan.hb;
   const int row = (own ? b_own * c.lq : 0) + min(wave_row + in_set, n_rows - 1);  // this lane's query row among all
   const int b = c.lq == 1 ? row : row / c.lq, row_in_b = row - b * c.lq;
@@ -266,9 +267,11 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
   constexpr int QRPI = F32 ? 1 : 64 / (D / 8), QL = 16 / QRPI;  // rows of a load instruction, loads of 16 rows
   struct QIn { uint16_t a[8]; u32x4 b[QL]; };
   [[maybe_unused]] QIn q_in[2];
-  const int q_chunks = (c.rq + 15) / 16, q_steps = rps * q_chunks;
-  [[maybe_unused]] auto request_q = [&](QIn& in, int n) __attribute__((always_inline)) {
-    const int in_row = n / q_chunks, r0 = n % q_chunks * 16;
+  // (steps in order: the ranks of a row, the next row)
+  struct QStep { int in_row, r0; };
+  [[maybe_unused]] auto after = [&](const QStep& n) __attribute__((always_inline)) { return n.r0 + 16 < c.rq ? QStep{n.in_row, n.r0 + 16} : QStep{n.in_row + 1, 0}; };
+  [[maybe_unused]] auto request_q = [&](QIn& in, const QStep& n) __attribute__((always_inline)) {
+    const auto [in_row, r0] = n;
     const int of = (own ? b_own * c.lq : 0) + min(wave_row + in_row, n_rows - 1), ob = c.lq == 1 ? of : of / c.lq;
     const uint16_t* const qa = static_cast<const uint16_t*>(c.qa.ptr) + ob * c.qa.stride_b + (of - ob * c.lq) * c.qa.stride_l + head;
     const uint16_t* const qb = static_cast<const uint16_t*>(c.qb.ptr) + ob * c.qb.stride_b + (of - ob * c.lq) * c.qb.stride_l + 8 * (l % (D / 8));
@@ -277,7 +280,7 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
 #pragma unroll
     for (int j = 0; j < 8; ++j) in.a[j] = qa[min(r0 + 8 * (j / 4) + 4 * g + j % 4, c.rq - 1) * c.qa.stride_r];
   };
-  if constexpr (!F32) request_q(q_in[0], 0);  // (in no branch, behind which the keys would be waited for together with it)
+  if constexpr (!F32) request_q(q_in[0], QStep{0, 0});  // (in no branch, behind which the keys would be waited for together with it)
 
   auto keys_of = [&](int x) __attribute__((always_inline)) {
     const int seen = keys_seen(c, length_of[x], row_of[x] - entry_of[x] * c.lq);
@@ -361,8 +364,8 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
     const BlockAt<uint16_t, D> q_at(l);
     uint16_t* const rows_at = reinterpret_cast<uint16_t*>(mem + Lds::kBuffer + w * (16 * D * 2));
     f32x16 sum[NDB];
-    auto use_q = [&](const QIn& in, int n) __attribute__((always_inline)) {
-      const int in_row = n / q_chunks, r0 = n % q_chunks * 16;
+    auto use_q = [&](const QIn& in, const QStep& n) __attribute__((always_inline)) {
+      const auto [in_row, r0] = n;
 #pragma unroll
       for (int x = 0; x < QL; ++x) {
         const int r = x * QRPI + l / (D / 8);
@@ -391,12 +394,17 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
           for (int v = 0; v < 16; ++v) o[db][v] = in_set == in_row ? sum[db][v] : o[db][v];
     };
     if (works) {
-      if (q_steps > 1) request_q(q_in[1], 1);
-      for (int n = 0; n < q_steps; n += 2) {
-        use_q(q_in[0], n);
-        if (n + 2 < q_steps) request_q(q_in[0], n + 2);
-        if (n + 1 < q_steps) use_q(q_in[1], n + 1);
-        if (n + 3 < q_steps) request_q(q_in[1], n + 3);
+      QStep now = {0, 0}, then = after(now);
+      if (then.in_row < rps) request_q(q_in[1], then);
+      for (;;) {
+        use_q(q_in[0], now);
+        if (then.in_row >= rps) break;
+        now = after(then);
+        if (now.in_row < rps) request_q(q_in[0], now);
+        use_q(q_in[1], then);
+        if (now.in_row >= rps) break;
+        then = after(now);
+        if (then.in_row < rps) request_q(q_in[1], then);
       }
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) {
@@ -423,7 +431,7 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   float m = -INFINITY, lsum = 0.f;
   const At at(l);
-  [[maybe_unused]] const int a_head = (16 * dhalf + 4 * (lp & 3)) % plan.hb;  // of the four columns whose a's this lane helps to transpose
+  [[maybe_unused]] const int a_head = in_block(16 * dhalf + 4 * (lp & 3));  // of the four columns whose a's this lane helps to transpose
   const int row_first = own ? c.prefix * RK : 0;
 
   struct Block { const T *kb, *vb, *ka, *va; int row0; };
