@@ -342,6 +342,30 @@ def test_autograd_with_and_without_weights(gpu, given):
                            torch.autograd.grad(tpa.tpa_norm_rope(q, k, **kw)[i], leaves[i], (dq, dk)[i])[0], want[i])
 
 
+@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("dtype,h,d,rq,rk", [(torch.bfloat16, 64, 64, 16, 8), (torch.bfloat16, 16, 128, 6, 2), (torch.float32, 24, 64, 3, 1)])
+def test_results_over_the_inputs(gpu, dtype, h, d, rq, rk, kernel):
+    """The C entry point takes the inputs' own memory for its results: bit for bit what it writes elsewhere."""
+    import ctypes
+
+    from tpa import _dispatch as dispatch
+
+    x = make(41, 3, 37, h, d, rq, rk, dtype)
+    kw = call(x, h, None, gpu)
+    q, k = x["q"].to(gpu), x["k"].to(gpu)
+    want = tpa.tpa_norm_rope(q, k, kernel=kernel, **kw)
+    positions = kw["positions"].contiguous()
+    f = {n + "a": dispatch.factor(t[..., :h]) for n, t in (("q", q), ("k", k))} | {n + "b": dispatch.factor(t[..., h:]) for n, t in (("q", q), ("k", k))}
+    args = dispatch.TpaNormRopeArgs(
+        **f, **{n + "_out": t for n, t in f.items()}, positions=positions.data_ptr(), rope_cos=kw["rope_cos"].data_ptr(), rope_sin=kw["rope_sin"].data_ptr(),
+        q_weight=kw["q_weight"].data_ptr(), k_weight=kw["k_weight"].data_ptr(), n_axes=1, sections=(ctypes.c_int32 * 4)(d // 2), B=3, l=37, H=h, D=d, rq=rq, rk=rk, rope_len=len(kw["rope_cos"]),
+        dtype=dispatch.dtype_code(dtype), weight_dtype=dispatch.dtype_code(kw["q_weight"].dtype), kernel=kernel, normalize=1, eps=kw.get("eps", 1e-6))
+    torch.cuda.synchronize()
+    assert dispatch.load_library().tpa_norm_rope(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
 def test_a_backward_pass_in_a_graph(gpu):
     """Captured with its gradients while nothing eager of the leaves lives; refused, before any of it is recorded, while something does."""
     h, d = 16, 64
