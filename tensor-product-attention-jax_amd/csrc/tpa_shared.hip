@@ -621,7 +621,8 @@ __device__ __forceinline__ void shared_part(const SharedMfmaParams& p, const Sha
     if (kw) return;
   }
   if (g == 0) {
-    p.part_m[to] = m;
+    // (a range in which all logits are NaN has not moved m, and -inf would say that it has no keys)
+    p.part_m[to] = lsum != lsum ? NAN : m;
     p.part_l[to] = lsum;
   }
 }
@@ -690,7 +691,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMfmaParams p) {
 #pragma unroll
     for (int x = 0; x < W - 1; ++x) sum += from_wave[x][lane % TPR];
   }
-  const bool empty = most == -INFINITY;
+  const bool empty = most == -INFINITY && total == 0.f;  // (the maxima above pass over NaN, the sums do not)
   const float inv = empty ? NAN : 1.f / (total * c.rk);
   T* const out = static_cast<T*>(c.o) + at * D + d;
   if (lane < TPR) {

@@ -342,3 +342,44 @@ def test_refusals(gpu):
     assert not o.any()
     with pytest.raises(ValueError):
         tpa.tpa_decode_shared(qa, qb, *caches, prefix_length=4, workspace=torch.empty(1, dtype=torch.uint8, device=gpu).expand(need))
+
+
+def ranges_of(b, lq, prefix, lk, h, d, rk, qa, qb, caches, table=None):
+    """Key ranges that the call's plan has (parts of D + 2 numbers a row and head), and blocks of 32 rows (token, rank) in all."""
+    size = tpa.decode_shared_workspace_bytes(qa, qb, *caches, prefix_length=prefix, page_table=table, kernel=2) - 256
+    of_block = 32 // rk
+    return size // (4 * b * lq * h * (d + 2)), -(-prefix // of_block) + -(-(lk - prefix // of_block * of_block) // of_block)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("where", ["own key", "block of the prefix", "prefix", "query", "query of the first"])
+def test_nan_is_not_taken_for_no_key(gpu, dtype, where):
+    """NaN where a row sees nothing else in a range of keys: the row's output and lse are NaN, as the formula has it; rows that do not see it keep
+    their results, one that sees no key its NaN and -inf."""
+    b, h, d, prefix, lk = 5, 16, 64, 160, 200
+    g = torch.Generator().manual_seed(11)
+    n = lambda *s: torch.randn(s, generator=g).to(dtype).to(gpu)
+    qa, qb, caches = n(b, 1, 5, h), n(b, 1, 5, d), [n(b, lk, 2, w) for w in (h, d, h, d)]
+    lengths = torch.tensor([161, 200, 160, 0, 40], dtype=torch.int32, device=gpu)
+    assert len(set(ranges_of(b, 1, prefix, lk, h, d, 2, qa, qb, caches))) == 1  # every block is a range of its own
+    call = lambda kernel: tpa.tpa_decode_shared(qa, qb, *caches, prefix_length=prefix, sm_scale=d**-0.5, kv_lengths=lengths, kernel=kernel)
+    clean = {kernel: call(kernel) for kernel in (1, 2)}
+    if where == "own key":
+        caches[1][0, 160], hit = math.nan, [0]  # the only one behind the prefix
+    elif where == "block of the prefix":
+        caches[1][0, 48:64], hit = math.nan, [0, 1, 2]
+    elif where == "prefix":
+        caches[0][0, :160], hit = math.nan, [0, 1, 2, 4]
+    elif where == "query":
+        qb[1, 0, 3, 7], hit = math.nan, [1]
+    else:
+        qa[0], hit = math.nan, [0]
+    for kernel in (1, 2):
+        o, lse = call(kernel)
+        for i in range(b):
+            if i in hit:
+                assert o[i].isnan().all() and lse[i].isnan().all(), (kernel, i)
+            elif i == 3:
+                assert o[i].isnan().all() and (lse[i] == -math.inf).all(), kernel
+            else:
+                assert torch.equal(o[i], clean[kernel][0][i]) and torch.equal(lse[i], clean[kernel][1][i]), (kernel, i)
