@@ -866,8 +866,11 @@ struct NormRopeOperator : torch::autograd::Function<NormRopeOperator> {
                                                 const std::optional<Tensor>& k_weight, const NormRope& c) {
     auto [yq, yk] = run_norm_rope(q, k, c);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, q_weight.value_or(Tensor()), k_weight.value_or(Tensor())});
-    ctx->saved_data["call"] = c10::IValue(std::make_tuple(c.positions, c.cos, c.sin, c.heads, c.sections, c.normalize, c.eps, (int64_t)c.kernel));
+    // positions and tables too: the node notices where one of them is written again before the backward (one made under inference mode counts no
+    // writes and cannot be saved: the node has a copy)
+    auto kept = [](const Tensor& t) { return t.defined() && t.is_inference() ? t.clone() : t; };
+    ctx->save_for_backward({q, k, q_weight.value_or(Tensor()), k_weight.value_or(Tensor()), kept(c.positions), kept(c.cos), kept(c.sin)});
+    ctx->saved_data["call"] = c10::IValue(std::make_tuple(c.heads, c.sections, c.normalize, c.eps, (int64_t)c.kernel));
     return {yq, yk};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d_out) {
@@ -877,9 +880,8 @@ struct NormRopeOperator : torch::autograd::Function<NormRopeOperator> {
     const auto call = ctx->saved_data["call"].toTuple();
     const auto& e = call->elements();
     NormRope c;
-    c.q_weight = saved[2]; c.k_weight = saved[3];
-    c.positions = e[0].toTensor(); c.cos = e[1].toTensor(); c.sin = e[2].toTensor();
-    c.heads = e[3].toInt(); c.sections = e[4].toIntVector(); c.normalize = e[5].toBool(); c.eps = e[6].toDouble(); c.kernel = (int)e[7].toInt();
+    c.q_weight = saved[2]; c.k_weight = saved[3]; c.positions = saved[4]; c.cos = saved[5]; c.sin = saved[6];
+    c.heads = e[0].toInt(); c.sections = e[1].toIntVector(); c.normalize = e[2].toBool(); c.eps = e[3].toDouble(); c.kernel = (int)e[4].toInt();
     const bool weights[2] = {c.q_weight.defined() && ctx->needs_input_grad(2), c.k_weight.defined() && ctx->needs_input_grad(c.q_weight.defined() ? 3 : 2)};
     try {
       run_norm_rope_bwd(saved[0], saved[1], c, d_out[0], d_out[1], weights, out.data());

@@ -455,3 +455,25 @@ def test_refusals(gpu):
     out = tpa.tpa_norm_rope(r, k, h, cos, sin)[0]
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(out.float().square().sum(), r, create_graph=True)
+
+
+@pytest.mark.parametrize("write", ["positions", "cos", "sin"])
+def test_arrays_written_again_before_the_backward(gpu, write):
+    """The gradients turn by the forward's positions: where these have been written over, torch says so.  What the call has converted is its own."""
+    h, d = 8, 64
+    x = make(43, 2, 9, h, d, 6, 2, torch.bfloat16)
+    kw = call(x, h, None, gpu)
+    q = x["q"].to(gpu).requires_grad_()
+    k, dq = x["k"].to(gpu), x["dq"].to(gpu)
+    arrays = dict(positions=kw["positions"].contiguous(), cos=kw["rope_cos"], sin=kw["rope_sin"])
+    kw.update(positions=arrays["positions"])
+    want = torch.autograd.grad(tpa.tpa_norm_rope(q, k, **kw)[0], q, dq)[0]
+    out = tpa.tpa_norm_rope(q, k, **kw)[0]
+    arrays[write].add_(0)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        torch.autograd.grad(out, q, dq)
+    wide = dict(positions=kw["positions"].long(), rope_cos=kw["rope_cos"].double(), rope_sin=kw["rope_sin"].double(), q_weight=kw["q_weight"], k_weight=kw["k_weight"], num_heads=h)
+    out = tpa.tpa_norm_rope(q, k, **wide)[0]
+    for n in ("positions", "rope_cos", "rope_sin"):
+        wide[n].zero_()
+    assert torch.equal(torch.autograd.grad(out, q, dq)[0], want)
