@@ -938,7 +938,9 @@ PyObject* norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   NormRope c = norm_rope_call(args + 2);
   check_norm_rope(q, k, c);
   one_device({q, k, c.cos, c.sin, c.q_weight, c.k_weight, c.positions});
-  no_tangents({q, k, c.q_weight, c.k_weight}, "tpa_norm_rope");
+  no_tangents({q, k, c.q_weight, c.k_weight, c.cos, c.sin}, "tpa_norm_rope");
+  if (at::GradMode::is_enabled() && (c.cos.requires_grad() || c.sin.requires_grad()))
+    throw Raise{PyExc_NotImplementedError, "tpa_norm_rope has no gradient for rope_cos and rope_sin: detach them"};
   std::pair<Tensor, Tensor> r;
   {
     WithoutGil free;

@@ -278,7 +278,8 @@ def tpa_norm_rope(
     rope_cos, rope_sin[rope_len, d/2] fp32 and the rotated pairs are those of `tpa_cache_append`.  `positions`: int [b, l] (default: 0 .. l-1), or
     [b, l, axes] with `sections`, the number of pairs that belong to each axis (time, height, width; up to four): pair j
     turns by its own axis' position, pairs past the last section do not turn.  `q_weight`, `k_weight` [d] (fp32 or bf16; default
-    ones).  `normalize=False` leaves the norms out.  Returns (q', k') in the inputs' shapes and type.
+    ones).  `normalize=False` leaves the norms out.  Returns (q', k') in the inputs' shapes and type.  Tables that ask for a gradient are
+    refused where one would be recorded; positions and tables must not be written again before the backward (torch raises).
     """
     return _call(
         _d.host_calls().norm_rope, (q, k, rope_cos, rope_sin, q_weight, k_weight, positions),

@@ -477,3 +477,21 @@ def test_arrays_written_again_before_the_backward(gpu, write):
     for n in ("positions", "rope_cos", "rope_sin"):
         wide[n].zero_()
     assert torch.equal(torch.autograd.grad(out, q, dq)[0], want)
+
+
+def test_tables_of_inference_and_tables_that_ask_for_gradients(gpu):
+    h, d = 8, 64
+    x = make(47, 2, 9, h, d, 6, 2, torch.bfloat16)
+    kw = call(x, h, None, gpu)
+    q = x["q"].to(gpu).requires_grad_()
+    k, dq = x["k"].to(gpu), x["dq"].to(gpu)
+    want = torch.autograd.grad(tpa.tpa_norm_rope(q, k, **kw)[0], q, dq)[0]
+    with torch.inference_mode():
+        made = {n: kw[n] + 0 for n in ("positions", "rope_cos", "rope_sin")}
+    assert torch.equal(torch.autograd.grad(tpa.tpa_norm_rope(q, k, **dict(kw, **made))[0], q, dq)[0], want)
+    for n in ("rope_cos", "rope_sin"):
+        asks = dict(kw, **{n: kw[n].clone().requires_grad_()})
+        with pytest.raises(NotImplementedError):
+            tpa.tpa_norm_rope(q, k, **asks)
+        with torch.no_grad():
+            tpa.tpa_norm_rope(q, k, **asks)
