@@ -554,6 +554,9 @@ std::pair<Tensor, Tensor> run_concat(const Tensor& q, const Tensor& k, const Ten
   return run_fwd(a, c, q.device(), q.scalar_type());
 }
 
+// writes that an array has seen; one made under inference mode counts none
+int64_t writes_of(const Tensor& t) { return t.defined() && !t.is_inference() ? (int64_t)t._version() : -1; }
+
 struct Operator : torch::autograd::Function<Operator> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                                                 int64_t h, const FwdCall& c) {
@@ -561,7 +564,8 @@ struct Operator : torch::autograd::Function<Operator> {
     ctx->mark_non_differentiable({lse});
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({q, k, v, o, lse});
-    ctx->saved_data["call"] = c10::IValue(std::make_tuple(h, c.qseg, c.kvseg, c.sm_scale, (int64_t)c.causal, (int64_t)c.causal_offset));
+    // segment ids stay where they are (hooks on what is saved see the floating-point tensors alone), with the count of their writes
+    ctx->saved_data["call"] = c10::IValue(std::make_tuple(h, c.qseg, c.kvseg, c.sm_scale, (int64_t)c.causal, (int64_t)c.causal_offset, writes_of(c.qseg), writes_of(c.kvseg)));
     return {o, lse};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d_out) {
@@ -575,6 +579,8 @@ struct Operator : torch::autograd::Function<Operator> {
     b.d_o = d_out[0];
     b.heads = e[0].toInt();
     b.qseg = e[1].toTensor(); b.kvseg = e[2].toTensor();
+    TORCH_CHECK(writes_of(b.qseg) == e[6].toInt() && writes_of(b.kvseg) == e[7].toInt(),
+                "segment ids needed for the gradient computation of tpa have been modified by an inplace operation");
     b.sm_scale = e[3].toDouble();
     b.causal = (int)e[4].toInt(); b.causal_offset = (int)e[5].toInt();
     try {

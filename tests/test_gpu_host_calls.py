@@ -113,3 +113,22 @@ def test_calls_of_several_threads_on_streams_of_their_own(gpu):
         for got, alone in zip(pool.map(worker, cases), want):
             for x, y in zip(got, alone):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("which", ["q", "kv"])
+def test_segment_ids_changed_between_forward_and_backward_are_an_error(gpu, which):
+    """The gradients' mask is the forward's; ids of another type are read from the caller's array again and have to be the same too."""
+    from tpa import tpa
+
+    q, k, v, do, ids = _training_inputs(gpu)
+    for dtype in (torch.int32, torch.int64):
+        both = dict(q=ids.to(dtype).clone(), kv=ids.to(dtype).clone())
+        o = tpa.tpa(q, k, v, 8, both["q"], both["kv"], sm_scale=0.125)
+        want = torch.autograd.grad(o, (q, k, v), do, retain_graph=True)
+        both[which].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(o, (q, k, v), do)
+        with torch.inference_mode():
+            made = ids + 0
+        got = torch.autograd.grad(tpa.tpa(q, k, v, 8, made, made, sm_scale=0.125), (q, k, v), do)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
