@@ -6,7 +6,8 @@
 // The gradient of |X_h|^2 is of the same kind: G a_h for the a's, and an R x R mixture of the b rows.
 //
 // G has signs, so |X_h|^2 may be far below the sum of its terms' sizes where ranks cancel.  It is summed in fp32 for bf16 factors,
-// whose products are exact there, and in 64 bits for fp32 factors.
+// whose products are exact there - heads that cancel are summed anew from X_h itself, see squares_of_vectors() - and in 64 bits for fp32
+// factors.
 #include <algorithm>
 #include <type_traits>
 
@@ -256,7 +257,8 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumParams p) {
 // holds row i's elements 32 s + 8 g + 0..7 of every chunk s, 16 bytes a load: at once the layout of both operands of G = B B^T and whole
 // pairs for the rotation.  G's result layout - column i, four rows - is, G being symmetric, that of an operand of the next product Y = G A, 16
 // heads a time; there lane (n, g) holds four rows of head n of Y and, as the other operand, the same four of A, so that |X_h|^2 = a_h . y_h is
-// a sum over a lane's registers and a few lanes.  Nothing goes through LDS.  For bf16 factors G goes into that product as three bf16
+// a sum over a lane's registers and a few lanes.  The b rows wait in LDS, which saves their registers while the heads go by (with them the kernel
+// of 16 heads of 128 takes 33 us in place of 19).  For bf16 factors G goes into that product as three bf16
 // numbers, 2^-27 of it off; for fp32 factors both are products in 64 bits.
 // The rows of a wave's tokens stand in one product, so a token's rows meet zeros for the other tokens'; where those are not finite, 0 * inf
 // would spread, and the tokens take turns.
@@ -502,22 +504,28 @@ __device__ __forceinline__ typename Sums<T>::V gram(const Chunk<T> (&x)[D / 32],
   finite = !__any(!fine);
   return G;
 }
+// two pairs of numbers of bf16
+__device__ __forceinline__ u32x2 packed(const float (&a)[4]) {
+  return u32x2{__builtin_amdgcn_perm(__float_as_uint(a[1]), __float_as_uint(a[0]), 0x07060302), __builtin_amdgcn_perm(__float_as_uint(a[3]), __float_as_uint(a[2]), 0x07060302)};
+}
+// four numbers as three of bf16 each, the largest part first: 2^-27 of them off
+__device__ __forceinline__ void in_three(f32x4 x, s16x4 (&part)[3]) {
+#pragma unroll
+  for (int n = 0; n < 3; ++n) {
+    const u32x2 p = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    part[n] = __builtin_bit_cast(s16x4, p);
+    x = f32x4{x[0] - bf16lo_to_f32(p[0]), x[1] - bf16hi_to_f32(p[0]), x[2] - bf16lo_to_f32(p[1]), x[3] - bf16hi_to_f32(p[1])};
+  }
+}
 // G as the operand of Y = G A
 template <typename T>
 struct GramOperand;
 template <>
 struct GramOperand<uint16_t> {
   s16x4 part[3];
-  __device__ __forceinline__ explicit GramOperand(f32x4 G) {
-#pragma unroll
-    for (int n = 0; n < 3; ++n) {
-      const u32x2 p = {pack_bf16(G[0], G[1]), pack_bf16(G[2], G[3])};
-      part[n] = __builtin_bit_cast(s16x4, p);
-      G = f32x4{G[0] - bf16lo_to_f32(p[0]), G[1] - bf16hi_to_f32(p[0]), G[2] - bf16lo_to_f32(p[1]), G[3] - bf16hi_to_f32(p[1])};
-    }
-  }
+  __device__ __forceinline__ explicit GramOperand(f32x4 G) { in_three(G, part); }
   __device__ __forceinline__ f32x4 times(const float (&a)[4]) const {  // a: numbers of bf16
-    const u32x2 p = {__builtin_amdgcn_perm(__float_as_uint(a[1]), __float_as_uint(a[0]), 0x07060302), __builtin_amdgcn_perm(__float_as_uint(a[3]), __float_as_uint(a[2]), 0x07060302)};
+    const u32x2 p = packed(a);
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 2; n >= 0; --n) y = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(part[n], __builtin_bit_cast(s16x4, p), y, 0, 0, 0);
@@ -555,6 +563,86 @@ __device__ __forceinline__ typename Sums<T>::V times_gram(const GramOperand<T>& 
   return y;
 }
 
+// b rows of a wave in LDS; the padding spreads the 16 rows that a transposing read meets over the banks
+template <typename T, int D>
+struct RowsInLds {
+  static constexpr int kStride = sizeof(T) == 2 ? D + 8 : D + 4;  // elements
+  static constexpr int kBytes = 16 * kStride * sizeof(T);
+};
+template <typename T, int D>
+__device__ __forceinline__ void rows_to_lds(const Chunk<T>& x, int s, int row, int g, T* rows) {
+#pragma unroll
+  for (int n = 0; n < (int)sizeof(T) / 2; ++n) reinterpret_cast<u32x4*>(rows + row * RowsInLds<T, D>::kStride + 32 * s + 8 * g)[n] = x.x[n];
+}
+// rows 4 g + 0..3 of the column that this lane stands for: 16 lanes bring 4 rows x 4 columns from `column` on each and get them transposed
+template <int D>
+__device__ __forceinline__ s16x4 rows_transposed(const uint16_t* rows, int row, int g, int column) {
+  const uint16_t* const from = rows + (4 * g + (row >> 2)) * RowsInLds<uint16_t, D>::kStride + column;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)from);
+}
+// Where ranks cancel a^T G a is off by the square of (sum of the terms' sizes / sum) in units of 2^-24, the head vectors themselves by the first
+// power.  The sum of the sizes is at most R^2 of the largest a_r^2 |b_r|^2: heads whose sum is less than 2^-10 of that, where the norm may be 2^-13 off,
+// are summed anew from R X_h[d] = sum_r b_r[d] a_r[h], whose terms are exact, 16 elements of 16 heads an instruction, which keeps none of them.
+// (4 x 4096 tokens, 16 heads of 128, ranks 6 and 2: forward 18.4 us with no such head, 25.5 with nothing else, backward 34.4 and 51.8; without the
+// comparison 17.7 and 36.3.)
+// A token's rows stand beside zeros for the other tokens', in the b rows too, which need not be finite.  `most`: |a_r| lengths_of(), of which the largest decides.
+constexpr float kCancelled = 1.f / 32;
+template <int D>
+__device__ __forceinline__ void squares_of_vectors(const uint16_t* rows, const float (&a)[4], const float (&most)[4], int row, int g, int lg, float (&square)[4]) {
+  float low[4];  // rows of the token that say so
+#pragma unroll
+  for (int j = 0; j < 4; ++j) low[j] = square[j] < most[j] * most[j] ? 1.f : 0.f;
+  over_token<uint16_t>(low, lg);
+  wave_lds_fence();
+  const u32x2 p = packed(a);
+#pragma unroll 1
+  for (int tt = 0; tt < 16 >> lg; ++tt) {
+    u32x2 keep;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) keep[n] = ((4 * g + 2 * n) >> lg == tt ? 0xffffu : 0u) | ((4 * g + 2 * n + 1) >> lg == tt ? 0xffff0000u : 0u);
+    const s16x4 of_token = __builtin_bit_cast(s16x4, p & keep);
+    float sum = 0.f;
+#pragma unroll 2
+    for (int x = 0; x < D / 16; ++x) {
+      const s16x4 f = __builtin_bit_cast(s16x4, __builtin_bit_cast(u32x2, rows_transposed<D>(rows, row, g, 16 * x + 4 * (row & 3))) & keep);
+      const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, of_token, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = fmaf(y[e], y[e], sum);
+    }
+    sum = with_lane(with_lane(sum, 16), 32);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) square[j] = low[j] != 0.f && (4 * g + j) >> lg == tt ? sum : square[j];
+  }
+}
+// R / 32 of |b_r| of this lane's four rows, off the diagonal of G
+__device__ __forceinline__ f32x4 lengths_of(const f32x4& G, int R, int g) {
+  f32x4 length;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) length[j] = kCancelled * R * __builtin_amdgcn_sqrtf(__shfl(G[j], 20 * g + j));
+  return length;
+}
+// the sums of squares of 16 heads, `y` = G a; bf16 factors: `rows` has the b rows, `length` is lengths_of()
+template <typename T, int D>
+__device__ __forceinline__ void squares_of(const float (&a)[4], const typename Sums<T>::V& y, [[maybe_unused]] const f32x4& length, [[maybe_unused]] const T* rows, [[maybe_unused]] int row,
+                                           [[maybe_unused]] int g, int lg, typename Sums<T>::S (&square)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) square[j] = a[j] * y[j];
+  over_token<T>(square, lg);
+  if constexpr (sizeof(T) == 2) {
+    float most[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most[j] = __builtin_fabsf(a[j] * length[j]);
+    bool low;
+    if (lg >= 2) {  // the four rows are one token's
+      const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+      low = square[0] < m * m;
+    } else {
+      low = lg && (square[0] < most[0] * most[0] || square[1] < most[1] * most[1] || square[2] < most[2] * most[2] || square[3] < most[3] * most[3]);
+    }
+    if (__any(low)) squares_of_vectors<D>(rows, a, most, row, g, lg, square);
+  }
+}
+
 // a wave's tokens, and this lane's row of theirs
 struct Rows {
   int bi, first;  // batch entry, its first token
@@ -572,7 +660,7 @@ struct Rows {
 };
 
 template <typename T, int D, bool AXES, int VH, bool CACHED>
-__device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Side& side, int group, const float* wt) {
+__device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Side& side, int group, const float* wt, [[maybe_unused]] T* rows) {
   constexpr int NS = D / 32;
   const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, R = side.R, H = p.H, lg = rows_log2(R);
   const Rows me(group, p.l, R, lg, lane);
@@ -624,6 +712,12 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
   typename Sums<T>::V G0 = {0, 0, 0, 0};
   if (p.normalize) G0 = gram<T, D>(x, row, g, lg, finite);
   const GramOperand<T> G(G0);
+  f32x4 length = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (sizeof(T) == 2) {
+    length = lengths_of(G0, R, g);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) rows_to_lds<T, D>(x[s], s, row, g, rows);  // where they wait for the heads too
+  }
   const typename Sums<T>::S inv = (typename Sums<T>::S)1 / (typename Sums<T>::S)(R * R * D);
   for (int h = VH * row; h - VH * row < H; h += 16 * VH) {
     float a[4][VH];
@@ -636,9 +730,7 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
         const float av[4] = {a[0][v], a[1][v], a[2][v], a[3][v]};
         const typename Sums<T>::V y = times_gram<T>(G, av, finite, g, lg);
         typename Sums<T>::S square[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) square[j] = av[j] * y[j];
-        over_token<T>(square, lg);
+        squares_of<T, D>(av, y, length, rows, row, g, lg, square);
         float scale[4];
         inverse_norms<T>(square, inv, p.eps, lg, scale);
 #pragma unroll
@@ -653,6 +745,7 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
   for (int s = 0; s < NS; ++s) {
     float y[8];
     const Chunk<float> w = load_chunk(wt + 32 * s + 8 * g);
+    if constexpr (sizeof(T) == 2) x[s] = load_chunk(rows + row * RowsInLds<T, D>::kStride + 32 * s + 8 * g);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float y0 = x[s][2 * e] * w[2 * e], y1 = x[s][2 * e + 1] * w[2 * e + 1];
@@ -661,6 +754,7 @@ __device__ __forceinline__ void norm_rope_rows(const NormRopeParams& p, const Si
     }
     if (stored) store_chunk(bo + 32 * s, y);
   }
+  if constexpr (sizeof(T) == 2) wave_lds_fence();  // the next tokens' rows go where these are
 }
 
 // V factors into their slots, 16 bytes a lane: chunks of a row of ranks, head factors first
@@ -686,14 +780,16 @@ __device__ __forceinline__ void copy_values(const NormRopeParams& p, int group) 
 template <typename T, int D, bool AXES, int VH, bool CACHED>
 __global__ __launch_bounds__(kNormWaves * 64, fwd_waves(sizeof(T), D)) void norm_rope_kernel(NormRopeParams p, int parts_q, int parts_k, int parts_v) {
   __shared__ __attribute__((aligned(16))) float wt[D];
+  __shared__ __attribute__((aligned(16))) unsigned char rows_mem[sizeof(T) == 2 ? kNormWaves * RowsInLds<T, D>::kBytes : 16];
   const int w = scalar(threadIdx.x >> 6), part = blockIdx.x;
+  T* const rows = reinterpret_cast<T*>(rows_mem + (sizeof(T) == 2 ? w * RowsInLds<T, D>::kBytes : 0));
   auto groups = [&](int R) { return (p.l + tokens_per_wave(R) - 1) / tokens_per_wave(R) * p.B; };
   if (part < parts_q) {
     weights_to_lds<D>(p.side[0].weight, p.weight_bf16, wt);
-    for (int group = part * kNormWaves + w; group < groups(p.side[0].R); group += parts_q * kNormWaves) norm_rope_rows<T, D, AXES, VH, false>(p, p.side[0], group, wt);
+    for (int group = part * kNormWaves + w; group < groups(p.side[0].R); group += parts_q * kNormWaves) norm_rope_rows<T, D, AXES, VH, false>(p, p.side[0], group, wt, rows);
   } else if (part < parts_q + parts_k) {
     weights_to_lds<D>(p.side[1].weight, p.weight_bf16, wt);
-    for (int group = (part - parts_q) * kNormWaves + w; group < groups(p.side[1].R); group += parts_k * kNormWaves) norm_rope_rows<T, D, AXES, VH, CACHED>(p, p.side[1], group, wt);
+    for (int group = (part - parts_q) * kNormWaves + w; group < groups(p.side[1].R); group += parts_k * kNormWaves) norm_rope_rows<T, D, AXES, VH, CACHED>(p, p.side[1], group, wt, rows);
   } else if constexpr (CACHED) {
     for (int group = (part - parts_q - parts_k) * kNormWaves + w; group < groups(p.side[1].R); group += parts_v * kNormWaves) copy_values<T, D>(p, group);
   }
@@ -704,8 +800,8 @@ __global__ __launch_bounds__(kNormWaves * 64, fwd_waves(sizeof(T), D)) void norm
 // factors w a and M are kept as two bf16 numbers each.
 template <typename T, int D>
 struct BwdLds {
-  static constexpr int kStride = sizeof(T) == 2 ? D : D + 4;  // of a b row (elements)
-  static constexpr size_t kRows = 16 * kStride * sizeof(T);
+  static constexpr int kStride = RowsInLds<T, D>::kStride;
+  static constexpr size_t kRows = RowsInLds<T, D>::kBytes;
   static size_t wave_bytes(int most_pairs) { return kRows + (size_t)(most_pairs + 3) / 4 * 16; }
   static size_t bytes(int most_pairs) { return kNormWaves * wave_bytes(most_pairs) + D * sizeof(float); }
 };
@@ -751,15 +847,12 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
   for (int s = 0; s < NS; ++s) x[s].keep(me.there);
   bool finite = true;
   typename Sums<T>::V G0 = {0, 0, 0, 0};
-  if (p.normalize) {
-    G0 = gram<T, D>(x, row, g, lg, finite);
-    if (finite)
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int n = 0; n < (int)sizeof(T) / 2; ++n) reinterpret_cast<u32x4*>(rows + row * Lds::kStride + 32 * s + 8 * g)[n] = x[s].x[n];
-  }
+  for (int s = 0; s < NS; ++s) rows_to_lds<T, D>(x[s], s, row, g, rows);  // where they wait for the heads too
+  if (p.normalize) G0 = gram<T, D>(x, row, g, lg, finite);
   const GramOperand<T> G(G0);
+  f32x4 length = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (sizeof(T) == 2) length = lengths_of(G0, R, g);
   const typename Sums<T>::S inv = (typename Sums<T>::S)1 / (typename Sums<T>::S)(R * R * D);
   for (int h = VH * row; h - VH * row < H; h += 16 * VH) {
     float a[4][VH], da[4][VH];
@@ -776,12 +869,9 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
         const typename Sums<T>::V y = times_gram<T>(G, av, finite, g, lg);
         typename Sums<T>::S square[4];
         float u[4];
+        squares_of<T, D>(av, y, length, rows, row, g, lg, square);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          square[j] = av[j] * y[j];
-          u[j] = da[j][v] * av[j];
-        }
-        over_token<T>(square, lg);
+        for (int j = 0; j < 4; ++j) u[j] = da[j][v] * av[j];
         over_token<T>(u, lg);
         float scale[4];
         inverse_norms<T>(square, inv, p.eps, lg, scale);
@@ -806,8 +896,8 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
   const Turns<D, AXES> turn(p.rot, turn_at, g);
   f32x4 M = {0.f, 0.f, 0.f, 0.f};  // M[4 g + e][row] of the token's rows
   u32x2 hi = {0, 0}, lo = {0, 0};  // in two bf16 numbers
+  wave_lds_fence();
   if (p.normalize) {
-    wave_lds_fence();
     const float* const w_of = W + (row >> lg) * H;
     for (int h = 8 * g; h - 8 * g < H; h += 32) {
       const bool there = me.there && h < H;
@@ -844,9 +934,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
   auto mix = [&](int n) __attribute__((always_inline)) {
     f32x4 out = {0.f, 0.f, 0.f, 0.f};
     if constexpr (sizeof(T) == 2) {
-      // rows 4 g + 0..3 of the column that this lane stands for: 16 lanes bring 4 rows x 16 columns and get them transposed
-      const T* const from = rows + (4 * g + (row >> 2)) * Lds::kStride + 32 * (n / 2) + 8 * (row & 3) + 4 * (n % 2);
-      const s16x4 f = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)from);
+      const s16x4 f = rows_transposed<D>(rows, row, g, 32 * (n / 2) + 8 * (row & 3) + 4 * (n % 2));
       out = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, lo), out, 0, 0, 0);
       return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, hi), out, 0, 0, 0);
     } else {
@@ -860,6 +948,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     f32x4 mixed[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const Chunk<T> xs = load_chunk(rows + row * Lds::kStride + 32 * s + 8 * g);
     if (p.normalize) {
       if (finite) {
         mixed[0] = mix(2 * s);
@@ -868,14 +957,14 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
         for (int tt = 0; tt < 16 >> lg; ++tt) {
           wave_lds_fence();
           const bool mine = row >> lg == tt;
-#pragma unroll
-          for (int n = 0; n < (int)sizeof(T) / 2; ++n)
-            reinterpret_cast<u32x4*>(rows + row * Lds::kStride + 32 * s + 8 * g)[n] = mine ? x[s].x[n] : u32x4{0, 0, 0, 0};
+          Chunk<T> one = xs;
+          one.keep(mine);
+          rows_to_lds<T, D>(one, s, row, g, rows);
           wave_lds_fence();
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const f32x4 one = mix(2 * s + n);
-            mixed[n] = mine ? one : mixed[n];
+            const f32x4 by_token = mix(2 * s + n);
+            mixed[n] = mine ? by_token : mixed[n];
           }
         }
       }
@@ -886,8 +975,8 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
     for (int e = 0; e < 4; ++e) {
       const float y0 = dy[s][2 * e], y1 = dy[s][2 * e + 1];
       const float e0 = y0 * turn.c[s][e] + y1 * turn.s[s][e], e1 = y1 * turn.c[s][e] - y0 * turn.s[s][e];
-      d_weight[8 * s + 2 * e] = fmaf(e0, x[s][2 * e], d_weight[8 * s + 2 * e]);
-      d_weight[8 * s + 2 * e + 1] = fmaf(e1, x[s][2 * e + 1], d_weight[8 * s + 2 * e + 1]);
+      d_weight[8 * s + 2 * e] = fmaf(e0, xs[2 * e], d_weight[8 * s + 2 * e]);
+      d_weight[8 * s + 2 * e + 1] = fmaf(e1, xs[2 * e + 1], d_weight[8 * s + 2 * e + 1]);
       y[2 * e] = fmaf(e0, w[2 * e], mixed[e / 2][2 * e % 4]);
       y[2 * e + 1] = fmaf(e1, w[2 * e + 1], mixed[e / 2][(2 * e + 1) % 4]);
     }

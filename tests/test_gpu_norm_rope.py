@@ -495,3 +495,62 @@ def test_tables_of_inference_and_tables_that_ask_for_gradients(gpu):
             tpa.tpa_norm_rope(q, k, **asks)
         with torch.no_grad():
             tpa.tpa_norm_rope(q, k, **asks)
+
+
+def first_power(x, h, weight, c, s, eps, dy):
+    """`side`'s results with the slack of norms that are summed over the head vectors themselves: with kappa as the sum of the terms' sizes over
+    their sum, an element of X_h is off by 2 R U of its terms' sizes, the norm by kappa^(1/2) of that, and by D + 16 roundings of its own.  fp32
+    factors have their norms in 64 bits, within the same."""
+    r, d = x.shape[2], x.shape[3] - h
+    a, b = x[..., :h], x[..., h:]
+    dense, sizes = torch.matmul(a.transpose(2, 3), b) / r, torch.matmul(a.abs().transpose(2, 3), b.abs()) / r
+    n = dense.square().mean(-1) + eps
+    scale = n.rsqrt()
+    rel_s = (2 * r * ((sizes.square().mean(-1) + eps) / n).sqrt() + d + 16) * U
+    out, _, grad, _, dw, _ = side(x, h, weight, c, s, eps, True, dy)
+    da = dy[..., :h]
+    w = scale**3 * (da * a).abs().sum(2) / (d * r * r)
+    m_size = torch.matmul(a.abs() * w[:, :, None], a.abs().transpose(2, 3))
+    worst = rel_s.amax(-1)[:, :, None, None]
+    # w comes from the norm and the sum over the ranks of da a; the gradients of a from G a, those of b from the mixture, each a sum of terms that cancel
+    # to the first power: G, M and w a are within 4 U of what they stand for
+    g_size = torch.matmul(b.abs(), b.abs().transpose(2, 3))
+    g_slack = torch.cat([(da * scale[:, :, None]).abs() * (rel_s[:, :, None] + 2 * U) + (w * 3 * rel_s)[:, :, None] * torch.matmul(b, dense.transpose(2, 3)).abs() * r
+                         + w[:, :, None] * torch.matmul(g_size, a.abs()) * (d + 3 * r + 20) * U,
+                         8 * U * dy[..., h:].abs().amax(-1, keepdim=True) * weight.abs() * 2 + torch.matmul((a.abs() * (3 * rel_s * w)[:, :, None]), dense.abs()) * r
+                         + torch.matmul(m_size, b.abs()) * (h + 3 * r + 24) * U], -1)
+    return out[..., :h], (a * scale[:, :, None]).abs() * rel_s[:, :, None], grad, g_slack
+
+
+def cancelling(apart, b, l, h, d, rq, rk, dtype):
+    """`make`'s arrays, every second rank the one before it with the other sign of a and a b that is off by 2^-apart: head vectors 2^apart smaller than
+    their terms."""
+    x = make(apart, b, l, h, d, rq, rk, torch.float32)
+    g = torch.Generator().manual_seed(apart)
+    for n in "qk":
+        y = x[n].to(torch.bfloat16).float()
+        y[:, :, 1::2, :h] = -y[:, :, ::2, :h]
+        y[:, :, 1::2, h:] = (y[:, :, ::2, h:] * (1 + 2.0**-apart * torch.randn(y[:, :, ::2, h:].shape, generator=g))).to(torch.bfloat16).float()
+        x[n] = y.to(dtype)
+        x["d" + n] = x["d" + n].to(dtype)
+    return x
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("h,d,rq,rk", [(16, 128, 2, 6), (32, 64, 4, 16), (8, 64, 8, 2)])
+@pytest.mark.parametrize("apart", [5, 7, 9])
+def test_ranks_that_cancel(gpu, dtype, h, d, rq, rk, apart, kernel):
+    """The norms of head vectors that are far smaller than their terms are as near as if the vectors had been formed; a token's do not depend on
+    the tokens beside it."""
+    x = cancelling(apart, 2, 21, h, d, rq, rk, dtype)
+    kw = call(x, h, None, gpu, kernel=kernel)
+    got = tpa.tpa_norm_rope(x["q"].to(gpu), x["k"].to(gpu), **kw)
+    c, s = angles(x["pos"], [d // 2], x["cos"], x["sin"], d)
+    others = make(apart, 2, 21, h, d, rq, rk, dtype)
+    for i, n in enumerate("qk"):
+        out, slack, _, _ = first_power(x[n].double(), h, x["w" + n].double(), c, s, 1e-6, x["d" + n].double())
+        near(got[i][..., :h], out, slack, dtype, n)
+        others[n][:, ::3] = x[n][:, ::3]
+    beside = tpa.tpa_norm_rope(others["q"].to(gpu), others["k"].to(gpu), **kw)
+    assert all(torch.equal(a[:, ::3], b[:, ::3]) for a, b in zip(got, beside))
