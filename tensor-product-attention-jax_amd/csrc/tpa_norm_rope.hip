@@ -797,7 +797,7 @@ __global__ __launch_bounds__(kNormWaves * 64, fwd_waves(sizeof(T), D)) void norm
 
 // ---- gradients.  The R x R sums M = A diag(w) A^T over the heads and the mixture M B of the b rows are products of the matrix cores
 // too: M's result layout is that of the second product's operand, whose other one are the b rows read back transposed from LDS.  For bf16
-// factors w a and M are kept as two bf16 numbers each.
+// factors w a and M are kept as three bf16 numbers each (2^-27 off: where ranks cancel the mixture is off by that times sum of sizes / sum).
 template <typename T, int D>
 struct BwdLds {
   static constexpr int kStride = RowsInLds<T, D>::kStride;
@@ -895,7 +895,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
   Chunk<T> ac = factors(8 * g);
   const Turns<D, AXES> turn(p.rot, turn_at, g);
   f32x4 M = {0.f, 0.f, 0.f, 0.f};  // M[4 g + e][row] of the token's rows
-  u32x2 hi = {0, 0}, lo = {0, 0};  // in two bf16 numbers
+  [[maybe_unused]] s16x4 M_part[3] = {};
   wave_lds_fence();
   if (p.normalize) {
     const float* const w_of = W + (row >> lg) * H;
@@ -907,15 +907,18 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = there ? ac[e] * w_of[h + e] : 0.f;
       if constexpr (sizeof(T) == 2) {
-        u32x4 wh, wl;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          wh[e] = pack_bf16(w[2 * e], w[2 * e + 1]);
-          wl[e] = pack_bf16(w[2 * e] - bf16lo_to_f32(wh[e]), w[2 * e + 1] - bf16hi_to_f32(wh[e]));
-        }
         const bf16x8 f = __builtin_bit_cast(bf16x8, ac.x[0]);
-        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, wl), M, 0, 0, 0);
-        M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, wh), M, 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+          u32x4 part;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            part[e] = pack_bf16(w[2 * e], w[2 * e + 1]);
+            w[2 * e] -= bf16lo_to_f32(part[e]);
+            w[2 * e + 1] -= bf16hi_to_f32(part[e]);
+          }
+          M = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, part), M, 0, 0, 0);
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) M = __builtin_amdgcn_mfma_f32_16x16x4f32(ac[e], w[e], M, 0, 0, 0);
@@ -925,18 +928,16 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if ((4 * g + e) >> lg != row >> lg) M[e] = 0.f;
-    if constexpr (sizeof(T) == 2) {
-      hi = u32x2{pack_bf16(M[0], M[1]), pack_bf16(M[2], M[3])};
-      lo = u32x2{pack_bf16(M[0] - bf16lo_to_f32(hi[0]), M[1] - bf16hi_to_f32(hi[0])), pack_bf16(M[2] - bf16lo_to_f32(hi[1]), M[3] - bf16hi_to_f32(hi[1]))};
-    }
+    if constexpr (sizeof(T) == 2) in_three(M, M_part);
   }
   // the mixture of the b rows for this lane's row: element e of piece n is d = 32 (n / 2) + 8 g + 4 (n % 2) + e
   auto mix = [&](int n) __attribute__((always_inline)) {
     f32x4 out = {0.f, 0.f, 0.f, 0.f};
     if constexpr (sizeof(T) == 2) {
       const s16x4 f = rows_transposed<D>(rows, row, g, 32 * (n / 2) + 8 * (row & 3) + 4 * (n % 2));
-      out = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, lo), out, 0, 0, 0);
-      return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, hi), out, 0, 0, 0);
+#pragma unroll
+      for (int x = 2; x >= 0; --x) out = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, M_part[x], out, 0, 0, 0);
+      return out;
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)

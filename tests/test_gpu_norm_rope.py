@@ -554,3 +554,18 @@ def test_ranks_that_cancel(gpu, dtype, h, d, rq, rk, apart, kernel):
         others[n][:, ::3] = x[n][:, ::3]
     beside = tpa.tpa_norm_rope(others["q"].to(gpu), others["k"].to(gpu), **kw)
     assert all(torch.equal(a[:, ::3], b[:, ::3]) for a, b in zip(got, beside))
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("h,d,rq,rk", [(16, 128, 2, 6), (32, 64, 4, 16), (8, 64, 8, 2)])
+@pytest.mark.parametrize("apart", [5, 7, 9])
+def test_gradients_of_ranks_that_cancel(gpu, dtype, h, d, rq, rk, apart, kernel):
+    """The same of the gradients, which hold the cube of the norm and sums over the ranks that cancel."""
+    x = cancelling(apart, 2, 21, h, d, rq, rk, dtype)
+    kw = call(x, h, None, gpu, kernel=kernel)
+    grads = tpa.tpa_norm_rope_bwd(x["q"].to(gpu), x["k"].to(gpu), dq_out=x["dq"].to(gpu), dk_out=x["dk"].to(gpu), **kw)
+    c, s = angles(x["pos"], [d // 2], x["cos"], x["sin"], d)
+    for i, n in enumerate("qk"):
+        _, _, grad, g_slack = first_power(x[n].double(), h, x["w" + n].double(), c, s, 1e-6, x["d" + n].double())
+        near(grads[i], grad, g_slack, dtype, "d" + n)
