@@ -343,7 +343,8 @@ typedef struct TpaNormRopeArgs {
   int32_t B, l, H, D, rq, rk;       /* D even, at most 256 */
   int32_t rope_len, dtype, weight_dtype;
   int32_t kernel;                   /* TPA_KERNEL_*: the MFMA kernel takes D in {64, 128}, H % 8 == 0, ranks up to 16, sections % 4 == 0 and
-                                       16-byte aligned rows */
+                                       16-byte aligned rows (cos, sin and factors); backward, whose workgroups hold a number for each head of up
+                                       to 4 * 16 tokens in 160 KiB of LDS, H up to 504, to 1008 where no rank is 1 */
   int32_t normalize;                /* 0: s_h = 1 */
   float eps;
 } TpaNormRopeArgs;

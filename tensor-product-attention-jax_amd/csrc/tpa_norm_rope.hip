@@ -51,6 +51,7 @@ struct NormRopeBwdParams {
   float eps;
   float* partial;  // [side][kPartials][D]
 };
+constexpr size_t kMostLds = 160 * 1024;
 constexpr int kPartials = 768;  // partial sums of each weight's gradient, at most
 
 __device__ __forceinline__ float weight_at(const void* w, int bf16, int d) {
@@ -1042,7 +1043,7 @@ bool fast_takes(const Args* a, const TpaFactor* const* fs, int n) {
     if ((reinterpret_cast<uintptr_t>(f.ptr) & 15) || f.stride_b % chunk || f.stride_l % chunk || f.stride_r % chunk) return false;
     if (f.stride_l < 0 || f.stride_r < 0 || f.stride_l > (1 << 25) || f.stride_r > (1 << 25)) return false;  // 16 tokens' offsets in 32 bits
   }
-  return !((reinterpret_cast<uintptr_t>(a->rope_cos) | reinterpret_cast<uintptr_t>(a->rope_sin) | reinterpret_cast<uintptr_t>(a->q_weight) | reinterpret_cast<uintptr_t>(a->k_weight)) & 15);
+  return !((reinterpret_cast<uintptr_t>(a->rope_cos) | reinterpret_cast<uintptr_t>(a->rope_sin)) & 15);
 }
 // entries that follow one another in every array are one: what positions count from then has to be given
 bool follows(const TpaFactor& f, int l) { return f.stride_b == f.stride_l * l; }
@@ -1073,6 +1074,10 @@ int launch_fast(NormRopeParams p, hipStream_t s) {
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
 inline int most_pairs(int rq, int rk, int H) { return (tokens_per_wave(rq) > tokens_per_wave(rk) ? tokens_per_wave(rq) : tokens_per_wave(rk)) * H; }
+size_t bwd_lds(int dtype, int D, int pairs) {
+  if (dtype == TPA_DTYPE_BF16) return D == 128 ? BwdLds<uint16_t, 128>::bytes(pairs) : BwdLds<uint16_t, 64>::bytes(pairs);
+  return D == 128 ? BwdLds<float, 128>::bytes(pairs) : BwdLds<float, 64>::bytes(pairs);
+}
 template <typename T, int D>
 int launch_fast_bwd(NormRopeBwdParams p, int (&parts)[2], hipStream_t s) {
   const int64_t tokens = (int64_t)p.B * p.l;
@@ -1089,25 +1094,29 @@ int launch_fast_bwd(NormRopeBwdParams p, int (&parts)[2], hipStream_t s) {
   // All workgroups are resident at once, and their waves take the same number of tokens' groups: what a wave has to do behind its last one - the weights'
   // gradients - is done once.  (With up to 768 workgroups
   // a side / so, us: 4 x 4096 tokens, 16 heads of 128, three axes 42.1 / 40.3, 4 x 2048, 24 heads 29.3 / 27.0.)
-  const int64_t resident = 256 * bwd_waves(sizeof(T), D, p.H > 16 ? 2 : 1);
+  const int pairs = most_pairs(p.side[0].R, p.side[1].R, p.H), wave = (int)BwdLds<T, D>::wave_bytes(pairs);
+  const size_t lds = BwdLds<T, D>::bytes(pairs);
+  const int64_t resident = 256 * std::min<int64_t>(bwd_waves(sizeof(T), D, p.H > 16 ? 2 : 1), kMostLds / lds);
   int64_t groups[2];
   for (int x = 0; x < 2; ++x) groups[x] = p.side[x].da_out.ptr ? (int64_t)p.B * ((p.l + tokens_per_wave(p.side[x].R) - 1) / tokens_per_wave(p.side[x].R)) : 0;
   auto parts_for = [&](int x, int64_t each) { return (groups[x] + each * kNormWaves - 1) / (each * kNormWaves); };
   int64_t each = std::max<int64_t>(1, (groups[0] + groups[1]) / (kNormWaves * resident));
   while (parts_for(0, each) + parts_for(1, each) > resident) ++each;
   for (int x = 0; x < 2; ++x) parts[x] = (int)parts_for(x, each);
-  const int pairs = most_pairs(p.side[0].R, p.side[1].R, p.H), wave = (int)BwdLds<T, D>::wave_bytes(pairs);
-  const size_t lds = BwdLds<T, D>::bytes(pairs);
   const bool axes = p.rot.n_axes > 1 || p.rot.last_of[3] < D / 2;
   const dim3 grid(parts[0] + parts[1]);
+  int rc = TPA_OK;
   with_heads(p.H, [&](auto vh) {
     constexpr int VH = decltype(vh)::value;
-    hipLaunchKernelGGL((axes ? norm_rope_bwd_kernel<T, D, true, VH> : norm_rope_bwd_kernel<T, D, false, VH>), grid, dim3(kNormWaves * 64), lds, s, p, parts[0], parts[1], wave);
+    auto kern = axes ? norm_rope_bwd_kernel<T, D, true, VH> : norm_rope_bwd_kernel<T, D, false, VH>;
+    static bool done[2][kMaxDevices] = {};
+    if (lds > 64 * 1024) rc = raise_lds_limit(done[axes], reinterpret_cast<const void*>(kern), kMostLds);
+    if (rc == TPA_OK) hipLaunchKernelGGL(kern, grid, dim3(kNormWaves * 64), lds, s, p, parts[0], parts[1], wave);
   });
+  if (rc != TPA_OK) return rc;
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
 
-constexpr size_t kMostLds = 160 * 1024;
 int check_sizes(int B, int l, int H, int D, int rq, int rk, int rope_len, int dtype, int weight_dtype, int kernel, int n_axes, const int32_t* sections) {
   if (dtype != TPA_DTYPE_F32 && dtype != TPA_DTYPE_BF16) return TPA_ERR_DTYPE;
   if (weight_dtype != TPA_DTYPE_F32 && weight_dtype != TPA_DTYPE_BF16) return TPA_ERR_DTYPE;
@@ -1200,8 +1209,7 @@ extern "C" int tpa_norm_rope_bwd(const TpaNormRopeBwdArgs* a, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   SumParams sum{p.partial, {p.side[0].d_weight, p.side[1].d_weight}, {0, 0}, a->D, p.weight_bf16};
   int rc;
-  if (fast_takes(a, &fs[0][0], 12) && (a->dtype == TPA_DTYPE_BF16 ? BwdLds<uint16_t, 128>::bytes(most_pairs(a->rq, a->rk, a->H))
-                                                                  : BwdLds<float, 128>::bytes(most_pairs(a->rq, a->rk, a->H))) <= 64 * 1024) {
+  if (fast_takes(a, &fs[0][0], 12) && bwd_lds(a->dtype, a->D, most_pairs(a->rq, a->rk, a->H)) <= kMostLds) {
     if (a->dtype == TPA_DTYPE_BF16) rc = a->D == 128 ? launch_fast_bwd<uint16_t, 128>(p, sum.count, s) : launch_fast_bwd<uint16_t, 64>(p, sum.count, s);
     else rc = a->D == 128 ? launch_fast_bwd<float, 128>(p, sum.count, s) : launch_fast_bwd<float, 64>(p, sum.count, s);
   } else {

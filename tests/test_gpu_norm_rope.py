@@ -569,3 +569,21 @@ def test_gradients_of_ranks_that_cancel(gpu, dtype, h, d, rq, rk, apart, kernel)
     for i, n in enumerate("qk"):
         _, _, grad, g_slack = first_power(x[n].double(), h, x["w" + n].double(), c, s, 1e-6, x["d" + n].double())
         near(grads[i], grad, g_slack, dtype, "d" + n)
+
+
+@pytest.mark.parametrize("dtype,h,d,rq,rk", [(torch.bfloat16, 192, 64, 1, 1), (torch.bfloat16, 192, 128, 1, 2), (torch.float32, 128, 64, 1, 1), (torch.float32, 128, 128, 2, 1), (torch.bfloat16, 512, 128, 1, 1)])
+def test_many_heads_at_rank_one(gpu, dtype, h, d, rq, rk):
+    """Sixteen tokens to a wave, each with a number for every head in LDS: the matrix-core kernels take them in both directions, weights at any address too."""
+    x = make(h, 2, 21, h, d, rq, rk, dtype)
+    kw = call(x, h, None, gpu, kernel=2)
+    for n in ("q_weight", "k_weight"):
+        kw[n] = torch.cat([kw[n].new_zeros(1), kw[n]])[1:]
+    q, k = (x[n].to(gpu) for n in "qk")
+    got = tpa.tpa_norm_rope(q, k, **kw)
+    grads = tpa.tpa_norm_rope_bwd(q, k, dq_out=x["dq"].to(gpu), dk_out=x["dk"].to(gpu), **kw)
+    c, s = angles(x["pos"], [d // 2], x["cos"], x["sin"], d)
+    for i, n in enumerate("qk"):
+        out, slack, grad, g_slack, dw, w_slack = side(x[n].double(), h, x["w" + n].double(), c, s, 1e-6, True, x["d" + n].double())
+        near(got[i], out, slack, dtype, n)
+        near(grads[i], grad, g_slack, dtype, "d" + n)
+        near(grads[2 + i], dw, w_slack, torch.float32, "dw" + n)
