@@ -354,7 +354,8 @@ typedef struct TpaNormRopeArgs {
  *   u_h = sum_r da'_r[h] a_r[h];  w_h = - s_h^3 u_h / (D R^2) (0 with normalize == 0)
  *   da_r[h] = s_h da'_r[h] + w_h sum_s G_rs a_s[h];   db_r = weight * e_r + sum_s (sum_h w_h a_r[h] a_s[h]) b_s
  *   d weight = sum over tokens and ranks of e_r * b_r
- * Every element of the gradients is written.  A side (q or k) whose d_a_out pointer is NULL has no gradient and none of its fields is read.
+ * Every element of the gradients is written.  A side (q or k) whose d_a_out pointer is NULL has no gradient, its weight among what has none, and
+ * none of its fields is read, its rank neither; without either side the call does nothing.
  */
 typedef struct TpaNormRopeBwdArgs {
   TpaFactor qa, qb, ka, kb;                 /* the forward's inputs */

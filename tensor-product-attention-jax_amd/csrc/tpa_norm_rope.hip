@@ -1032,8 +1032,8 @@ __global__ __launch_bounds__(kNormWaves * 64, bwd_waves(sizeof(T), D, VH)) void 
 
 // ---------------------------------------------------------------------------------------------- checks
 template <typename Args>
-bool fast_takes(const Args* a, const TpaFactor* const* fs, int n) {
-  if (a->kernel == TPA_KERNEL_GENERIC || (a->D != 64 && a->D != 128) || a->H % 8 || a->rq > 16 || a->rk > 16) return false;
+bool fast_takes(const Args* a, int rq, int rk, const TpaFactor* const* fs, int n) {
+  if (a->kernel == TPA_KERNEL_GENERIC || (a->D != 64 && a->D != 128) || a->H % 8 || rq > 16 || rk > 16) return false;
   if ((int64_t)a->B * a->l > (1 << 26)) return false;  // groups of tokens of every entry in 32 bits
   for (int i = 0; i < a->n_axes; ++i)
     if (a->sections[i] % 4) return false;
@@ -1168,7 +1168,7 @@ extern "C" int tpa_norm_rope(const TpaNormRopeArgs* a, void* stream) {
   p.B = a->B; p.l = a->l; p.H = a->H; p.D = a->D;
   p.weight_bf16 = a->weight_dtype == TPA_DTYPE_BF16; p.normalize = a->normalize != 0; p.eps = a->eps;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (fast_takes(a, fs, a->slots ? 12 : 8)) {
+  if (fast_takes(a, a->rq, a->rk, fs, a->slots ? 12 : 8)) {
     if (a->dtype == TPA_DTYPE_BF16) return a->D == 128 ? launch_fast<uint16_t, 128>(p, s) : launch_fast<uint16_t, 64>(p, s);
     return a->D == 128 ? launch_fast<float, 128>(p, s) : launch_fast<float, 64>(p, s);
   }
@@ -1190,15 +1190,25 @@ extern "C" size_t tpa_norm_rope_bwd_workspace_bytes(int32_t B, int32_t l, int32_
 extern "C" int tpa_norm_rope_bwd(const TpaNormRopeBwdArgs* a, void* stream) {
   using namespace tpa;
   if (!a) return TPA_ERR_NULL;
-  if (const int rc = check_sizes(a->B, a->l, a->H, a->D, a->rq, a->rk, a->rope_len, a->dtype, a->weight_dtype, a->kernel, a->n_axes, a->sections); rc != TPA_OK) return rc;
-  const TpaFactor* fs[2][6] = {{&a->qa, &a->qb, &a->dqa_out, &a->dqb_out, &a->dqa, &a->dqb}, {&a->ka, &a->kb, &a->dka_out, &a->dkb_out, &a->dka, &a->dkb}};
-  for (auto& side : fs)
-    for (const TpaFactor* f : side)
-      if (side[2]->ptr && !f->ptr) return TPA_ERR_NULL;
+  // a side without a gradient is as if it had the other's: nothing of its own is looked at
+  const bool q = a->dqa_out.ptr, k = a->dka_out.ptr;
+  const int rq = q || !k ? a->rq : a->rk, rk = k || !q ? a->rk : a->rq;
+  if (const int rc = check_sizes(a->B, a->l, a->H, a->D, q || k ? rq : 1, q || k ? rk : 1, a->rope_len, a->dtype, a->weight_dtype, a->kernel, a->n_axes, a->sections); rc != TPA_OK) return rc;
+  if (!q && !k) return TPA_OK;
+  const TpaFactor* fs[12] = {};
+  int n = 0;
+  if (q)
+    for (const TpaFactor* f : {&a->qa, &a->qb, &a->dqa_out, &a->dqb_out, &a->dqa, &a->dqb}) fs[n++] = f;
+  if (k)
+    for (const TpaFactor* f : {&a->ka, &a->kb, &a->dka_out, &a->dkb_out, &a->dka, &a->dkb}) fs[n++] = f;
+  for (int i = 0; i < n; ++i)
+    if (!fs[i]->ptr) return TPA_ERR_NULL;
   if (!a->rope_cos || !a->rope_sin) return TPA_ERR_NULL;
   NormRopeBwdParams p{};
-  p.side[0] = {a->qa, a->qb, a->dqa_out, a->dqb_out, a->dqa, a->dqb, a->q_weight, a->dqa_out.ptr ? a->dq_weight : nullptr, a->rq};
-  p.side[1] = {a->ka, a->kb, a->dka_out, a->dkb_out, a->dka, a->dkb, a->k_weight, a->dka_out.ptr ? a->dk_weight : nullptr, a->rk};
+  if (q) p.side[0] = {a->qa, a->qb, a->dqa_out, a->dqb_out, a->dqa, a->dqb, a->q_weight, a->dq_weight, rq};
+  if (k) p.side[1] = {a->ka, a->kb, a->dka_out, a->dkb_out, a->dka, a->dkb, a->k_weight, a->dk_weight, rk};
+  p.side[0].R = rq;
+  p.side[1].R = rk;
   const bool sums = p.side[0].d_weight || p.side[1].d_weight;
   if (sums && (!a->workspace || a->workspace_bytes < tpa_norm_rope_bwd_workspace_bytes(a->B, a->l, a->D))) return TPA_ERR_WORKSPACE;
   if (sums && (reinterpret_cast<uintptr_t>(a->workspace) & 15)) return TPA_ERR_ALIGN;
@@ -1209,12 +1219,12 @@ extern "C" int tpa_norm_rope_bwd(const TpaNormRopeBwdArgs* a, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   SumParams sum{p.partial, {p.side[0].d_weight, p.side[1].d_weight}, {0, 0}, a->D, p.weight_bf16};
   int rc;
-  if (fast_takes(a, &fs[0][0], 12) && bwd_lds(a->dtype, a->D, most_pairs(a->rq, a->rk, a->H)) <= kMostLds) {
+  if (fast_takes(a, rq, rk, fs, n) && bwd_lds(a->dtype, a->D, most_pairs(rq, rk, a->H)) <= kMostLds) {
     if (a->dtype == TPA_DTYPE_BF16) rc = a->D == 128 ? launch_fast_bwd<uint16_t, 128>(p, sum.count, s) : launch_fast_bwd<uint16_t, 64>(p, sum.count, s);
     else rc = a->D == 128 ? launch_fast_bwd<float, 128>(p, sum.count, s) : launch_fast_bwd<float, 64>(p, sum.count, s);
   } else {
     if (a->kernel == TPA_KERNEL_MFMA) return TPA_ERR_UNSUPPORTED;
-    const size_t lds = any_lds(a->rq > a->rk ? a->rq : a->rk, a->H, a->D, true);
+    const size_t lds = any_lds(rq > rk ? rq : rk, a->H, a->D, true);
     if (lds > kMostLds) return TPA_ERR_SHAPE;
     const int64_t tokens = (int64_t)a->B * a->l;
     const int groups = sum.count[0] = sum.count[1] = (int)(tokens < kPartials ? tokens : kPartials);

@@ -587,3 +587,36 @@ def test_many_heads_at_rank_one(gpu, dtype, h, d, rq, rk):
         near(got[i], out, slack, dtype, n)
         near(grads[i], grad, g_slack, dtype, "d" + n)
         near(grads[2 + i], dw, w_slack, torch.float32, "dw" + n)
+
+
+@pytest.mark.parametrize("gone", ["q", "k", "qk"])
+def test_a_side_without_a_gradient_is_not_looked_at(gpu, gone):
+    """The C entry point with one side's gradient, the other side's fields left as anything."""
+    import ctypes
+
+    from tpa import _dispatch as dispatch
+
+    h, d, rq, rk = 16, 64, 6, 2
+    x = make(53, 2, 37, h, d, rq, rk, torch.bfloat16)
+    kw = call(x, h, None, gpu)
+    arrays = {n: x[n].to(gpu) for n in ("q", "k", "dq", "dk")}
+    want = tpa.tpa_norm_rope_bwd(arrays["q"], arrays["k"], dq_out=arrays["dq"], dk_out=arrays["dk"], kernel=2, **kw)
+    grads, d_weights, fields = {}, {}, {}
+    for n in "qk":
+        grads[n], d_weights[n] = torch.zeros_like(arrays[n]), torch.zeros(d, device=gpu)
+        for part, at in (("a", slice(0, h)), ("b", slice(h, None))):
+            for name, t in ((n + part, arrays[n]), (f"d{n}{part}_out", arrays["d" + n]), (f"d{n}{part}", grads[n])):
+                fields[name] = dispatch.factor(t[..., at]) if n not in gone else dispatch.TpaFactor(None if name.endswith("a_out") else 6, 3, -5, 7)
+    ws = torch.empty(1 << 22, dtype=torch.uint8, device=gpu)
+    positions = kw["positions"].contiguous()
+    args = dispatch.TpaNormRopeBwdArgs(
+        **fields, dq_weight=d_weights["q"].data_ptr(), dk_weight=d_weights["k"].data_ptr(), positions=positions.data_ptr(), rope_cos=kw["rope_cos"].data_ptr(),
+        rope_sin=kw["rope_sin"].data_ptr(), q_weight=3 if "q" in gone else kw["q_weight"].data_ptr(), k_weight=3 if "k" in gone else kw["k_weight"].data_ptr(), n_axes=1,
+        sections=(ctypes.c_int32 * 4)(d // 2), B=2, l=37, H=h, D=d, rq=-1 if "q" in gone else rq, rk=99 if "k" in gone else rk, rope_len=len(kw["rope_cos"]),
+        dtype=1, weight_dtype=0, kernel=2, normalize=1, eps=1e-6, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    torch.cuda.synchronize()
+    assert dispatch.load_library().tpa_norm_rope_bwd(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    for i, n in enumerate("qk"):
+        assert torch.equal(grads[n], torch.zeros_like(grads[n]) if n in gone else want[i])
+        assert torch.equal(d_weights[n], torch.zeros_like(d_weights[n]) if n in gone else want[2 + i])
