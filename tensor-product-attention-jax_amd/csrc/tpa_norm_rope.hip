@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kAnyThreads) void norm_rope_bwd_any_kernel(NormRope
     for (int h = tid; h < H; h += kAnyThreads) {
       float u = 0.f;
       for (int r = 0; r < R; ++r) u += da[r * H + h] * a[r * H + h];
-      w[h] = p.normalize ? -s[h] * s[h] * s[h] * u / ((float)D * R * R) : 0.f;
+      w[h] = p.normalize ? -(s[h] * u) * (s[h] / ((float)D * R * R)) * s[h] : 0.f;  // (the cube alone may pass 2^128)
       for (int r = 0; r < R; ++r) {
         double y = 0;
         if (p.normalize)
@@ -878,7 +878,7 @@ __device__ __forceinline__ void norm_rope_bwd_rows(const NormRopeBwdParams& p, c
         inverse_norms<T>(square, inv, p.eps, lg, scale);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float w = -scale[j] * scale[j] * scale[j] * u[j] * (float)inv;
+          const float w = -(scale[j] * u[j]) * (scale[j] * (float)inv) * scale[j];  // (the cube alone may pass 2^128)
           da[j][v] = da[j][v] * scale[j] + w * (float)y[j];
           const int rj = Sums<T>::row(g, j);
           if ((rj & ((1 << lg) - 1)) == 0 && h < H) W[(rj >> lg) * H + h + v] = w;

@@ -620,3 +620,19 @@ def test_a_side_without_a_gradient_is_not_looked_at(gpu, gone):
     for i, n in enumerate("qk"):
         assert torch.equal(grads[n], torch.zeros_like(grads[n]) if n in gone else want[i])
         assert torch.equal(d_weights[n], torch.zeros_like(d_weights[n]) if n in gone else want[2 + i])
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_small_head_vectors_without_eps(gpu, dtype, kernel):
+    """Head vectors of about 2^-43 and eps 0: the cube of 2^43 is no number of 32 bits, the gradients are."""
+    h, d = 8, 128
+    x = make(59, 1, 11, h, d, 16, 15, dtype)
+    for n in "qk":
+        x[n][..., h:] *= 2.0**-41
+    kw = call(x, h, None, gpu, kernel=kernel, eps=0.0)
+    grads = tpa.tpa_norm_rope_bwd(x["q"].to(gpu), x["k"].to(gpu), dq_out=x["dq"].to(gpu), dk_out=x["dk"].to(gpu), **kw)
+    c, s = angles(x["pos"], [d // 2], x["cos"], x["sin"], d)
+    for i, n in enumerate("qk"):
+        _, _, grad, g_slack, _, _ = side(x[n].double(), h, x["w" + n].double(), c, s, 0.0, True, x["d" + n].double())
+        near(grads[i], grad, g_slack, dtype, "d" + n)
