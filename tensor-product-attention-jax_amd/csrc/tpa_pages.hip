@@ -93,9 +93,9 @@ __global__ __launch_bounds__(kThreads) void page_tables_kernel(PageTablesParams 
   }
   __syncthreads();
 
-  const int64_t begin = (int64_t)blockIdx.x * p.rows_per_group;
-  const int stop = (int)min(begin + p.rows_per_group, (int64_t)p.num_tokens);
-  for (int r = (int)begin + tid; r < stop; r += kThreads) {
+  const uint32_t begin = blockIdx.x * (uint32_t)p.rows_per_group, stop = min(begin + (uint32_t)p.rows_per_group, (uint32_t)p.num_tokens);
+  for (uint32_t next = begin + tid; next < stop; next += kThreads) {  // (behind the last row up to 2^31 + 255)
+    const int r = (int)next;
     if (r >= ends[p.B - 1]) {
       p.slots[r] = -1;
       p.positions[r] = 0;

@@ -142,3 +142,14 @@ def test_under_inference_mode(gpu):
         after = after + 1
     assert slots.tolist() == [20, 21, 22, 24, 25, 26, 27, 28, 29, 30, 31, 32, -1, -1] and starts.tolist() == [0, 3, 12]
     assert after.tolist() == [4, 10] and int(start) == 4 and table.tolist() == [[5, -1, -1, -1], [6, 7, 8, -1]] and positions[:3].tolist() == [0, 1, 2]
+
+
+@pytest.mark.parametrize("rows", [2**31 - 1, 2**31 - 300])
+def test_the_most_rows(gpu, rows):
+    """As many rows as 31 bits hold: the padding behind the tokens ends with the arrays."""
+    table, free = torch.zeros((2, 4), dtype=torch.int32, device=gpu), torch.arange(9, dtype=torch.int32, device=gpu)
+    slots, positions, starts, after, start = tpa.tpa_page_tables(torch.tensor([0, 3], device=gpu), torch.tensor([2, 1], device=gpu), table, free, page_size=4, num_tokens=rows)
+    assert slots[:3].tolist() == [0, 1, 3] and positions[:3].tolist() == [0, 1, 3] and starts.tolist() == [0, 2, 3] and after.tolist() == [2, 4] and start.tolist() == [1]
+    for first in range(3, rows, 2**28):
+        assert (slots[first : first + 2**28] == -1).all() and not positions[first : first + 2**28].any()
+    assert len(slots) == len(positions) == rows
