@@ -297,6 +297,7 @@ size_t tpa_cache_append_workspace_bytes(int32_t B, int32_t n, int32_t d_model, i
  *   than the row has room for), come from free_pages[free_start ..], the requests served in order, and are written into the row;
  *   new_kv_lengths[b] = kv_lengths[b] + its new tokens that have a page: tokens past the table's row or the last free page have none
  *   positions[row] = kv_lengths[b] + (row - starts[b]);  slots[row] = page * page_size + position % page_size, or -1 without a page
+ *   and for a page below zero or one whose slots 31 bits do not hold
  *   rows from starts[B] on: slot -1, position 0.   new_free_start = free_start + pages taken.
  * Lengths and counts below zero count as zero, lengths past the table's row as its end.  Nothing else of page_table is written.
  */

@@ -113,11 +113,16 @@ __global__ __launch_bounds__(kThreads) void page_tables_kernel(PageTablesParams 
     if (pos < cap) {
       const int nth = (int)pos / p.page_size, in_page = (int)pos - nth * p.page_size;
       int32_t* const entry = p.page_table + (int64_t)lo * p.pages_per_seq + nth;
+      // of a page that 31 bits do not number, or none: no slot
+      auto slot_of = [&](int page) {
+        const int64_t at = (int64_t)page * p.page_size + in_page;
+        return page >= 0 && at <= INT32_MAX ? (int)at : -1;
+      };
       if (nth < have) {
-        slot = *entry * p.page_size + in_page;
+        slot = slot_of(*entry);
       } else if (const int64_t at = (int64_t)firsts[lo] + nth - have; at < p.num_free) {
         const int page = p.free_pages[at];
-        slot = page * p.page_size + in_page;
+        slot = slot_of(page);
         if (in_page == 0) *entry = page;  // the token that opens a page
       }
     }

@@ -153,3 +153,14 @@ def test_the_most_rows(gpu, rows):
     for first in range(3, rows, 2**28):
         assert (slots[first : first + 2**28] == -1).all() and not positions[first : first + 2**28].any()
     assert len(slots) == len(positions) == rows
+
+
+def test_pages_whose_slots_31_bits_do_not_hold(gpu):
+    """A page so far back, or no page at all (-1, or anything below zero), gives no slot, never another page's."""
+    far = 2**31 // 16
+    table = torch.tensor([[far, 3], [-1, 3], [-far - 1, 3], [far - 1, 3]], dtype=torch.int32, device=gpu)
+    free = torch.tensor([far * 2, -5, far + 7, far - 2], dtype=torch.int32, device=gpu)
+    got = tpa.tpa_page_tables(torch.tensor([2, 2, 2, 2], device=gpu), torch.ones(4, dtype=torch.int32, device=gpu), table, free, page_size=16, num_tokens=4)
+    assert got[0].tolist() == [-1, -1, -1, (far - 1) * 16 + 2] and got[1].tolist() == [2] * 4
+    got = tpa.tpa_page_tables(torch.tensor([16, 16, 16, 16], device=gpu), torch.ones(4, dtype=torch.int32, device=gpu), table, free, page_size=16, num_tokens=4)
+    assert got[0].tolist() == [-1, -1, -1, (far - 2) * 16] and got[4].tolist() == [4]
