@@ -59,6 +59,7 @@ __global__ __launch_bounds__(kThreads) void page_tables_kernel(PageTablesParams 
 
   // this thread's requests, side by side: their tokens, then the pages that these open, then both in LDS
   const int each = (p.B + kThreads - 1) / kThreads, b0 = min(tid * each, p.B), b1 = min(b0 + each, p.B);
+  auto pages_of = [&](int tokens) { return (int)(((uint32_t)tokens + (uint32_t)p.page_size - 1) / (uint32_t)p.page_size); };  // (both below 2^31)
   auto length_of = [&](int b) { return max(0, min(p.kv_lengths[b], cap)); };
   uint32_t tokens = 0;
   for (int b = b0; b < b1; ++b) tokens = stop_at(tokens, (uint32_t)max(p.new_tokens[b], 0), p.num_tokens);
@@ -68,9 +69,9 @@ __global__ __launch_bounds__(kThreads) void page_tables_kernel(PageTablesParams 
     const uint32_t next = stop_at(row, (uint32_t)max(p.new_tokens[b], 0), p.num_tokens);
     len = length_of(b);
     end = min((int)(next - row), cap - len) + len;
-    have = (len + p.page_size - 1) / p.page_size;
+    have = pages_of(len);
     row = next;
-    return (end + p.page_size - 1) / p.page_size - have;
+    return pages_of(end) - have;
   };
   uint32_t pages = 0, row = row0;
   for (int b = b0, len, end, have; b < b1; ++b) pages = stop_at(pages, place(b, row, len, end, have), p.num_free);
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(kThreads) void page_tables_kernel(PageTablesParams 
       if (ends[mid] > r) hi = mid;
       else lo = mid + 1;
     }
-    const int len = length_of(lo), have = (len + p.page_size - 1) / p.page_size;
+    const int len = length_of(lo), have = pages_of(len);
     const int64_t pos = (int64_t)len + r - (lo ? ends[lo - 1] : 0);
     int slot = -1;
     if (pos < cap) {

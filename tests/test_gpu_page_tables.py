@@ -164,3 +164,30 @@ def test_pages_whose_slots_31_bits_do_not_hold(gpu):
     assert got[0].tolist() == [-1, -1, -1, (far - 1) * 16 + 2] and got[1].tolist() == [2] * 4
     got = tpa.tpa_page_tables(torch.tensor([16, 16, 16, 16], device=gpu), torch.ones(4, dtype=torch.int32, device=gpu), table, free, page_size=16, num_tokens=4)
     assert got[0].tolist() == [-1, -1, -1, (far - 2) * 16] and got[4].tolist() == [4]
+
+
+@pytest.mark.parametrize("page,pages", [(2**31 - 1, 1), (2**30, 1), (2**30 - 1, 2), (2**29 + 5, 3)])
+def test_the_largest_pages(gpu, page, pages):
+    """Pages whose sizes 31 bits just hold, request by request in Python's integers; a slot past 31 bits is none, a position past them is their end."""
+    cap, n_free, rows, most = page * pages, 9, 23, 2**31 - 1
+    lengths, news = [0, 1, 2, cap - 3, cap, page, page - 1, cap - 1], [3, 1, 4, 9, 2, 1, 2, 1]
+    ids = list(range(len(lengths) * pages + n_free))
+    table, free = [ids[i * pages : (i + 1) * pages] for i in range(len(lengths))], ids[len(lengths) * pages :]
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu)
+    got_table = dev(table)
+    got = tpa.tpa_page_tables(dev(lengths), dev(news), got_table, dev(free), page_size=page, num_tokens=rows, free_start=dev([1]))
+    slots, positions, starts, after, at = [], [], [0], [], 1
+    for row, length, new in zip(table, lengths, news):
+        have = -(-length // page)
+        opened = max(0, -(-min(length + new, cap) // page) - have)
+        row[have : have + opened] = free[at : at + opened]
+        at += opened
+        for position in range(length, length + new):
+            slot = row[position // page] * page + position % page if position < cap else -1
+            slots.append(slot if slot <= most else -1)
+            positions.append(min(position, most))
+        starts.append(len(slots))
+        after.append(min(length + new, cap))
+    assert len(slots) == rows and at <= n_free
+    for name, g, w in zip(("slots", "positions", "starts", "new_kv_lengths", "new_free_start", "page_table"), (*got, got_table), (slots, positions, starts, after, [at], table)):
+        assert g.tolist() == w, name
