@@ -731,16 +731,24 @@ PyObject* page_tables(PyObject*, PyObject* const* args, Py_ssize_t n) {
       out[i].unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
       at += (sizes[i] + 63) / 64 * 64;
     }
-    TpaPageTablesArgs a{};
-    a.kv_lengths = ids_ptr(len); a.new_tokens = ids_ptr(fresh);
-    a.page_table = static_cast<int32_t*>(table.data_ptr());
-    a.free_pages = ids_ptr(pool); a.free_start = ids_ptr(start);
-    int32_t* to[5];
-    for (int i = 0; i < 5; ++i) to[i] = static_cast<int32_t*>(out[i].data_ptr());
-    a.slots = to[0]; a.positions = to[1]; a.starts = to[2]; a.new_kv_lengths = to[3]; a.new_free_start = to[4];
-    a.B = (int)b; a.pages_per_seq = (int)table.size(1); a.page_size = (int)page; a.num_free = (int)pool.numel(); a.num_tokens = (int)rows;
-    check("tpa_page_tables", lib.tpa_page_tables(&a, stream_of(device)));
-    written(table);
+    if (b) {
+      TpaPageTablesArgs a{};
+      a.kv_lengths = ids_ptr(len); a.new_tokens = ids_ptr(fresh);
+      a.page_table = static_cast<int32_t*>(table.data_ptr());
+      a.free_pages = ids_ptr(pool); a.free_start = ids_ptr(start);
+      int32_t* to[5];
+      for (int i = 0; i < 5; ++i) to[i] = static_cast<int32_t*>(out[i].data_ptr());
+      a.slots = to[0]; a.positions = to[1]; a.starts = to[2]; a.new_kv_lengths = to[3]; a.new_free_start = to[4];
+      a.B = (int)b; a.pages_per_seq = (int)table.size(1); a.page_size = (int)page; a.num_free = (int)pool.numel(); a.num_tokens = (int)rows;
+      check("tpa_page_tables", lib.tpa_page_tables(&a, stream_of(device)));
+      written(table);
+    } else {  // no requests: rows of padding, no page taken
+      out[0].fill_(-1);
+      out[1].zero_();
+      out[2].zero_();
+      if (start.defined()) out[4].copy_(start.view({1}).clamp(0, pool.numel()));
+      else out[4].zero_();
+    }
   }
   return tuple_of({out[0], out[1], out[2], out[3], out[4]});
   END_CALL

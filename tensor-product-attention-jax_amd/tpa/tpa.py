@@ -252,6 +252,8 @@ def tpa_page_tables(kv_lengths, new_tokens, page_table, free_pages, *, page_size
         starts[b + 1]          first row of every request
         new_kv_lengths[b]      lengths with the new tokens that have a slot, for `tpa_decode` and the next step
         new_free_start[1]      `free_start` and the pages taken
+
+    A step without requests (b = 0) is one of padding.
     """
     return _call(
         _d.host_calls().page_tables, (kv_lengths, new_tokens, free_pages, free_start), page_table, int(page_size), int(num_tokens)

@@ -191,3 +191,12 @@ def test_the_largest_pages(gpu, page, pages):
     assert len(slots) == rows and at <= n_free
     for name, g, w in zip(("slots", "positions", "starts", "new_kv_lengths", "new_free_start", "page_table"), (*got, got_table), (slots, positions, starts, after, [at], table)):
         assert g.tolist() == w, name
+
+
+def test_no_requests(gpu):
+    """A step in which nothing runs: rows of padding, no page taken; the free list's start inside the list."""
+    none = torch.zeros(0, dtype=torch.int32, device=gpu)
+    table, free = torch.zeros((0, 4), dtype=torch.int32, device=gpu), torch.arange(9, dtype=torch.int32, device=gpu)
+    for rows, start, want in ((5, None, 0), (0, 3, 3), (700, 99, 9), (1, -2, 0)):
+        got = tpa.tpa_page_tables(none, none, table, free, page_size=4, num_tokens=rows, free_start=None if start is None else torch.tensor([start], device=gpu))
+        assert [t.tolist() for t in got] == [[-1] * rows, [0] * rows, [0], [], [want]] and all(t.dtype == torch.int32 for t in got)
