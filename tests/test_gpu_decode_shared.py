@@ -383,3 +383,70 @@ def test_nan_is_not_taken_for_no_key(gpu, dtype, where):
                 assert o[i].isnan().all() and (lse[i] == -math.inf).all(), kernel
             else:
                 assert torch.equal(o[i], clean[kernel][0][i]) and torch.equal(lse[i], clean[kernel][1][i]), (kernel, i)
+
+
+@pytest.mark.parametrize(
+    "b,lq,prefix,own,h,d,rk,dtype,page",
+    [
+        (64, 1, 6000, 40, 32, 128, 2, BF, 64),      # eight waves of columns over the prefix
+        (64, 1, 5000, 40, 32, 128, 2, BF, 0),
+        (64, 2, 70, 3000, 32, 128, 2, BF, 64),      # own keys
+        (24, 4, 500, 2500, 64, 64, 4, BF, 32),      # two blocks of heads, rank 4
+        (100, 4, 500, 1500, 8, 128, 8, BF, 0),      # rank 8, a set of four rows
+        (33, 3, 1200, 2500, 24, 64, 1, BF, 64),     # 24 heads, rank 1
+        (64, 1, 4000, 40, 32, 128, 2, F32, 64),
+        (64, 1, 300, 1600, 16, 128, 2, F32, 0),
+        (70, 2, 1500, 1500, 32, 64, 4, F32, 48),
+    ],
+)
+def test_ranges_of_many_tiles(gpu, b, lq, prefix, own, h, d, rk, dtype, page):
+    """Workgroups that go round the two tile buffers several times, over the prefix and over own keys of all lengths."""
+    rq, lk, scale = 6, prefix + own, d**-0.5
+    if page:
+        lk = -(-lk // page) * page
+    g = torch.Generator(device=gpu).manual_seed(b + prefix)
+    n = lambda *s: torch.randn(s, generator=g, device=gpu)
+    qa, qb = (rq**0.5 * n(b, lq, rq, h)).to(dtype), n(b, lq, rq, d).to(dtype)
+    length = prefix + lq + torch.arange(b) * 7919 % (own - lq + 1)
+    length[b // 2] = prefix + own
+    if page:  # a pool in which nothing but the prefix and the rows' own tokens is a number
+        pages, whole = lk // page, prefix // page
+        ids = torch.randperm(whole + b * (pages - whole), generator=g, device=gpu)
+        table = torch.cat([ids[:whole].expand(b, whole), ids[whole:].view(b, -1)], 1)
+        caches = [torch.full((len(ids), page, rk, w), math.nan, dtype=dtype, device=gpu) for w in (h, d, h, d)]
+        place = lambda i, t: (table[i, t // page], t % page)
+    else:
+        table = None
+        caches = [torch.full((b, lk, rk, w), math.nan, dtype=dtype, device=gpu) for w in (h, d, h, d)]
+        place = lambda i, t: (torch.full_like(t, i), t)
+    first = torch.arange(prefix, device=gpu)
+    for x, c in enumerate(caches):
+        c[place(0, first)] = (n(prefix, rk, c.shape[3]) * (rk**0.5 if x == 0 else 1)).to(dtype)
+        for i in range(b):
+            t = torch.arange(prefix, int(length[i]), device=gpu)
+            c[place(i, t)] = (n(len(t), rk, c.shape[3]) * (rk**0.5 if x == 0 else 1)).to(dtype)
+    more = {} if table is None else dict(page_table=table.to(torch.int32).contiguous())
+    ranges, blocks = ranges_of(b, lq, prefix, lk, h, d, rk, qa, qb, caches, more.get("page_table"))
+    assert blocks >= 3 * (4 if dtype == BF else 2) * ranges
+    call = lambda: tpa.tpa_decode_shared(qa, qb, *caches, prefix_length=prefix, sm_scale=scale, kernel=2, kv_lengths=length.to(gpu), causal=2, **more)
+    got, got_lse = call()
+    assert all(torch.equal(x, y) for x, y in zip(call(), (got, got_lse)))
+    assert not got.isnan().any() and not got_lse.isnan().any()
+    half, split = torch.finfo(dtype).eps / 2, 2.0**-16 if dtype == BF else 0
+    for i in sorted({0, 1, b // 3, b // 2, b - 1}):
+        t = torch.arange(prefix, int(length[i]), device=gpu)
+        kv = [torch.cat([c[place(0, first)], c[place(i, t)]])[None] for c in caches]
+        with torch.device(gpu):
+            o, lse, size, xs = oracle(qa[i : i + 1], qb[i : i + 1], kv, prefix, length[i : i + 1].to(gpu), scale, 2, 0)
+        logit = (split + (2 * d + rk * rq) * U) * xs
+        slack = 2 * logit.transpose(1, 2)[..., None] * size + (half if dtype == BF else 0) * size + (lk + 16) * U * size
+        assert ((got_lse[i].double() - lse[0]).abs() <= (logit + (lk + 8) * U + 4 * U * lse.abs())[0]).all(), i
+        assert ((got[i].double() - o[0]).abs() <= (half * o.abs() + slack * (1 + half))[0]).all(), i
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_pages_whose_rows_are_no_power_of_two(gpu, dtype):
+    """Pages of 48 and 80 tokens at rank 2, of 24 at rank 4, of 96 at rank 1: whole blocks of rows, of which a page holds 3 or 5."""
+    for page, rk, prefix, lengths in ((48, 2, 200, [230, 480, 201, 192, 300]), (80, 2, 160, [161, 400, 240]), (24, 4, 100, [180, 101, 144]), (96, 1, 96, [97, 300, 96])):
+        check(gpu, len(lengths), 1, prefix, max(lengths) - prefix, 16, 64, 6, rk, dtype, 2, page=page, lengths=lengths)
+        check(gpu, len(lengths), 3, prefix, max(lengths) - prefix, 8, 128, 6, rk, dtype, 2, page=page, lengths=lengths, causal=2)

@@ -636,3 +636,35 @@ def test_small_head_vectors_without_eps(gpu, dtype, kernel):
     for i, n in enumerate("qk"):
         _, _, grad, g_slack, _, _ = side(x[n].double(), h, x["w" + n].double(), c, s, 0.0, True, x["d" + n].double())
         near(grads[i], grad, g_slack, dtype, "d" + n)
+
+
+@pytest.mark.parametrize(
+    "b,l,h,d,rq,rk,dtype,kernel,sections",
+    [
+        (3, 7001, 16, 128, 6, 2, torch.bfloat16, 2, None),          # several groups of tokens to a wave of the backward, unequal shares
+        (2, 9003, 64, 64, 16, 8, torch.bfloat16, 2, [8, 12, 12]),   # and, past 16384 groups, of the forward
+        (1, 20011, 8, 64, 6, 2, torch.float32, 2, None),
+        (1, 17003, 32, 128, 9, 3, torch.float32, 2, None),
+        (1, 5003, 8, 64, 6, 2, torch.bfloat16, 1, None),            # more tokens than workgroups of the plain kernels
+        (5, 1009, 3, 10, 5, 2, torch.float32, 0, None),
+    ],
+)
+def test_many_tokens(gpu, b, l, h, d, rq, rk, dtype, kernel, sections):
+    """Waves and workgroups that serve several groups of tokens.  A sum of a weight's gradient is a chain of what a lane or thread meets and 76 more."""
+    x = make(l, b, l, h, d, rq, rk, dtype, axes=len(sections or [0]))
+    kw = call(x, h, sections, gpu, kernel=kernel)
+    q, k = (x[n].to(gpu) for n in "qk")
+    got = tpa.tpa_norm_rope(q, k, **kw)
+    grads = tpa.tpa_norm_rope_bwd(q, k, dq_out=x["dq"].to(gpu), dk_out=x["dk"].to(gpu), **kw)
+    again = tpa.tpa_norm_rope_bwd(q, k, dq_out=x["dq"].to(gpu), dk_out=x["dk"].to(gpu), **kw)
+    assert all(torch.equal(g, w) for g, w in zip(grads, again))
+    with torch.device(gpu):
+        c, s = angles(x["pos"].to(gpu), sections or [d // 2], x["cos"].to(gpu), x["sin"].to(gpu), d)
+        for i, n in enumerate("qk"):
+            r = (rq, rk)[i]
+            chain = -(-b * l // 768) * r + 76  # at most: a workgroup of the plain kernels has every 768th token, a lane of the others fewer rows
+            ingredients = side(x[n].to(gpu).double(), h, x["w" + n].to(gpu).double(), c, s, 1e-6, True, x["d" + n].to(gpu).double())
+            out, slack, grad, g_slack, dw, w_slack = (t.cpu() for t in ingredients)
+            near(got[i], out, slack, dtype, n)
+            near(grads[i], grad, g_slack, dtype, "d" + n)
+            near(grads[2 + i], dw, w_slack * (chain / 128), torch.float32, "dw" + n)
