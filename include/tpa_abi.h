@@ -517,6 +517,8 @@ size_t tpa_norm_rope_bwd_workspace_bytes(int32_t B, int32_t l, int32_t D);
  * are taken to be those of entry 0, whose cache (or pages) alone is read for them, once for all entries; every entry's other
  * tokens are its own.  kv_lengths count both; an entry shorter than the prefix sees as much of it as its length says.  Entry 0's cache (row 0
  * of page_table) has to hold the prefix as far as any entry sees it, whatever entry 0's own length is.
+ * NaN in the logits of keys that a row sees gives the row NaN in o and lse; V factors that are not finite may reach, as 0 * inf, rows from
+ * which their token is hidden but which others of the batch that do see it are computed with.
  * num_splits must be 0; B lq H below 2^24.  Needs `workspace` of at least tpa_decode_shared_workspace_bytes(...) bytes, 256-byte aligned.  Matrix-core kernels take
  * bf16 and fp32 with dk == dv in {64, 128}, H % 8 == 0, rk in {1, 2, 4, 8} and rows as tpa_decode has them; any other problem,
  * paged ones too, runs on the vector units.

@@ -263,15 +263,15 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumParams p) {
 // numbers, 2^-27 of it off; for fp32 factors both are products in 64 bits.
 // The rows of a wave's tokens stand in one product, so a token's rows meet zeros for the other tokens'; where those are not finite, 0 * inf
 // would spread, and the tokens take turns.
-// HBM bounds it: a token's factors come once and go once, forward at 4.1 to 4.9 TB/s in the cases below, backward, whose chain of products is longer, at
-// 3.1 to 3.7, where a plain copy of their size has about 4.5.  (With
+// HBM bounds it: a token's factors come once and go once, forward at 3.9 to 4.8 TB/s in the cases below, backward, whose chain of products is longer, at
+// 3.5 to 3.6, where a copy of 1 GiB has 5.15.  (With
 // G through LDS and R^2 products a head on the vector units, 310 registers and 1300 vector instructions per 16 rows, their backward
 // took 66 and 256 us.)
 typedef __attribute__((ext_vector_type(4))) double f64x4;
 constexpr int kNormWaves = 4;
 // Waves of a SIMD that the registers are kept to.  More of them hide more of the loads until they cost much scratch memory: us of the backward of
-// 4 x 4096 tokens, 16 heads of 128, at 2 / 3 waves 42.0 / 38.6, of 4 x 2048, 24 heads 29.1 / 37.5; of 8 x 2048, 64 heads of 64, ranks 16 and 8, at 3 / 4
-// 83 / 137; forward of the last at 4 / 5 / 6 waves 41.3 / 44.9 / 105.  (The factors of the next tokens asked for ahead take the registers of
+// 4 x 4096 tokens, 16 heads of 128, at 2 / 3 waves 39.0 / 34.3, of 4099 tokens, 32 heads, three axes 20.7 / 24.5; of 8 x 2048, 64 heads of 64, ranks 16
+// and 8, at 2 / 3 / 4 108 / 85 / 152; forward of the last at 3 / 4 / 5 / 6 waves 42.2 / 41.5 / 63.2 / 138.  (The factors of the next tokens asked for ahead take the registers of
 // a wave, which costs more than it hides.)
 constexpr int fwd_waves(int size, int d) { return size == 2 ? 4 : d == 64 ? 3 : 2; }
 constexpr int bwd_waves(int size, int d, int heads_of_lane) { return size == 2 && (d == 64 || heads_of_lane == 1) ? 3 : 2; }

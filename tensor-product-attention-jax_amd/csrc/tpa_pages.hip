@@ -6,7 +6,7 @@
 // reads, and then serves its own tokens from LDS.  Nothing passes between workgroups, and nothing depends on their order: a token
 // that reads the table reads entries below ceil(length / page size), one that writes it writes those above.
 //
-// Latency bounds it: the requests' lengths, two sums over the workgroup, a search, a table entry.  3.5 us for a token of each of 64 requests, 5.8 us for 384
+// Latency bounds it: the requests' lengths, two sums over the workgroup, a search, a table entry.  3.4 us for a token of each of 64 requests, 5.6 us for 384
 // requests with up to 512 tokens each (0.3 MB read and written, 0.06 us at the rate of a copy); the host's call takes 7.
 #include "tpa_common.h"
 

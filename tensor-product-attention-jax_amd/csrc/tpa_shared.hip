@@ -5,7 +5,7 @@
 //
 // What bounds it: over a long prefix the matrix cores, at the power that the chip has for them - a tile of 4 blocks (64 tokens of rank 2, 256 columns of
 // 128) takes 5.8 us, of which its 768 matrix instructions are 3.7 by themselves and LDS 3.0 - and the way in and out: 6 us to a
-// first tile, 2 to 3 for the parts, 4 to 9 for the merge.  64 sequences over 8192 + 700 tokens, 32 heads: 51.5 us; 32 over 32768 + 300: 76.4; 4 over
+// first tile, 2 to 3 for the parts, 4 to 9 for the merge.  64 sequences over 8192 + 700 tokens, 32 heads: 50.6 us; 32 over 32768 + 300: 76.2; 4 over
 // 1500 + 120, 16 heads: 15.2, as long as the host's call.
 #include <algorithm>
 #include <cmath>
@@ -129,7 +129,8 @@ __global__ __launch_bounds__(kAnyThreads) void shared_any_kernel(SharedParams p)
 // products of the rows (t, r) with the columns.  The rows serve every column, so a workgroup takes a tile of 4 blocks of 32 rows
 // once for up to 256 columns: the columns of the prefix are those of all sequences, 32 to a wave; where there are fewer (a sequence's
 // own keys, few sequences) waves share the tile's blocks and are joined at the end.  Tiles go from memory straight to LDS, two
-// buffers.  (Dense keys would halve the matrix work at rank 2, but every wave would have to build them: 32 columns a head use a key once.)
+// buffers.  (Dense keys would halve the matrix work at rank 2, but every wave would have to build them: 32 columns a head use a key
+// once.  By count only; sets of 32 query rows of one head, which would use a key 32 times, were not built either.)
 // Qm is kept as two bf16 numbers, 2^-17 of it off: with one the logits carry the rounding of Qm, 2^-9 each, and the output's error
 // grows by half; the second costs 8 of 24 matrix instructions a block.  The weights p va are rounded to bf16 once, sums are fp32.
 // In fp32 nothing is rounded, a tile has 2 blocks, and what a product takes is read as it lies: over d the halves of a wave take d = 8 m + 4 g + e
