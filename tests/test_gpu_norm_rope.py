@@ -668,3 +668,46 @@ def test_many_tokens(gpu, b, l, h, d, rq, rk, dtype, kernel, sections):
             near(got[i], out, slack, dtype, n)
             near(grads[i], grad, g_slack, dtype, "d" + n)
             near(grads[2 + i], dw, w_slack * (chain / 128), torch.float32, "dw" + n)
+
+
+@pytest.mark.parametrize("h,d,rq,rk", [(16, 128, 2, 6), (32, 64, 4, 16), (8, 64, 8, 2), (24, 128, 16, 4)])
+def test_ranks_that_cancel_in_a_cache_and_beside_values_that_are_not_finite(gpu, h, d, rq, rk):
+    """Written into a cache bit for bit what tpa_norm_rope gives; infinities and NaN of some tokens, a zero token, and tokens that do not cancel stay
+    with themselves, in both directions."""
+    x = cancelling(8, 2, 21, h, d, rq, rk, torch.bfloat16)
+    plain = make(61, 2, 21, h, d, rq, rk, torch.bfloat16)
+    for n in "qk":
+        x[n][:, 1::4] = plain[n][:, 1::4]
+    kw = call(x, h, None, gpu)
+    q, k, v, dq, dk = (x[n].to(torch.bfloat16).to(gpu) for n in ("q", "k", "v", "dq", "dk"))
+    want = tpa.tpa_norm_rope(q, k, kernel=2, **kw)
+    grads = tpa.tpa_norm_rope_bwd(q, k, dq_out=dq, dk_out=dk, kernel=2, **kw)
+    pools = [torch.zeros((4, 16, rk, w), dtype=torch.bfloat16, device=gpu) for w in (h, d, h, d)]
+    slots = torch.randperm(64, generator=torch.Generator().manual_seed(2))[:42].view(2, 21).to(gpu)
+    got = tpa.tpa_norm_rope_write(q, k, v, h, kw["rope_cos"], kw["rope_sin"], *pools, slots, kw["q_weight"], kw["k_weight"], kw["positions"], kernel=2)
+    assert torch.equal(got, want[0])
+    for pool, part in zip(pools, (want[1][..., :h], want[1][..., h:], v[..., :h], v[..., h:])):
+        assert torch.equal(pool.flatten(0, 1)[slots], part)
+    for y in (q, k):
+        y[0, 2, -1, h + 1], y[0, 5, 0, h + d - 1], y[1, 11, -1, 0], y[1, 14] = float("inf"), float("nan"), float("-inf"), 0
+    others = torch.ones(2, 21, dtype=torch.bool, device=gpu)
+    others[0, [2, 5]] = others[1, [11, 14]] = False
+    again = tpa.tpa_norm_rope(q, k, kernel=2, **kw)
+    again_grads = tpa.tpa_norm_rope_bwd(q, k, dq_out=dq, dk_out=dk, kernel=2, **kw)
+    for a, b in zip((*again, *again_grads[:2]), (*want, *grads[:2])):
+        assert torch.equal(a[others], b[others]) and not torch.equal(a, b)
+
+
+def test_the_most_heads(gpu):
+    """As many heads at rank 1 as the header names for every type and head size; one block more is the plain kernel's, or refused."""
+    for h, kernel in ((504, 2), (512, 0)):
+        x = make(h, 1, 17, h, 128, 1, 1, torch.float32)
+        kw = call(x, h, None, gpu, kernel=kernel)
+        q, k = (x[n].to(gpu) for n in "qk")
+        grads = tpa.tpa_norm_rope_bwd(q, k, dq_out=x["dq"].to(gpu), dk_out=x["dk"].to(gpu), **kw)
+        c, s = angles(x["pos"], [64], x["cos"], x["sin"], 128)
+        for i, n in enumerate("qk"):
+            _, _, grad, g_slack, _, _ = side(x[n].double(), h, x["w" + n].double(), c, s, 1e-6, True, x["d" + n].double())
+            near(grads[i], grad, g_slack, torch.float32, "d" + n)
+    with pytest.raises(RuntimeError):
+        tpa.tpa_norm_rope_bwd(q, k, dq_out=x["dq"].to(gpu), dk_out=x["dk"].to(gpu), **dict(kw, kernel=2))
