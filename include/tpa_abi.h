@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define TPA_ABI_VERSION 12
+#define TPA_ABI_VERSION 13
 
 /* element types of the factor / output arrays */
 enum { TPA_DTYPE_F32 = 0, TPA_DTYPE_BF16 = 1 };
@@ -379,6 +379,154 @@ typedef struct TpaNormRopeBwdArgs {
   size_t workspace_bytes;
 } TpaNormRopeBwdArgs;
 
+/*
+ * A cache in 4 bits.  No counterpart in the reference.  A row holds the K (or V) factors of one token and rank, H + D numbers:
+ *   ceil(D/2) bytes of codes of b, ceil(H/2) bytes of codes of a, ceil(D/32) scales of b, ceil(H/32) scales of a, then bytes without a
+ *   meaning up to a multiple of four: tpa_fp4_row_bytes(H, D) in all.  Number 2i of a part is the low half of its byte i, 2i + 1 the high half.
+ * A code's lower three bits stand for 0, 0.5, 1, 1.5, 2, 3, 4, 6, its highest for the sign; the 32 numbers of a block (the last one may have
+ * fewer) are code * 2^(scale - 127).  Scale 255: every number of the block is NaN.
+ * Writing takes the power of two 2^e with e = floor(log2 m) - 2, m the block's largest magnitude, and the next one where m > 7.25 * 2^e (with
+ * 6, below which nothing is cut off, the values of a normal distribution are off by 0.1155 of their root mean square, with 8, where
+ * 2^e never goes up, 0.1149, with 7.25 0.1116); e between -125 and 125; codes to the nearest, halves to even, at most 6.  A block
+ * with an infinity or a NaN has scale 255.
+ */
+size_t tpa_fp4_row_bytes(int32_t H, int32_t D); /* 0 if a size is not positive */
+
+/*
+ * tpa_cache_write_fp4 / tpa_cache_read_fp4 arguments.  Token i of batch entry b is at place slots[b, i] % page_size of page slots[b, i] / page_size
+ * of the pools.  Writing reads the factors and drops tokens whose slot is outside 0 .. num_slots - 1; no slot may be there twice.
+ * Reading writes the factors (through their ptr), rounded once to dtype, zeros for such a token.
+ */
+typedef struct TpaFp4RowsArgs {
+  TpaFactor ka, kb, va, vb;     /* [B, l, rk, H|dk|H|dv], element type = dtype */
+  TpaFactor k_cache, v_cache;   /* pools of rows [page, token_in_page, rk, tpa_fp4_row_bytes(H, dk|dv)]; strides in bytes */
+  const int32_t* slots;         /* [B, l] */
+  int32_t page_size, num_slots; /* num_slots = pages of the pools * page_size */
+  int32_t B, l, H, dk, dv, rk;
+  int32_t dtype;
+} TpaFp4RowsArgs;
+
+/*
+ * tpa_decode_fp4 arguments: those of tpa_decode over a cache of rows in 4 bits.  Q, logits, mask and results are TpaFwdArgs', with K and V made from
+ * the numbers that the rows stand for.
+ */
+typedef struct TpaDecodeFp4Args {
+  TpaFactor qa, qb;             /* [B, lq, rq, H|dk], element type = dtype */
+  TpaFactor k_cache, v_cache;   /* [B, lk, rk, bytes], or with page_table pools [page, token_in_page, rk, bytes]; strides in bytes */
+  void* o;                      /* [B, lq, H, dv] contiguous, element type = dtype */
+  float* lse;                   /* [B, H, lq] or NULL */
+  int32_t B, lq, lk, H, dk, dv, rq, rk;
+  int32_t dtype;
+  float sm_scale;
+  int32_t causal, causal_offset; /* as in TpaFwdArgs */
+  int32_t kernel;               /* TPA_KERNEL_*: the MFMA kernel takes dk == dv in {64, 128}, H % 8 == 0, rk in {1, 2, 4, 8}, rows and strides of the cache at
+                                   multiples of 4 bytes */
+  const int32_t* kv_lengths;    /* [B] or NULL */
+  const int32_t* page_table;    /* [B, pages_per_seq] or NULL */
+  int32_t page_size, pages_per_seq; /* pages_per_seq * page_size >= lk */
+  int32_t num_pages;            /* of the pools: a page of the table outside them is read as the nearest one */
+  void* workspace;              /* tpa_decode_fp4_workspace_bytes(...), 256-byte aligned */
+  size_t workspace_bytes;
+} TpaDecodeFp4Args;
+
+/*
+ * tpa_beam_select arguments: the continuations of a step of beam search.  No counterpart in the reference.  Of request i the candidate (beam j, token v)
+ * has the value scores[i, j] + logits[i, j, v] - log sum_w exp(logits[i, j, w]); a finished beam has one candidate, (j, eos_token) with
+ * the value scores[i, j].  A value that is NaN or +inf counts as -inf.  The num_out largest values of each request, in falling order, equal ones by the lower beam * vocab + token:
+ *   new_scores[i, r] = the value;  parents[i, r] = i * beams + beam, the row of beams that it goes on from;  tokens[i, r];
+ *   new_finished[i, r] = finished[i, j], or the token is eos_token
+ * Values are compared in 64 bits; the logarithms in them are right to about 1e-7.
+ */
+typedef struct TpaBeamSelectArgs {
+  const void* logits;        /* [B, beams, vocab], element type = dtype, the last dimension contiguous */
+  int64_t stride_b, stride_n; /* elements between requests and beams */
+  const float* scores;       /* [B, beams] */
+  const uint8_t* finished;   /* [B, beams], 0 or 1, or NULL (no beam is) */
+  float* new_scores;         /* [B, num_out] */
+  int32_t* parents;          /* [B, num_out] */
+  int32_t* tokens;           /* [B, num_out] */
+  uint8_t* new_finished;     /* [B, num_out] */
+  int32_t B, beams, vocab, num_out; /* beams and num_out at most TPA_BEAM_MAX, vocab at most 2^30, beams * vocab below 2^31, num_out <= beams * vocab */
+  int32_t eos_token;         /* -1: none (then `finished` must be NULL) */
+  int32_t dtype;
+  void* workspace;           /* tpa_beam_select_workspace_bytes(...), 16-byte aligned */
+  size_t workspace_bytes;
+} TpaBeamSelectArgs;
+#define TPA_BEAM_MAX 64
+
+/* A pool of pages [num_pages, page_size, token_bytes], the tokens of a page without gaps. */
+typedef struct TpaPool {
+  void* ptr;
+  int64_t page_stride; /* bytes between pages, at least page_size * token_bytes */
+  int64_t token_bytes;
+} TpaPool;
+
+/*
+ * tpa_pages_fork arguments: sequences that go on from chosen ones (beams, samples of one prompt, requests that end or change their row).  No counterpart in
+ * the reference.  Sequence i of the new batch goes on from sequence s = parents[i] of the old one; outside 0 .. B - 1: it is empty.  With
+ * n = kv_lengths[s], f = n / page_size, t = n % page_size:
+ *   its first f pages are s's.  If t > 0, the first new sequence (the lowest i) of s keeps s's last page where page_shares has 0 for it; every
+ *   other one gets the next of free_pages[free_start ..], the new sequences served in order, and a copy of its t tokens in every pool.  Without
+ *   a page left (or with one outside the pools) it ends with its f whole pages: new_kv_lengths[i] = f * page_size, n otherwise.
+ *   new_page_table[i]: its pages, then zeros.
+ * page_shares[p] = sequences that hold page p, beyond the first (0 for a page that tpa_page_tables has just opened).  new_page_shares has
+ * it after the step: a page of f gains (new sequences of s) - 1 for every old sequence s that holds it, a last page that no new sequence keeps loses 1.  A
+ * page whose count falls below 0 is released: its count is 0 again, and the pages released stand, in rising order, in new_free_pages right before
+ * the first page that is still free, whose place new_free_start names (the first one released: those for which the list has no room before are left
+ * out).  The list has room for every page that was taken from it.
+ * Table entries outside 0 .. num_pages - 1 are passed on and hold no page.  Lengths past the table's row count as its end, counts and lengths below 0 as 0.
+ * Outputs must not overlap inputs.  Two launches (one more for every TPA_MAX_POOLS pools).
+ */
+typedef struct TpaPagesForkArgs {
+  const int32_t* page_table;   /* [B, pages_per_seq] */
+  const int32_t* kv_lengths;   /* [B] */
+  const int32_t* parents;      /* [M] */
+  const int32_t* page_shares;  /* [num_pages] */
+  const int32_t* free_pages;   /* [num_free], or NULL with num_free == 0 */
+  const int32_t* free_start;   /* [1], or NULL (0) */
+  int32_t* new_page_table;     /* [M, pages_per_seq] */
+  int32_t* new_kv_lengths;     /* [M] */
+  int32_t* new_page_shares;    /* [num_pages] */
+  int32_t* new_free_pages;     /* [num_free] */
+  int32_t* new_free_start;     /* [1] */
+  const TpaPool* pools;        /* num_pools of them, in host memory; or NULL with num_pools == 0 */
+  int32_t num_pools;
+  int32_t B, M;                /* at most TPA_PAGE_TABLES_MAX_REQUESTS each */
+  int32_t pages_per_seq, page_size, num_pages, num_free; /* pages_per_seq * page_size and num_pages * page_size below 2^31 */
+  void* workspace;             /* tpa_pages_workspace_bytes(...), 16-byte aligned */
+  size_t workspace_bytes;
+} TpaPagesForkArgs;
+#define TPA_MAX_POOLS 96
+
+/*
+ * tpa_pages_compact arguments: the pages in use move to the front of their pools.  No counterpart in the reference.  In use are all pages that do not stand in
+ * free_pages[free_start ..], n of them.  Those at n and behind it go, in rising order, to the free pages before n, in every pool:
+ *   moved[p] = where page p is now, p itself for a page that is free;  new_page_shares has the counts at the new places, 0 from n on;
+ *   new_page_table: the entries of each row's ceil(kv_lengths / page_size) pages at their new places (an entry outside 0 .. num_pages - 1 as
+ *   it was), then zeros;  new_free_pages ends with n .. num_pages - 1, new_free_start names the place of n.
+ * Every holder of pages that is not a row of this table is to look its pages up in `moved`.  Outputs must not overlap inputs.  Two launches (one more for every
+ * TPA_MAX_POOLS pools).
+ */
+typedef struct TpaPagesCompactArgs {
+  const int32_t* page_table;   /* [B, pages_per_seq] */
+  const int32_t* kv_lengths;   /* [B] */
+  const int32_t* page_shares;  /* [num_pages] */
+  const int32_t* free_pages;   /* [num_free], or NULL with num_free == 0 */
+  const int32_t* free_start;   /* [1], or NULL (0) */
+  int32_t* new_page_table;     /* [B, pages_per_seq] */
+  int32_t* new_page_shares;    /* [num_pages] */
+  int32_t* new_free_pages;     /* [num_free] */
+  int32_t* new_free_start;     /* [1] */
+  int32_t* moved;              /* [num_pages] */
+  const TpaPool* pools;
+  int32_t num_pools;
+  int32_t B;                   /* may be 0 */
+  int32_t pages_per_seq, page_size, num_pages, num_free; /* num_pages at most TPA_COMPACT_MAX_PAGES */
+  void* workspace;             /* tpa_pages_workspace_bytes(...), 16-byte aligned */
+  size_t workspace_bytes;
+} TpaPagesCompactArgs;
+#define TPA_COMPACT_MAX_PAGES (1 << 20)
+
 /* ABI version of the loaded library (TPA_ABI_VERSION it was built with). */
 int tpa_abi_version(void);
 
@@ -528,6 +676,29 @@ int tpa_decode_shared(const TpaFwdArgs* args, int32_t prefix_length, void* strea
 /* Bytes of workspace that tpa_decode_shared needs for this call; 0 if it would refuse it.  `workspace`, `workspace_bytes` and the
    outputs are not looked at. */
 size_t tpa_decode_shared_workspace_bytes(const TpaFwdArgs* args, int32_t prefix_length);
+
+/* K and V factors of new tokens into a paged cache in 4 bits, and the factors that slots of one stand for (see TpaFp4RowsArgs).  One launch each. */
+int tpa_cache_write_fp4(const TpaFp4RowsArgs* args, void* stream);
+int tpa_cache_read_fp4(const TpaFp4RowsArgs* args, void* stream);
+
+/*
+ * tpa_decode over a cache in 4 bits (see TpaDecodeFp4Args).  A number of V that is NaN may reach, as 0 * NaN, the rows of its batch entry from which the causal
+ * mask hides its token; tokens past kv_lengths are not read.
+ */
+int tpa_decode_fp4(const TpaDecodeFp4Args* args, void* stream);
+
+/* Bytes of workspace that tpa_decode_fp4 needs for this call; 0 if it would refuse it or needs none.  `workspace` and the outputs are not looked at. */
+size_t tpa_decode_fp4_workspace_bytes(const TpaDecodeFp4Args* args);
+
+/* The best continuations of every request's beams (see TpaBeamSelectArgs).  Two launches. */
+int tpa_beam_select(const TpaBeamSelectArgs* args, void* stream);
+size_t tpa_beam_select_workspace_bytes(int32_t B, int32_t beams, int32_t vocab, int32_t num_out, int32_t dtype);
+
+/* Pages of sequences that go on from chosen ones (see TpaPagesForkArgs), and pages moved to the front of their pools (see TpaPagesCompactArgs). */
+int tpa_pages_fork(const TpaPagesForkArgs* args, void* stream);
+int tpa_pages_compact(const TpaPagesCompactArgs* args, void* stream);
+/* Bytes of workspace that either needs; M = 0 for tpa_pages_compact. */
+size_t tpa_pages_workspace_bytes(int32_t M, int32_t num_pages);
 
 #ifdef __cplusplus
 }

@@ -38,7 +38,8 @@ using at::Tensor;
   X(tpa_fwd) X(tpa_decode) X(tpa_cache_append) X(tpa_bwd) X(tpa_strerror) X(tpa_fwd_call_workspace_bytes) \
   X(tpa_decode_call_workspace_bytes) X(tpa_cache_append_workspace_bytes) X(tpa_bwd_workspace_bytes)             \
   X(tpa_page_tables) X(tpa_norm_rope) X(tpa_norm_rope_bwd) X(tpa_norm_rope_bwd_workspace_bytes) X(tpa_decode_shared) \
-  X(tpa_decode_shared_workspace_bytes)
+  X(tpa_decode_shared_workspace_bytes) X(tpa_fp4_row_bytes) X(tpa_cache_write_fp4) X(tpa_cache_read_fp4) X(tpa_decode_fp4) \
+  X(tpa_decode_fp4_workspace_bytes) X(tpa_beam_select) X(tpa_beam_select_workspace_bytes) X(tpa_pages_fork) X(tpa_pages_compact) X(tpa_pages_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
   TPA_CALLS(X)
@@ -1049,6 +1050,382 @@ PyObject* norm_rope_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_CALL
 }
 
+// ------------------------------------------------------------------------------------------------ a cache in 4 bits
+// A cache of rows [pages or batch entries, tokens, rk, bytes]; `bytes` = what H + D numbers take
+void check_fp4_cache(const Tensor& t, const char* name, int64_t rk, int64_t h, int64_t d) {
+  if (t.scalar_type() != at::kByte) throw Raise{PyExc_TypeError, std::string(name) + " holds rows of bytes (uint8), got " + c10::toString(t.scalar_type())};
+  const int64_t bytes = h <= INT32_MAX && d <= INT32_MAX ? (int64_t)lib.tpa_fp4_row_bytes((int)h, (int)d) : 0;
+  if (t.dim() != 4 || t.size(2) != rk || t.size(3) != bytes)
+    throw Raise{PyExc_ValueError, std::string(name) + " must be [pages, page_size, " + std::to_string(rk) + ", " + std::to_string(bytes) + "] for " + std::to_string(h) + " heads of " +
+                                      std::to_string(d) + ", got " + sizes_of(t)};
+}
+void fits_int(std::initializer_list<int64_t> sizes, const char* name) {
+  for (int64_t s : sizes)
+    if (s > INT32_MAX) throw CallFailed{name, TPA_ERR_SHAPE};
+}
+// what writing and reading have in common; false: nothing to do
+bool describe_fp4_rows(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& slots, int64_t h, const char* name, TpaFp4RowsArgs& a) {
+  expect(kc.sizes().slice(0, 3) == vc.sizes().slice(0, 3), vc);
+  if (!is_shape(slots, {k.size(0), k.size(1)}))
+    throw Raise{PyExc_ValueError, "slots must have shape (" + std::to_string(k.size(0)) + ", " + std::to_string(k.size(1)) + "), got " + sizes_of(slots)};
+  fits_int({k.size(0), k.size(1), k.size(2), k.size(3), v.size(3), kc.size(0), kc.size(1)}, name);
+  if (kc.size(0) && kc.size(1) > INT32_MAX / kc.size(0)) throw CallFailed{name, TPA_ERR_SHAPE};
+  if (!k.size(0) || !k.size(1) || !k.size(2)) return false;
+  a.ka = factor_of<TpaFactor>(k); a.kb = factor_of<TpaFactor>(k, h);
+  a.va = factor_of<TpaFactor>(v); a.vb = factor_of<TpaFactor>(v, h);
+  a.k_cache = factor_of<TpaFactor>(kc); a.v_cache = factor_of<TpaFactor>(vc);
+  a.slots = ids_ptr(slots);
+  a.page_size = std::max((int)kc.size(1), 1);
+  a.num_slots = (int)(kc.size(0) * kc.size(1));
+  a.B = (int)k.size(0); a.l = (int)k.size(1); a.rk = (int)k.size(2); a.H = (int)h; a.dk = (int)(k.size(3) - h); a.dv = (int)(v.size(3) - h);
+  a.dtype = dtype_code(k.scalar_type());
+  return true;
+}
+
+// cache_write_fp4(k, v, slots, k_cache, v_cache, num_heads)
+PyObject* cache_write_fp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("cache_write_fp4", n, 6);
+  if (!gpu_tensors(args + 3, 2)) throw Raise{PyExc_TypeError, "the cache is written in place: k_cache and v_cache must be GPU tensors"};
+  if (!gpu_tensors(args, 3)) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor k = THPVariable_Unpack(args[0]), v = THPVariable_Unpack(args[1]), kc = THPVariable_Unpack(args[3]), vc = THPVariable_Unpack(args[4]);
+  Tensor slots = THPVariable_Unpack(args[2]);
+  const int64_t h = integer(args[5]);
+  one_device({k, v, slots, kc, vc});
+  if (k.dim() != 4 || v.dim() != 4) throw Raise{PyExc_ValueError, "k, v must be [b, l, r, h + d]"};
+  expect(v.sizes().slice(0, 3) == k.sizes().slice(0, 3), v);
+  if (!(0 < h && h < k.size(3) && h < v.size(3))) throw Raise{PyExc_AssertionError, "num_heads = " + std::to_string(h) + ", " + sizes_of(k) + ", " + sizes_of(v)};
+  const Tensor two[2] = {k, v};
+  static const char* const names[2] = {"k", "v"};
+  check_dtypes(two, names, 2);
+  (void)dtype_code(k.scalar_type());
+  check_fp4_cache(kc, "k_cache", k.size(2), h, k.size(3) - h);
+  check_fp4_cache(vc, "v_cache", v.size(2), h, v.size(3) - h);
+  {
+    WithoutGil free;
+    const c10::DeviceGuard guard(k.device());
+    slots = ints(slots);
+    TpaFp4RowsArgs a{};
+    if (describe_fp4_rows(k, v, kc, vc, slots, h, "tpa_cache_write_fp4", a)) {
+      check("tpa_cache_write_fp4", lib.tpa_cache_write_fp4(&a, stream_of(k.device())));
+      written(kc);
+      written(vc);
+    }
+  }
+  Py_RETURN_NONE;
+  END_CALL
+}
+
+// cache_read_fp4(k_cache, v_cache, slots, num_heads, head_dim, v_head_dim, bf16)
+PyObject* cache_read_fp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("cache_read_fp4", n, 7);
+  if (!gpu_tensors(args, 3)) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor kc = THPVariable_Unpack(args[0]), vc = THPVariable_Unpack(args[1]);
+  Tensor slots = THPVariable_Unpack(args[2]), k, v;
+  const int64_t h = integer(args[3]), dk = integer(args[4]), dv = integer(args[5]);
+  const at::ScalarType dtype = integer(args[6]) ? at::kBFloat16 : at::kFloat;
+  one_device({kc, vc, slots});
+  if (h <= 0 || dk <= 0 || dv <= 0) throw Raise{PyExc_ValueError, "num_heads and the head sizes must be positive"};
+  if (kc.dim() != 4) throw Raise{PyExc_ValueError, "k_cache must be [pages, page_size, rk, bytes], got " + sizes_of(kc)};
+  check_fp4_cache(kc, "k_cache", kc.size(2), h, dk);
+  check_fp4_cache(vc, "v_cache", kc.size(2), h, dv);
+  if (slots.dim() != 2) throw Raise{PyExc_ValueError, "slots must be [b, l], got " + sizes_of(slots)};
+  {
+    WithoutGil free;
+    const c10::DeviceGuard guard(kc.device());
+    slots = ints(slots);
+    const auto options = at::TensorOptions().device(kc.device()).dtype(dtype);
+    k = at::empty({slots.size(0), slots.size(1), kc.size(2), h + dk}, options);
+    v = at::empty({slots.size(0), slots.size(1), kc.size(2), h + dv}, options);
+    TpaFp4RowsArgs a{};
+    if (describe_fp4_rows(k, v, kc, vc, slots, h, "tpa_cache_read_fp4", a)) check("tpa_cache_read_fp4", lib.tpa_cache_read_fp4(&a, stream_of(kc.device())));
+  }
+  return tuple_of({k, v});
+  END_CALL
+}
+
+// decode_fp4(qa, qb, k_cache, v_cache, kv_lengths, page_table, workspace, sm_scale, kernel, causal, causal_offset, v_head_dim)
+PyObject* decode_fp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("decode_fp4", n, 12);
+  if (!gpu_tensors(args, 4) || !none_or_gpu(args[4]) || !none_or_gpu(args[5]) || !none_or_gpu(args[6])) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor qa = THPVariable_Unpack(args[0]), qb = THPVariable_Unpack(args[1]), kc = THPVariable_Unpack(args[2]), vc = THPVariable_Unpack(args[3]);
+  Tensor pages = tensor_or_none(args[5]), ws = tensor_or_none(args[6]);
+  one_device({qa, qb, kc, vc, tensor_or_none(args[4]), pages, ws});
+  TpaDecodeFp4Args a{};
+  a.sm_scale = (float)real(args[7]);
+  a.kernel = (int)integer(args[8]);
+  a.causal = (int)integer(args[9]);
+  a.causal_offset = (int)integer(args[10]);
+  const int64_t given_dv = integer(args[11]);
+  if (qa.dim() != 4 || qb.dim() != 4) throw Raise{PyExc_ValueError, "qa, qb must be [b, lq, rq, x], got " + sizes_of(qa) + ", " + sizes_of(qb)};
+  expect(qb.sizes().slice(0, 3) == qa.sizes().slice(0, 3), qb);
+  const Tensor two[2] = {qa, qb};
+  static const char* const names[2] = {"qa", "qb"};
+  check_dtypes(two, names, 2);
+  a.dtype = dtype_code(qa.scalar_type());
+  const int64_t h = qa.size(3), dk = qb.size(3), dv = given_dv < 0 ? dk : given_dv;
+  if (h <= 0 || dk <= 0 || dv <= 0 || qa.size(2) <= 0) throw CallFailed{"tpa_decode_fp4", TPA_ERR_SHAPE};
+  if (kc.dim() != 4) throw Raise{PyExc_ValueError, "k_cache must be [pages, page_size, rk, bytes], got " + sizes_of(kc)};
+  check_fp4_cache(kc, "k_cache", kc.size(2), h, dk);
+  check_fp4_cache(vc, "v_cache", kc.size(2), h, dv);
+  expect(kc.sizes().slice(0, 3) == vc.sizes().slice(0, 3), vc);
+  fits_int({qa.size(0), qa.size(1), qa.size(2), h, dk, dv, kc.size(0), kc.size(1), kc.size(2)}, "tpa_decode_fp4");
+  std::pair<Tensor, Tensor> r;
+  {
+    WithoutGil free;
+    const at::Device device = qa.device();
+    const c10::DeviceGuard guard(device);
+    a.B = (int)qa.size(0); a.lq = (int)qa.size(1); a.rq = (int)qa.size(2); a.H = (int)h; a.dk = (int)dk; a.dv = (int)dv; a.rk = (int)kc.size(2);
+    if (pages.defined()) {
+      pages = ints(pages);
+      expect(pages.dim() == 2 && pages.size(0) == a.B, pages);
+      fits_int({pages.size(1), pages.size(1) * kc.size(1)}, "tpa_decode_fp4");
+      a.page_table = ids_ptr(pages);
+      a.page_size = (int)kc.size(1);
+      a.pages_per_seq = (int)pages.size(1);
+      a.num_pages = (int)kc.size(0);
+      a.lk = a.page_size * a.pages_per_seq;
+    } else {
+      expect(kc.size(0) == a.B, kc);
+      a.lk = (int)kc.size(1);
+    }
+    a.qa = factor_of<TpaFactor>(qa); a.qb = factor_of<TpaFactor>(qb);
+    a.k_cache = factor_of<TpaFactor>(kc); a.v_cache = factor_of<TpaFactor>(vc);
+    const Tensor kvlen = lengths(tensor_or_none(args[4]), a.B);
+    a.kv_lengths = ids_ptr(kvlen);
+    const auto options = at::TensorOptions().device(device);
+    r.first = at::empty({a.B, a.lq, a.H, a.dv}, options.dtype(qa.scalar_type()));
+    r.second = at::empty({a.B, a.H, a.lq}, options.dtype(at::kFloat));
+    if (r.first.numel() && a.lk && kc.numel() && vc.numel()) {
+      const size_t need = lib.tpa_decode_fp4_workspace_bytes(&a);
+      if (!ws.defined() && need) ws = bytes_on(device, need + 256);
+      if (ws.defined()) take_workspace(ws, 256, a);
+      a.o = r.first.data_ptr();
+      a.lse = f32_ptr(r.second);
+      check("tpa_decode_fp4", lib.tpa_decode_fp4(&a, stream_of(device)));
+    } else {  // no rows, or none that sees a key
+      r.first.fill_(NAN);
+      r.second.fill_(-INFINITY);
+    }
+  }
+  return pair(std::move(r));
+  END_CALL
+}
+
+// ------------------------------------------------------------------------------------------------ beams
+// beam_select(logits, scores, finished, num_out, eos_token)
+PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("beam_select", n, 5);
+  if (!gpu_tensors(args, 2) || !none_or_gpu(args[2])) Py_RETURN_NOTIMPLEMENTED;
+  Tensor logits = THPVariable_Unpack(args[0]), scores = THPVariable_Unpack(args[1]), finished = tensor_or_none(args[2]), out[4];
+  const int64_t given = integer(args[3]), eos = integer(args[4]);
+  one_device({logits, scores, finished});
+  if (logits.dim() != 3) throw Raise{PyExc_ValueError, "logits must be [b, beams, vocab], got " + sizes_of(logits)};
+  const int64_t b = logits.size(0), beams = logits.size(1), vocab = logits.size(2), k = given < 0 ? beams : given;
+  const int dtype = dtype_code(logits.scalar_type());
+  for (const Tensor* t : {&scores, &finished})
+    if (t->defined() && !is_shape(*t, {b, beams}))
+      throw Raise{PyExc_ValueError, std::string(t == &scores ? "scores" : "finished") + " must have shape (" + std::to_string(b) + ", " + std::to_string(beams) + "), got " + sizes_of(*t)};
+  if (!at::isFloatingType(scores.scalar_type())) throw Raise{PyExc_TypeError, std::string("scores are floating-point numbers, got ") + c10::toString(scores.scalar_type())};
+  if (finished.defined() && finished.scalar_type() != at::kBool) throw Raise{PyExc_TypeError, std::string("finished holds truth values, got ") + c10::toString(finished.scalar_type())};
+  if (finished.defined() && eos < 0) throw Raise{PyExc_ValueError, "finished beams need an eos_token"};
+  if (eos < -1 || eos >= vocab) throw Raise{PyExc_ValueError, "eos_token must be below the vocabulary's " + std::to_string(vocab) + ", got " + std::to_string(eos)};
+  if (k < 1 || beams < 1 || vocab < 1 || k > beams * vocab)
+    throw Raise{PyExc_ValueError, "num_out must be between 1 and beams * vocab, got " + std::to_string(k) + " of " + sizes_of(logits)};
+  fits_int({b, beams, vocab, k}, "tpa_beam_select");
+  {
+    WithoutGil free;
+    const at::Device device = logits.device();
+    const c10::DeviceGuard guard(device);
+    if (vocab > 1 && logits.stride(2) != 1) logits = logits.contiguous();
+    scores = scores.to(at::kFloat).contiguous();
+    if (finished.defined()) finished = finished.contiguous();
+    const auto options = at::TensorOptions().device(device);
+    out[0] = at::empty({b, k}, options.dtype(at::kFloat));
+    out[1] = at::empty({b, k}, options.dtype(at::kInt));
+    out[2] = at::empty({b, k}, options.dtype(at::kInt));
+    out[3] = at::empty({b, k}, options.dtype(at::kBool));
+    if (b) {
+      TpaBeamSelectArgs a{};
+      a.logits = logits.data_ptr();
+      a.stride_b = logits.stride(0); a.stride_n = logits.stride(1);
+      a.scores = f32_ptr(scores);
+      a.finished = finished.defined() ? static_cast<const uint8_t*>(finished.data_ptr()) : nullptr;
+      a.new_scores = f32_ptr(out[0]);
+      a.parents = static_cast<int32_t*>(out[1].data_ptr());
+      a.tokens = static_cast<int32_t*>(out[2].data_ptr());
+      a.new_finished = static_cast<uint8_t*>(out[3].data_ptr());
+      a.B = (int)b; a.beams = (int)beams; a.vocab = (int)vocab; a.num_out = (int)k; a.eos_token = (int)eos; a.dtype = dtype;
+      const Tensor ws = bytes_on(device, lib.tpa_beam_select_workspace_bytes(a.B, a.beams, a.vocab, a.num_out, a.dtype) + 16);
+      take_workspace(ws, 16, a);
+      check("tpa_beam_select", lib.tpa_beam_select(&a, stream_of(device)));
+    }
+  }
+  return tuple_of({out[0], out[1], out[2], out[3]});
+  END_CALL
+}
+
+// ------------------------------------------------------------------------------------------------ pages between sequences
+// The pools of a call: GPU tensors [num_pages, page_size, ..] whose pages have no gaps
+std::vector<Tensor> pools_of(PyObject* arg) {
+  PyObject* const list = PySequence_Fast(arg, "pools is a list of tensors");
+  if (!list) throw python_error();
+  std::vector<Tensor> pools;
+  bool ok = true;
+  for (Py_ssize_t i = 0; ok && i < PySequence_Fast_GET_SIZE(list); ++i) {
+    PyObject* const item = PySequence_Fast_GET_ITEM(list, i);
+    ok = gpu_tensors(&item, 1);
+    if (ok) pools.push_back(THPVariable_Unpack(item));
+  }
+  Py_DECREF(list);
+  if (!ok) throw Raise{PyExc_TypeError, "pages are moved in place: pools must be GPU tensors"};
+  return pools;
+}
+std::vector<TpaPool> describe_pools(const std::vector<Tensor>& pools, int64_t num_pages, int64_t page_size) {
+  std::vector<TpaPool> out;
+  for (const Tensor& t : pools) {
+    if (t.dim() < 2 || t.size(0) != num_pages || t.size(1) != page_size)
+      throw Raise{PyExc_ValueError, "pools must be [" + std::to_string(num_pages) + ", " + std::to_string(page_size) + ", ..], got " + sizes_of(t)};
+    if (!t.numel()) continue;  // nothing in a page
+    int64_t each = 1;          // elements of a token, then of a page
+    bool whole = true;
+    for (int64_t d = t.dim() - 1; d >= 1; --d) {
+      if (t.size(d) > 1 && t.stride(d) != each) whole = false;
+      each *= t.size(d);
+    }
+    if (!whole || (num_pages > 1 && t.stride(0) < each)) throw Raise{PyExc_ValueError, "the pages of a pool must be contiguous and apart"};
+    const int64_t e = t.element_size();
+    out.push_back(TpaPool{t.data_ptr(), std::max(t.stride(0), each) * e, each / page_size * e});
+  }
+  return out;
+}
+// int32 results of the given sizes in one allocation
+void allocate_ints(const at::Device& device, std::initializer_list<std::vector<int64_t>> shapes, Tensor* out) {
+  int64_t at = 0, total = 0;
+  auto room = [](const std::vector<int64_t>& s) {
+    int64_t n = 1;
+    for (int64_t x : s) n *= x;
+    return (n + 63) / 64 * 64;
+  };
+  for (const auto& s : shapes) total += room(s);
+  const Tensor all = at::empty({total}, at::TensorOptions().device(device).dtype(at::kInt));
+  int i = 0;
+  for (const auto& s : shapes) {
+    out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+    out[i].unsafeGetTensorImpl()->set_storage_offset(at);
+    out[i++].unsafeGetTensorImpl()->set_sizes_contiguous(s);
+    at += room(s);
+  }
+}
+// what both calls take: a table, lengths, counts, a list of free pages and the place in it
+struct PageState {
+  Tensor table, len, shares, free, start;
+  int64_t page_size = 0;
+};
+void check_page_state(const PageState& s, const char* name) {
+  if (s.table.dim() != 2) throw Raise{PyExc_ValueError, "page_table must be [b, pages_per_seq], got " + sizes_of(s.table)};
+  const int64_t b = s.table.size(0);
+  if (!is_shape(s.len, {b})) throw Raise{PyExc_ValueError, "kv_lengths must have shape (" + std::to_string(b) + ",), got " + sizes_of(s.len)};
+  if (s.shares.dim() != 1 || !s.shares.size(0)) throw Raise{PyExc_ValueError, "page_shares has a number for every page, got shape " + sizes_of(s.shares)};
+  if (s.free.dim() != 1) throw Raise{PyExc_ValueError, "free_pages is a list of pages, got shape " + sizes_of(s.free)};
+  if (s.start.defined() && s.start.numel() != 1) throw Raise{PyExc_ValueError, "free_start is one number, got shape " + sizes_of(s.start)};
+  if (s.page_size < 1 || s.page_size > INT32_MAX) throw Raise{PyExc_ValueError, "page_size must be positive, got " + std::to_string(s.page_size)};
+  if (!s.table.size(1)) throw Raise{PyExc_ValueError, "page_table must be [b, pages_per_seq], got " + sizes_of(s.table)};
+  fits_int({b, s.table.size(1), s.shares.size(0), s.free.size(0)}, name);
+}
+void settle(PageState& s) {
+  s.table = ints(s.table);
+  s.len = ints(s.len);
+  s.shares = ints(s.shares);
+  s.free = ints(s.free);
+  if (s.start.defined()) s.start = ints(s.start);
+}
+template <typename Args>
+void describe_pages(const PageState& s, const std::vector<TpaPool>& pools, Args& a) {
+  a.page_table = ids_ptr(s.table); a.kv_lengths = ids_ptr(s.len); a.page_shares = ids_ptr(s.shares); a.free_pages = ids_ptr(s.free); a.free_start = ids_ptr(s.start);
+  a.pools = pools.data(); a.num_pools = (int)pools.size();
+  a.B = (int)s.table.size(0); a.pages_per_seq = (int)s.table.size(1); a.page_size = (int)s.page_size;
+  a.num_pages = (int)s.shares.size(0); a.num_free = (int)s.free.size(0);
+}
+int32_t* int_ptr(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+// pages_fork(page_table, kv_lengths, parents, page_shares, free_pages, free_start, pools, page_size)
+PyObject* pages_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("pages_fork", n, 8);
+  if (!gpu_tensors(args, 5) || !none_or_gpu(args[5])) Py_RETURN_NOTIMPLEMENTED;
+  PageState s;
+  s.table = THPVariable_Unpack(args[0]); s.len = THPVariable_Unpack(args[1]); s.shares = THPVariable_Unpack(args[3]); s.free = THPVariable_Unpack(args[4]);
+  s.start = tensor_or_none(args[5]);
+  Tensor parents = THPVariable_Unpack(args[2]), out[5];
+  const std::vector<Tensor> pools = pools_of(args[6]);
+  s.page_size = integer(args[7]);
+  one_device({s.table, s.len, parents, s.shares, s.free, s.start});
+  for (const Tensor& t : pools) one_device({s.table, t});
+  check_page_state(s, "tpa_pages_fork");
+  if (parents.dim() < 1) throw Raise{PyExc_ValueError, "parents has a number for every new sequence, got shape " + sizes_of(parents)};
+  fits_int({parents.numel()}, "tpa_pages_fork");
+  const std::vector<TpaPool> described = describe_pools(pools, s.shares.size(0), s.page_size);
+  {
+    WithoutGil free;
+    const at::Device device = s.table.device();
+    const c10::DeviceGuard guard(device);
+    settle(s);
+    parents = ints(parents);
+    const int64_t m = parents.numel();
+    allocate_ints(device, {{m, s.table.size(1)}, {m}, {s.shares.size(0)}, {s.free.size(0)}, {1}}, out);
+    TpaPagesForkArgs a{};
+    describe_pages(s, described, a);
+    a.parents = ids_ptr(parents);
+    a.M = (int)m;
+    a.new_page_table = int_ptr(out[0]); a.new_kv_lengths = int_ptr(out[1]); a.new_page_shares = int_ptr(out[2]);
+    a.new_free_pages = int_ptr(out[3]); a.new_free_start = int_ptr(out[4]);
+    const Tensor ws = bytes_on(device, lib.tpa_pages_workspace_bytes(a.M, a.num_pages) + 16);
+    take_workspace(ws, 16, a);
+    check("tpa_pages_fork", lib.tpa_pages_fork(&a, stream_of(device)));
+    for (const Tensor& t : pools) written(t);
+  }
+  return tuple_of({out[0], out[1], out[2], out[3], out[4]});
+  END_CALL
+}
+
+// pages_compact(page_table, kv_lengths, page_shares, free_pages, free_start, pools, page_size)
+PyObject* pages_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  BEGIN_CALL
+  count("pages_compact", n, 7);
+  if (!gpu_tensors(args, 4) || !none_or_gpu(args[4])) Py_RETURN_NOTIMPLEMENTED;
+  PageState s;
+  s.table = THPVariable_Unpack(args[0]); s.len = THPVariable_Unpack(args[1]); s.shares = THPVariable_Unpack(args[2]); s.free = THPVariable_Unpack(args[3]);
+  s.start = tensor_or_none(args[4]);
+  Tensor out[5];
+  const std::vector<Tensor> pools = pools_of(args[5]);
+  s.page_size = integer(args[6]);
+  one_device({s.table, s.len, s.shares, s.free, s.start});
+  for (const Tensor& t : pools) one_device({s.table, t});
+  check_page_state(s, "tpa_pages_compact");
+  const std::vector<TpaPool> described = describe_pools(pools, s.shares.size(0), s.page_size);
+  {
+    WithoutGil free;
+    const at::Device device = s.table.device();
+    const c10::DeviceGuard guard(device);
+    settle(s);
+    allocate_ints(device, {{s.table.size(0), s.table.size(1)}, {s.shares.size(0)}, {s.free.size(0)}, {1}, {s.shares.size(0)}}, out);
+    TpaPagesCompactArgs a{};
+    describe_pages(s, described, a);
+    a.new_page_table = int_ptr(out[0]); a.new_page_shares = int_ptr(out[1]); a.new_free_pages = int_ptr(out[2]); a.new_free_start = int_ptr(out[3]);
+    a.moved = int_ptr(out[4]);
+    const Tensor ws = bytes_on(device, lib.tpa_pages_workspace_bytes(0, a.num_pages) + 16);
+    take_workspace(ws, 16, a);
+    check("tpa_pages_compact", lib.tpa_pages_compact(&a, stream_of(device)));
+    for (const Tensor& t : pools) written(t);
+  }
+  return tuple_of({out[0], out[1], out[2], out[3], out[4]});
+  END_CALL
+}
+
 // ------------------------------------------------------------------------------------------------ module
 // bind(path of libtpa_gfx950.so, TpaError)
 PyObject* bind(PyObject*, PyObject* args) {
@@ -1075,7 +1452,8 @@ PyObject* bind(PyObject*, PyObject* args) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(factors), FAST(decode), FAST(append), FAST(backward), FAST(tpa), FAST(decode_shared), FAST(page_tables),
-                         FAST(norm_rope), FAST(norm_rope_backward), FAST(norm_rope_write), {nullptr, nullptr, 0, nullptr}};
+                         FAST(norm_rope), FAST(norm_rope_backward), FAST(norm_rope_write),
+                         FAST(cache_write_fp4), FAST(cache_read_fp4), FAST(decode_fp4), FAST(beam_select), FAST(pages_fork), FAST(pages_compact), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tpa_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,673 @@
+// Decode over the factored KV cache in 4 bits: a few query tokens against a long cache.
+//
+// As in the decode over 16-bit factors, K and V are never formed: with Qm[c, :] = (scale / (Rq Rk)) sum_i qa[i, h] qb[i, :] for every column c = (query row,
+// head) the logits are s[c, t] = sum_j a_k[t, j, h] (Qm[c, :] . b_k[t, j, :]), and o[c, :] = (1/Rk) sum_t sum_j (p[c, t] a_v[t, j, h]) b_v[t, j, :]: two
+// products of the matrix cores with the rows of a block of 32 (token, rank) rows and 32 columns.
+//
+// A lane reads half a row, 32 bytes of codes for 128 numbers.  The product with Q sums over the numbers in any order, so Q takes the order in which they lie in
+// that half and the codes go from memory to the matrix cores through the registers: four conversions a word, exact in bf16, the block's scale within them.
+// V is contracted over the rows: its numbers go through LDS as bf16 and come back transposed, and so do the head factors of both.
+//
+// The blocks of all sequences, one behind the other, are dealt to the workgroups in equal shares (of whole rounds of four blocks, one for each wave), whatever
+// the lengths are; a workgroup that meets several sequences leaves a part for each, and a second launch joins the parts of a sequence by maximum and sum.
+#include <algorithm>
+
+#include "tpa_fp4.h"
+
+namespace tpa {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kRows = 32;  // (token, rank) rows of a block
+
+struct Fp4Params {
+  TpaFactor qa, qb, kc, vc;
+  void* o;
+  float* lse;
+  const int32_t *kvlen, *table;
+  float *part_o, *part_m, *part_l;  // [slot, column, D], [slot, column], [slot, column]
+  int32_t* plan;                    // [B + 1] rounds before each sequence
+  int page_size, page_shift, pages_per_seq, num_pages;
+  int B, lq, lk, H, dk, dv, rq, rk, cols;
+  int causal, coff;
+  int groups;   // workgroups that share out the rounds, at most
+  float scale;  // of Q: sm_scale log2(e) / (rq rk); of the vector-unit kernel: sm_scale
+};
+
+// keys that query row `row` of a sequence of `length` keys sees
+__device__ __forceinline__ int keys_seen(const Fp4Params& p, int length, int row) {
+  const int len = max(0, min(length, p.lk));
+  if (!p.causal) return len;
+  const int64_t last = (int64_t)row + p.coff + 1 + (p.causal == TPA_CAUSAL_BOTTOM_RIGHT ? len - p.lq : 0);
+  return (int)max((int64_t)0, min((int64_t)len, last));
+}
+__device__ __forceinline__ int length_of(const Fp4Params& p, int b) { return p.kvlen ? p.kvlen[b] : p.lk; }
+// rounds of blocks of a sequence: those of the last row, which sees the most
+template <int RK>
+__device__ __forceinline__ int rounds_of(const Fp4Params& p, int b) {
+  return (int)(((int64_t)keys_seen(p, length_of(p, b), p.lq - 1) * RK + kRows * kWaves - 1) / (kRows * kWaves));
+}
+
+// sum over the threads before this one and over all; `red` = an int per wave
+__device__ __forceinline__ int sum_before(int x, int* red, int& total) {
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int upto = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(upto, d);
+    if (lane >= d) upto += y;
+  }
+  if (lane == 63) red[w] = upto;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) before += red[i];
+    total += red[i];
+  }
+  return before + upto - x;
+}
+
+template <int D, int NC, int NS>
+struct Fp4Lds {
+  static constexpr int kV = kRows * D;                            // elements of V's tile
+  static constexpr int kA = kRows * 32;                           // of the head factors of 32 columns
+  static constexpr int kPerWave = kV + 2 * NC * kA;               // bf16 elements
+  static constexpr int kHalf = D / 2, kRowStride = kHalf + 4;     // the waves are joined in two halves of D
+  static_assert(4 * (32 * kRowStride + 64) <= 2 * kPerWave, "the join takes the room of the tiles");
+  static constexpr int kQ = NC * NS * (D / 16) * 64 * 16;         // bytes of Q's fragments
+  static constexpr size_t kBytes = 2 * (size_t)kPerWave * kWaves + kQ;
+};
+
+// a [32][D] bf16 tile: 16-byte chunk c of row r at chunk c ^ (r mod chunks)
+template <int D>
+__device__ __forceinline__ int tile_write_at(int row, int chunk) { return row * D + 8 * (chunk ^ (row & (D / 8 - 1))); }
+// transposed read: lane (i, g) gets rows 16 kk + 8 hi + 4 g + 0..3 of column 32 db + i
+template <int D>
+__device__ __forceinline__ bf16x8 tile_tr(const uint16_t* tile, int l, int kk, int db) {
+  constexpr int CPR = D / 8;
+  const int g = l >> 5, lp = l & 15, dhalf = (l >> 4) & 1;
+  auto at = [&](int hi) {
+    const int r = 16 * kk + 8 * hi + 4 * g + (lp >> 2);
+    return r * D + 8 * ((4 * db + 2 * dhalf + ((lp & 3) >> 1)) ^ (r & (CPR - 1))) + 4 * (lp & 1);
+  };
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(tile + at(0)));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(tile + at(1)));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// x as a sum of NS bf16 numbers (3: all 24 bits), two at a time
+template <int NS>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NS]) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    out[s] = pack_bf16(x, y);
+    x -= bf16lo_to_f32(out[s]);
+    y -= bf16hi_to_f32(out[s]);
+  }
+}
+
+// T: of the queries and the output.  NC: sets of 32 columns of a workgroup.  QS, PS: bf16 numbers that stand for one of Q and of the weighted probabilities.
+template <typename T, int D, int RK, int NC, int QS, int PS>
+__global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 : 1) void decode_fp4_kernel(Fp4Params p) {
+  using Lds = Fp4Lds<D, NC, QS>;
+  constexpr int NKS = D / 16, NDB = D / 32, NW = D / 64;  // NW: 16-byte words of half a row's codes
+  constexpr int NTOK = RK <= 4 ? 16 / RK : 32 / RK;       // tokens whose rows this lane has logits of
+  constexpr int NV = RK <= 4 ? RK : RK / 2;               // rows of a token in this half of the wave
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem_fp4[];
+  __shared__ int red[kWaves], found[2];
+  const int tid = threadIdx.x, w = scalar(tid >> 6), l = tid & 63, i = l & 31, g = l >> 5;
+  const int c0 = blockIdx.y * 32 * NC;
+
+  // ---- this workgroup's share of the rounds
+  const int each = (p.B + kThreads - 1) / kThreads, e0 = min(tid * each, p.B), e1 = min(e0 + each, p.B);
+  int mine = 0, total;
+  for (int b = e0; b < e1; ++b) mine += rounds_of<RK>(p, b);
+  int before = sum_before(mine, red, total);
+  const int groups = min(p.groups, total);
+  const bool writes_plan = blockIdx.x == 0 && blockIdx.y == 0;
+  const int64_t share = blockIdx.x;
+  if (share >= groups && !writes_plan) return;
+  int r0 = groups ? (int)(share * total / groups) : 0;
+  const int r1 = groups ? (int)((share + 1) * total / groups) : 0;
+  for (int b = e0; b < e1; ++b) {
+    const int n = rounds_of<RK>(p, b);
+    if (writes_plan) p.plan[b] = before;
+    if (r0 >= before && r0 < before + n) { found[0] = b; found[1] = before; }
+    before += n;
+  }
+  if (writes_plan && tid == 0) p.plan[p.B] = total;
+  if (share >= groups) return;
+  __syncthreads();
+  int b = scalar(found[0]), first_round = scalar(found[1]);
+
+  uint16_t* const lds_v = smem_fp4 + w * Lds::kPerWave;
+  uint16_t* const lds_a = lds_v + Lds::kV;  // [set][K, V][32 rows][32 columns]
+  u32x4* const lds_q = reinterpret_cast<u32x4*>(smem_fp4 + kWaves * Lds::kPerWave);
+
+  const Fp4Row parts(p.H, D);
+  // where the head factors of this lane's columns lie in a row: two chunks of 8 for every set
+  int a_at[NC][2], a_scale_at[NC][2];
+#pragma unroll
+  for (int s = 0; s < NC; ++s)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int h = (c0 + 32 * s + 16 * g + 8 * q) % p.H;
+      a_at[s][q] = parts.a_codes + h / 2;
+      a_scale_at[s][q] = parts.a_scales + h / 32;
+    }
+  int row_of_col[NC];  // query row of this lane's column in every set (past the last: the last)
+#pragma unroll
+  for (int s = 0; s < NC; ++s) row_of_col[s] = min(c0 + 32 * s + i, p.cols - 1) / p.H;
+
+  while (r0 < r1) {
+    const int rounds = rounds_of<RK>(p, b);
+    if (r0 >= first_round + rounds) {  // (a sequence without keys, or one whose end is a share's)
+      first_round += rounds;
+      ++b;
+      continue;
+    }
+    const int stop = min(r1, first_round + rounds);
+    const int len = length_of(p, b);
+    int last_of[NC];
+#pragma unroll
+    for (int s = 0; s < NC; ++s) last_of[s] = keys_seen(p, len, row_of_col[s]) * RK - 1;
+    const int last_row = keys_seen(p, len, p.lq - 1) * RK - 1;  // not below 0 here
+    const int blk_begin = (r0 - first_round) * kWaves + w, blk_end = min((stop - first_round) * kWaves, last_row / kRows + 1);
+
+    // ---- loads of a block: this lane's row (one past the last: that one), its place looked up a visit ahead
+    struct Raw {
+      u32x4 k[NW], v[NW];
+      uint32_t k_scales, v_scales, ka[NC][2], va[NC][2];
+      uint8_t ka_scale[NC][2], va_scale[NC][2];
+    } raw[2];
+    auto token_of = [&](int blk) __attribute__((always_inline)) { return min(blk * kRows + i, last_row) / RK; };
+    auto page_of = [&](int token) __attribute__((always_inline)) { return p.page_shift >= 0 ? token >> p.page_shift : token / p.page_size; };
+    auto lookup = [&](int blk) __attribute__((always_inline)) { return p.table ? p.table[(int64_t)b * p.pages_per_seq + page_of(token_of(blk))] : 0; };
+    int ahead[2];
+    auto issue = [&](Raw& x, int& page_ahead, int blk) __attribute__((always_inline)) {
+      const int token = token_of(blk), rank = min(blk * kRows + i, last_row) % RK;
+      int64_t page = b;
+      int in_page = token;
+      if (p.table) {
+        page = max(0, min(page_ahead, p.num_pages - 1));
+        in_page = token - page_of(token) * p.page_size;
+      }
+      const uint8_t* const k = static_cast<const uint8_t*>(p.kc.ptr) + page * p.kc.stride_b + in_page * p.kc.stride_l + rank * p.kc.stride_r;
+      const uint8_t* const v = static_cast<const uint8_t*>(p.vc.ptr) + page * p.vc.stride_b + in_page * p.vc.stride_l + rank * p.vc.stride_r;
+      typedef u32x4 __attribute__((aligned(4))) Word;
+#pragma unroll
+      for (int n = 0; n < NW; ++n) {
+        x.k[n] = *reinterpret_cast<const Word*>(k + g * (D / 4) + 16 * n);
+        x.v[n] = *reinterpret_cast<const Word*>(v + g * (D / 4) + 16 * n);
+      }
+      x.k_scales = *reinterpret_cast<const uint32_t*>(k + parts.b_scales);
+      x.v_scales = *reinterpret_cast<const uint32_t*>(v + parts.b_scales);
+#pragma unroll
+      for (int s = 0; s < NC; ++s)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          x.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + a_at[s][q]);
+          x.va[s][q] = *reinterpret_cast<const uint32_t*>(v + a_at[s][q]);
+          x.ka_scale[s][q] = k[a_scale_at[s][q]];
+          x.va_scale[s][q] = v[a_scale_at[s][q]];
+        }
+      page_ahead = lookup(blk + 2 * kWaves);
+    };
+    ahead[0] = lookup(blk_begin);
+    ahead[1] = lookup(blk_begin + kWaves);
+    issue(raw[0], ahead[0], blk_begin);
+    issue(raw[1], ahead[1], blk_begin + kWaves);
+
+    // ---- Q's fragments: lane (column, g) of step ks holds numbers g D/2 + 8 ks + 0..7
+    __syncthreads();  // the sequence before has left LDS
+    for (int item = tid; item < 32 * NC * (D / 8); item += kThreads) {
+      const int col = item / (D / 8), chunk = item % (D / 8), c = min(c0 + col, p.cols - 1), qi = c / p.H, h = c - qi * p.H;
+      const T* const qa = static_cast<const T*>(p.qa.ptr) + b * p.qa.stride_b + qi * p.qa.stride_l + h;
+      const T* const qb = static_cast<const T*>(p.qb.ptr) + b * p.qb.stride_b + qi * p.qb.stride_l + 8 * chunk;
+      float x[8] = {};
+#pragma unroll 2
+      for (int r = 0; r < p.rq; ++r) {
+        const float a = load_as_f32(qa + r * p.qa.stride_r);
+        const T* const row = qb + r * p.qb.stride_r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += a * load_as_f32(row + j);
+      }
+      uint32_t words[4][QS];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_pair<QS>(x[2 * j] * p.scale, x[2 * j + 1] * p.scale, words[j]);
+      const int half = chunk / NKS, ks = chunk % NKS;
+#pragma unroll
+      for (int q = 0; q < QS; ++q)
+        lds_q[(((col >> 5) * QS + q) * NKS + ks) * 64 + 32 * half + (col & 31)] = u32x4{words[0][q], words[1][q], words[2][q], words[3][q]};
+    }
+    __syncthreads();
+    constexpr bool kHeldQ = NC * QS == 1;  // in registers
+    bf16x8 qf[kHeldQ ? NKS : 1];
+    if constexpr (kHeldQ) {
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, lds_q[ks * 64 + l]);
+    }
+
+    f32x16 o[NC][NDB];
+    float m[NC], sum[NC];
+#pragma unroll
+    for (int s = 0; s < NC; ++s) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[s][db][v] = 0.f;
+      m[s] = -INFINITY;
+      sum[s] = 0.f;
+    }
+
+    auto block = [&](const Raw& x, int blk, bf16x8 (&kf)[NKS]) __attribute__((always_inline)) {
+      // ---- numbers of K to fragments, of V and of the head factors to LDS
+      float scale[2][NW];
+#pragma unroll
+      for (int n = 0; n < NW; ++n) {
+        const int shift = 8 * (NW * g + n);
+        scale[0][n] = fp4_scale((x.k_scales >> shift) & 255);
+        scale[1][n] = fp4_scale((x.v_scales >> shift) & 255);
+      }
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        kf[ks] = fp4_bf16x8(x.k[ks / 4][ks % 4], scale[0][ks / 4]);
+        *reinterpret_cast<bf16x8*>(lds_v + tile_write_at<D>(i, NKS * g + ks)) = fp4_bf16x8(x.v[ks / 4][ks % 4], scale[1][ks / 4]);
+      }
+#pragma unroll
+      for (int s = 0; s < NC; ++s)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint16_t* const at = lds_a + 2 * s * Lds::kA + i * 32 + 16 * g + 8 * q;
+          *reinterpret_cast<bf16x8*>(at) = fp4_bf16x8(x.ka[s][q], fp4_scale(x.ka_scale[s][q]));
+          *reinterpret_cast<bf16x8*>(at + Lds::kA) = fp4_bf16x8(x.va[s][q], fp4_scale(x.va_scale[s][q]));
+        }
+    };
+    auto consume = [&](int blk, const bf16x8 (&kf)[NKS]) __attribute__((always_inline)) {
+      const int lp = l & 15, dhalf = (l >> 4) & 1, row0 = blk * kRows;
+#pragma unroll
+      for (int s = 0; s < NC; ++s) {
+        if constexpr (NC > 1) __builtin_amdgcn_sched_barrier(0);
+        float ak[16], av[16];  // of this lane's column, rows 8q + 4g + 0..3
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = 2 * s * Lds::kA + (8 * q + 4 * g + (lp >> 2)) * 32 + 16 * dhalf + 4 * (lp & 3);
+          const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + at));
+          const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + Lds::kA + at));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
+            av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
+          }
+        }
+        f32x16 sp;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sp[v] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+          for (int q = 0; q < QS; ++q) {
+            const bf16x8 qv = kHeldQ ? qf[kHeldQ ? ks : 0] : __builtin_bit_cast(bf16x8, lds_q[((s * QS + q) * NKS + ks) * 64 + l]);
+            sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qv, sp, 0, 0, 0);
+          }
+
+        // ---- logits per token (log2 domain); from rank 8 on a token's rows span both halves of the wave
+        float st[NTOK], most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NTOK; ++t) {
+          const int v0 = t * NV;
+          float acc = 0.f;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) acc = fmaf(ak[v0 + j], sp[v0 + j], acc);
+          if constexpr (RK >= 8) acc = halves_sum(acc);
+          const int row = RK >= 8 ? row0 + RK * t : row0 + 8 * (v0 >> 2) + 4 * g + (v0 & 3);  // the token's first row
+          if (row > last_of[s]) acc = -INFINITY;
+          st[t] = acc;
+          most = fmaxf(most, acc);
+        }
+        most = halves_max(most);
+        // the reference is a whole number: a weight then has the same significand, and is rounded the same way, however the keys are dealt to
+        // waves and workgroups, and every factor that joins them is a power of two
+        const float m_new = fmaxf(m[s], __builtin_ceilf(most)), m_use = m_new == -INFINITY ? 0.f : m_new;
+        if (__any(m_new > m[s])) {
+          const float alpha = __builtin_amdgcn_exp2f(m[s] - m_use);
+          sum[s] *= alpha;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[s][db][v] *= alpha;
+          m[s] = m_new;
+        }
+        float pp[16];
+#pragma unroll
+        for (int t = 0; t < NTOK; ++t) {
+          const float pt = __builtin_amdgcn_exp2f(st[t] - m_use);
+          sum[s] += RK >= 8 ? 0.5f * pt : pt;  // both halves hold the token: each adds half of it
+#pragma unroll
+          for (int j = 0; j < NV; ++j) pp[t * NV + j] = pt * av[t * NV + j];
+        }
+        // ---- O^T[d, column] += sum over the rows of V[row, d] P'[row, column]; slot (g, j) = row 16 kk + 8 (j / 4) + 4 g + j % 4
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          uint32_t words[4][PS];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) split_pair<PS>(pp[8 * kk + 2 * j], pp[8 * kk + 2 * j + 1], words[j]);
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            const bf16x8 vf = tile_tr<D>(lds_v, l, kk, db);
+#pragma unroll
+            for (int q = 0; q < PS; ++q)
+              o[s][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(bf16x8, u32x4{words[0][q], words[1][q], words[2][q], words[3][q]}), o[s][db], 0, 0, 0);
+          }
+        }
+      }
+    };
+    for (int blk = blk_begin; blk < blk_end; blk += 2 * kWaves) {
+      bf16x8 kf[NKS];
+      block(raw[0], blk, kf);
+      issue(raw[0], ahead[0], blk + 2 * kWaves);
+      consume(blk, kf);
+      if (blk + kWaves < blk_end) {
+        block(raw[1], blk + kWaves, kf);
+        issue(raw[1], ahead[1], blk + 3 * kWaves);
+        consume(blk + kWaves, kf);
+      }
+    }
+
+    // ---- join the waves through LDS, half of D at a time, and leave the part
+    const int64_t slot = (int64_t)share + b;
+    float* const red_o = reinterpret_cast<float*>(lds_v);
+    constexpr int RS = Lds::kRowStride, HB = NDB / 2;
+#pragma unroll
+    for (int s = 0; s < NC; ++s) {
+      const int n_cols = min(32, p.cols - c0 - 32 * s);
+      if (n_cols <= 0) break;
+      const float all = halves_sum(sum[s]);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        __syncthreads();
+#pragma unroll
+        for (int db = 0; db < HB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x16& x = o[s][half * HB + db];
+            *reinterpret_cast<f32x4*>(red_o + i * RS + 32 * db + 8 * q + 4 * g) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+          }
+        if (g == 0) {
+          red_o[32 * RS + i] = m[s];
+          red_o[32 * RS + 32 + i] = all;
+        }
+        __syncthreads();
+        const int64_t base = slot * p.cols + c0 + 32 * s;
+        for (int idx = tid; idx < n_cols * (D / 8); idx += kThreads) {
+          const int c = idx / (D / 8), d = 4 * (idx % (D / 8));
+          float mw[kWaves], lw[kWaves], most = -INFINITY;
+#pragma unroll
+          for (int ww = 0; ww < kWaves; ++ww) {
+            const float* const from = reinterpret_cast<const float*>(smem_fp4 + ww * Lds::kPerWave);
+            mw[ww] = from[32 * RS + c];
+            lw[ww] = from[32 * RS + 32 + c];
+            most = fmaxf(most, mw[ww]);
+          }
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+          float lacc = 0.f;
+#pragma unroll
+          for (int ww = 0; ww < kWaves; ++ww) {
+            const float* const from = reinterpret_cast<const float*>(smem_fp4 + ww * Lds::kPerWave);
+            const float f = lw[ww] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mw[ww] - most);  // 0: no key of this wave
+            acc += f * *reinterpret_cast<const f32x4*>(from + c * RS + d);
+            lacc += f * lw[ww];
+          }
+          *reinterpret_cast<f32x4*>(p.part_o + (base + c) * D + half * (D / 2) + d) = acc;
+          if (half == 0 && d == 0) {
+            p.part_m[base + c] = most;
+            p.part_l[base + c] = lacc;
+          }
+        }
+      }
+    }
+    r0 = stop;
+  }
+}
+
+// The parts of a sequence's column joined: a workgroup for each column, its threads' slices over the parts.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void join_kernel(Fp4Params p) {
+  constexpr int LANES = D / 4, SLICES = kThreads / LANES;
+  __shared__ f32x4 part[SLICES][LANES];
+  __shared__ float part_m[SLICES], part_l[SLICES];
+  const int b = blockIdx.x / p.cols, c = blockIdx.x - b * p.cols, at = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+  const int64_t total = p.plan[p.B], first = p.plan[b], rounds = p.plan[b + 1] - first, groups = min((int64_t)p.groups, total);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, sum = 0.f;
+  if (rounds > 0) {
+    const int from = (int)(((first + 1) * groups - 1) / total), to = (int)(((first + rounds) * groups - 1) / total);
+    for (int share = from + slice; share <= to; share += SLICES) {
+      const int64_t base = (int64_t)(share + b) * p.cols + c;
+      const float ms = p.part_m[base], ls = p.part_l[base];
+      const f32x4 os = *reinterpret_cast<const f32x4*>(p.part_o + base * D + 4 * at);
+      if (ls == 0.f) continue;  // no key of this column
+      const float most = fmaxf(m, ms), use = most == -INFINITY ? 0.f : most;
+      const float f = __builtin_amdgcn_exp2f(m - use), fs = __builtin_amdgcn_exp2f(ms - use);
+      acc = acc * f + os * fs;
+      sum = sum * f + ls * fs;
+      m = most;
+    }
+  }
+  part[slice][at] = acc;
+  if (at == 0) { part_m[slice] = m; part_l[slice] = sum; }
+  __syncthreads();
+  if (slice) return;
+  float most = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < SLICES; ++s) most = fmaxf(most, part_m[s]);
+  const float use = most == -INFINITY ? 0.f : most;
+  acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < SLICES; ++s) {
+    if (part_l[s] == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(part_m[s] - use);
+    acc += f * part[s][at];
+    sum += f * part_l[s];
+  }
+  const float inv = sum == 0.f ? NAN : 1.f / (sum * p.rk);
+  T* const o = static_cast<T*>(p.o) + ((int64_t)b * p.cols + c) * D + 4 * at;
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
+  else *reinterpret_cast<f32x4*>(o) = acc * inv;
+  if (p.lse && at == 0) {
+    const int qi = c / p.H, h = c - qi * p.H;
+    p.lse[((int64_t)b * p.H + h) * p.lq + qi] = sum == 0.f ? -INFINITY : (most + log2f(sum)) * kLn2;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ any shape
+// A workgroup per query row and head, 256 keys at a time: a thread's key by itself, then the threads' output columns over the keys.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void decode_fp4_any_kernel(Fp4Params p) {
+  __shared__ float q[256], weight[kThreads], red[2][kWaves], out[kThreads];
+  __shared__ int64_t v_row[kThreads];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int b = blockIdx.x / p.cols, c = blockIdx.x - b * p.cols, qi = c / p.H, h = c - qi * p.H;
+  const Fp4Row k_parts(p.H, p.dk), v_parts(p.H, p.dv);
+  for (int d = tid; d < p.dk; d += kThreads) {
+    float x = 0.f;
+    for (int r = 0; r < p.rq; ++r)
+      x += load_as_f32(static_cast<const T*>(p.qa.ptr) + b * p.qa.stride_b + qi * p.qa.stride_l + r * p.qa.stride_r + h) *
+           load_as_f32(static_cast<const T*>(p.qb.ptr) + b * p.qb.stride_b + qi * p.qb.stride_l + r * p.qb.stride_r + d);
+    q[d] = x / p.rq;
+  }
+  const int keys = keys_seen(p, length_of(p, b), qi);
+  const int columns = kThreads / p.dv, d = tid % p.dv, slice = tid / p.dv;  // (dv <= 256) threads past the last slice idle
+  float m = -INFINITY, sum = 0.f, acc = 0.f;
+  __syncthreads();
+  for (int t0 = 0; t0 < keys; t0 += kThreads) {
+    const int t = t0 + tid;
+    float x = -INFINITY;
+    if (t < keys) {
+      int64_t page = b;
+      int in_page = t;
+      if (p.table) {
+        const int nth = t / p.page_size;
+        page = max(0, min(p.table[(int64_t)b * p.pages_per_seq + nth], p.num_pages - 1));
+        in_page = t - nth * p.page_size;
+      }
+      v_row[tid] = page * p.vc.stride_b + in_page * p.vc.stride_l;
+      const uint8_t* const k = static_cast<const uint8_t*>(p.kc.ptr) + page * p.kc.stride_b + in_page * p.kc.stride_l;
+      x = 0.f;
+      for (int r = 0; r < p.rk; ++r) {
+        const uint8_t* const row = k + r * p.kc.stride_r;
+        float dot = 0.f;
+        for (int j = 0; j < p.dk; ++j) dot += q[j] * fp4_number(row, row + k_parts.b_scales, j);
+        x += dot * fp4_number(row + k_parts.a_codes, row + k_parts.a_scales, h);
+      }
+      x *= p.scale / p.rk;
+    }
+    float most = x;
+#pragma unroll
+    for (int s = 32; s; s /= 2) most = fmaxf(most, __shfl_xor(most, s));
+    if (lane == 0) red[0][w] = most;
+    __syncthreads();
+    most = m;
+    for (int s = 0; s < kWaves; ++s) most = fmaxf(most, red[0][s]);
+    const float use = most == -INFINITY ? 0.f : most, f = expf(m - use);
+    m = most;
+    float part = t < keys ? expf(x - use) : 0.f;
+    weight[tid] = part;
+#pragma unroll
+    for (int s = 32; s; s /= 2) part += __shfl_xor(part, s);
+    if (lane == 0) red[1][w] = part;
+    __syncthreads();
+    sum *= f;
+    for (int s = 0; s < kWaves; ++s) sum += red[1][s];
+    acc *= f;
+    if (slice < columns)
+      for (int u = slice; u < min(kThreads, keys - t0); u += columns) {
+        const uint8_t* const v = static_cast<const uint8_t*>(p.vc.ptr) + v_row[u];
+        float x = 0.f;
+        for (int r = 0; r < p.rk; ++r) {
+          const uint8_t* const row = v + r * p.vc.stride_r;
+          x += fp4_number(row + v_parts.a_codes, row + v_parts.a_scales, h) * fp4_number(row, row + v_parts.b_scales, d);
+        }
+        acc += weight[u] * x;
+      }
+    __syncthreads();
+  }
+  out[tid] = acc;
+  __syncthreads();
+  if (tid < p.dv) {
+    float x = 0.f;
+    for (int s = 0; s < columns; ++s) x += out[s * p.dv + tid];
+    store_from_f32(static_cast<T*>(p.o) + ((int64_t)b * p.cols + c) * p.dv + tid, sum == 0.f ? NAN : x / (sum * p.rk));
+  }
+  if (p.lse && tid == 0) p.lse[((int64_t)b * p.H + h) * p.lq + qi] = sum == 0.f ? -INFINITY : m + logf(sum);
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+bool mfma_takes(const TpaDecodeFp4Args* a) {
+  if (a->dk != a->dv || (a->dk != 64 && a->dk != 128) || a->H % 8 || (a->rk != 1 && a->rk != 2 && a->rk != 4 && a->rk != 8)) return false;
+  if ((int64_t)a->B * ((int64_t)a->lk * a->rk / (kRows * kWaves) + 1) > INT32_MAX) return false;  // rounds
+  for (const TpaFactor* f : {&a->k_cache, &a->v_cache})
+    if (reinterpret_cast<uintptr_t>(f->ptr) % 4 || f->stride_b % 4 || f->stride_l % 4 || f->stride_r % 4) return false;
+  return true;
+}
+
+struct Plan { int sets, col_groups, groups; int64_t slots; size_t plan_bytes, bytes; };
+Plan plan_of(const TpaDecodeFp4Args* a) {
+  Plan p;
+  const int64_t cols = (int64_t)a->lq * a->H;
+  p.sets = cols > 32 ? 2 : 1;
+  p.col_groups = (int)((cols + 32 * p.sets - 1) / (32 * p.sets));
+  const int64_t rounds = a->B * (((int64_t)a->lk * a->rk + kRows * kWaves - 1) / (kRows * kWaves));
+  p.groups = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / p.col_groups));
+  p.slots = (int64_t)p.groups + a->B;
+  p.plan_bytes = (4 * ((size_t)a->B + 1) + 255) / 256 * 256;
+  p.bytes = p.plan_bytes + 4 * (size_t)p.slots * cols * (a->dv + 2);
+  return p;
+}
+
+int check_args(const TpaDecodeFp4Args* a) {
+  if (!a) return TPA_ERR_NULL;
+  if (a->dtype != TPA_DTYPE_F32 && a->dtype != TPA_DTYPE_BF16) return TPA_ERR_DTYPE;
+  if (a->B <= 0 || a->lq <= 0 || a->lk <= 0 || a->H <= 0 || a->dk <= 0 || a->dv <= 0 || a->rq <= 0 || a->rk <= 0) return TPA_ERR_SHAPE;
+  if (a->dk > 256 || a->dv > 256 || (int64_t)a->B * a->lq * a->H > 1 << 24 || (int64_t)a->lk * a->rk > INT32_MAX / 2) return TPA_ERR_SHAPE;
+  if (a->causal < TPA_CAUSAL_NONE || a->causal > TPA_CAUSAL_BOTTOM_RIGHT) return TPA_ERR_UNSUPPORTED;
+  if (a->kernel != TPA_KERNEL_AUTO && a->kernel != TPA_KERNEL_GENERIC && a->kernel != TPA_KERNEL_MFMA) return TPA_ERR_UNSUPPORTED;
+  for (const TpaFactor* f : {&a->qa, &a->qb, &a->k_cache, &a->v_cache})
+    if (!f->ptr) return TPA_ERR_NULL;
+  if (a->page_table && (a->page_size <= 0 || a->pages_per_seq <= 0 || a->num_pages <= 0 || (int64_t)a->page_size * a->pages_per_seq < a->lk)) return TPA_ERR_SHAPE;
+  if (a->kernel == TPA_KERNEL_MFMA && !mfma_takes(a)) return TPA_ERR_UNSUPPORTED;
+  return TPA_OK;
+}
+
+template <typename T, int D, int RK, int NC, int QS, int PS>
+int launch(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+  auto kern = decode_fp4_kernel<T, D, RK, NC, QS, PS>;
+  constexpr size_t lds = Fp4Lds<D, NC, QS>::kBytes;
+  static bool configured[kMaxDevices] = {};
+  if (int rc = raise_lds_limit(configured, reinterpret_cast<const void*>(kern), lds); rc != TPA_OK) return rc;
+  hipLaunchKernelGGL(kern, dim3(p.groups, plan.col_groups), dim3(kThreads), lds, stream, p);
+  if (hipGetLastError() != hipSuccess) return TPA_ERR_LAUNCH;
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(p.B * p.cols)), dim3(kThreads), 0, stream, p);
+  return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
+}
+template <typename T, int D, int RK>
+int launch_sets(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) return plan.sets == 1 ? launch<T, D, RK, 1, 2, 1>(p, plan, stream) : launch<T, D, RK, 2, 2, 1>(p, plan, stream);
+  else return plan.sets == 1 ? launch<T, D, RK, 1, 3, 3>(p, plan, stream) : launch<T, D, RK, 2, 3, 3>(p, plan, stream);
+}
+template <typename T, int D>
+int launch_rank(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+  switch (p.rk) {
+    case 1: return launch_sets<T, D, 1>(p, plan, stream);
+    case 2: return launch_sets<T, D, 2>(p, plan, stream);
+    case 4: return launch_sets<T, D, 4>(p, plan, stream);
+    default: return launch_sets<T, D, 8>(p, plan, stream);
+  }
+}
+
+}  // namespace
+}  // namespace tpa
+
+extern "C" size_t tpa_decode_fp4_workspace_bytes(const TpaDecodeFp4Args* a) {
+  using namespace tpa;
+  if (check_args(a) != TPA_OK || a->kernel == TPA_KERNEL_GENERIC || !mfma_takes(a)) return 0;
+  return plan_of(a).bytes;
+}
+
+extern "C" int tpa_decode_fp4(const TpaDecodeFp4Args* a, void* stream) {
+  using namespace tpa;
+  if (int rc = check_args(a); rc != TPA_OK) return rc;
+  if (!a->o) return TPA_ERR_NULL;
+  Fp4Params p{};
+  p.qa = a->qa; p.qb = a->qb; p.kc = a->k_cache; p.vc = a->v_cache;
+  p.o = a->o; p.lse = a->lse; p.kvlen = a->kv_lengths; p.table = a->page_table;
+  p.page_size = a->page_size > 0 ? a->page_size : 1; p.pages_per_seq = a->pages_per_seq; p.num_pages = a->num_pages;
+  p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
+  p.B = a->B; p.lq = a->lq; p.lk = a->lk; p.H = a->H; p.dk = a->dk; p.dv = a->dv; p.rq = a->rq; p.rk = a->rk; p.cols = a->lq * a->H;
+  p.causal = a->causal;
+  if (a->causal) {
+    const int far = a->causal == TPA_CAUSAL_BOTTOM_RIGHT ? a->lq + a->lk : a->lk;
+    p.coff = clamp_causal_offset(a->causal_offset, a->causal == TPA_CAUSAL_BOTTOM_RIGHT ? -far : -a->lq, far);
+  }
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (a->kernel == TPA_KERNEL_GENERIC || !mfma_takes(a)) {
+    p.scale = a->sm_scale;
+    const dim3 grid((unsigned)(p.B * p.cols));
+    if (a->dtype == TPA_DTYPE_BF16) hipLaunchKernelGGL(decode_fp4_any_kernel<uint16_t>, grid, dim3(kThreads), 0, on, p);
+    else hipLaunchKernelGGL(decode_fp4_any_kernel<float>, grid, dim3(kThreads), 0, on, p);
+    return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
+  }
+  const Plan plan = plan_of(a);
+  if (!a->workspace || a->workspace_bytes < plan.bytes) return TPA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 256 || reinterpret_cast<uintptr_t>(a->o) % 16) return TPA_ERR_ALIGN;
+  p.scale = a->sm_scale * kLog2e / ((float)a->rq * (float)a->rk);
+  p.groups = plan.groups;
+  p.plan = static_cast<int32_t*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.plan_bytes);
+  p.part_m = p.part_o + plan.slots * p.cols * p.dv;
+  p.part_l = p.part_m + plan.slots * p.cols;
+  if (a->dtype == TPA_DTYPE_BF16) return a->dk == 128 ? launch_rank<uint16_t, 128>(p, plan, on) : launch_rank<uint16_t, 64>(p, plan, on);
+  return a->dk == 128 ? launch_rank<float, 128>(p, plan, on) : launch_rank<float, 64>(p, plan, on);
+}

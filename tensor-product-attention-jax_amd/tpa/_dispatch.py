@@ -24,7 +24,7 @@ KERNEL_AUTO = 0
 KERNEL_GENERIC = 1
 KERNEL_MFMA = 2
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 
 class TpaFactor(ctypes.Structure):
@@ -298,6 +298,138 @@ class TpaNormRopeBwdArgs(ctypes.Structure):
     ]
 
 
+class TpaFp4RowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("ka", TpaFactor),
+        ("kb", TpaFactor),
+        ("va", TpaFactor),
+        ("vb", TpaFactor),
+        ("k_cache", TpaFactor),
+        ("v_cache", TpaFactor),
+        ("slots", ctypes.c_void_p),
+        ("page_size", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("l", ctypes.c_int32),
+        ("H", ctypes.c_int32),
+        ("dk", ctypes.c_int32),
+        ("dv", ctypes.c_int32),
+        ("rk", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class TpaDecodeFp4Args(ctypes.Structure):
+    _fields_ = [
+        ("qa", TpaFactor),
+        ("qb", TpaFactor),
+        ("k_cache", TpaFactor),
+        ("v_cache", TpaFactor),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("B", ctypes.c_int32),
+        ("lq", ctypes.c_int32),
+        ("lk", ctypes.c_int32),
+        ("H", ctypes.c_int32),
+        ("dk", ctypes.c_int32),
+        ("dv", ctypes.c_int32),
+        ("rq", ctypes.c_int32),
+        ("rk", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("causal_offset", ctypes.c_int32),
+        ("kernel", ctypes.c_int32),
+        ("kv_lengths", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("page_size", ctypes.c_int32),
+        ("pages_per_seq", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class TpaBeamSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_n", ctypes.c_int64),
+        ("scores", ctypes.c_void_p),
+        ("finished", ctypes.c_void_p),
+        ("new_scores", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("tokens", ctypes.c_void_p),
+        ("new_finished", ctypes.c_void_p),
+        ("B", ctypes.c_int32),
+        ("beams", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("num_out", ctypes.c_int32),
+        ("eos_token", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class TpaPool(ctypes.Structure):
+    _fields_ = [
+        ("ptr", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("token_bytes", ctypes.c_int64),
+    ]
+
+
+class TpaPagesForkArgs(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("kv_lengths", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("page_shares", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_start", ctypes.c_void_p),
+        ("new_page_table", ctypes.c_void_p),
+        ("new_kv_lengths", ctypes.c_void_p),
+        ("new_page_shares", ctypes.c_void_p),
+        ("new_free_pages", ctypes.c_void_p),
+        ("new_free_start", ctypes.c_void_p),
+        ("pools", ctypes.POINTER(TpaPool)),
+        ("num_pools", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("M", ctypes.c_int32),
+        ("pages_per_seq", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("num_free", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class TpaPagesCompactArgs(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("kv_lengths", ctypes.c_void_p),
+        ("page_shares", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_start", ctypes.c_void_p),
+        ("new_page_table", ctypes.c_void_p),
+        ("new_page_shares", ctypes.c_void_p),
+        ("new_free_pages", ctypes.c_void_p),
+        ("new_free_start", ctypes.c_void_p),
+        ("moved", ctypes.c_void_p),
+        ("pools", ctypes.POINTER(TpaPool)),
+        ("num_pools", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("pages_per_seq", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("num_free", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class TpaError(RuntimeError):
     """A non-zero return code of the C ABI."""
 
@@ -374,6 +506,20 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.tpa_decode_shared.argtypes = [ctypes.POINTER(TpaFwdArgs), ctypes.c_int32, ctypes.c_void_p]
         lib.tpa_decode_shared_workspace_bytes.restype = ctypes.c_size_t
         lib.tpa_decode_shared_workspace_bytes.argtypes = [ctypes.POINTER(TpaFwdArgs), ctypes.c_int32]
+        for name, args in (
+            ("tpa_cache_write_fp4", TpaFp4RowsArgs), ("tpa_cache_read_fp4", TpaFp4RowsArgs), ("tpa_decode_fp4", TpaDecodeFp4Args),
+            ("tpa_beam_select", TpaBeamSelectArgs), ("tpa_pages_fork", TpaPagesForkArgs), ("tpa_pages_compact", TpaPagesCompactArgs),
+        ):
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        for name, args in (
+            ("tpa_fp4_row_bytes", [ctypes.c_int32] * 2), ("tpa_decode_fp4_workspace_bytes", [ctypes.POINTER(TpaDecodeFp4Args)]),
+            ("tpa_beam_select_workspace_bytes", [ctypes.c_int32] * 5), ("tpa_pages_workspace_bytes", [ctypes.c_int32] * 2),
+        ):
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_size_t
+            fn.argtypes = args
         if lib.tpa_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{p}: ABI version {lib.tpa_abi_version()} != {ABI_VERSION}")
         if path is None:

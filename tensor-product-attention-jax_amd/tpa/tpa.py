@@ -39,6 +39,7 @@ from . import _dispatch as _d
 __all__ = [
     "BlockSizes", "tpa", "tpa_factors", "tpa_decode", "tpa_cache_append", "tpa_factors_bwd", "_tpa_fwd", "_tpa_bwd", "_fwd", "_bwd",
     "_precompute_delta", "_lse", "_lse_accum", "tpa_decode_shared", "tpa_page_tables", "tpa_norm_rope", "tpa_norm_rope_bwd", "tpa_norm_rope_write",
+    "fp4_row_bytes", "tpa_cache_write_fp4", "tpa_cache_read_fp4", "tpa_decode_fp4", "tpa_beam_select", "tpa_pages_fork", "tpa_pages_compact",
 ]
 
 
@@ -332,6 +333,125 @@ def tpa_norm_rope_write(
     return _call(
         _d.host_calls().norm_rope_write, (q, k, v, slots, rope_cos, rope_sin, q_weight, k_weight, positions),
         int(num_heads), sections, bool(normalize), float(eps), int(kernel), ka, kb, va, vb,
+    )
+
+
+def fp4_row_bytes(num_heads: int, head_dim: int) -> int:
+    """Bytes of a row of a cache in 4 bits: the K (or V) factors of one token and rank, h + d numbers in 4 bits with a scale byte for each 32 of
+    the h and of the d, up to a multiple of four (`include/tpa_abi.h` has the layout)."""
+    return int(_d.load_library().tpa_fp4_row_bytes(int(num_heads), int(head_dim)))
+
+
+def tpa_cache_write_fp4(k, v, num_heads: int, k_cache, v_cache, slots):
+    """The K and V factors of new tokens into a paged cache that holds them in 4 bits (an addition).
+
+    k[b,l,rk,h+dk], v[b,l,rk,h+dv] of the new tokens, packed (b = 1) or not, as `tpa_norm_rope` leaves them; `slots` int [b, l] of
+    `tpa_page_tables`: token i's rows go to place slots[i] % page_size of page slots[i] // page_size of k_cache and v_cache, uint8
+    [pages, page_size, rk, fp4_row_bytes(h, dk|dv)], which `tpa_decode_fp4` reads; slots outside the pools (-1) are dropped, and no slot may be there twice.
+    A contiguous cache [b, cache_len, rk, bytes] is a pool whose pages are the batch entries.  Each 32 numbers share a power of two as their scale; a
+    number is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it, or a negative of these, to the nearest.  32 numbers with an infinity or a NaN among them are
+    all NaN afterwards.  No gradient flows through this call.
+    """
+    return _call(_d.host_calls().cache_write_fp4, (k, v, slots), k_cache, v_cache, int(num_heads))
+
+
+def tpa_cache_read_fp4(k_cache, v_cache, num_heads: int, slots, *, head_dim: int, v_head_dim: int | None = None, dtype=torch.bfloat16):
+    """The K and V factors that slots of a cache in 4 bits stand for (an addition): (k[b,l,rk,h+dk], v[b,l,rk,h+dv]) as `tpa` and `tpa_norm_rope`
+    take them, zeros for slots outside the pools.  dk = `head_dim`, dv = `v_head_dim` (default the same); every number a cache holds is exact in
+    either dtype.  With it a chunk of new tokens runs through `tpa` over cached ones."""
+    return _call(
+        _d.host_calls().cache_read_fp4, (k_cache, v_cache, slots), int(num_heads), int(head_dim), int(head_dim if v_head_dim is None else v_head_dim),
+        int(_d.dtype_code(dtype) == _d.TPA_DTYPE_BF16),
+    )
+
+
+def tpa_decode_fp4(
+    qa, qb, k_cache, v_cache,
+    sm_scale: float = 1.0,
+    workspace: torch.Tensor | None = None,
+    kernel: int = _d.KERNEL_AUTO,
+    kv_lengths=None,
+    page_table=None,
+    causal: bool = False,
+    causal_offset: int = 0,
+    v_head_dim: int | None = None,
+):
+    """`tpa_decode` over a cache in 4 bits (an addition): the rows that `tpa_cache_write_fp4` wrote, 352 bytes a token where bf16 factors take 1280 (32 heads
+    of 128, rank 2).  qa[b,lq,rq,h], qb[b,lq,rq,dk] in bf16 or fp32; k_cache, v_cache uint8 [b, lk, rk, fp4_row_bytes(h, dk|dv)], or with
+    `page_table` (int32 [b, pages_per_seq]) pools [pages, page_size, rk, bytes] with pages of any size; dv = `v_head_dim` (default dk).  The
+    other arguments and the results are `tpa_decode`'s.  Pages outside the pools are read as the nearest one.  `workspace` (uint8, at least `decode_fp4_workspace_bytes(...)`) may
+    be passed to avoid the allocation; a workspace serves one call at a time.
+    Returns (o[b,lq,h,dv], lse[b,h,lq]).
+    """
+    return _call(
+        _d.host_calls().decode_fp4, (qa, qb, k_cache, v_cache, kv_lengths, page_table, workspace),
+        sm_scale, int(kernel), _causal_code(causal), int(causal_offset), -1 if v_head_dim is None else int(v_head_dim),
+    )
+
+
+def decode_fp4_workspace_bytes(qa, qb, k_cache, v_cache, *, page_table=None, v_head_dim: int | None = None, kernel: int = _d.KERNEL_AUTO) -> int:
+    """What `tpa_decode_fp4` needs for operands of these shapes and layouts (room to align it among it)."""
+    b, lq, rq, h = qa.shape
+    rows, per, rk, _ = k_cache.shape
+    args = _d.TpaDecodeFp4Args(
+        qa=_d.factor(qa), qb=_d.factor(qb), k_cache=_d.factor(k_cache), v_cache=_d.factor(v_cache),
+        B=b, lq=lq, lk=per if page_table is None else page_table.shape[1] * per, H=h, dk=qb.shape[-1], dv=qb.shape[-1] if v_head_dim is None else v_head_dim,
+        rq=rq, rk=rk, dtype=_d.dtype_code(qa.dtype), sm_scale=1.0, kernel=int(kernel),
+        page_table=None if page_table is None else page_table.data_ptr(), page_size=0 if page_table is None else per,
+        pages_per_seq=0 if page_table is None else page_table.shape[1], num_pages=rows,
+    )
+    return int(_d.load_library().tpa_decode_fp4_workspace_bytes(ctypes.byref(args))) + 256
+
+
+def tpa_beam_select(logits, scores, *, num_out: int | None = None, finished=None, eos_token: int | None = None):
+    """The continuations that a step of beam search goes on with (an addition).
+
+    logits[b, beams, vocab] (bf16 or fp32), scores[b, beams]: of every request, the `num_out` (default: beams; up to 64) largest of
+    score + logit - log(sum(exp(logits of the beam))) over its beams and the vocabulary, in falling order, equal ones by the lower beam and then token.  A beam
+    that is `finished` (bool [b, beams], with `eos_token`) has one continuation, itself with that token, and keeps its score.  Values that are
+    NaN or +inf count as -inf.  All results stay on the GPU (no synchronisation):
+
+        new_scores[b, num_out]   fp32
+        parents[b, num_out]      int32: the row i * beams + beam that each goes on from, for `tpa_pages_fork`
+        tokens[b, num_out]       int32
+        new_finished[b, num_out] bool: the beam was finished, or the token is `eos_token`
+    """
+    return _call(
+        _d.host_calls().beam_select, (logits, scores, finished), -1 if num_out is None else int(num_out), -1 if eos_token is None else int(eos_token)
+    )
+
+
+def tpa_pages_fork(page_table, kv_lengths, parents, page_shares, free_pages, pools, *, page_size: int, free_start=None):
+    """Sequences that go on from chosen ones, in a paged cache (an addition): beams after `tpa_beam_select`, samples of one prompt, requests that end (no
+    new sequence names them) or change their row.
+
+    New sequence i (of as many as `parents`, int, has) goes on from sequence parents[i] of the old ones, whose pages and lengths are `page_table` [b,
+    pages_per_seq] and `kv_lengths` [b]; another number (-1) makes it empty.  It shares the whole pages.  The last page, if only partly filled, stays with
+    the first new sequence of its old one, if no other sequence holds it; the others get a page of `free_pages` from index `free_start` (int32
+    [1], 0 if not given) on, and the tokens are copied into it in every tensor of `pools` ([pages, page_size, ..], any type, in place: the layers' K and V).
+    Without a free page left a sequence ends with its whole pages, as new_kv_lengths says.  `page_shares` (int [pages]) counts the sequences that hold a page
+    beyond the first: zeros at the start, and `tpa_page_tables` need not know it.  Pages that nobody holds any more come back to the list, in rising order,
+    before the first page that is still free; the list has room for every page that was taken from it.  All results are new int32 tensors on the GPU:
+
+        new_page_table[len(parents), pages_per_seq], new_kv_lengths[len(parents)], new_page_shares[pages],
+        new_free_pages (as long as free_pages), new_free_start[1]
+    """
+    return _call(
+        _d.host_calls().pages_fork, (page_table, kv_lengths, parents, page_shares, free_pages, free_start), pools, int(page_size)
+    )
+
+
+def tpa_pages_compact(page_table, kv_lengths, page_shares, free_pages, pools, *, page_size: int, free_start=None):
+    """The pages in use moved to the front of their pools (an addition), so that the rest of the pools can be given away.
+
+    In use are the n pages that do not stand in `free_pages` from `free_start` on; those at n and behind go to the free pages before n, in rising order, in
+    every tensor of `pools`.  Arguments are those of `tpa_pages_fork`.  Returns new int32 tensors on the GPU:
+
+        new_page_table, new_page_shares[pages], new_free_pages (n .. pages - 1 at its end), new_free_start[1],
+        moved[pages]   where each page is now, for holders of pages that are not in this table
+    """
+    return _call(
+        _d.host_calls().pages_compact, (page_table, kv_lengths, page_shares, free_pages, free_start), pools, int(page_size)
     )
 
 
