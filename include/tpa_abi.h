@@ -475,7 +475,7 @@ typedef struct TpaPool {
  * the first page that is still free, whose place new_free_start names (the first one released: those for which the list has no room before are left
  * out).  The list has room for every page that was taken from it.
  * Table entries outside 0 .. num_pages - 1 are passed on and hold no page.  Lengths past the table's row count as its end, counts and lengths below 0 as 0.
- * Outputs must not overlap inputs.  Two launches (one more for every TPA_MAX_POOLS pools).
+ * Outputs must not overlap inputs.  One launch for up to 8192 pages, 2048 sequences and TPA_MAX_POOLS pools, otherwise two, and one more for every further TPA_MAX_POOLS pools.
  */
 typedef struct TpaPagesForkArgs {
   const int32_t* page_table;   /* [B, pages_per_seq] */
@@ -504,8 +504,8 @@ typedef struct TpaPagesForkArgs {
  *   moved[p] = where page p is now, p itself for a page that is free;  new_page_shares has the counts at the new places, 0 from n on;
  *   new_page_table: the entries of each row's ceil(kv_lengths / page_size) pages at their new places (an entry outside 0 .. num_pages - 1 as
  *   it was), then zeros;  new_free_pages ends with n .. num_pages - 1, new_free_start names the place of n.
- * Every holder of pages that is not a row of this table is to look its pages up in `moved`.  Outputs must not overlap inputs.  Two launches (one more for every
- * TPA_MAX_POOLS pools).
+ * Every holder of pages that is not a row of this table is to look its pages up in `moved`.  Outputs must not overlap inputs.
+ * One launch for up to 8192 pages and TPA_MAX_POOLS pools, otherwise two, and one more for every further TPA_MAX_POOLS pools.
  */
 typedef struct TpaPagesCompactArgs {
   const int32_t* page_table;   /* [B, pages_per_seq] */
@@ -697,8 +697,8 @@ size_t tpa_beam_select_workspace_bytes(int32_t B, int32_t beams, int32_t vocab, 
 /* Pages of sequences that go on from chosen ones (see TpaPagesForkArgs), and pages moved to the front of their pools (see TpaPagesCompactArgs). */
 int tpa_pages_fork(const TpaPagesForkArgs* args, void* stream);
 int tpa_pages_compact(const TpaPagesCompactArgs* args, void* stream);
-/* Bytes of workspace that either needs; M = 0 for tpa_pages_compact. */
-size_t tpa_pages_workspace_bytes(int32_t M, int32_t num_pages);
+/* Bytes of workspace that tpa_pages_fork needs, or with M = 0 tpa_pages_compact (and a fork without new sequences); 0 where one launch does the work. */
+size_t tpa_pages_workspace_bytes(int32_t B, int32_t M, int32_t num_pages, int32_t num_pools);
 
 #ifdef __cplusplus
 }

@@ -1241,13 +1241,18 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Device device = logits.device();
     const c10::DeviceGuard guard(device);
     if (vocab > 1 && logits.stride(2) != 1) logits = logits.contiguous();
-    scores = scores.to(at::kFloat).contiguous();
+    if (scores.scalar_type() != at::kFloat) scores = scores.to(at::kFloat);
+    scores = scores.contiguous();
     if (finished.defined()) finished = finished.contiguous();
-    const auto options = at::TensorOptions().device(device);
-    out[0] = at::empty({b, k}, options.dtype(at::kFloat));
-    out[1] = at::empty({b, k}, options.dtype(at::kInt));
-    out[2] = at::empty({b, k}, options.dtype(at::kInt));
-    out[3] = at::empty({b, k}, options.dtype(at::kBool));
+    // one allocation for four small results, each at a multiple of 256 bytes
+    const int64_t each = (b * k * 4 + 255) / 256 * 256;
+    const Tensor all = bytes_on(device, 4 * each);
+    const at::ScalarType types[4] = {at::kFloat, at::kInt, at::kInt, at::kBool};
+    for (int i = 0; i < 4; ++i) {
+      out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(types[i]));
+      out[i].unsafeGetTensorImpl()->set_storage_offset(i * each / (int64_t)c10::elementSize(types[i]));
+      out[i].unsafeGetTensorImpl()->set_sizes_contiguous({b, k});
+    }
     if (b) {
       TpaBeamSelectArgs a{};
       a.logits = logits.data_ptr();
@@ -1383,8 +1388,8 @@ PyObject* pages_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.M = (int)m;
     a.new_page_table = int_ptr(out[0]); a.new_kv_lengths = int_ptr(out[1]); a.new_page_shares = int_ptr(out[2]);
     a.new_free_pages = int_ptr(out[3]); a.new_free_start = int_ptr(out[4]);
-    const Tensor ws = bytes_on(device, lib.tpa_pages_workspace_bytes(a.M, a.num_pages) + 16);
-    take_workspace(ws, 16, a);
+    Tensor ws;
+    if (const size_t need = lib.tpa_pages_workspace_bytes(a.B, a.M, a.num_pages, a.num_pools)) take_workspace(ws = bytes_on(device, need + 16), 16, a);
     check("tpa_pages_fork", lib.tpa_pages_fork(&a, stream_of(device)));
     for (const Tensor& t : pools) written(t);
   }
@@ -1417,8 +1422,8 @@ PyObject* pages_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
     describe_pages(s, described, a);
     a.new_page_table = int_ptr(out[0]); a.new_page_shares = int_ptr(out[1]); a.new_free_pages = int_ptr(out[2]); a.new_free_start = int_ptr(out[3]);
     a.moved = int_ptr(out[4]);
-    const Tensor ws = bytes_on(device, lib.tpa_pages_workspace_bytes(0, a.num_pages) + 16);
-    take_workspace(ws, 16, a);
+    Tensor ws;
+    if (const size_t need = lib.tpa_pages_workspace_bytes(a.B, 0, a.num_pages, a.num_pools)) take_workspace(ws = bytes_on(device, need + 16), 16, a);
     check("tpa_pages_compact", lib.tpa_pages_compact(&a, stream_of(device)));
     for (const Tensor& t : pools) written(t);
   }

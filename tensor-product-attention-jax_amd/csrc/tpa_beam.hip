@@ -1,9 +1,9 @@
 // The continuations of a step of beam search: the largest values of score + logit - log sum exp over a request's beams and vocabulary.
 //
-// First launch: a wave reads a chunk of a beam's logits once.  Every lane keeps a sum of exponentials against a maximum of its own; the largest logits of the
-// chunk stand sorted in the lanes of the wave (lane r: the r-th), and a logit goes in only if it beats the last of them, which after the first few hundred
-// hardly any does: num_out * ln(chunk / 512) on average.  (Inside a beam the order of the values is that of the logits.)
-// Second launch: a workgroup for each request joins the sums and picks num_out times the largest of the chunks' candidates, in 64 bits.
+// First launch: a wave holds a chunk of a beam's logits in its registers.  Every lane sums exponentials against a maximum of its own; the k-th largest of
+// the lanes' maxima bounds the chunk's k largest logits from below, and what is above it is put into a list sorted over the lanes (lane r: the r-th).
+// (Inside a beam the order of the values is that of the logits.)
+// Second launch: a workgroup for each request joins the sums and ranks the chunks' candidates, in 64 bits, behind a bound found in the same way.
 // Equal values go to the lower index: logits are put in by rising index, behind their equals, and the last step compares value and index.
 //
 // HBM bounds it where there are many beams, the latency of two launches where there are few.
@@ -16,8 +16,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBatch = 512;      // logits that a wave looks at together, eight a lane
-constexpr int kAhead = 4;        // batches asked for together
-constexpr int kHeld = 8192;      // candidates that the second launch holds in LDS
+constexpr int kHeld = 4096;      // candidates that the second launch holds in LDS
+constexpr int kListed = 512;     // candidates that it ranks among each other
 // log2(e) in two parts: one alone is off by 1.3e-8 of itself, which a logit of 12 makes 2e-7 of every term
 constexpr float kLog2eHigh = 1.44269502f, kLog2eLow = 1.92596299e-8f;
 
@@ -34,7 +34,7 @@ struct BeamParams {
   uint8_t* new_finished;
   Sum* sums;              // [B, beams, chunks]
   Candidate* candidates;  // [B, beams, chunks, k]
-  int B, n, vocab, k, eos, chunk, chunks;
+  int B, n, vocab, k, eos, chunks;
 };
 
 __device__ __forceinline__ float max8(const float (&x)[8]) {
@@ -64,6 +64,10 @@ struct Eight<uint16_t> {
       x[2 * j + 1] = bf16hi_to_f32(w[j]);
     }
   }
+  __device__ __forceinline__ void load_part(const uint16_t* p, int n) {  // the first n of them, -inf behind
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = (2 * j < n ? (uint32_t)p[2 * j] : 0xff80u) | (2 * j + 1 < n ? (uint32_t)p[2 * j + 1] : 0xff80u) << 16;
+  }
 };
 template <>
 struct Eight<float> {
@@ -80,9 +84,18 @@ struct Eight<float> {
       x[4 + j] = hi[j];
     }
   }
+  __device__ __forceinline__ void load_part(const float* p, int n) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lo[j] = j < n ? p[j] : -INFINITY;
+      hi[j] = 4 + j < n ? p[4 + j] : -INFINITY;
+    }
+  }
 };
 
-template <typename T>
+// NB: batches of a chunk.  The chunk stays in registers: all of it is asked for at once, and when the lanes' maxima are known, the k-th largest of
+// them leaves hardly more than k logits to put in.
+template <typename T, int NB>
 __global__ __launch_bounds__(kThreads) void chunk_kernel(BeamParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + scalar((int)(threadIdx.x >> 6));
@@ -90,35 +103,53 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(BeamParams p) {
   const int row = (int)(id / p.chunks), chunk = (int)(id - (int64_t)row * p.chunks), b = row / p.n, beam = row - b * p.n;
   if (p.finished && p.finished[row]) return;  // its one candidate needs no logits
   const T* const logits = static_cast<const T*>(p.logits) + b * p.stride_b + beam * p.stride_n;
-  const int begin = chunk * p.chunk, end = begin + min(p.chunk, p.vocab - begin);
+  const int begin = chunk * (NB * kBatch), end = begin + min(NB * kBatch, p.vocab - begin);
 
-  float r = -INFINITY, s = 0.f;             // this lane's logits: sum of exp2(x log2 e - r)
-  float best = -INFINITY;                   // lane i: the i-th largest logit so far
-  int token = -1;
-  float least = -INFINITY;                  // the k-th largest: what a logit has to beat
-  auto look = [&](const float (&x)[8], int first, bool fill) __attribute__((always_inline)) {
-    const float most = max8(x);
-    const float rn = fmaxf(r, most * kLog2eHigh), ru = rn == -INFINITY ? 0.f : rn;
+  Eight<T> held[NB];
+  if (end - begin == NB * kBatch) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) held[n].load(logits + begin + n * kBatch + 8 * lane);
+  } else {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) held[n].load_part(logits + begin + n * kBatch + 8 * lane, end - begin - n * kBatch - 8 * lane);
+  }
+
+  float r = -INFINITY, s = 0.f;  // this lane's logits: sum of exp2(x log2 e - r)
+  float most[NB], top = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    float x[8];
+    held[n].get(x);
+    most[n] = max8(x);
+    top = fmaxf(top, most[n]);
+    const float rn = fmaxf(r, most[n] * kLog2eHigh), ru = rn == -INFINITY ? 0.f : rn;
     float terms[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) terms[j] = __builtin_amdgcn_exp2f(fmaf(x[j], kLog2eLow, fmaf(x[j], kLog2eHigh, -ru)));
     s = fmaf(s, __builtin_amdgcn_exp2f(r - ru), ((terms[0] + terms[1]) + (terms[2] + terms[3])) + ((terms[4] + terms[5]) + (terms[6] + terms[7])));
     r = rn;
-    if (fill) {
-      // the k-th largest of the lanes' maxima: at least k logits of the first batch are no smaller
-      int key = ordered(most), at = 0;
-      for (int i = 0; i < p.k; ++i) {
-        at = wave_max(key);
-        const uint64_t there = __ballot(key == at);
-        if (lane == __builtin_ctzll(there)) key = INT32_MIN;
-      }
-      // the number below it, for what is not below the maximum goes in: -inf for that of -inf (whose neighbour is a NaN), and no zero, which
-      // the zero on its other side does not beat
-      least = fmaxf(from_ordered(max(at, INT32_MIN + 1) - 1), -INFINITY);
-      if (least == 0.f) least = __uint_as_float(0x80000001u);
-    }
-    uint64_t lanes = __ballot(most > least);
-    while (lanes) {
+  }
+
+  // the k-th largest of the lanes' maxima: at least k logits are no smaller
+  int key = ordered(top), at_key = 0;
+  for (int i = 0; i < p.k; ++i) {
+    at_key = wave_max(key);
+    const uint64_t there = __ballot(key == at_key);
+    if (lane == __builtin_ctzll(there)) key = INT32_MIN;
+  }
+  // what a logit has to beat: the number below that one, -inf for that of -inf (whose neighbour is a NaN), and no zero, which the zero on its
+  // other side does not beat
+  float least = fmaxf(from_ordered(max(at_key, INT32_MIN + 1) - 1), -INFINITY);
+  if (least == 0.f) least = __uint_as_float(0x80000001u);
+  float best = -INFINITY;  // lane i: the i-th largest logit so far
+  int token = -1;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    uint64_t lanes = __ballot(most[n] > least);
+    if (!lanes) continue;
+    float x[8];
+    held[n].get(x);
+    do {
       const int from = __builtin_ctzll(lanes);
       lanes &= lanes - 1;
 #pragma unroll
@@ -129,38 +160,11 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(BeamParams p) {
           const float best_before = __int_as_float(lane_before(__float_as_int(best)));
           const int token_before = lane_before(token);
           best = lane > at ? best_before : lane == at ? v : best;
-          token = lane > at ? token_before : lane == at ? first + 8 * from + j : token;
+          token = lane > at ? token_before : lane == at ? begin + n * kBatch + 8 * from + j : token;
           least = fmaxf(least, lane_value(best, p.k - 1));
         }
       }
-    }
-  };
-
-  Eight<T> now[kAhead], next[kAhead];
-  const int whole = (end - begin) / kBatch;  // batches without a missing logit
-  auto request = [&](Eight<T>(&to)[kAhead], int batch) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) to[u].load(logits + begin + (int64_t)min(batch + u, whole - 1) * kBatch + 8 * lane);
-  };
-  if (whole > 0) request(now, 0);
-  for (int batch = 0; batch < whole; batch += kAhead) {
-    if (batch + kAhead < whole) request(next, batch + kAhead);
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (batch + u >= whole) break;
-      float x[8];
-      now[u].get(x);
-      look(x, begin + (batch + u) * kBatch, batch + u == 0);
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
-  }
-  if (begin + whole * kBatch < end) {
-    float x[8];
-    const int first = begin + whole * kBatch;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = first + 8 * lane + j < end ? load_as_f32(logits + first + 8 * lane + j) : -INFINITY;
-    look(x, first, whole == 0);
+    } while (lanes);
   }
 
   const float rw = from_ordered(wave_max(ordered(r))), ru = rw == -INFINITY ? 0.f : rw;
@@ -177,7 +181,8 @@ __global__ __launch_bounds__(kThreads) void select_kernel(BeamParams p) {
   __shared__ double red_value[kThreads / 64];
   __shared__ int red_flat[kThreads / 64];
   __shared__ double won_value[TPA_BEAM_MAX];
-  __shared__ int won[TPA_BEAM_MAX];
+  __shared__ int won[TPA_BEAM_MAX], listed, list_flat[kListed];
+  __shared__ double list_value[kListed];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int per_beam = p.chunks * p.k, total = p.n * per_beam;
   const Candidate* const all = p.candidates + (int64_t)b * total;
@@ -206,46 +211,82 @@ __global__ __launch_bounds__(kThreads) void select_kernel(BeamParams p) {
   }
   __syncthreads();
 
-  // the best candidate of this thread's behind (value, flat index); values that are no number, or infinite, are none
-  auto best_behind = [&](double value, int flat, double& best, int& best_flat) {
-    best = -INFINITY;
-    best_flat = INT32_MAX;
-    auto consider = [&](double v, int f) {
-      if (!(fabs(v) < INFINITY)) return;
-      if (!(v < value || (v == value && f > flat))) return;
-      if (v > best || (v == best && f < best_flat)) { best = v; best_flat = f; }
-    };
+  // this thread's candidates; values that are no number, or infinite, are none
+  auto for_each = [&](auto visit) __attribute__((always_inline)) {
     for (int i = tid; i < total; i += kThreads) {
       const int j = i / per_beam;
       const Candidate c = hold ? held[i] : all[i];
-      if (c.token >= 0) consider(base[j] + (double)c.logit, j * p.vocab + c.token);
+      const double v = base[j] + (double)c.logit;
+      if (c.token >= 0 && fabs(v) < INFINITY) visit(v, j * p.vocab + c.token);
     }
-    if (p.finished && tid < p.n && p.finished[b * p.n + tid]) consider((double)p.scores[b * p.n + tid], tid * p.vocab + p.eos);
+    if (p.finished && tid < p.n && p.finished[b * p.n + tid]) {
+      const double v = (double)p.scores[b * p.n + tid];
+      if (fabs(v) < INFINITY) visit(v, tid * p.vocab + p.eos);
+    }
   };
+  // the best of them behind (value, flat index)
+  auto best_behind = [&](double value, int flat, double& best, int& best_flat) {
+    best = -INFINITY;
+    best_flat = INT32_MAX;
+    for_each([&](double v, int f) {
+      if (!(v < value || (v == value && f > flat))) return;
+      if (v > best || (v == best && f < best_flat)) { best = v; best_flat = f; }
+    });
+  };
+  // A bound: in every wave the k-th largest of the lanes' best candidates, as fp32 rounded down; the largest of the waves' leaves k candidates or more
   double best;
   int flat;
   best_behind(INFINITY, -1, best, flat);
+  int key = ordered((float)best) - ((double)(float)best > best), at_key = 0;
+  for (int i = 0; i < p.k; ++i) {
+    at_key = wave_max(key);
+    const uint64_t there = __ballot(key == at_key);
+    if (lane == __builtin_ctzll(there)) key = INT32_MIN;
+  }
+  if (lane == 0) red_flat[w] = at_key;
+  if (tid == 0) listed = 0;
+  __syncthreads();
+  const float bound = from_ordered(max(max(max(red_flat[0], red_flat[1]), max(red_flat[2], red_flat[3])), ordered(-INFINITY)));
+  for_each([&](double v, int f) {
+    if (v < (double)bound) return;
+    const int at = atomicAdd(&listed, 1);
+    if (at < kListed) { list_value[at] = v; list_flat[at] = f; }
+  });
+  __syncthreads();
   int found = 0;
-  for (; found < p.k; ++found) {
-    double v = best;
-    int f = flat;
-#pragma unroll
-    for (int d = 32; d; d /= 2) {
-      const double ov = __shfl_xor(v, d);
-      const int of = __shfl_xor(f, d);
-      if (ov > v || (ov == v && of < f)) { v = ov; f = of; }
+  if (listed <= kListed) {
+    // in whatever order they stand: each one's place is the number of those that beat it
+    found = min(listed, p.k);
+    for (int i = tid; i < listed; i += kThreads) {
+      const double v = list_value[i];
+      const int f = list_flat[i];
+      int place = 0;
+      for (int j = 0; j < listed; ++j) place += list_value[j] > v || (list_value[j] == v && list_flat[j] < f);
+      if (place < p.k) { won_value[place] = v; won[place] = f; }
     }
-    if (lane == 0) { red_value[w] = v; red_flat[w] = f; }
-    __syncthreads();
-    v = red_value[0];
-    f = red_flat[0];
+  } else {
+    // many that are alike: the best one, k times
+    for (; found < p.k; ++found) {
+      double v = best;
+      int f = flat;
 #pragma unroll
-    for (int i = 1; i < kThreads / 64; ++i)
-      if (red_value[i] > v || (red_value[i] == v && red_flat[i] < f)) { v = red_value[i]; f = red_flat[i]; }
-    if (f == INT32_MAX) break;  // no candidate is left (the same in every thread)
-    if (tid == 0) { won_value[found] = v; won[found] = f; }
-    if (f == flat) best_behind(v, f, best, flat);
-    __syncthreads();
+      for (int d = 32; d; d /= 2) {
+        const double ov = __shfl_xor(v, d);
+        const int of = __shfl_xor(f, d);
+        if (ov > v || (ov == v && of < f)) { v = ov; f = of; }
+      }
+      if (lane == 0) { red_value[w] = v; red_flat[w] = f; }
+      __syncthreads();
+      v = red_value[0];
+      f = red_flat[0];
+#pragma unroll
+      for (int i = 1; i < kThreads / 64; ++i)
+        if (red_value[i] > v || (red_value[i] == v && red_flat[i] < f)) { v = red_value[i]; f = red_flat[i]; }
+      if (f == INT32_MAX) break;  // no candidate is left (the same in every thread)
+      if (tid == 0) { won_value[found] = v; won[found] = f; }
+      if (f == flat) best_behind(v, f, best, flat);
+      __syncthreads();
+    }
   }
   __syncthreads();
   // places without a candidate: values of -inf, the lowest indices that have not won
@@ -270,10 +311,16 @@ __global__ __launch_bounds__(kThreads) void select_kernel(BeamParams p) {
   }
 }
 
-// Logits of a wave: as many as leave about 4096 waves, between 2 and 32 batches.
-int chunk_of(int64_t B, int64_t n, int64_t vocab) {
-  const int64_t each = (B * n * vocab / 4096 + kBatch - 1) / kBatch * kBatch;
-  return (int)std::max<int64_t>(2 * kBatch, std::min<int64_t>(each, 32 * kBatch));
+// Batches of a chunk: as many as leave about 4096 waves, as far as a chunk fits the registers
+int batches_of(int64_t B, int64_t n, int64_t vocab, int dtype) {
+  const int64_t logits = B * n * vocab;
+  int batches = 2;
+  while (batches < (dtype == TPA_DTYPE_BF16 ? 16 : 8) && logits > (int64_t)4096 * batches * kBatch) batches *= 2;
+  return batches;
+}
+int64_t chunks_of(int64_t B, int64_t n, int64_t vocab, int dtype) {
+  const int64_t chunk = (int64_t)batches_of(B, n, vocab, dtype) * kBatch;
+  return (vocab + chunk - 1) / chunk;
 }
 
 }  // namespace
@@ -282,9 +329,7 @@ int chunk_of(int64_t B, int64_t n, int64_t vocab) {
 extern "C" size_t tpa_beam_select_workspace_bytes(int32_t B, int32_t beams, int32_t vocab, int32_t num_out, int32_t dtype) {
   using namespace tpa;
   if (B <= 0 || beams <= 0 || vocab <= 0 || num_out <= 0 || beams > TPA_BEAM_MAX || num_out > TPA_BEAM_MAX) return 0;
-  (void)dtype;
-  const int chunk = chunk_of(B, beams, vocab);
-  const size_t parts = (size_t)B * beams * (((size_t)vocab + chunk - 1) / chunk);
+  const size_t parts = (size_t)B * beams * chunks_of(B, beams, vocab, dtype);
   return parts * (sizeof(Sum) + num_out * sizeof(Candidate));
 }
 
@@ -299,8 +344,7 @@ extern "C" int tpa_beam_select(const TpaBeamSelectArgs* a, void* stream) {
   if (!a->logits || !a->scores || !a->new_scores || !a->parents || !a->tokens || !a->new_finished) return TPA_ERR_NULL;
   if (a->finished && a->eos_token < 0) return TPA_ERR_UNSUPPORTED;
   BeamParams p{};
-  p.chunk = chunk_of(a->B, a->beams, a->vocab);
-  p.chunks = (a->vocab + p.chunk - 1) / p.chunk;
+  p.chunks = (int)chunks_of(a->B, a->beams, a->vocab, a->dtype);
   const int64_t parts = (int64_t)a->B * a->beams * p.chunks, groups = (parts + kThreads / 64 - 1) / (kThreads / 64);
   if (groups > INT32_MAX || (int64_t)a->beams * p.chunks * a->num_out > INT32_MAX) return TPA_ERR_SHAPE;
   if (!a->workspace || a->workspace_bytes < tpa_beam_select_workspace_bytes(a->B, a->beams, a->vocab, a->num_out, a->dtype)) return TPA_ERR_WORKSPACE;
@@ -311,8 +355,15 @@ extern "C" int tpa_beam_select(const TpaBeamSelectArgs* a, void* stream) {
   p.candidates = reinterpret_cast<Candidate*>(p.sums + parts);
   p.B = a->B; p.n = a->beams; p.vocab = a->vocab; p.k = a->num_out; p.eos = a->eos_token;
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (a->dtype == TPA_DTYPE_BF16) hipLaunchKernelGGL(chunk_kernel<uint16_t>, dim3((unsigned)groups), dim3(kThreads), 0, on, p);
-  else hipLaunchKernelGGL(chunk_kernel<float>, dim3((unsigned)groups), dim3(kThreads), 0, on, p);
+  const bool bf16 = a->dtype == TPA_DTYPE_BF16;
+  void (*kern)(BeamParams) = nullptr;
+  switch (batches_of(a->B, a->beams, a->vocab, a->dtype)) {
+    case 2: kern = bf16 ? chunk_kernel<uint16_t, 2> : chunk_kernel<float, 2>; break;
+    case 4: kern = bf16 ? chunk_kernel<uint16_t, 4> : chunk_kernel<float, 4>; break;
+    case 8: kern = bf16 ? chunk_kernel<uint16_t, 8> : chunk_kernel<float, 8>; break;
+    default: kern = chunk_kernel<uint16_t, 16>;
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(kThreads), 0, on, p);
   if (hipGetLastError() != hipSuccess) return TPA_ERR_LAUNCH;
   const int64_t total = (int64_t)p.n * p.chunks * p.k;
   static bool configured[kMaxDevices] = {};

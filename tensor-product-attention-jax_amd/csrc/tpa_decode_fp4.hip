@@ -48,24 +48,15 @@ __device__ __forceinline__ int rounds_of(const Fp4Params& p, int b) {
   return (int)(((int64_t)keys_seen(p, length_of(p, b), p.lq - 1) * RK + kRows * kWaves - 1) / (kRows * kWaves));
 }
 
-// sum over the threads before this one and over all; `red` = an int per wave
-__device__ __forceinline__ int sum_before(int x, int* red, int& total) {
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int upto = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(upto, d);
-    if (lane >= d) upto += y;
-  }
-  if (lane == 63) red[w] = upto;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int i = 0; i < kWaves; ++i) {
-    if (i < w) before += red[i];
-    total += red[i];
-  }
-  return before + upto - x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_from(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int wave_prefix_sum(int x) {  // lane i: sum of lanes 0 .. i
+  x = add_from<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: inside rows of 16 lanes
+  x = add_from<0x112, 0xf>(x);
+  x = add_from<0x114, 0xf>(x);
+  x = add_from<0x118, 0xf>(x);
+  x = add_from<0x142, 0xa>(x);  // row_bcast 15: the last lane of rows 0 and 2 to rows 1 and 3
+  return add_from<0x143, 0xc>(x);  // row_bcast 31: lane 31 to rows 2 and 3
 }
 
 template <int D, int NC, int NS>
@@ -79,17 +70,24 @@ struct Fp4Lds {
   static constexpr size_t kBytes = 2 * (size_t)kPerWave * kWaves + kQ;
 };
 
-// a [32][D] bf16 tile: 16-byte chunk c of row r at chunk c ^ (r mod chunks)
+// a [32][D] bf16 tile: 16-byte chunk c of row r at chunk c ^ turn(r).  The 16 lanes of a transposed read take two neighbouring chunks of four rows, those of a
+// write one chunk of sixteen rows: turn() sends both to places of their own among the 16 of a line of banks (with r mod chunks, under which two
+// rows have the same two places, and the head factors' tile as it comes, 202 of a block's 500 LDS cycles were conflicts).
 template <int D>
-__device__ __forceinline__ int tile_write_at(int row, int chunk) { return row * D + 8 * (chunk ^ (row & (D / 8 - 1))); }
+__device__ __forceinline__ int turn(int row) {
+  return D == 128 ? (row << 1 | (row >> 3 & 1)) & 15 : (row & 6) | (row >> 3 & 1);
+}
+template <int D>
+__device__ __forceinline__ int tile_write_at(int row, int chunk) { return row * D + 8 * (chunk ^ turn<D>(row)); }
+// a [32][32] bf16 tile of head factors: the same with four chunks
+__device__ __forceinline__ int a_write_at(int row, int chunk) { return row * 32 + 8 * (chunk ^ (row >> 2 & 3)); }
 // transposed read: lane (i, g) gets rows 16 kk + 8 hi + 4 g + 0..3 of column 32 db + i
 template <int D>
 __device__ __forceinline__ bf16x8 tile_tr(const uint16_t* tile, int l, int kk, int db) {
-  constexpr int CPR = D / 8;
   const int g = l >> 5, lp = l & 15, dhalf = (l >> 4) & 1;
   auto at = [&](int hi) {
     const int r = 16 * kk + 8 * hi + 4 * g + (lp >> 2);
-    return r * D + 8 * ((4 * db + 2 * dhalf + ((lp & 3) >> 1)) ^ (r & (CPR - 1))) + 4 * (lp & 1);
+    return tile_write_at<D>(r, 4 * db + 2 * dhalf + ((lp & 3) >> 1)) + 4 * (lp & 1);
   };
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(tile + at(0)));
   const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(tile + at(1)));
@@ -107,39 +105,64 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NS]
   }
 }
 
+// eight elements from a place that need not be aligned
+template <typename T>
+struct Eight;
+template <>
+struct Eight<uint16_t> {
+  typedef u32x4 __attribute__((aligned(2))) Raw;
+  u32x4 w;
+  __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ float get(int j) const { return j & 1 ? bf16hi_to_f32(w[j >> 1]) : bf16lo_to_f32(w[j >> 1]); }
+};
+template <>
+struct Eight<float> {
+  typedef f32x4 __attribute__((aligned(4))) Raw;
+  f32x4 w[2];
+  __device__ __forceinline__ void load(const float* p) {
+    w[0] = *reinterpret_cast<const Raw*>(p);
+    w[1] = *reinterpret_cast<const Raw*>(p + 4);
+  }
+  __device__ __forceinline__ float get(int j) const { return w[j >> 2][j & 3]; }
+};
+
 // T: of the queries and the output.  NC: sets of 32 columns of a workgroup.  QS, PS: bf16 numbers that stand for one of Q and of the weighted probabilities.
-template <typename T, int D, int RK, int NC, int QS, int PS>
+// PAIR: whole groups of 16 heads, so that a lane's two chunks of head factors are neighbours in one block of 32.
+template <typename T, int D, int RK, int NC, int QS, int PS, bool PAIR>
 __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 : 1) void decode_fp4_kernel(Fp4Params p) {
   using Lds = Fp4Lds<D, NC, QS>;
   constexpr int NKS = D / 16, NDB = D / 32, NW = D / 64;  // NW: 16-byte words of half a row's codes
   constexpr int NTOK = RK <= 4 ? 16 / RK : 32 / RK;       // tokens whose rows this lane has logits of
   constexpr int NV = RK <= 4 ? RK : RK / 2;               // rows of a token in this half of the wave
+  constexpr int NA = PAIR ? 1 : 2;                        // pieces of this lane's head factors of a set
   extern __shared__ __attribute__((aligned(16))) uint16_t smem_fp4[];
-  __shared__ int red[kWaves], found[2];
   const int tid = threadIdx.x, w = scalar(tid >> 6), l = tid & 63, i = l & 31, g = l >> 5;
   const int c0 = blockIdx.y * 32 * NC;
 
-  // ---- this workgroup's share of the rounds
-  const int each = (p.B + kThreads - 1) / kThreads, e0 = min(tid * each, p.B), e1 = min(e0 + each, p.B);
-  int mine = 0, total;
+  // ---- this workgroup's share of the rounds, which every wave finds for itself: a lane has neighbouring sequences
+  const int each = (p.B + 63) / 64, e0 = min(l * each, p.B), e1 = min(e0 + each, p.B);
+  int mine = 0;
   for (int b = e0; b < e1; ++b) mine += rounds_of<RK>(p, b);
-  int before = sum_before(mine, red, total);
+  const int upto = wave_prefix_sum(mine), total = __builtin_amdgcn_readlane(upto, 63);
   const int groups = min(p.groups, total);
-  const bool writes_plan = blockIdx.x == 0 && blockIdx.y == 0;
   const int64_t share = blockIdx.x;
-  if (share >= groups && !writes_plan) return;
-  int r0 = groups ? (int)(share * total / groups) : 0;
-  const int r1 = groups ? (int)((share + 1) * total / groups) : 0;
-  for (int b = e0; b < e1; ++b) {
-    const int n = rounds_of<RK>(p, b);
-    if (writes_plan) p.plan[b] = before;
-    if (r0 >= before && r0 < before + n) { found[0] = b; found[1] = before; }
-    before += n;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && w == 0) {
+    int before = upto - mine;
+    for (int b = e0; b < e1; ++b) {
+      p.plan[b] = before;
+      before += rounds_of<RK>(p, b);
+    }
+    if (l == 0) p.plan[p.B] = total;
   }
-  if (writes_plan && tid == 0) p.plan[p.B] = total;
   if (share >= groups) return;
-  __syncthreads();
-  int b = scalar(found[0]), first_round = scalar(found[1]);
+  int r0 = (int)(share * total / groups);
+  const int r1 = (int)((share + 1) * total / groups);
+  int b = e0, first_round = upto - mine;
+  if (r0 >= first_round && r0 < upto)
+    for (int n; r0 >= first_round + (n = rounds_of<RK>(p, b)); ++b) first_round += n;
+  const int there = __builtin_ctzll(__ballot(r0 >= upto - mine && r0 < upto));
+  b = __builtin_amdgcn_readlane(b, there);
+  first_round = __builtin_amdgcn_readlane(first_round, there);
 
   uint16_t* const lds_v = smem_fp4 + w * Lds::kPerWave;
   uint16_t* const lds_a = lds_v + Lds::kV;  // [set][K, V][32 rows][32 columns]
@@ -147,15 +170,18 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
 
   const Fp4Row parts(p.H, D);
   // where the head factors of this lane's columns lie in a row: two chunks of 8 for every set
-  int a_at[NC][2], a_scale_at[NC][2];
+  int a_at[NC][NA], a_scale_at[NC][NA];
 #pragma unroll
   for (int s = 0; s < NC; ++s)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < NA; ++q) {
       const int h = (c0 + 32 * s + 16 * g + 8 * q) % p.H;
       a_at[s][q] = parts.a_codes + h / 2;
       a_scale_at[s][q] = parts.a_scales + h / 32;
     }
+  // this lane's row of a block: always the same rank
+  const uint8_t* const k_base = static_cast<const uint8_t*>(p.kc.ptr) + (i % RK) * p.kc.stride_r;
+  const uint8_t* const v_base = static_cast<const uint8_t*>(p.vc.ptr) + (i % RK) * p.vc.stride_r;
   int row_of_col[NC];  // query row of this lane's column in every set (past the last: the last)
 #pragma unroll
   for (int s = 0; s < NC; ++s) row_of_col[s] = min(c0 + 32 * s + i, p.cols - 1) / p.H;
@@ -175,49 +201,50 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     const int last_row = keys_seen(p, len, p.lq - 1) * RK - 1;  // not below 0 here
     const int blk_begin = (r0 - first_round) * kWaves + w, blk_end = min((stop - first_round) * kWaves, last_row / kRows + 1);
 
-    // ---- loads of a block: this lane's row (one past the last: that one), its place looked up a visit ahead
+    // ---- loads of a block: this lane's row (of a token past the last: that one's), its page looked up a block ahead
+    const int last_token = last_row / RK;
     struct Raw {
       u32x4 k[NW], v[NW];
       uint32_t k_scales, v_scales, ka[NC][2], va[NC][2];
-      uint8_t ka_scale[NC][2], va_scale[NC][2];
-    } raw[2];
-    auto token_of = [&](int blk) __attribute__((always_inline)) { return min(blk * kRows + i, last_row) / RK; };
+      uint8_t ka_scale[NC][NA], va_scale[NC][NA];
+    } raw;
+    auto token_of = [&](int blk) __attribute__((always_inline)) { return min(blk * (kRows / RK) + i / RK, last_token); };
     auto page_of = [&](int token) __attribute__((always_inline)) { return p.page_shift >= 0 ? token >> p.page_shift : token / p.page_size; };
-    auto lookup = [&](int blk) __attribute__((always_inline)) { return p.table ? p.table[(int64_t)b * p.pages_per_seq + page_of(token_of(blk))] : 0; };
-    int ahead[2];
-    auto issue = [&](Raw& x, int& page_ahead, int blk) __attribute__((always_inline)) {
-      const int token = token_of(blk), rank = min(blk * kRows + i, last_row) % RK;
-      int64_t page = b;
-      int in_page = token;
-      if (p.table) {
-        page = max(0, min(page_ahead, p.num_pages - 1));
-        in_page = token - page_of(token) * p.page_size;
-      }
-      const uint8_t* const k = static_cast<const uint8_t*>(p.kc.ptr) + page * p.kc.stride_b + in_page * p.kc.stride_l + rank * p.kc.stride_r;
-      const uint8_t* const v = static_cast<const uint8_t*>(p.vc.ptr) + page * p.vc.stride_b + in_page * p.vc.stride_l + rank * p.vc.stride_r;
+    auto lookup = [&](int blk) __attribute__((always_inline)) { return p.table ? p.table[(int64_t)b * p.pages_per_seq + page_of(token_of(blk))] : b; };
+    int page_ahead;
+    auto issue = [&](int blk) __attribute__((always_inline)) {
+      const int token = token_of(blk);
+      const int page = p.table ? max(0, min(page_ahead, p.num_pages - 1)) : b, in_page = p.table ? token - page_of(token) * p.page_size : token;
+      const uint8_t* const k = k_base + page * p.kc.stride_b + in_page * p.kc.stride_l;
+      const uint8_t* const v = v_base + page * p.vc.stride_b + in_page * p.vc.stride_l;
       typedef u32x4 __attribute__((aligned(4))) Word;
+      typedef u32x2 __attribute__((aligned(4))) Pair;
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
-        x.k[n] = *reinterpret_cast<const Word*>(k + g * (D / 4) + 16 * n);
-        x.v[n] = *reinterpret_cast<const Word*>(v + g * (D / 4) + 16 * n);
+        raw.k[n] = *reinterpret_cast<const Word*>(k + g * (D / 4) + 16 * n);
+        raw.v[n] = *reinterpret_cast<const Word*>(v + g * (D / 4) + 16 * n);
       }
-      x.k_scales = *reinterpret_cast<const uint32_t*>(k + parts.b_scales);
-      x.v_scales = *reinterpret_cast<const uint32_t*>(v + parts.b_scales);
+      raw.k_scales = *reinterpret_cast<const uint32_t*>(k + parts.b_scales);
+      raw.v_scales = *reinterpret_cast<const uint32_t*>(v + parts.b_scales);
 #pragma unroll
       for (int s = 0; s < NC; ++s)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          x.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + a_at[s][q]);
-          x.va[s][q] = *reinterpret_cast<const uint32_t*>(v + a_at[s][q]);
-          x.ka_scale[s][q] = k[a_scale_at[s][q]];
-          x.va_scale[s][q] = v[a_scale_at[s][q]];
+        for (int q = 0; q < NA; ++q) {
+          if constexpr (PAIR) {
+            const u32x2 kw = *reinterpret_cast<const Pair*>(k + a_at[s][0]), vw = *reinterpret_cast<const Pair*>(v + a_at[s][0]);
+            raw.ka[s][0] = kw[0]; raw.ka[s][1] = kw[1];
+            raw.va[s][0] = vw[0]; raw.va[s][1] = vw[1];
+          } else {
+            raw.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + a_at[s][q]);
+            raw.va[s][q] = *reinterpret_cast<const uint32_t*>(v + a_at[s][q]);
+          }
+          raw.ka_scale[s][q] = k[a_scale_at[s][q]];
+          raw.va_scale[s][q] = v[a_scale_at[s][q]];
         }
-      page_ahead = lookup(blk + 2 * kWaves);
+      page_ahead = lookup(blk + kWaves);
     };
-    ahead[0] = lookup(blk_begin);
-    ahead[1] = lookup(blk_begin + kWaves);
-    issue(raw[0], ahead[0], blk_begin);
-    issue(raw[1], ahead[1], blk_begin + kWaves);
+    page_ahead = lookup(blk_begin);
+    issue(blk_begin);
 
     // ---- Q's fragments: lane (column, g) of step ks holds numbers g D/2 + 8 ks + 0..7
     __syncthreads();  // the sequence before has left LDS
@@ -226,12 +253,21 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       const T* const qa = static_cast<const T*>(p.qa.ptr) + b * p.qa.stride_b + qi * p.qa.stride_l + h;
       const T* const qb = static_cast<const T*>(p.qb.ptr) + b * p.qb.stride_b + qi * p.qb.stride_l + 8 * chunk;
       float x[8] = {};
-#pragma unroll 2
-      for (int r = 0; r < p.rq; ++r) {
-        const float a = load_as_f32(qa + r * p.qa.stride_r);
-        const T* const row = qb + r * p.qb.stride_r;
+      for (int r0 = 0; r0 < p.rq; r0 += 4) {  // four ranks asked for together, those past the last again the last, which counts once
+        float a[4];
+        Eight<T> row[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += a * load_as_f32(row + j);
+        for (int u = 0; u < 4; ++u) {
+          const int r = min(r0 + u, p.rq - 1);
+          a[u] = load_as_f32(qa + r * p.qa.stride_r);
+          row[u].load(qb + r * p.qb.stride_r);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (r0 + u < p.rq) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = fmaf(a[u], row[u].get(j), x[j]);
+          }
       }
       uint32_t words[4][QS];
 #pragma unroll
@@ -242,11 +278,11 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         lds_q[(((col >> 5) * QS + q) * NKS + ks) * 64 + 32 * half + (col & 31)] = u32x4{words[0][q], words[1][q], words[2][q], words[3][q]};
     }
     __syncthreads();
-    constexpr bool kHeldQ = NC * QS == 1;  // in registers
-    bf16x8 qf[kHeldQ ? NKS : 1];
+    constexpr bool kHeldQ = NC == 1 && QS <= 2;  // in registers: read from LDS for every block they are two fifths of its traffic
+    bf16x8 qf[kHeldQ ? QS * NKS : 1];
     if constexpr (kHeldQ) {
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, lds_q[ks * 64 + l]);
+      for (int n = 0; n < QS * NKS; ++n) qf[n] = __builtin_bit_cast(bf16x8, lds_q[n * 64 + l]);
     }
 
     f32x16 o[NC][NDB];
@@ -261,30 +297,41 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       sum[s] = 0.f;
     }
 
-    auto block = [&](const Raw& x, int blk, bf16x8 (&kf)[NKS]) __attribute__((always_inline)) {
-      // ---- numbers of K to fragments, of V and of the head factors to LDS
+    // products of the rows of K with Q; numbers of V and of the head factors to LDS
+    auto unpack = [&](f32x16 (&sp)[NC]) __attribute__((always_inline)) {
       float scale[2][NW];
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
         const int shift = 8 * (NW * g + n);
-        scale[0][n] = fp4_scale((x.k_scales >> shift) & 255);
-        scale[1][n] = fp4_scale((x.v_scales >> shift) & 255);
+        scale[0][n] = fp4_scale((raw.k_scales >> shift) & 255);
+        scale[1][n] = fp4_scale((raw.v_scales >> shift) & 255);
       }
 #pragma unroll
+      for (int s = 0; s < NC; ++s)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sp[s][v] = 0.f;
+#pragma unroll
       for (int ks = 0; ks < NKS; ++ks) {
-        kf[ks] = fp4_bf16x8(x.k[ks / 4][ks % 4], scale[0][ks / 4]);
-        *reinterpret_cast<bf16x8*>(lds_v + tile_write_at<D>(i, NKS * g + ks)) = fp4_bf16x8(x.v[ks / 4][ks % 4], scale[1][ks / 4]);
+        const bf16x8 kf = fp4_bf16x8(raw.k[ks / 4][ks % 4], scale[0][ks / 4]);
+#pragma unroll
+        for (int s = 0; s < NC; ++s)
+#pragma unroll
+          for (int q = 0; q < QS; ++q) {
+            const bf16x8 qv = kHeldQ ? qf[kHeldQ ? q * NKS + ks : 0] : __builtin_bit_cast(bf16x8, lds_q[((s * QS + q) * NKS + ks) * 64 + l]);
+            sp[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qv, sp[s], 0, 0, 0);
+          }
+        *reinterpret_cast<bf16x8*>(lds_v + tile_write_at<D>(i, NKS * g + ks)) = fp4_bf16x8(raw.v[ks / 4][ks % 4], scale[1][ks / 4]);
       }
 #pragma unroll
       for (int s = 0; s < NC; ++s)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          uint16_t* const at = lds_a + 2 * s * Lds::kA + i * 32 + 16 * g + 8 * q;
-          *reinterpret_cast<bf16x8*>(at) = fp4_bf16x8(x.ka[s][q], fp4_scale(x.ka_scale[s][q]));
-          *reinterpret_cast<bf16x8*>(at + Lds::kA) = fp4_bf16x8(x.va[s][q], fp4_scale(x.va_scale[s][q]));
+          uint16_t* const at = lds_a + 2 * s * Lds::kA + a_write_at(i, 2 * g + q);
+          *reinterpret_cast<bf16x8*>(at) = fp4_bf16x8(raw.ka[s][q], fp4_scale(raw.ka_scale[s][PAIR ? 0 : q]));
+          *reinterpret_cast<bf16x8*>(at + Lds::kA) = fp4_bf16x8(raw.va[s][q], fp4_scale(raw.va_scale[s][PAIR ? 0 : q]));
         }
     };
-    auto consume = [&](int blk, const bf16x8 (&kf)[NKS]) __attribute__((always_inline)) {
+    auto consume = [&](int blk, const f32x16 (&products)[NC]) __attribute__((always_inline)) {
       const int lp = l & 15, dhalf = (l >> 4) & 1, row0 = blk * kRows;
 #pragma unroll
       for (int s = 0; s < NC; ++s) {
@@ -292,7 +339,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         float ak[16], av[16];  // of this lane's column, rows 8q + 4g + 0..3
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int at = 2 * s * Lds::kA + (8 * q + 4 * g + (lp >> 2)) * 32 + 16 * dhalf + 4 * (lp & 3);
+          const int at = 2 * s * Lds::kA + a_write_at(8 * q + 4 * g + (lp >> 2), 2 * dhalf + ((lp & 3) >> 1)) + 4 * (lp & 1);
           const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + at));
           const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + Lds::kA + at));
 #pragma unroll
@@ -301,17 +348,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
             av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
           }
         }
-        f32x16 sp;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) sp[v] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
-#pragma unroll
-          for (int q = 0; q < QS; ++q) {
-            const bf16x8 qv = kHeldQ ? qf[kHeldQ ? ks : 0] : __builtin_bit_cast(bf16x8, lds_q[((s * QS + q) * NKS + ks) * 64 + l]);
-            sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qv, sp, 0, 0, 0);
-          }
-
+        const f32x16& sp = products[s];
         // ---- logits per token (log2 domain); from rank 8 on a token's rows span both halves of the wave
         float st[NTOK], most = -INFINITY;
 #pragma unroll
@@ -363,16 +400,11 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         }
       }
     };
-    for (int blk = blk_begin; blk < blk_end; blk += 2 * kWaves) {
-      bf16x8 kf[NKS];
-      block(raw[0], blk, kf);
-      issue(raw[0], ahead[0], blk + 2 * kWaves);
-      consume(blk, kf);
-      if (blk + kWaves < blk_end) {
-        block(raw[1], blk + kWaves, kf);
-        issue(raw[1], ahead[1], blk + 3 * kWaves);
-        consume(blk + kWaves, kf);
-      }
+    for (int blk = blk_begin; blk < blk_end; blk += kWaves) {
+      f32x16 sp[NC];
+      unpack(sp);
+      issue(blk + kWaves);
+      consume(blk, sp);
     }
 
     // ---- join the waves through LDS, half of D at a time, and leave the part
@@ -431,54 +463,70 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
   }
 }
 
-// The parts of a sequence's column joined: a workgroup for each column, its threads' slices over the parts.
-template <typename T, int D>
+// The parts of a sequence's columns joined: D / 4 threads have a column, or SLICES times as many, which share out its parts where there are many (128 sequences of 12 000
+// keys, five parts each: 7.5 us in eight slices).
+template <typename T, int D, int SLICES>
 __global__ __launch_bounds__(kThreads) void join_kernel(Fp4Params p) {
-  constexpr int LANES = D / 4, SLICES = kThreads / LANES;
-  __shared__ f32x4 part[SLICES][LANES];
-  __shared__ float part_m[SLICES], part_l[SLICES];
-  const int b = blockIdx.x / p.cols, c = blockIdx.x - b * p.cols, at = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+  constexpr int LANES = D / 4, COLS = kThreads / LANES / SLICES;
+  __shared__ f32x4 part[SLICES > 1 ? kThreads : 1];
+  __shared__ float part_m[SLICES > 1 ? COLS * SLICES : 1], part_l[SLICES > 1 ? COLS * SLICES : 1];
+  const int at = threadIdx.x % LANES, slice = threadIdx.x / LANES % SLICES, mine = threadIdx.x / LANES / SLICES;
+  const int64_t column = (int64_t)blockIdx.x * COLS + mine, last = (int64_t)p.B * p.cols - 1;
+  const int b = (int)(min(column, last) / p.cols), c = (int)(min(column, last) - (int64_t)b * p.cols);
   const int64_t total = p.plan[p.B], first = p.plan[b], rounds = p.plan[b + 1] - first, groups = min((int64_t)p.groups, total);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, sum = 0.f;
   if (rounds > 0) {
     const int from = (int)(((first + 1) * groups - 1) / total), to = (int)(((first + rounds) * groups - 1) / total);
-    for (int share = from + slice; share <= to; share += SLICES) {
-      const int64_t base = (int64_t)(share + b) * p.cols + c;
-      const float ms = p.part_m[base], ls = p.part_l[base];
-      const f32x4 os = *reinterpret_cast<const f32x4*>(p.part_o + base * D + 4 * at);
-      if (ls == 0.f) continue;  // no key of this column
-      const float most = fmaxf(m, ms), use = most == -INFINITY ? 0.f : most;
-      const float f = __builtin_amdgcn_exp2f(m - use), fs = __builtin_amdgcn_exp2f(ms - use);
-      acc = acc * f + os * fs;
-      sum = sum * f + ls * fs;
-      m = most;
+    constexpr int kTogether = 4;
+    for (int share = from + slice; share <= to; share += kTogether * SLICES) {
+      float ms[kTogether], ls[kTogether];
+      f32x4 os[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const int64_t base = (int64_t)(min(share + u * SLICES, to) + b) * p.cols + c;
+        ms[u] = p.part_m[base];
+        ls[u] = share + u * SLICES <= to ? p.part_l[base] : 0.f;
+        os[u] = *reinterpret_cast<const f32x4*>(p.part_o + base * D + 4 * at);
+      }
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        if (ls[u] == 0.f) continue;  // no key of this column
+        const float most = fmaxf(m, ms[u]), use = most == -INFINITY ? 0.f : most;
+        const float f = __builtin_amdgcn_exp2f(m - use), fs = __builtin_amdgcn_exp2f(ms[u] - use);
+        acc = acc * f + os[u] * fs;
+        sum = sum * f + ls[u] * fs;
+        m = most;
+      }
     }
   }
-  part[slice][at] = acc;
-  if (at == 0) { part_m[slice] = m; part_l[slice] = sum; }
-  __syncthreads();
-  if (slice) return;
-  float most = -INFINITY;
+  if constexpr (SLICES > 1) {
+    part[threadIdx.x] = acc;
+    if (at == 0) { part_m[mine * SLICES + slice] = m; part_l[mine * SLICES + slice] = sum; }
+    __syncthreads();
+    if (slice) return;
+    m = -INFINITY;
 #pragma unroll
-  for (int s = 0; s < SLICES; ++s) most = fmaxf(most, part_m[s]);
-  const float use = most == -INFINITY ? 0.f : most;
-  acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  sum = 0.f;
+    for (int s = 0; s < SLICES; ++s) m = fmaxf(m, part_m[mine * SLICES + s]);
+    const float use = m == -INFINITY ? 0.f : m;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    sum = 0.f;
 #pragma unroll
-  for (int s = 0; s < SLICES; ++s) {
-    if (part_l[s] == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(part_m[s] - use);
-    acc += f * part[s][at];
-    sum += f * part_l[s];
+    for (int s = 0; s < SLICES; ++s) {
+      if (part_l[mine * SLICES + s] == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(part_m[mine * SLICES + s] - use);
+      acc += f * part[(mine * SLICES + s) * LANES + at];
+      sum += f * part_l[mine * SLICES + s];
+    }
   }
+  if (column > last) return;
   const float inv = sum == 0.f ? NAN : 1.f / (sum * p.rk);
-  T* const o = static_cast<T*>(p.o) + ((int64_t)b * p.cols + c) * D + 4 * at;
+  T* const o = static_cast<T*>(p.o) + column * D + 4 * at;
   if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
   else *reinterpret_cast<f32x4*>(o) = acc * inv;
   if (p.lse && at == 0) {
     const int qi = c / p.H, h = c - qi * p.H;
-    p.lse[((int64_t)b * p.H + h) * p.lq + qi] = sum == 0.f ? -INFINITY : (most + log2f(sum)) * kLn2;
+    p.lse[((int64_t)b * p.H + h) * p.lq + qi] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
   }
 }
 
@@ -601,21 +649,31 @@ int check_args(const TpaDecodeFp4Args* a) {
   return TPA_OK;
 }
 
-template <typename T, int D, int RK, int NC, int QS, int PS>
+template <typename T, int D, int RK, int NC, int QS, int PS, bool PAIR>
 int launch(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
-  auto kern = decode_fp4_kernel<T, D, RK, NC, QS, PS>;
+  auto kern = decode_fp4_kernel<T, D, RK, NC, QS, PS, PAIR>;
   constexpr size_t lds = Fp4Lds<D, NC, QS>::kBytes;
   static bool configured[kMaxDevices] = {};
   if (int rc = raise_lds_limit(configured, reinterpret_cast<const void*>(kern), lds); rc != TPA_OK) return rc;
   hipLaunchKernelGGL(kern, dim3(p.groups, plan.col_groups), dim3(kThreads), lds, stream, p);
-  if (hipGetLastError() != hipSuccess) return TPA_ERR_LAUNCH;
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(p.B * p.cols)), dim3(kThreads), 0, stream, p);
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
+}
+template <typename T, int D, int SLICES>
+int launch_join(const Fp4Params& p, hipStream_t stream) {
+  constexpr int cols = kThreads / (D / 4) / SLICES;
+  hipLaunchKernelGGL((join_kernel<T, D, SLICES>), dim3((unsigned)(((int64_t)p.B * p.cols + cols - 1) / cols)), dim3(kThreads), 0, stream, p);
+  return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
+}
+template <typename T, int D, int RK, int NC>
+int launch_pairs(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+  constexpr int QS = sizeof(T) == 2 ? 2 : 3, PS = sizeof(T) == 2 ? 1 : 3;
+  return p.H % 16 == 0 ? launch<T, D, RK, NC, QS, PS, true>(p, plan, stream) : launch<T, D, RK, NC, QS, PS, false>(p, plan, stream);
 }
 template <typename T, int D, int RK>
 int launch_sets(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2) return plan.sets == 1 ? launch<T, D, RK, 1, 2, 1>(p, plan, stream) : launch<T, D, RK, 2, 2, 1>(p, plan, stream);
-  else return plan.sets == 1 ? launch<T, D, RK, 1, 3, 3>(p, plan, stream) : launch<T, D, RK, 2, 3, 3>(p, plan, stream);
+  const int rc = plan.sets == 1 ? launch_pairs<T, D, RK, 1>(p, plan, stream) : launch_pairs<T, D, RK, 2>(p, plan, stream);
+  if (rc != TPA_OK) return rc;
+  return p.groups > 8 * (int64_t)p.B ? launch_join<T, D, 8>(p, stream) : launch_join<T, D, 1>(p, stream);
 }
 template <typename T, int D>
 int launch_rank(const Fp4Params& p, const Plan& plan, hipStream_t stream) {

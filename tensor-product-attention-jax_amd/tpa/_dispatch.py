@@ -515,7 +515,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
             fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         for name, args in (
             ("tpa_fp4_row_bytes", [ctypes.c_int32] * 2), ("tpa_decode_fp4_workspace_bytes", [ctypes.POINTER(TpaDecodeFp4Args)]),
-            ("tpa_beam_select_workspace_bytes", [ctypes.c_int32] * 5), ("tpa_pages_workspace_bytes", [ctypes.c_int32] * 2),
+            ("tpa_beam_select_workspace_bytes", [ctypes.c_int32] * 5), ("tpa_pages_workspace_bytes", [ctypes.c_int32] * 4),
         ):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_size_t

@@ -151,12 +151,24 @@ def pages(fork, pool=None, **changed):
     [(SHAPE, {k: 0}) for k in ("pages_per_seq", "page_size", "num_pages")]
     + [(SHAPE, {k: -1}) for k in ("B", "num_free", "num_pools")]
     + [(SHAPE, dict(B=8193)), (SHAPE, dict(pages_per_seq=1 << 30)), (SHAPE, dict(num_pages=1 << 30)), (SHAPE, dict(pool=(P, 4 * 88, 0))), (SHAPE, dict(pool=(P, 1 << 40, 1 << 30))), (UNSUPPORTED, dict(pool=(P, 4 * 88 - 1, 88))),
-       (NULL, dict(pool=(None, 400, 88))), (WORKSPACE, dict(workspace=None)), (WORKSPACE, dict(workspace_bytes=64)), (ALIGN, dict(workspace=P + 4)), (UNSUPPORTED, dict(new_page_table="page_table")),
+       (NULL, dict(pool=(None, 400, 88))), (WORKSPACE, dict(num_pages=9000, workspace=None)), (WORKSPACE, dict(num_pages=9000, workspace_bytes=64)), (ALIGN, dict(num_pages=9000, workspace=P + 4)), (UNSUPPORTED, dict(new_page_table="page_table")),
        (UNSUPPORTED, dict(new_page_shares="page_shares")), (UNSUPPORTED, dict(new_free_start="free_start")), (UNSUPPORTED, dict(new_free_pages="new_page_shares"))]
     + [(NULL, {k: None}) for k in ("page_table", "kv_lengths", "page_shares", "free_pages", "new_page_table", "new_page_shares", "new_free_pages", "new_free_start")],
 )
 def test_pages_refuse(fork, code, changed):
     assert pages(fork, **changed) == code
+
+
+def test_pages_workspace():
+    from tpa import _dispatch as d
+
+    size = d.load_library().tpa_pages_workspace_bytes
+    assert size(2048, 2048, 8192, 96) == 0 and size(8192, 0, 8192, 96) == 0
+    for b, m, total in ((2049, 1, 100), (1, 2049, 100), (1, 1, 8193), (1, 0, 8193)):  # the size it names is the size it needs
+        need = size(b, m, total, 1)
+        assert need > 0 and pages(m > 0, B=b, num_pages=total, workspace_bytes=need - 1, **({"M": m} if m else {})) == WORKSPACE
+    assert size(1, 1, 8192, 97) > 0
+    assert size(1, -1, 9000, 1) == 0 and size(1, 1, 0, 1) == 0
 
 
 def test_pages_refuse_what_only_one_call_has():
