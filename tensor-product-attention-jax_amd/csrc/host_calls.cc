@@ -1195,9 +1195,17 @@ PyObject* decode_fp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.k_cache = factor_of<TpaFactor>(kc); a.v_cache = factor_of<TpaFactor>(vc);
     const Tensor kvlen = lengths(tensor_or_none(args[4]), a.B);
     a.kv_lengths = ids_ptr(kvlen);
-    const auto options = at::TensorOptions().device(device);
-    r.first = at::empty({a.B, a.lq, a.H, a.dv}, options.dtype(qa.scalar_type()));
-    r.second = at::empty({a.B, a.H, a.lq}, options.dtype(at::kFloat));
+    // output and logsumexp in one allocation
+    const int64_t first = ((int64_t)a.B * a.lq * a.H * a.dv * qa.element_size() + 255) / 256 * 256;
+    const Tensor all = bytes_on(device, first + (int64_t)4 * a.B * a.H * a.lq);
+    auto part = [&](int64_t at, at::ScalarType type, std::initializer_list<int64_t> sizes) {
+      Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+      t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+      t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+      return t;
+    };
+    r.first = part(0, qa.scalar_type(), {a.B, a.lq, a.H, a.dv});
+    r.second = part(first, at::kFloat, {a.B, a.H, a.lq});
     if (r.first.numel() && a.lk && kc.numel() && vc.numel()) {
       const size_t need = lib.tpa_decode_fp4_workspace_bytes(&a);
       if (!ws.defined() && need) ws = bytes_on(device, need + 256);

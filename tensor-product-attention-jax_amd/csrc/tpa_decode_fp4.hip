@@ -19,6 +19,17 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kRows = 32;  // (token, rank) rows of a block
+constexpr int kMostGroups = 512;                 // workgroups that share out the rounds: two on a compute unit
+constexpr int64_t kNarrow = (1ll << 31) / kMostGroups;  // rounds up to which their shares are quotients of 32 bits (of 64 they take a microsecond)
+
+// x / d and the rest of small numbers (below 2^24), inv = 1 / d rounded: off by one at most, which the rest shows
+__device__ __forceinline__ int small_quotient(int x, int d, float inv, int& rest) {
+  int q = (int)((float)x * inv);
+  rest = x - q * d;
+  if (rest < 0) { --q; rest += d; }
+  if (rest >= d) { ++q; rest -= d; }
+  return q;
+}
 
 struct Fp4Params {
   TpaFactor qa, qb, kc, vc;
@@ -26,11 +37,12 @@ struct Fp4Params {
   float* lse;
   const int32_t *kvlen, *table;
   float *part_o, *part_m, *part_l;  // [slot, column, D], [slot, column], [slot, column]
-  int32_t* plan;                    // [B + 1] rounds before each sequence
+  int32_t* plan;                    // [B + 1] rounds before each sequence (rounds_of)
   int page_size, page_shift, pages_per_seq, num_pages;
   int B, lq, lk, H, dk, dv, rq, rk, cols;
   int causal, coff;
   int groups;   // workgroups that share out the rounds, at most
+  float inv_h;  // 1 / H
   float scale;  // of Q: sm_scale log2(e) / (rq rk); of the vector-unit kernel: sm_scale
 };
 
@@ -42,10 +54,13 @@ __device__ __forceinline__ int keys_seen(const Fp4Params& p, int length, int row
   return (int)max((int64_t)0, min((int64_t)len, last));
 }
 __device__ __forceinline__ int length_of(const Fp4Params& p, int b) { return p.kvlen ? p.kvlen[b] : p.lk; }
-// rounds of blocks of a sequence: those of the last row, which sees the most
+// Rounds of blocks of a sequence, those of the last row, which sees the most, and kStart more that stand for what it costs to begin one: Q's fragments, the first block's
+// way, the part.  (Without them workgroups that met two sequences ended last, 101 us after the start where the median was at 88.)
+constexpr int kStart = 3;
 template <int RK>
 __device__ __forceinline__ int rounds_of(const Fp4Params& p, int b) {
-  return (int)(((int64_t)keys_seen(p, length_of(p, b), p.lq - 1) * RK + kRows * kWaves - 1) / (kRows * kWaves));
+  const int n = (int)(((int64_t)keys_seen(p, length_of(p, b), p.lq - 1) * RK + kRows * kWaves - 1) / (kRows * kWaves));
+  return n ? n + kStart : 0;
 }
 
 template <int CTRL, int ROWS>
@@ -59,15 +74,20 @@ __device__ __forceinline__ int wave_prefix_sum(int x) {  // lane i: sum of lanes
   return add_from<0x143, 0xc>(x);  // row_bcast 31: lane 31 to rows 2 and 3
 }
 
-template <int D, int NC, int NS>
+enum { kRowsApart, kDense, kFewHeads };  // LAYOUT of the kernel
+
+// LDS: the tiles of the waves, the parts of Q that are not held in registers.  (Those that are held are made where the tiles will be.)
+template <int D, int NC, int QS, int LAYOUT>
 struct Fp4Lds {
   static constexpr int kV = kRows * D;                            // elements of V's tile
   static constexpr int kA = kRows * 32;                           // of the head factors of 32 columns
   static constexpr int kPerWave = kV + 2 * NC * kA;               // bf16 elements
   static constexpr int kHalf = D / 2, kRowStride = kHalf + 4;     // the waves are joined in two halves of D
   static_assert(4 * (32 * kRowStride + 64) <= 2 * kPerWave, "the join takes the room of the tiles");
-  static constexpr int kQ = NC * NS * (D / 16) * 64 * 16;         // bytes of Q's fragments
-  static constexpr size_t kBytes = 2 * (size_t)kPerWave * kWaves + kQ;
+  static constexpr int kPart = NC * (D / 16) * 64;                // 16-byte words of a part of Q
+  static constexpr int kHeld = QS > 2 || (NC == 2 && D == 64) ? 0 : NC == 1 && (D == 64 || LAYOUT == kFewHeads) ? QS : 1;  // parts in registers: as far as they go there
+  static_assert(16 * kHeld * kPart <= 2 * kPerWave * kWaves, "the held parts of Q take the room of the tiles");
+  static constexpr size_t kBytes = 2 * (size_t)kPerWave * kWaves + 16 * (size_t)(QS - kHeld) * kPart;
 };
 
 // a [32][D] bf16 tile: 16-byte chunk c of row r at chunk c ^ turn(r).  The 16 lanes of a transposed read take two neighbouring chunks of four rows, those of a
@@ -105,18 +125,8 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NS]
   }
 }
 
-// eight elements from a place that need not be aligned
-template <typename T>
-struct Eight;
-template <>
-struct Eight<uint16_t> {
-  typedef u32x4 __attribute__((aligned(2))) Raw;
-  u32x4 w;
-  __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const Raw*>(p); }
-  __device__ __forceinline__ float get(int j) const { return j & 1 ? bf16hi_to_f32(w[j >> 1]) : bf16lo_to_f32(w[j >> 1]); }
-};
-template <>
-struct Eight<float> {
+// eight numbers from a place that need not be aligned
+struct Eight {
   typedef f32x4 __attribute__((aligned(4))) Raw;
   f32x4 w[2];
   __device__ __forceinline__ void load(const float* p) {
@@ -127,14 +137,18 @@ struct Eight<float> {
 };
 
 // T: of the queries and the output.  NC: sets of 32 columns of a workgroup.  QS, PS: bf16 numbers that stand for one of Q and of the weighted probabilities.
-// PAIR: whole groups of 16 heads, so that a lane's two chunks of head factors are neighbours in one block of 32.
-template <typename T, int D, int RK, int NC, int QS, int PS, bool PAIR>
+// LAYOUT: kRowsApart: every lane finds its row by itself.  kDense: the 32 rows of every block lie one behind the other, all of them in memory (pages of whole blocks), so
+// that a block has one address and a lane's place in it never changes.  kFewHeads: kDense and 8, 16 or 32 heads, so that all columns of a set have their head
+// factors in one block of 32: its scale goes into those of K's and V's numbers, and the codes themselves are transposed, to fp32 right from there.
+// What bounds the kernel is the issue of instructions, 2.9 of 5.5 thousand cycles a block in the softmax and its surroundings and none in waiting for memory:
+// 128 sequences of 12 000 keys, 32 heads of 128, rank 2 (308, 268 and 224 vector instructions a block):
+template <typename T, int D, int RK, int NC, int QS, int PS, int LAYOUT>
 __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 : 1) void decode_fp4_kernel(Fp4Params p) {
-  using Lds = Fp4Lds<D, NC, QS>;
+  using Lds = Fp4Lds<D, NC, QS, LAYOUT>;
   constexpr int NKS = D / 16, NDB = D / 32, NW = D / 64;  // NW: 16-byte words of half a row's codes
   constexpr int NTOK = RK <= 4 ? 16 / RK : 32 / RK;       // tokens whose rows this lane has logits of
   constexpr int NV = RK <= 4 ? RK : RK / 2;               // rows of a token in this half of the wave
-  constexpr int NA = PAIR ? 1 : 2;                        // pieces of this lane's head factors of a set
+  constexpr int NA = LAYOUT == kFewHeads ? 1 : NC;        // different sets of head factors
   extern __shared__ __attribute__((aligned(16))) uint16_t smem_fp4[];
   const int tid = threadIdx.x, w = scalar(tid >> 6), l = tid & 63, i = l & 31, g = l >> 5;
   const int c0 = blockIdx.y * 32 * NC;
@@ -155,8 +169,14 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     if (l == 0) p.plan[p.B] = total;
   }
   if (share >= groups) return;
-  int r0 = (int)(share * total / groups);
-  const int r1 = (int)((share + 1) * total / groups);
+  int r0, r1;
+  if (total < kNarrow) {
+    r0 = (int)((uint32_t)share * (uint32_t)total / (uint32_t)groups);
+    r1 = (int)(((uint32_t)share + 1) * (uint32_t)total / (uint32_t)groups);
+  } else {
+    r0 = (int)(share * total / groups);
+    r1 = (int)((share + 1) * total / groups);
+  }
   int b = e0, first_round = upto - mine;
   if (r0 >= first_round && r0 < upto)
     for (int n; r0 >= first_round + (n = rounds_of<RK>(p, b)); ++b) first_round += n;
@@ -166,16 +186,19 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
 
   uint16_t* const lds_v = smem_fp4 + w * Lds::kPerWave;
   uint16_t* const lds_a = lds_v + Lds::kV;  // [set][K, V][32 rows][32 columns]
-  u32x4* const lds_q = reinterpret_cast<u32x4*>(smem_fp4 + kWaves * Lds::kPerWave);
+  u32x4* const lds_q = reinterpret_cast<u32x4*>(smem_fp4);  // parts in registers later
+  u32x4* const lds_q_rest = reinterpret_cast<u32x4*>(smem_fp4 + kWaves * Lds::kPerWave);
+  constexpr int kHeld = Lds::kHeld;
 
   const Fp4Row parts(p.H, D);
   // where the head factors of this lane's columns lie in a row: two chunks of 8 for every set
-  int a_at[NC][NA], a_scale_at[NC][NA];
+  int a_at[NA][2], a_scale_at[NA][2];
 #pragma unroll
-  for (int s = 0; s < NC; ++s)
+  for (int s = 0; s < NA; ++s)
 #pragma unroll
-    for (int q = 0; q < NA; ++q) {
-      const int h = (c0 + 32 * s + 16 * g + 8 * q) % p.H;
+    for (int q = 0; q < 2; ++q) {
+      int h;
+      small_quotient(c0 + 32 * s + 16 * g + 8 * q, p.H, p.inv_h, h);
       a_at[s][q] = parts.a_codes + h / 2;
       a_scale_at[s][q] = parts.a_scales + h / 32;
     }
@@ -184,7 +207,10 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
   const uint8_t* const v_base = static_cast<const uint8_t*>(p.vc.ptr) + (i % RK) * p.vc.stride_r;
   int row_of_col[NC];  // query row of this lane's column in every set (past the last: the last)
 #pragma unroll
-  for (int s = 0; s < NC; ++s) row_of_col[s] = min(c0 + 32 * s + i, p.cols - 1) / p.H;
+  for (int s = 0; s < NC; ++s) {
+    int h;
+    row_of_col[s] = small_quotient(min(c0 + 32 * s + i, p.cols - 1), p.H, p.inv_h, h);
+  }
 
   while (r0 < r1) {
     const int rounds = rounds_of<RK>(p, b);
@@ -193,96 +219,180 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       ++b;
       continue;
     }
-    const int stop = min(r1, first_round + rounds);
+    const int stop = min(r1, first_round + rounds), begin = max(r0 - first_round - kStart, 0), end = stop - first_round - kStart;
+    r0 = stop;
+    if (end <= begin) continue;  // nothing but a share of its start
     const int len = length_of(p, b);
-    int last_of[NC];
+    int last_of[NC], least_last[NC];
 #pragma unroll
-    for (int s = 0; s < NC; ++s) last_of[s] = keys_seen(p, len, row_of_col[s]) * RK - 1;
+    for (int s = 0; s < NC; ++s) {
+      last_of[s] = keys_seen(p, len, row_of_col[s]) * RK - 1;
+      least_last[s] = scalar(__builtin_amdgcn_readfirstlane(last_of[s]));  // of the first column, whose row sees the fewest keys
+    }
     const int last_row = keys_seen(p, len, p.lq - 1) * RK - 1;  // not below 0 here
-    const int blk_begin = (r0 - first_round) * kWaves + w, blk_end = min((stop - first_round) * kWaves, last_row / kRows + 1);
+    const int blk_begin = begin * kWaves + w, blk_end = min(end * kWaves, last_row / kRows + 1);
 
-    // ---- loads of a block: this lane's row (of a token past the last: that one's), its page looked up a block ahead
-    const int last_token = last_row / RK;
+    // ---- loads of a block; its page is looked up a block ahead
+    typedef u32x4 __attribute__((aligned(4))) Word;
+    typedef u32x2 __attribute__((aligned(4))) Pair;
     struct Raw {
       u32x4 k[NW], v[NW];
-      uint32_t k_scales, v_scales, ka[NC][2], va[NC][2];
-      uint8_t ka_scale[NC][NA], va_scale[NC][NA];
+      uint32_t k_scales, v_scales;           // kFewHeads: of b and of a, k_scales and v_scales the first and second word of K's row (g = 0) or V's
+      u32x2 ka[NA], va[NA];                  // kFewHeads: heads of the first 16 columns and of the others of K's row (g = 0) or V's
+      uint8_t ka_scale[NA][2], va_scale[NA][2];  // (not kFewHeads)
     } raw;
-    auto token_of = [&](int blk) __attribute__((always_inline)) { return min(blk * (kRows / RK) + i / RK, last_token); };
-    auto page_of = [&](int token) __attribute__((always_inline)) { return p.page_shift >= 0 ? token >> p.page_shift : token / p.page_size; };
-    auto lookup = [&](int blk) __attribute__((always_inline)) { return p.table ? p.table[(int64_t)b * p.pages_per_seq + page_of(token_of(blk))] : b; };
-    int page_ahead;
-    auto issue = [&](int blk) __attribute__((always_inline)) {
-      const int token = token_of(blk);
-      const int page = p.table ? max(0, min(page_ahead, p.num_pages - 1)) : b, in_page = p.table ? token - page_of(token) * p.page_size : token;
-      const uint8_t* const k = k_base + page * p.kc.stride_b + in_page * p.kc.stride_l;
-      const uint8_t* const v = v_base + page * p.vc.stride_b + in_page * p.vc.stride_l;
-      typedef u32x4 __attribute__((aligned(4))) Word;
-      typedef u32x2 __attribute__((aligned(4))) Pair;
+    // this lane's half of K's row and of V's, and their ends
+    auto take = [&](const uint8_t* k, const uint8_t* v, uint32_t at_k, uint32_t at_v) __attribute__((always_inline)) {
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
-        raw.k[n] = *reinterpret_cast<const Word*>(k + g * (D / 4) + 16 * n);
-        raw.v[n] = *reinterpret_cast<const Word*>(v + g * (D / 4) + 16 * n);
+        raw.k[n] = *reinterpret_cast<const Word*>(k + (at_k + g * (D / 4)) + 16 * n);
+        raw.v[n] = *reinterpret_cast<const Word*>(v + (at_v + g * (D / 4)) + 16 * n);
       }
-      raw.k_scales = *reinterpret_cast<const uint32_t*>(k + parts.b_scales);
-      raw.v_scales = *reinterpret_cast<const uint32_t*>(v + parts.b_scales);
+      raw.k_scales = *reinterpret_cast<const uint32_t*>(k + (at_k + parts.b_scales));
+      raw.v_scales = *reinterpret_cast<const uint32_t*>(v + (at_v + parts.b_scales));
 #pragma unroll
-      for (int s = 0; s < NC; ++s)
+      for (int s = 0; s < NA; ++s)
 #pragma unroll
-        for (int q = 0; q < NA; ++q) {
-          if constexpr (PAIR) {
-            const u32x2 kw = *reinterpret_cast<const Pair*>(k + a_at[s][0]), vw = *reinterpret_cast<const Pair*>(v + a_at[s][0]);
-            raw.ka[s][0] = kw[0]; raw.ka[s][1] = kw[1];
-            raw.va[s][0] = vw[0]; raw.va[s][1] = vw[1];
-          } else {
-            raw.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + a_at[s][q]);
-            raw.va[s][q] = *reinterpret_cast<const uint32_t*>(v + a_at[s][q]);
-          }
-          raw.ka_scale[s][q] = k[a_scale_at[s][q]];
-          raw.va_scale[s][q] = v[a_scale_at[s][q]];
+        for (int q = 0; q < 2; ++q) {
+          raw.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + (at_k + a_at[s][q]));
+          raw.va[s][q] = *reinterpret_cast<const uint32_t*>(v + (at_v + a_at[s][q]));
+          raw.ka_scale[s][q] = k[at_k + a_scale_at[s][q]];
+          raw.va_scale[s][q] = v[at_v + a_scale_at[s][q]];
         }
+    };
+    // the same with the whole end of K's row in one half of the wave and of V's in the other: three loads instead of six (8 heads: what is read behind
+    // them is not used)
+    auto take_few = [&](const uint8_t* k, const uint8_t* v, uint32_t at_k, uint32_t at_v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < NW; ++n) {
+        raw.k[n] = *reinterpret_cast<const Word*>(k + (at_k + g * (D / 4)) + 16 * n);
+        raw.v[n] = *reinterpret_cast<const Word*>(v + (at_v + g * (D / 4)) + 16 * n);
+      }
+      const uint8_t* const mine = g ? v + at_v : k + at_k;
+      raw.ka[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes);
+      raw.va[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes + (p.H == 32 ? 8 : 0));
+      if constexpr (D == 128) {
+        const u32x2 x = *reinterpret_cast<const Pair*>(mine + parts.b_scales);
+        raw.k_scales = x[0];
+        raw.v_scales = x[1];
+      } else {
+        raw.k_scales = *reinterpret_cast<const uint32_t*>(mine + parts.b_scales);
+      }
+    };
+    auto page_of = [&](int token) __attribute__((always_inline)) { return p.page_shift >= 0 ? token >> p.page_shift : token / p.page_size; };
+    const int last_token = last_row / RK;
+    auto token_of = [&](int blk) __attribute__((always_inline)) {  // the block's first, or this lane's (of a row past the last: the last)
+      return LAYOUT != kRowsApart ? min(blk, last_row / kRows) * (kRows / RK) : min(blk * (kRows / RK) + i / RK, last_token);
+    };
+    auto lookup = [&](int blk) __attribute__((always_inline)) { return p.table ? p.table[(int64_t)b * p.pages_per_seq + page_of(token_of(blk))] : b; };
+    int page_ahead = lookup(blk_begin);
+    auto issue = [&](int blk) __attribute__((always_inline)) {
+      const int token = token_of(blk);
+      int page = p.table ? max(0, min(page_ahead, p.num_pages - 1)) : b;
+      const int in_page = p.table ? token - page_of(token) * p.page_size : token;
+      if constexpr (LAYOUT != kRowsApart) {
+        page = scalar(page);
+        const int64_t k = page * p.kc.stride_b + in_page * p.kc.stride_l, v = page * p.vc.stride_b + in_page * p.vc.stride_l;
+        const uint8_t *const k_block = static_cast<const uint8_t*>(p.kc.ptr) + k, *const v_block = static_cast<const uint8_t*>(p.vc.ptr) + v;
+        if constexpr (LAYOUT == kFewHeads) take_few(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
+        else take(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
+      } else {
+        take(k_base + page * p.kc.stride_b + in_page * p.kc.stride_l, v_base + page * p.vc.stride_b + in_page * p.vc.stride_l, 0, 0);
+      }
       page_ahead = lookup(blk + kWaves);
     };
-    page_ahead = lookup(blk_begin);
     issue(blk_begin);
 
     // ---- Q's fragments: lane (column, g) of step ks holds numbers g D/2 + 8 ks + 0..7
     __syncthreads();  // the sequence before has left LDS
-    for (int item = tid; item < 32 * NC * (D / 8); item += kThreads) {
-      const int col = item / (D / 8), chunk = item % (D / 8), c = min(c0 + col, p.cols - 1), qi = c / p.H, h = c - qi * p.H;
-      const T* const qa = static_cast<const T*>(p.qa.ptr) + b * p.qa.stride_b + qi * p.qa.stride_l + h;
-      const T* const qb = static_cast<const T*>(p.qb.ptr) + b * p.qb.stride_b + qi * p.qb.stride_l + 8 * chunk;
-      float x[8] = {};
-      for (int r0 = 0; r0 < p.rq; r0 += 4) {  // four ranks asked for together, those past the last again the last, which counts once
-        float a[4];
-        Eight<T> row[4];
+    auto part_q = [&](int q) __attribute__((always_inline)) { return q < kHeld ? lds_q + q * Lds::kPart : lds_q_rest + (q - kHeld) * Lds::kPart; };
+    auto place_q = [&](int col, int d) __attribute__((always_inline)) {  // of number d of a column in a part of Q
+      const int half = d / (D / 2), ks = d % (D / 2) / 8;
+      return ((col >> 5) * NKS + ks) * 64 + 32 * half + (col & 31);
+    };
+    if constexpr (sizeof(T) == 2) {
+      // by the matrix cores, 32 numbers of 32 columns a wave: rows d, columns c, contraction over the ranks, whose loads are all on their way at once.
+      // (On the vector units, eight numbers a thread, the loads waited for four times: 6100 of the 18 800 cycles of the shortest call.)
+      for (int item = w; item < NC * NDB; item += kWaves) {
+        const int set = item / NDB, db = item % NDB;
+        int h;
+        const int qi = small_quotient(min(c0 + 32 * set + i, p.cols - 1), p.H, p.inv_h, h);
+        const uint16_t* const qa = static_cast<const uint16_t*>(p.qa.ptr) + b * p.qa.stride_b + qi * p.qa.stride_l + h;
+        // (columns of one set are of several query rows: their b rows differ, so a product for each of these rows, of which a column takes its own)
+        const int first_row = small_quotient(min(c0 + 32 * set, p.cols - 1), p.H, p.inv_h, h), last = small_quotient(min(c0 + 32 * set + 31, p.cols - 1), p.H, p.inv_h, h);
+        f32x16 x;
+        for (int row = first_row; row <= last; ++row) {
+          const uint16_t* const qb = static_cast<const uint16_t*>(p.qb.ptr) + b * p.qb.stride_b + row * p.qb.stride_l + 32 * db + i;
+          f32x16 acc;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = min(r0 + u, p.rq - 1);
-          a[u] = load_as_f32(qa + r * p.qa.stride_r);
-          row[u].load(qb + r * p.qb.stride_r);
+          for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+          for (int r0 = 0; r0 < p.rq; r0 += 16) {
+            uint16_t av[8], bv[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int r = min(r0 + 8 * g + j, p.rq - 1);
+              av[j] = qa[r * p.qa.stride_r];
+              bv[j] = qb[r * p.qb.stride_r];
+            }
+            u32x4 aw, bw;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int r = r0 + 8 * g + 2 * j;  // ranks past the last count as zero in both
+              aw[j] = (r < p.rq ? (uint32_t)av[2 * j] : 0u) | (r + 1 < p.rq ? (uint32_t)av[2 * j + 1] << 16 : 0u);
+              bw[j] = (r < p.rq ? (uint32_t)bv[2 * j] : 0u) | (r + 1 < p.rq ? (uint32_t)bv[2 * j + 1] << 16 : 0u);
+            }
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bw), __builtin_bit_cast(bf16x8, aw), acc, 0, 0, 0);
+          }
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[v] = row == first_row || row == qi ? acc[v] : x[v];
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (r0 + u < p.rq) {
+        for (int n = 0; n < 4; ++n) {  // numbers 32 db + 8 n + 4 g + 0..3
+          uint32_t lo[QS], hi[QS];
+          split_pair<QS>(x[4 * n] * p.scale, x[4 * n + 1] * p.scale, lo);
+          split_pair<QS>(x[4 * n + 2] * p.scale, x[4 * n + 3] * p.scale, hi);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = fmaf(a[u], row[u].get(j), x[j]);
-          }
+          for (int q = 0; q < QS; ++q)
+            reinterpret_cast<u32x2*>(part_q(q))[2 * place_q(32 * set + i, 32 * db + 8 * n) + g] = u32x2{lo[q], hi[q]};
+        }
       }
-      uint32_t words[4][QS];
+    } else {
+      for (int item = tid; item < 32 * NC * (D / 8); item += kThreads) {
+        const int col = item / (D / 8), chunk = item % (D / 8);
+        int h;
+        const int qi = small_quotient(min(c0 + col, p.cols - 1), p.H, p.inv_h, h);
+        const T* const qa = static_cast<const T*>(p.qa.ptr) + b * p.qa.stride_b + qi * p.qa.stride_l + h;
+        const T* const qb = static_cast<const T*>(p.qb.ptr) + b * p.qb.stride_b + qi * p.qb.stride_l + 8 * chunk;
+        float x[8] = {};
+        for (int r0 = 0; r0 < p.rq; r0 += 6) {  // six ranks asked for together, those past the last again the last, which counts once
+          float a[6];
+          Eight row[6];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) split_pair<QS>(x[2 * j] * p.scale, x[2 * j + 1] * p.scale, words[j]);
-      const int half = chunk / NKS, ks = chunk % NKS;
+          for (int u = 0; u < 6; ++u) {
+            const int r = min(r0 + u, p.rq - 1);
+            a[u] = qa[r * p.qa.stride_r];
+            row[u].load(qb + r * p.qb.stride_r);
+          }
 #pragma unroll
-      for (int q = 0; q < QS; ++q)
-        lds_q[(((col >> 5) * QS + q) * NKS + ks) * 64 + 32 * half + (col & 31)] = u32x4{words[0][q], words[1][q], words[2][q], words[3][q]};
+          for (int u = 0; u < 6; ++u)
+            if (r0 + u < p.rq) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = fmaf(a[u], row[u].get(j), x[j]);
+            }
+        }
+        uint32_t words[4][QS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair<QS>(x[2 * j] * p.scale, x[2 * j + 1] * p.scale, words[j]);
+#pragma unroll
+        for (int q = 0; q < QS; ++q) part_q(q)[place_q(col, 8 * chunk)] = u32x4{words[0][q], words[1][q], words[2][q], words[3][q]};
+      }
     }
     __syncthreads();
-    constexpr bool kHeldQ = NC == 1 && QS <= 2;  // in registers: read from LDS for every block they are two fifths of its traffic
-    bf16x8 qf[kHeldQ ? QS * NKS : 1];
-    if constexpr (kHeldQ) {
+    bf16x8 qf[kHeld ? kHeld * NC * NKS : 1];
+    if constexpr (kHeld > 0) {
 #pragma unroll
-      for (int n = 0; n < QS * NKS; ++n) qf[n] = __builtin_bit_cast(bf16x8, lds_q[n * 64 + l]);
+      for (int n = 0; n < kHeld * NC * NKS; ++n) qf[n] = __builtin_bit_cast(bf16x8, lds_q[n * 64 + l]);
+      __syncthreads();  // the tiles take their place
     }
 
     f32x16 o[NC][NDB];
@@ -298,13 +408,41 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     }
 
     // products of the rows of K with Q; numbers of V and of the head factors to LDS
-    auto unpack = [&](f32x16 (&sp)[NC]) __attribute__((always_inline)) {
+    auto unpack = [&](int blk, f32x16 (&sp)[NC]) __attribute__((always_inline)) {
+      uint32_t k_scales = raw.k_scales, v_scales = raw.v_scales;
+      float ka_scale = 1.f, va_scale = 1.f;
+      if constexpr (LAYOUT == kFewHeads) {
+        const auto first = __builtin_amdgcn_permlane32_swap(raw.k_scales, raw.k_scales, false, false);
+        k_scales = first[0];
+        v_scales = first[1];
+        if constexpr (D == 128) {
+          const auto second = __builtin_amdgcn_permlane32_swap(raw.v_scales, raw.v_scales, false, false);
+          ka_scale = fp4_scale(second[0] & 255);
+          va_scale = fp4_scale(second[1] & 255);
+        } else {
+          ka_scale = fp4_scale(k_scales >> 16 & 255);
+          va_scale = fp4_scale(v_scales >> 16 & 255);
+        }
+      }
+      if (LAYOUT != kRowsApart && blk * kRows + kRows - 1 > last_row && blk * kRows + i > last_row) {
+        // behind the last token: whatever is there, numbers that a weight of 0 leaves at 0
+        v_scales = 0;
+        va_scale = 1.f;
+        if constexpr (LAYOUT != kFewHeads) {
+#pragma unroll
+          for (int s = 0; s < NA; ++s) raw.va_scale[s][0] = raw.va_scale[s][1] = 0;
+        }
+      }
       float scale[2][NW];
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
         const int shift = 8 * (NW * g + n);
-        scale[0][n] = fp4_scale((raw.k_scales >> shift) & 255);
-        scale[1][n] = fp4_scale((raw.v_scales >> shift) & 255);
+        scale[0][n] = fp4_scale((k_scales >> shift) & 255);
+        scale[1][n] = fp4_scale((v_scales >> shift) & 255);
+        if constexpr (LAYOUT == kFewHeads) {  // (a product past 2^127 is infinity, which the conversions make NaN of)
+          scale[0][n] *= ka_scale;
+          scale[1][n] *= va_scale;
+        }
       }
 #pragma unroll
       for (int s = 0; s < NC; ++s)
@@ -317,37 +455,63 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         for (int s = 0; s < NC; ++s)
 #pragma unroll
           for (int q = 0; q < QS; ++q) {
-            const bf16x8 qv = kHeldQ ? qf[kHeldQ ? q * NKS + ks : 0] : __builtin_bit_cast(bf16x8, lds_q[((s * QS + q) * NKS + ks) * 64 + l]);
+            const bf16x8 qv = q < kHeld ? qf[q < kHeld ? (q * NC + s) * NKS + ks : 0] : __builtin_bit_cast(bf16x8, part_q(q)[(s * NKS + ks) * 64 + l]);
             sp[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qv, sp[s], 0, 0, 0);
           }
         *reinterpret_cast<bf16x8*>(lds_v + tile_write_at<D>(i, NKS * g + ks)) = fp4_bf16x8(raw.v[ks / 4][ks % 4], scale[1][ks / 4]);
       }
+      if constexpr (LAYOUT == kFewHeads) {
+        if (p.H == 8) { raw.ka[0][1] = raw.ka[0][0]; raw.va[0][1] = raw.va[0][0]; }
+        reinterpret_cast<u32x4*>(lds_a)[l] = u32x4{raw.ka[0][0], raw.ka[0][1], raw.va[0][0], raw.va[0][1]};  // [K, V][32 rows][32 codes]
+      } else {
 #pragma unroll
-      for (int s = 0; s < NC; ++s)
+        for (int s = 0; s < NA; ++s)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint16_t* const at = lds_a + 2 * s * Lds::kA + a_write_at(i, 2 * g + q);
-          *reinterpret_cast<bf16x8*>(at) = fp4_bf16x8(raw.ka[s][q], fp4_scale(raw.ka_scale[s][PAIR ? 0 : q]));
-          *reinterpret_cast<bf16x8*>(at + Lds::kA) = fp4_bf16x8(raw.va[s][q], fp4_scale(raw.va_scale[s][PAIR ? 0 : q]));
-        }
+          for (int q = 0; q < 2; ++q) {
+            uint16_t* const at = lds_a + 2 * s * Lds::kA + a_write_at(i, 2 * g + q);
+            *reinterpret_cast<bf16x8*>(at) = fp4_bf16x8(raw.ka[s][q], fp4_scale(raw.ka_scale[s][q]));
+            *reinterpret_cast<bf16x8*>(at + Lds::kA) = fp4_bf16x8(raw.va[s][q], fp4_scale(raw.va_scale[s][q]));
+          }
+      }
     };
     auto consume = [&](int blk, const f32x16 (&products)[NC]) __attribute__((always_inline)) {
       const int lp = l & 15, dhalf = (l >> 4) & 1, row0 = blk * kRows;
+      float ak[16], av[16];  // of this lane's column, rows 8q + 4g + 0..3
+      auto head_factors = [&](int s) __attribute__((always_inline)) {
+        if constexpr (LAYOUT == kFewHeads) {
+          // lane lp of 16 names row 8 (lp / 4) + 4 g + lp % 4, and gets its own column's codes of the sixteen rows
+          typedef int s32x2 __attribute__((ext_vector_type(2)));
+          const int at = 8 * (2 * (8 * (lp >> 2) + 4 * g + (lp & 3)) + dhalf);
+          const s32x2 tk = __builtin_amdgcn_ds_read_tr4_b64_v2i32((s32x2 __attribute__((address_space(3)))*)(reinterpret_cast<uint8_t*>(lds_a) + at));
+          const s32x2 tv = __builtin_amdgcn_ds_read_tr4_b64_v2i32((s32x2 __attribute__((address_space(3)))*)(reinterpret_cast<uint8_t*>(lds_a) + 512 + at));
+          float x[8];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            fp4_f32x8((uint32_t)tk[n], 1.f, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ak[8 * n + j] = x[j];
+            fp4_f32x8((uint32_t)tv[n], 1.f, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) av[8 * n + j] = x[j];
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int at = 2 * s * Lds::kA + a_write_at(8 * q + 4 * g + (lp >> 2), 2 * dhalf + ((lp & 3) >> 1)) + 4 * (lp & 1);
+            const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + at));
+            const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + Lds::kA + at));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
+              av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
+            }
+          }
+        }
+      };
 #pragma unroll
       for (int s = 0; s < NC; ++s) {
         if constexpr (NC > 1) __builtin_amdgcn_sched_barrier(0);
-        float ak[16], av[16];  // of this lane's column, rows 8q + 4g + 0..3
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int at = 2 * s * Lds::kA + a_write_at(8 * q + 4 * g + (lp >> 2), 2 * dhalf + ((lp & 3) >> 1)) + 4 * (lp & 1);
-          const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + at));
-          const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + Lds::kA + at));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
-            av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
-          }
-        }
+        if (LAYOUT != kFewHeads || s == 0) head_factors(s);
         const f32x16& sp = products[s];
         // ---- logits per token (log2 domain); from rank 8 on a token's rows span both halves of the wave
         float st[NTOK], most = -INFINITY;
@@ -358,11 +522,18 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
 #pragma unroll
           for (int j = 0; j < NV; ++j) acc = fmaf(ak[v0 + j], sp[v0 + j], acc);
           if constexpr (RK >= 8) acc = halves_sum(acc);
-          const int row = RK >= 8 ? row0 + RK * t : row0 + 8 * (v0 >> 2) + 4 * g + (v0 & 3);  // the token's first row
-          if (row > last_of[s]) acc = -INFINITY;
           st[t] = acc;
-          most = fmaxf(most, acc);
         }
+        if (row0 + kRows - 1 > least_last[s]) {  // (the same in all lanes)
+          asm volatile("");                      // a branch: it is taken for the last keys alone
+#pragma unroll
+          for (int t = 0; t < NTOK; ++t) {
+            const int v0 = t * NV, row = RK >= 8 ? row0 + RK * t : row0 + 8 * (v0 >> 2) + 4 * g + (v0 & 3);  // the token's first row
+            if (row > last_of[s]) st[t] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NTOK; ++t) most = fmaxf(most, st[t]);
         most = halves_max(most);
         // the reference is a whole number: a weight then has the same significand, and is rounded the same way, however the keys are dealt to
         // waves and workgroups, and every factor that joins them is a power of two
@@ -402,7 +573,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     };
     for (int blk = blk_begin; blk < blk_end; blk += kWaves) {
       f32x16 sp[NC];
-      unpack(sp);
+      unpack(blk, sp);
       issue(blk + kWaves);
       consume(blk, sp);
     }
@@ -459,7 +630,6 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         }
       }
     }
-    r0 = stop;
   }
 }
 
@@ -473,11 +643,18 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Fp4Params p) {
   const int at = threadIdx.x % LANES, slice = threadIdx.x / LANES % SLICES, mine = threadIdx.x / LANES / SLICES;
   const int64_t column = (int64_t)blockIdx.x * COLS + mine, last = (int64_t)p.B * p.cols - 1;
   const int b = (int)(min(column, last) / p.cols), c = (int)(min(column, last) - (int64_t)b * p.cols);
-  const int64_t total = p.plan[p.B], first = p.plan[b], rounds = p.plan[b + 1] - first, groups = min((int64_t)p.groups, total);
+  const int64_t total = p.plan[p.B], first = p.plan[b] + kStart, rounds = p.plan[b + 1] - first, groups = min((int64_t)p.groups, total);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, sum = 0.f;
   if (rounds > 0) {
-    const int from = (int)(((first + 1) * groups - 1) / total), to = (int)(((first + rounds) * groups - 1) / total);
+    int from, to;
+    if (total < kNarrow) {
+      from = (int)((((uint32_t)first + 1) * (uint32_t)groups - 1) / (uint32_t)total);
+      to = (int)((((uint32_t)first + (uint32_t)rounds) * (uint32_t)groups - 1) / (uint32_t)total);
+    } else {
+      from = (int)(((first + 1) * groups - 1) / total);
+      to = (int)(((first + rounds) * groups - 1) / total);
+    }
     constexpr int kTogether = 4;
     for (int share = from + slice; share <= to; share += kTogether * SLICES) {
       float ms[kTogether], ls[kTogether];
@@ -615,20 +792,28 @@ __global__ __launch_bounds__(kThreads) void decode_fp4_any_kernel(Fp4Params p) {
 // ------------------------------------------------------------------------------------------------ host side
 bool mfma_takes(const TpaDecodeFp4Args* a) {
   if (a->dk != a->dv || (a->dk != 64 && a->dk != 128) || a->H % 8 || (a->rk != 1 && a->rk != 2 && a->rk != 4 && a->rk != 8)) return false;
-  if ((int64_t)a->B * ((int64_t)a->lk * a->rk / (kRows * kWaves) + 1) > INT32_MAX) return false;  // rounds
+  if ((int64_t)a->B * ((int64_t)a->lk * a->rk / (kRows * kWaves) + 1 + kStart) > INT32_MAX) return false;  // rounds
   for (const TpaFactor* f : {&a->k_cache, &a->v_cache})
     if (reinterpret_cast<uintptr_t>(f->ptr) % 4 || f->stride_b % 4 || f->stride_l % 4 || f->stride_r % 4) return false;
   return true;
 }
 
-struct Plan { int sets, col_groups, groups; int64_t slots; size_t plan_bytes, bytes; };
+// whether rows lie one behind the other and blocks of 32 of them are inside a page (a block is then less than 2^31 bytes)
+bool dense_rows(const TpaDecodeFp4Args* a) {
+  for (const TpaFactor* f : {&a->k_cache, &a->v_cache})
+    if (f->stride_r < 0 || f->stride_r > 1 << 20 || f->stride_l != a->rk * f->stride_r) return false;
+  return (a->page_table ? (int64_t)a->page_size * a->rk : (int64_t)a->lk * a->rk) % kRows == 0;
+}
+
+struct Plan { int sets, col_groups, groups; bool dense; int64_t slots; size_t plan_bytes, bytes; };
 Plan plan_of(const TpaDecodeFp4Args* a) {
   Plan p;
   const int64_t cols = (int64_t)a->lq * a->H;
   p.sets = cols > 32 ? 2 : 1;
   p.col_groups = (int)((cols + 32 * p.sets - 1) / (32 * p.sets));
-  const int64_t rounds = a->B * (((int64_t)a->lk * a->rk + kRows * kWaves - 1) / (kRows * kWaves));
-  p.groups = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / p.col_groups));
+  const int64_t rounds = a->B * (((int64_t)a->lk * a->rk + kRows * kWaves - 1) / (kRows * kWaves) + kStart);
+  p.groups = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, kMostGroups / p.col_groups));
+  p.dense = dense_rows(a);
   p.slots = (int64_t)p.groups + a->B;
   p.plan_bytes = (4 * ((size_t)a->B + 1) + 255) / 256 * 256;
   p.bytes = p.plan_bytes + 4 * (size_t)p.slots * cols * (a->dv + 2);
@@ -649,10 +834,10 @@ int check_args(const TpaDecodeFp4Args* a) {
   return TPA_OK;
 }
 
-template <typename T, int D, int RK, int NC, int QS, int PS, bool PAIR>
+template <typename T, int D, int RK, int NC, int QS, int PS, int LAYOUT>
 int launch(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
-  auto kern = decode_fp4_kernel<T, D, RK, NC, QS, PS, PAIR>;
-  constexpr size_t lds = Fp4Lds<D, NC, QS>::kBytes;
+  auto kern = decode_fp4_kernel<T, D, RK, NC, QS, PS, LAYOUT>;
+  constexpr size_t lds = Fp4Lds<D, NC, QS, LAYOUT>::kBytes;
   static bool configured[kMaxDevices] = {};
   if (int rc = raise_lds_limit(configured, reinterpret_cast<const void*>(kern), lds); rc != TPA_OK) return rc;
   hipLaunchKernelGGL(kern, dim3(p.groups, plan.col_groups), dim3(kThreads), lds, stream, p);
@@ -665,13 +850,15 @@ int launch_join(const Fp4Params& p, hipStream_t stream) {
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
 template <typename T, int D, int RK, int NC>
-int launch_pairs(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+int launch_layout(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
   constexpr int QS = sizeof(T) == 2 ? 2 : 3, PS = sizeof(T) == 2 ? 1 : 3;
-  return p.H % 16 == 0 ? launch<T, D, RK, NC, QS, PS, true>(p, plan, stream) : launch<T, D, RK, NC, QS, PS, false>(p, plan, stream);
+  if (!plan.dense) return launch<T, D, RK, NC, QS, PS, kRowsApart>(p, plan, stream);
+  if (p.H == 8 || p.H == 16 || p.H == 32) return launch<T, D, RK, NC, QS, PS, kFewHeads>(p, plan, stream);
+  return launch<T, D, RK, NC, QS, PS, kDense>(p, plan, stream);
 }
 template <typename T, int D, int RK>
 int launch_sets(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
-  const int rc = plan.sets == 1 ? launch_pairs<T, D, RK, 1>(p, plan, stream) : launch_pairs<T, D, RK, 2>(p, plan, stream);
+  const int rc = plan.sets == 1 ? launch_layout<T, D, RK, 1>(p, plan, stream) : launch_layout<T, D, RK, 2>(p, plan, stream);
   if (rc != TPA_OK) return rc;
   return p.groups > 8 * (int64_t)p.B ? launch_join<T, D, 8>(p, stream) : launch_join<T, D, 1>(p, stream);
 }
@@ -722,6 +909,7 @@ extern "C" int tpa_decode_fp4(const TpaDecodeFp4Args* a, void* stream) {
   if (reinterpret_cast<uintptr_t>(a->workspace) % 256 || reinterpret_cast<uintptr_t>(a->o) % 16) return TPA_ERR_ALIGN;
   p.scale = a->sm_scale * kLog2e / ((float)a->rq * (float)a->rk);
   p.groups = plan.groups;
+  p.inv_h = 1.f / (float)a->H;
   p.plan = static_cast<int32_t*>(a->workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.plan_bytes);
   p.part_m = p.part_o + plan.slots * p.cols * p.dv;
