@@ -3,10 +3,13 @@
 // First launch: a wave holds a chunk of a beam's logits in its registers.  Every lane sums exponentials against a maximum of its own; the k-th largest of
 // the lanes' maxima bounds the chunk's k largest logits from below, and what is above it is put into a list sorted over the lanes (lane r: the r-th).
 // (Inside a beam the order of the values is that of the logits.)
-// Second launch: a workgroup for each request joins the sums and ranks the chunks' candidates, in 64 bits, behind a bound found in the same way.
+// Second launch: a workgroup for each request joins the sums and ranks the chunks' candidates, in 64 bits, behind a bound found in the same way.  It has
+// 1024 threads where there are many lists: each sum's and each list's reading is a wait of about 1 us (16 beams, 16 continuations, 160 000 fp32 logits, one
+// request: 15.3 us, with 256 threads 23.3; all candidates read in place of each list's first ones: 54), and 256 elsewhere (its barriers are cheaper).
 // Equal values go to the lower index: logits are put in by rising index, behind their equals, and the last step compares value and index.
 //
-// HBM bounds it where there are many beams, the latency of two launches where there are few.
+// HBM bounds it where there are many beams (64 requests, 4 beams, 131 072 bf16 logits: 18.7 + 5.4 us, 67 MB at 3.6 TB/s in the first), the latency of two
+// launches where there are few (one request, 4 beams, 50 021 fp32 logits: 5.2 + 5.6 us).
 #include <algorithm>
 
 #include "tpa_common.h"
@@ -15,6 +18,7 @@ namespace tpa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMostThreads = 1024;  // of the second launch, where a request has many lists
 constexpr int kBatch = 512;      // logits that a wave looks at together, eight a lane
 constexpr int kHeld = 4096;      // candidates that the second launch holds in LDS
 constexpr int kListed = 512;     // candidates that it ranks among each other
@@ -23,6 +27,8 @@ constexpr float kLog2eHigh = 1.44269502f, kLog2eLow = 1.92596299e-8f;
 
 struct Sum { double s; float r; int unused; };  // sum of exp2(x log2 e - r)
 struct Candidate { float logit; int token; };    // token < 0: none
+
+struct alignas(16) Ranked { double v; int flat, unused; };
 
 struct BeamParams {
   const void* logits;
@@ -175,23 +181,29 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(BeamParams p) {
   if (lane < p.k) p.candidates[id * p.k + lane] = Candidate{best, token};
 }
 
-__global__ __launch_bounds__(kThreads) void select_kernel(BeamParams p) {
+// Candidates of each list that the second launch copies to LDS first, in loads that do not wait for each other: all, if they fit, or the best one
+__host__ __device__ inline int held_of_each(int lists, int k) { return (int64_t)lists * k <= kHeld ? k : lists <= kHeld ? 1 : 0; }
+
+__global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
   extern __shared__ __attribute__((aligned(8))) char smem_beam[];
   __shared__ double base[TPA_BEAM_MAX];  // of a beam: what is added to its logits
-  __shared__ double red_value[kThreads / 64];
-  __shared__ int red_flat[kThreads / 64];
+  __shared__ double red_value[kMostThreads / 64];
+  __shared__ int red_flat[kMostThreads / 64];
   __shared__ double won_value[TPA_BEAM_MAX];
-  __shared__ int won[TPA_BEAM_MAX], listed, list_flat[kListed];
-  __shared__ double list_value[kListed];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int per_beam = p.chunks * p.k, total = p.n * per_beam;
-  const Candidate* const all = p.candidates + (int64_t)b * total;
+  __shared__ int won[TPA_BEAM_MAX], listed;
+  __shared__ Ranked list[kListed];
+  __shared__ int keys[kMostThreads];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, threads = blockDim.x, waves = threads / 64;
+  const int lists = p.n * p.chunks;
+  const Candidate* const all = p.candidates + (int64_t)b * lists * p.k;
   Candidate* const held = reinterpret_cast<Candidate*>(smem_beam);
-  const bool hold = total <= kHeld;
-  if (hold)
-    for (int i = tid; i < total; i += kThreads) held[i] = all[i];
+  const int hold = held_of_each(lists, p.k);
+  if (hold == 1)
+    for (int i = tid; i < lists; i += threads) held[i] = all[i * p.k];
+  else
+    for (int i = tid; i < lists * hold; i += threads) held[i] = all[i];
 
-  for (int j = w; j < p.n; j += kThreads / 64) {
+  for (int j = w; j < p.n; j += waves) {
     const int row = b * p.n + j;
     double value = NAN;  // a finished beam's chunks have no candidates: nothing was written there
     if (!(p.finished && p.finished[row])) {
@@ -211,61 +223,78 @@ __global__ __launch_bounds__(kThreads) void select_kernel(BeamParams p) {
   }
   __syncthreads();
 
-  // this thread's candidates; values that are no number, or infinite, are none
+  // This thread's candidates, list by list, each list's best first; values that are no number, or infinite, are none.  `visit` says whether it wants
+  // more of a list: of most lists only the first candidate is looked at, which is what keeps many beams with many continuations cheap.
   auto for_each = [&](auto visit) __attribute__((always_inline)) {
-    for (int i = tid; i < total; i += kThreads) {
-      const int j = i / per_beam;
-      const Candidate c = hold ? held[i] : all[i];
-      const double v = base[j] + (double)c.logit;
-      if (c.token >= 0 && fabs(v) < INFINITY) visit(v, j * p.vocab + c.token);
+    for (int i = tid; i < lists; i += threads) {
+      const int j = i / p.chunks;
+      for (int r = 0; r < p.k; ++r) {
+        const Candidate c = r < hold ? held[i * hold + r] : all[i * p.k + r];
+        const double v = base[j] + (double)c.logit;
+        if (c.token < 0 || !(fabs(v) < INFINITY) || !visit(v, j * p.vocab + c.token)) break;
+      }
     }
     if (p.finished && tid < p.n && p.finished[b * p.n + tid]) {
       const double v = (double)p.scores[b * p.n + tid];
       if (fabs(v) < INFINITY) visit(v, tid * p.vocab + p.eos);
     }
   };
-  // the best of them behind (value, flat index)
-  auto best_behind = [&](double value, int flat, double& best, int& best_flat) {
-    best = -INFINITY;
-    best_flat = INT32_MAX;
-    for_each([&](double v, int f) {
-      if (!(v < value || (v == value && f > flat))) return;
-      if (v > best || (v == best && f < best_flat)) { best = v; best_flat = f; }
-    });
-  };
-  // A bound: in every wave the k-th largest of the lanes' best candidates, as fp32 rounded down; the largest of the waves' leaves k candidates or more
-  double best;
-  int flat;
-  best_behind(INFINITY, -1, best, flat);
-  int key = ordered((float)best) - ((double)(float)best > best), at_key = 0;
-  for (int i = 0; i < p.k; ++i) {
-    at_key = wave_max(key);
-    const uint64_t there = __ballot(key == at_key);
-    if (lane == __builtin_ctzll(there)) key = INT32_MIN;
-  }
-  if (lane == 0) red_flat[w] = at_key;
+  // A bound: the k-th largest of the threads' best candidates, as fp32 rounded down, leaves k candidates or hardly more (every wave looks for it)
+  double most = -INFINITY;
+  for_each([&](double v, int) { most = fmax(most, v); return false; });
+  keys[tid] = ordered((float)most) - ((double)(float)most > most);
   if (tid == 0) listed = 0;
   __syncthreads();
-  const float bound = from_ordered(max(max(max(red_flat[0], red_flat[1]), max(red_flat[2], red_flat[3])), ordered(-INFINITY)));
+  int key[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) key[j] = keys[64 * j + lane];
+  for (int i = kThreads; i < threads; i += kThreads)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) key[j] = max(key[j], keys[i + 64 * j + lane]);
+  int at_key = 0;
+  for (int i = 0; i < p.k; ++i) {
+    const int of_lane = max(max(key[0], key[1]), max(key[2], key[3]));
+    at_key = wave_max(of_lane);
+    const uint64_t there = __ballot(of_lane == at_key);
+    bool here = lane == __builtin_ctzll(there);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (here && key[j] == at_key) { key[j] = INT32_MIN; here = false; }
+  }
+  const float bound = from_ordered(max(at_key, ordered(-INFINITY)));
   for_each([&](double v, int f) {
-    if (v < (double)bound) return;
+    if (v < (double)bound) return false;
     const int at = atomicAdd(&listed, 1);
-    if (at < kListed) { list_value[at] = v; list_flat[at] = f; }
+    if (at < kListed) list[at] = Ranked{v, f, 0};
+    return true;
   });
   __syncthreads();
   int found = 0;
   if (listed <= kListed) {
     // in whatever order they stand: each one's place is the number of those that beat it
     found = min(listed, p.k);
-    for (int i = tid; i < listed; i += kThreads) {
-      const double v = list_value[i];
-      const int f = list_flat[i];
+    for (int i = tid; i < listed; i += threads) {
+      const double v = list[i].v;
+      const int f = list[i].flat;
       int place = 0;
-      for (int j = 0; j < listed; ++j) place += list_value[j] > v || (list_value[j] == v && list_flat[j] < f);
+#pragma unroll 8
+      for (int j = 0; j < listed; ++j) place += list[j].v > v || (list[j].v == v && list[j].flat < f);
       if (place < p.k) { won_value[place] = v; won[place] = f; }
     }
   } else {
-    // many that are alike: the best one, k times
+    // many that are alike: the best one behind the last, k times
+    double best;
+    int flat;
+    auto best_behind = [&](double value, int after) {
+      best = -INFINITY;
+      flat = INT32_MAX;
+      for_each([&](double v, int f) {
+        if (v < best) return false;
+        if ((v < value || (v == value && f > after)) && (v > best || f < flat)) { best = v; flat = f; }
+        return true;
+      });
+    };
+    best_behind(INFINITY, -1);
     for (; found < p.k; ++found) {
       double v = best;
       int f = flat;
@@ -279,12 +308,11 @@ __global__ __launch_bounds__(kThreads) void select_kernel(BeamParams p) {
       __syncthreads();
       v = red_value[0];
       f = red_flat[0];
-#pragma unroll
-      for (int i = 1; i < kThreads / 64; ++i)
+      for (int i = 1; i < waves; ++i)
         if (red_value[i] > v || (red_value[i] == v && red_flat[i] < f)) { v = red_value[i]; f = red_flat[i]; }
       if (f == INT32_MAX) break;  // no candidate is left (the same in every thread)
       if (tid == 0) { won_value[found] = v; won[found] = f; }
-      if (f == flat) best_behind(v, f, best, flat);
+      if (f == flat) best_behind(v, f);
       __syncthreads();
     }
   }
@@ -365,9 +393,9 @@ extern "C" int tpa_beam_select(const TpaBeamSelectArgs* a, void* stream) {
   }
   hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(kThreads), 0, on, p);
   if (hipGetLastError() != hipSuccess) return TPA_ERR_LAUNCH;
-  const int64_t total = (int64_t)p.n * p.chunks * p.k;
+  const int lists = p.n * p.chunks;
   static bool configured[kMaxDevices] = {};
   if (int rc = raise_lds_limit(configured, reinterpret_cast<const void*>(select_kernel), kHeld * sizeof(Candidate)); rc != TPA_OK) return rc;
-  hipLaunchKernelGGL(select_kernel, dim3(a->B), dim3(kThreads), total <= kHeld ? total * sizeof(Candidate) : 0, on, p);
+  hipLaunchKernelGGL(select_kernel, dim3(a->B), dim3(lists > 2 * kThreads ? kMostThreads : kThreads), (size_t)lists * held_of_each(lists, p.k) * sizeof(Candidate), on, p);
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }

@@ -68,6 +68,17 @@ def test_a_large_vocabulary(gpu, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("b,n,k,vocab", [(1, 16, 16, 160000), (2, 64, 64, 5000), (1, 64, 8, 70001), (3, 5, 64, 20000)])
+def test_many_beams_with_many_continuations(gpu, b, n, k, vocab, dtype):
+    """More candidates than the second launch copies, in more lists than it copies the first of, and lists that hold most of what wins."""
+    logits, scores = inputs(gpu, 11, b, n, vocab, dtype)
+    check(logits, scores, k=k)
+    logits[:, 0, 100:100 + k] += 20.0
+    check(logits, scores, k=k)
+    check(torch.zeros_like(logits), torch.zeros_like(scores), k=k)
+
+
+@BOTH
 def test_ties_go_to_the_lower_index(gpu, dtype):
     for b, n, vocab, levels in ((2, 1, 3000, 3), (1, 1, 2100, 1), (2, 4, 700, 2)):
         x = torch.randint(0, levels, (b, 1, vocab), generator=torch.Generator().manual_seed(vocab)).to(dtype).to(gpu).expand(b, n, vocab)
