@@ -74,7 +74,7 @@ __device__ __forceinline__ int wave_prefix_sum(int x) {  // lane i: sum of lanes
   return add_from<0x143, 0xc>(x);  // row_bcast 31: lane 31 to rows 2 and 3
 }
 
-enum { kRowsApart, kDense, kFewHeads };  // LAYOUT of the kernel
+enum { kRowsApart, kDense, kFewHeads, kWholeSets };  // LAYOUT of the kernel
 
 // LDS: the tiles of the waves, the parts of Q that are not held in registers.  (Those that are held are made where the tiles will be.)
 template <int D, int NC, int QS, int LAYOUT>
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
 
   const Fp4Row parts(p.H, D);
   // where the head factors of this lane's columns lie in a row: two chunks of 8 for every set
-  int a_at[NA][2], a_scale_at[NA][2];
+  int a_at[NA][2], a_scale_at[NA][2];  // (kWholeSets: 32 heads from a_at[s][0] on, their scale's place among the scales of a in a_scale_at[s][0])
 #pragma unroll
   for (int s = 0; s < NA; ++s)
 #pragma unroll
@@ -201,6 +201,10 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       small_quotient(c0 + 32 * s + 16 * g + 8 * q, p.H, p.inv_h, h);
       a_at[s][q] = parts.a_codes + h / 2;
       a_scale_at[s][q] = parts.a_scales + h / 32;
+      if constexpr (LAYOUT == kWholeSets) {
+        a_at[s][q] -= 8 * g;
+        a_scale_at[s][q] = h / 32;
+      }
     }
   // this lane's row of a block: always the same rank
   const uint8_t* const k_base = static_cast<const uint8_t*>(p.kc.ptr) + (i % RK) * p.kc.stride_r;
@@ -240,6 +244,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       uint32_t k_scales, v_scales;           // kFewHeads: of b and of a, k_scales and v_scales the first and second word of K's row (g = 0) or V's
       u32x2 ka[NA], va[NA];                  // kFewHeads: heads of the first 16 columns and of the others of K's row (g = 0) or V's
       uint8_t ka_scale[NA][2], va_scale[NA][2];  // (not kFewHeads)
+      u32x4 a[NA];                               // kWholeSets: heads of every set, of K's row (g = 0) or V's, whose scale words are as for kFewHeads
     } raw;
     // this lane's half of K's row and of V's, and their ends
     auto take = [&](const uint8_t* k, const uint8_t* v, uint32_t at_k, uint32_t at_v) __attribute__((always_inline)) {
@@ -269,8 +274,13 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         raw.v[n] = *reinterpret_cast<const Word*>(v + (at_v + g * (D / 4)) + 16 * n);
       }
       const uint8_t* const mine = g ? v + at_v : k + at_k;
-      raw.ka[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes);
-      raw.va[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes + (p.H == 32 ? 8 : 0));
+      if constexpr (LAYOUT == kWholeSets) {
+#pragma unroll
+        for (int s = 0; s < NA; ++s) raw.a[s] = *reinterpret_cast<const Word*>(mine + a_at[s][0]);
+      } else {
+        raw.ka[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes);
+        raw.va[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes + (p.H == 32 ? 8 : 0));
+      }
       if constexpr (D == 128) {
         const u32x2 x = *reinterpret_cast<const Pair*>(mine + parts.b_scales);
         raw.k_scales = x[0];
@@ -294,7 +304,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         page = scalar(page);
         const int64_t k = page * p.kc.stride_b + in_page * p.kc.stride_l, v = page * p.vc.stride_b + in_page * p.vc.stride_l;
         const uint8_t *const k_block = static_cast<const uint8_t*>(p.kc.ptr) + k, *const v_block = static_cast<const uint8_t*>(p.vc.ptr) + v;
-        if constexpr (LAYOUT == kFewHeads) take_few(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
+        if constexpr (LAYOUT != kDense) take_few(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
         else take(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
       } else {
         take(k_base + page * p.kc.stride_b + in_page * p.kc.stride_l, v_base + page * p.vc.stride_b + in_page * p.vc.stride_l, 0, 0);
@@ -410,12 +420,14 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     // products of the rows of K with Q; numbers of V and of the head factors to LDS
     auto unpack = [&](int blk, f32x16 (&sp)[NC]) __attribute__((always_inline)) {
       uint32_t k_scales = raw.k_scales, v_scales = raw.v_scales;
+      uint32_t a_scales = D == 128 ? raw.v_scales : raw.k_scales >> 16;  // kWholeSets: of this half's matrix
       float ka_scale = 1.f, va_scale = 1.f;
-      if constexpr (LAYOUT == kFewHeads) {
+      if constexpr (LAYOUT == kFewHeads || LAYOUT == kWholeSets) {
         const auto first = __builtin_amdgcn_permlane32_swap(raw.k_scales, raw.k_scales, false, false);
         k_scales = first[0];
         v_scales = first[1];
-        if constexpr (D == 128) {
+        if constexpr (LAYOUT == kWholeSets) {
+        } else if constexpr (D == 128) {
           const auto second = __builtin_amdgcn_permlane32_swap(raw.v_scales, raw.v_scales, false, false);
           ka_scale = fp4_scale(second[0] & 255);
           va_scale = fp4_scale(second[1] & 255);
@@ -428,7 +440,8 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         // behind the last token: whatever is there, numbers that a weight of 0 leaves at 0
         v_scales = 0;
         va_scale = 1.f;
-        if constexpr (LAYOUT != kFewHeads) {
+        a_scales = 0;
+        if constexpr (LAYOUT == kRowsApart || LAYOUT == kDense) {
 #pragma unroll
           for (int s = 0; s < NA; ++s) raw.va_scale[s][0] = raw.va_scale[s][1] = 0;
         }
@@ -463,6 +476,14 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       if constexpr (LAYOUT == kFewHeads) {
         if (p.H == 8) { raw.ka[0][1] = raw.ka[0][0]; raw.va[0][1] = raw.va[0][0]; }
         reinterpret_cast<u32x4*>(lds_a)[l] = u32x4{raw.ka[0][0], raw.ka[0][1], raw.va[0][0], raw.va[0][1]};  // [K, V][32 rows][32 codes]
+      } else if constexpr (LAYOUT == kWholeSets) {
+#pragma unroll
+        for (int s = 0; s < NA; ++s) {
+          const float scale_of_set = fp4_scale(a_scales >> 8 * a_scale_at[s][0] & 255);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<bf16x8*>(lds_a + (2 * s + g) * Lds::kA + a_write_at(i, q)) = fp4_bf16x8(raw.a[s][q], scale_of_set);
+        }
       } else {
 #pragma unroll
         for (int s = 0; s < NA; ++s)
@@ -854,6 +875,7 @@ int launch_layout(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
   constexpr int QS = sizeof(T) == 2 ? 2 : 3, PS = sizeof(T) == 2 ? 1 : 3;
   if (!plan.dense) return launch<T, D, RK, NC, QS, PS, kRowsApart>(p, plan, stream);
   if (p.H == 8 || p.H == 16 || p.H == 32) return launch<T, D, RK, NC, QS, PS, kFewHeads>(p, plan, stream);
+  if (p.H % 32 == 0 && D / 32 + p.H / 32 <= D / 16) return launch<T, D, RK, NC, QS, PS, kWholeSets>(p, plan, stream);
   return launch<T, D, RK, NC, QS, PS, kDense>(p, plan, stream);
 }
 template <typename T, int D, int RK>
