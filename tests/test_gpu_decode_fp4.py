@@ -161,6 +161,65 @@ def test_numbers_that_are_not_finite(gpu, dtype):
         assert torch.isfinite(o[2, ..., :32]).all() and o[2, ..., 32:].isnan().all() and torch.isfinite(lse[2]).all()
 
 
+# heads of a few, of whole sets of 32 and of any number, whose rows a block has one behind the other
+LAYOUTS = pytest.mark.parametrize("h,d,rk", [(8, 64, 2), (8, 128, 4), (16, 128, 1), (32, 64, 8), (32, 128, 2), (64, 64, 4), (64, 128, 1), (96, 128, 2), (128, 128, 2), (24, 64, 2), (40, 128, 8), (96, 64, 1), (160, 128, 2)])
+
+
+@BOTH
+@LAYOUTS
+@pytest.mark.parametrize("page", [64, None])
+def test_what_is_behind_the_last_token(gpu, h, d, rk, page, dtype):
+    """The rest of a block, a page and a pool holds bytes that stand for NaN."""
+    lengths, tokens = [1, 77, 192, 0, 33], 192
+    q, kc, vc, table = problem(h, 5, 2, h, d, 6, rk, tokens, dtype, page)
+    for i, n in enumerate(lengths):
+        for t in range(n, tokens):
+            at = (i, t) if page is None else (table[i, t // page], t % page)
+            kc[at], vc[at] = 255, 255
+    if page:
+        for unused in set(range(len(kc))) - set(table.ravel()):
+            kc[unused], vc[unused] = 255, 255
+    dev = lambda x: None if x is None else torch.as_tensor(x).to(gpu)
+    got = tpa.tpa_decode_fp4(dev(q[..., :h]), dev(q)[..., h:], dev(kc), dev(vc), 0.1, kv_lengths=dev(np.array(lengths, np.int32)), page_table=dev(table), causal=BOTTOM_RIGHT)
+    compare(got, exact(q, kc, vc, table, h, d, d, 0.1, lengths, BOTTOM_RIGHT, 0), d, 6, rk, dtype)
+
+
+@BOTH
+@LAYOUTS
+def test_every_scale_that_is_no_number(gpu, h, d, rk, dtype):
+    """One scale byte of a row at a time, of K in one call and of V in another: what it belongs to is NaN and nothing else (the last sequence has none);
+    scales far apart in V."""
+    page, tokens, lq = 32, 128, 2
+    first, scales = (d + 1) // 2 + h // 2, d // 32 + -(-h // 32)
+    q, kc, vc, table = problem(h + 1, scales + 1, lq, h, d, 6, rk, tokens, dtype, page)
+    vc = fp4.random_rows(np.random.default_rng(h + d), vc.shape[:-1], h, d, (90, 165))
+    dev = lambda x: torch.as_tensor(x).to(gpu)
+    for which in (0, 1):
+        caches = [kc.copy(), vc.copy()]
+        for i in range(scales):
+            t = (31 * i + 5) % tokens
+            caches[which][table[i, t // page], t % page, i % rk, first + i] = 255
+        got = tpa.tpa_decode_fp4(dev(q[..., :h]), dev(q)[..., h:], dev(caches[0]), dev(caches[1]), 0.1, page_table=dev(table))
+        want = exact(q, *caches, table, h, d, d, 0.1, None, NONE, 0)
+        assert np.isnan(want[0]).any() and not np.isnan(want[0]).all()
+        assert np.array_equal(np.isnan(got[1].cpu().numpy()), np.isnan(want[1]))
+        compare(got, want, d, 6, rk, dtype)
+
+
+@BOTH
+@LAYOUTS
+def test_rows_with_room_between_them(gpu, h, d, rk, dtype):
+    """Rows of a wider array, one behind the other, at 4 bytes behind a 16-byte place."""
+    q, kc, vc, table = problem(h + 2, 2, 3, h, d, 5, rk, 160, dtype, 32)
+    dev = lambda x: torch.as_tensor(x).to(gpu)
+    n = kc.shape[-1]
+    wide = [torch.full((*c.shape[:-1], n + 20), 255, dtype=torch.uint8, device=gpu) for c in (kc, vc)]
+    for x, c in zip(wide, (kc, vc)):
+        x[..., 4 : 4 + n] = dev(c)
+    got = tpa.tpa_decode_fp4(dev(q[..., :h]), dev(q)[..., h:], *(x[..., 4 : 4 + n] for x in wide), 0.1, kv_lengths=dev(np.array([160, 95], np.int32)), page_table=dev(table), causal=TOP_LEFT, causal_offset=120)
+    compare(got, exact(q, kc, vc, table, h, d, d, 0.1, [160, 95], TOP_LEFT, 120), d, 5, rk, dtype)
+
+
 @BOTH
 def test_tables_with_pages_outside_the_pools(gpu, dtype):
     """They are read as the nearest page, and other sequences are not touched by them."""
