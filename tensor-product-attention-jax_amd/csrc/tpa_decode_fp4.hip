@@ -74,7 +74,7 @@ __device__ __forceinline__ int wave_prefix_sum(int x) {  // lane i: sum of lanes
   return add_from<0x143, 0xc>(x);  // row_bcast 31: lane 31 to rows 2 and 3
 }
 
-enum { kRowsApart, kDense, kFewHeads, kWholeSets };  // LAYOUT of the kernel
+enum { kRowsApart, kFewHeads, kWholeSets };  // LAYOUT of the kernel
 
 // LDS: the tiles of the waves, the parts of Q that are not held in registers.  (Those that are held are made where the tiles will be.)
 template <int D, int NC, int QS, int LAYOUT>
@@ -137,11 +137,18 @@ struct Eight {
 };
 
 // T: of the queries and the output.  NC: sets of 32 columns of a workgroup.  QS, PS: bf16 numbers that stand for one of Q and of the weighted probabilities.
-// LAYOUT: kRowsApart: every lane finds its row by itself.  kDense: the 32 rows of every block lie one behind the other, all of them in memory (pages of whole blocks), so
-// that a block has one address and a lane's place in it never changes.  kFewHeads: kDense and 8, 16 or 32 heads, so that all columns of a set have their head
-// factors in one block of 32: its scale goes into those of K's and V's numbers, and the codes themselves are transposed, to fp32 right from there.
-// What bounds the kernel is the issue of instructions, 2.9 of 5.5 thousand cycles a block in the softmax and its surroundings and none in waiting for memory:
-// 128 sequences of 12 000 keys, 32 heads of 128, rank 2 (308, 268 and 224 vector instructions a block):
+// LAYOUT: kRowsApart: every lane finds its row by itself and loads 8 heads and a scale at a time.
+// The others take blocks whose 32 rows lie one behind the other, all of them in memory (pages of whole blocks): a block has one address, a lane's place in it
+// never changes, and the ends of K's rows come in one half of the wave, those of V's in the other.
+// kFewHeads: 8, 16 or 32 heads: all columns of a set have their head factors in one block of 32, so its scale goes into those of K's and V's numbers, and the
+// codes themselves are transposed, to fp32 right from there.
+// kWholeSets: 64 heads, or 96 or 128 of 128 numbers: a set has a whole block of 32 heads, which is one load, and all scales of a row are in its last words.
+// What bounds the kernel is the issue of vector instructions and the first-level cache, which had work in 69 % of its cycles, none in waiting for memory:
+//   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 94 us, kRowsApart 104; 64 of 8192: 37, kRowsApart 42 (vector instructions of a block 228 and 308)
+//   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 42, kRowsApart 46; 48 of 8192, one row, 64 heads of 128, rank 2: 88, kRowsApart 107
+// (24 heads with one address a block and all else as for kRowsApart: 41.9 against 42.6, which is not worth a variant.)
+// Where there are few blocks, what is done once counts: 9 us with a block for every wave, 0.8 of them to find the share, 1.5 until the block is asked for,
+// 1.1 for Q, 2.1 for the block and 1.8 to join the waves.
 template <typename T, int D, int RK, int NC, int QS, int PS, int LAYOUT>
 __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 : 1) void decode_fp4_kernel(Fp4Params p) {
   using Lds = Fp4Lds<D, NC, QS, LAYOUT>;
@@ -247,27 +254,27 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       u32x4 a[NA];                               // kWholeSets: heads of every set, of K's row (g = 0) or V's, whose scale words are as for kFewHeads
     } raw;
     // this lane's half of K's row and of V's, and their ends
-    auto take = [&](const uint8_t* k, const uint8_t* v, uint32_t at_k, uint32_t at_v) __attribute__((always_inline)) {
+    auto take = [&](const uint8_t* k, const uint8_t* v) __attribute__((always_inline)) {
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
-        raw.k[n] = *reinterpret_cast<const Word*>(k + (at_k + g * (D / 4)) + 16 * n);
-        raw.v[n] = *reinterpret_cast<const Word*>(v + (at_v + g * (D / 4)) + 16 * n);
+        raw.k[n] = *reinterpret_cast<const Word*>(k + g * (D / 4) + 16 * n);
+        raw.v[n] = *reinterpret_cast<const Word*>(v + g * (D / 4) + 16 * n);
       }
-      raw.k_scales = *reinterpret_cast<const uint32_t*>(k + (at_k + parts.b_scales));
-      raw.v_scales = *reinterpret_cast<const uint32_t*>(v + (at_v + parts.b_scales));
+      raw.k_scales = *reinterpret_cast<const uint32_t*>(k + parts.b_scales);
+      raw.v_scales = *reinterpret_cast<const uint32_t*>(v + parts.b_scales);
 #pragma unroll
       for (int s = 0; s < NA; ++s)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          raw.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + (at_k + a_at[s][q]));
-          raw.va[s][q] = *reinterpret_cast<const uint32_t*>(v + (at_v + a_at[s][q]));
-          raw.ka_scale[s][q] = k[at_k + a_scale_at[s][q]];
-          raw.va_scale[s][q] = v[at_v + a_scale_at[s][q]];
+          raw.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + a_at[s][q]);
+          raw.va[s][q] = *reinterpret_cast<const uint32_t*>(v + a_at[s][q]);
+          raw.ka_scale[s][q] = k[a_scale_at[s][q]];
+          raw.va_scale[s][q] = v[a_scale_at[s][q]];
         }
     };
     // the same with the whole end of K's row in one half of the wave and of V's in the other: three loads instead of six (8 heads: what is read behind
     // them is not used)
-    auto take_few = [&](const uint8_t* k, const uint8_t* v, uint32_t at_k, uint32_t at_v) __attribute__((always_inline)) {
+    auto take_ends = [&](const uint8_t* k, const uint8_t* v, uint32_t at_k, uint32_t at_v) __attribute__((always_inline)) {
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
         raw.k[n] = *reinterpret_cast<const Word*>(k + (at_k + g * (D / 4)) + 16 * n);
@@ -304,10 +311,9 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         page = scalar(page);
         const int64_t k = page * p.kc.stride_b + in_page * p.kc.stride_l, v = page * p.vc.stride_b + in_page * p.vc.stride_l;
         const uint8_t *const k_block = static_cast<const uint8_t*>(p.kc.ptr) + k, *const v_block = static_cast<const uint8_t*>(p.vc.ptr) + v;
-        if constexpr (LAYOUT != kDense) take_few(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
-        else take(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
+        take_ends(k_block, v_block, i * (uint32_t)p.kc.stride_r, i * (uint32_t)p.vc.stride_r);
       } else {
-        take(k_base + page * p.kc.stride_b + in_page * p.kc.stride_l, v_base + page * p.vc.stride_b + in_page * p.vc.stride_l, 0, 0);
+        take(k_base + page * p.kc.stride_b + in_page * p.kc.stride_l, v_base + page * p.vc.stride_b + in_page * p.vc.stride_l);
       }
       page_ahead = lookup(blk + kWaves);
     };
@@ -422,29 +428,24 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       uint32_t k_scales = raw.k_scales, v_scales = raw.v_scales;
       uint32_t a_scales = D == 128 ? raw.v_scales : raw.k_scales >> 16;  // kWholeSets: of this half's matrix
       float ka_scale = 1.f, va_scale = 1.f;
-      if constexpr (LAYOUT == kFewHeads || LAYOUT == kWholeSets) {
+      if constexpr (LAYOUT != kRowsApart) {
         const auto first = __builtin_amdgcn_permlane32_swap(raw.k_scales, raw.k_scales, false, false);
         k_scales = first[0];
         v_scales = first[1];
-        if constexpr (LAYOUT == kWholeSets) {
-        } else if constexpr (D == 128) {
-          const auto second = __builtin_amdgcn_permlane32_swap(raw.v_scales, raw.v_scales, false, false);
-          ka_scale = fp4_scale(second[0] & 255);
-          va_scale = fp4_scale(second[1] & 255);
-        } else {
-          ka_scale = fp4_scale(k_scales >> 16 & 255);
-          va_scale = fp4_scale(v_scales >> 16 & 255);
-        }
+      }
+      if constexpr (LAYOUT == kFewHeads && D == 128) {
+        const auto second = __builtin_amdgcn_permlane32_swap(raw.v_scales, raw.v_scales, false, false);
+        ka_scale = fp4_scale(second[0] & 255);
+        va_scale = fp4_scale(second[1] & 255);
+      } else if constexpr (LAYOUT == kFewHeads) {
+        ka_scale = fp4_scale(k_scales >> 16 & 255);
+        va_scale = fp4_scale(v_scales >> 16 & 255);
       }
       if (LAYOUT != kRowsApart && blk * kRows + kRows - 1 > last_row && blk * kRows + i > last_row) {
         // behind the last token: whatever is there, numbers that a weight of 0 leaves at 0
         v_scales = 0;
         va_scale = 1.f;
         a_scales = 0;
-        if constexpr (LAYOUT == kRowsApart || LAYOUT == kDense) {
-#pragma unroll
-          for (int s = 0; s < NA; ++s) raw.va_scale[s][0] = raw.va_scale[s][1] = 0;
-        }
       }
       float scale[2][NW];
 #pragma unroll
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         const int shift = 8 * (NW * g + n);
         scale[0][n] = fp4_scale((k_scales >> shift) & 255);
         scale[1][n] = fp4_scale((v_scales >> shift) & 255);
-        if constexpr (LAYOUT == kFewHeads) {  // (a product past 2^127 is infinity, which the conversions make NaN of)
+        if constexpr (LAYOUT == kFewHeads) {  // (a product past 2^127 is infinity, which the conversions make NaN of; one below 2^-127 counts as that)
           scale[0][n] *= ka_scale;
           scale[1][n] *= va_scale;
         }
@@ -876,7 +877,7 @@ int launch_layout(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
   if (!plan.dense) return launch<T, D, RK, NC, QS, PS, kRowsApart>(p, plan, stream);
   if (p.H == 8 || p.H == 16 || p.H == 32) return launch<T, D, RK, NC, QS, PS, kFewHeads>(p, plan, stream);
   if (p.H % 32 == 0 && D / 32 + p.H / 32 <= D / 16) return launch<T, D, RK, NC, QS, PS, kWholeSets>(p, plan, stream);
-  return launch<T, D, RK, NC, QS, PS, kDense>(p, plan, stream);
+  return launch<T, D, RK, NC, QS, PS, kRowsApart>(p, plan, stream);
 }
 template <typename T, int D, int RK>
 int launch_sets(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
