@@ -683,7 +683,9 @@ int tpa_cache_read_fp4(const TpaFp4RowsArgs* args, void* stream);
 
 /*
  * tpa_decode over a cache in 4 bits (see TpaDecodeFp4Args).  A number of V that is NaN may reach, as 0 * NaN, the rows of its batch entry from which the causal
- * mask hides its token; tokens past kv_lengths are not read.
+ * mask hides its token; what is behind kv_lengths counts for nothing.
+ * The two scales of a number's factors may be multiplied first: where the product is past 2^127 the number is NaN, below 2^-127 it may count as up to 2^-122.
+ * Two launches; one on the vector units.
  */
 int tpa_decode_fp4(const TpaDecodeFp4Args* args, void* stream);
 

@@ -815,6 +815,7 @@ __global__ __launch_bounds__(kThreads) void decode_fp4_any_kernel(Fp4Params p) {
 bool mfma_takes(const TpaDecodeFp4Args* a) {
   if (a->dk != a->dv || (a->dk != 64 && a->dk != 128) || a->H % 8 || (a->rk != 1 && a->rk != 2 && a->rk != 4 && a->rk != 8)) return false;
   if ((int64_t)a->B * ((int64_t)a->lk * a->rk / (kRows * kWaves) + 1 + kStart) > INT32_MAX) return false;  // rounds
+  if ((int64_t)a->lq * a->H > 64 * 65535) return false;  // sets of columns are the second dimension of the grid
   for (const TpaFactor* f : {&a->k_cache, &a->v_cache})
     if (reinterpret_cast<uintptr_t>(f->ptr) % 4 || f->stride_b % 4 || f->stride_l % 4 || f->stride_r % 4) return false;
   return true;
