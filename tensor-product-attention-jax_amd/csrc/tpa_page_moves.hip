@@ -163,26 +163,23 @@ __device__ __forceinline__ int deal_pages(const ForkParams& p, const int32_t* fi
 // in LDS: holders that pages lo .. lo + n - 1 gain or lose.  A wave takes eight sequences at a time, a lane a page of each: sequences that go on once have
 // nothing to count but the last page.
 __device__ __forceinline__ void count_holders(const ForkParams& p, const int32_t* children, const int32_t* length, int32_t* change, int lo, int n) {
+  // last pages: lost unless a new sequence keeps it
+  for (int s = threadIdx.x; s < p.B; s += kPlanThreads)
+    if (length[s] % p.page != 0) {
+      const int page = p.table[(int64_t)s * p.P + length[s] / p.page];
+      if (page >= lo && page < lo + n && (children[s] == 0 || shares_of(p, page) != 0)) atomicAdd(&change[page - lo], -1);
+    }
   constexpr int kTogether = 8;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int s0 = wave * kTogether; s0 < p.B; s0 += kPlanThreads / 64 * kTogether) {
     int most = 0, full[kTogether], by[kTogether];
-    bool tail[kTogether];
 #pragma unroll
     for (int u = 0; u < kTogether; ++u) {
-      const int s = min(s0 + u, p.B - 1), len = length[s];
-      full[u] = len / p.page;
-      tail[u] = s0 + u < p.B && len % p.page != 0;
+      const int s = min(s0 + u, p.B - 1);
+      full[u] = length[s] / p.page;
       by[u] = s0 + u < p.B ? children[s] - 1 : 0;
       most = max(most, (by[u] ? full[u] : 0));
     }
-    // last pages, one lane for each sequence: lost unless a new sequence keeps it
-#pragma unroll
-    for (int u = 0; u < kTogether; ++u)
-      if (lane == u && tail[u]) {
-        const int page = p.table[(int64_t)(s0 + u) * p.P + full[u]];
-        if (page >= lo && page < lo + n && (by[u] < 0 || shares_of(p, page) != 0)) atomicAdd(&change[page - lo], -1);
-      }
     for (int e = lane; e < most; e += 64) {
       int page[kTogether];
 #pragma unroll
@@ -196,28 +193,51 @@ __device__ __forceinline__ void count_holders(const ForkParams& p, const int32_t
     }
   }
 }
-// counts of pages lo .. lo + n - 1 after the step; this thread's kEach pages that are released as bits, how many in `count`
-constexpr int kEach = kRange / kPlanThreads;
-__device__ __forceinline__ uint32_t settle_counts(const ForkParams& p, const int32_t* change, int lo, int n, int& count) {
-  count = 0;
-  uint32_t gone = 0;
+// Counts of pages lo .. lo + n - 1 after the step, page j * kPlanThreads + i of them by thread i; put(rank, how many there are, page) for those that are released,
+// in rising order.  Returns how many.  `slabs` = kSlabs ints
+constexpr int kEach = kRange / kPlanThreads, kSlabs = kEach * (kPlanThreads / 64);
+template <typename Put>
+__device__ __forceinline__ int settle_counts(const ForkParams& p, const int32_t* change, int lo, int n, int* slabs, Put put) {
+  static_assert(kSlabs == 128, "two of them a lane");
+  const int tid = threadIdx.x, lane = tid & 63, w = scalar(tid >> 6);
+  int before[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) before[j] = shares_of(p, lo + min(j * kPlanThreads + tid, n - 1));  // all on their way together
+  uint64_t gone[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    const int i = threadIdx.x * kEach + j;
-    if (i >= n) break;
-    const int now = shares_of(p, lo + i) + change[i];
-    p.new_shares[lo + i] = max(now, 0);
-    if (now < 0) { gone |= 1u << j; ++count; }
+    const int i = j * kPlanThreads + tid, now = i < n ? before[j] + change[i] : 0;
+    if (i < n) p.new_shares[lo + i] = max(now, 0);
+    gone[j] = __ballot(now < 0);
+    if (lane == 0) slabs[j * (kPlanThreads / 64) + w] = __popcll(gone[j]);
   }
-  return gone;
+  __syncthreads();
+  // every wave: released pages before each slab of 64
+  const int first = slabs[2 * lane], both = first + slabs[2 * lane + 1];
+  int upto = both;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(upto, d);
+    if (lane >= d) upto += y;
+  }
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int slab = j * (kPlanThreads / 64) + w;
+    const int base = __builtin_amdgcn_readlane(upto - both, slab >> 1) + (slab & 1 ? __builtin_amdgcn_readlane(first, slab >> 1) : 0);
+    if (gone[j] >> lane & 1) put(base + __popcll(gone[j] & ((1ull << lane) - 1)), total, lo + j * kPlanThreads + tid);
+  }
+  return total;
 }
 
 // ---- one launch, for pages of one range and no more than kSmall sequences: the first workgroup counts holders and makes the list, every other one makes the plan for
-// itself and carries out its share (a second launch costs the host 3.5 us; with it, 256 sequences over 4170 pages took 16.4 + 5.4 us)
+// itself and carries out its share (a second launch costs the host 3.5 us; with it, 256 sequences over 4170 pages and 15 MB of copies took 16.4 + 5.4 us, with one
+// 17.8; 12.3 since the first workgroup, which is the last to end, reads the last pages, the counts and the table's rows in as few rounds of waiting as there
+// are).  One of these workgroups fits a compute unit (76 registers; at 64, for two, 60 bytes go to scratch memory: 15.9 us).
 constexpr int kSmall = 2048;
 __global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(ForkParams p, Pools pools) {
   extern __shared__ int32_t smem[];
-  __shared__ int red[kPlanThreads / 64];
+  __shared__ int red[kPlanThreads / 64], slabs[kSlabs];
   int32_t* const children = smem;
   int32_t* const first = children + p.B;
   int32_t* const length = first + p.B;
@@ -232,18 +252,12 @@ __global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(ForkParams p, 
     const int taken = deal_pages(p, first, length, start, red, moves, [&](int i, int, int len) { p.new_lengths[i] = len; }, [](int, Move) {});
     count_holders(p, children, length, rest, 0, p.N);
     __syncthreads();
-    int count, released;
-    const uint32_t gone = settle_counts(p, rest, 0, p.N, count);
-    int at = sum_before(count, red, released);
-    const int end = start + taken, begin = end - released;
+    const int end = start + taken;
+    const int begin = end - settle_counts(p, rest, 0, p.N, slabs, [&](int rank, int released, int page) {
+      if (end - released + rank >= 0) p.new_free[end - released + rank] = page;
+    });
     for (int j = tid; j < p.F; j += kPlanThreads)
       if (j < begin || j >= end) p.new_free[j] = p.free_pages[j];
-#pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (gone >> j & 1) {
-        if (begin + at >= 0) p.new_free[begin + at] = tid * kEach + j;
-        ++at;
-      }
     if (tid == 0) p.new_start[0] = max(begin, 0);
     return;
   }
@@ -255,7 +269,8 @@ __global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(ForkParams p, 
   const int block = blockIdx.x - 1, blocks = gridDim.x - 1;
   copy_pages(pools, moves, [&](int m) { return Move{move[3 * m], move[3 * m + 1], move[3 * m + 2], 0}; }, (int64_t)(tid / kCopyThreads) * blocks + block,
              (int64_t)kGroups * blocks);
-  for (int64_t at = (int64_t)block * kPlanThreads + tid; at < (int64_t)p.M * p.P; at += (int64_t)blocks * kPlanThreads) {
+  // the table from the last groups on, which have the fewest chunks
+  for (int64_t at = ((int64_t)(kGroups - 1 - tid / kCopyThreads) * blocks + block) * kCopyThreads + tid % kCopyThreads; at < (int64_t)p.M * p.P; at += (int64_t)blocks * kPlanThreads) {
     const int i = (int)(at / p.P), e = (int)(at - (int64_t)i * p.P);
     int page = 0;
     if ((int64_t)e * p.page < len[i]) {
@@ -269,7 +284,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(ForkParams p, 
 // ---- two launches
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
   extern __shared__ int32_t smem[];
-  __shared__ int red[kPlanThreads / 64];
+  __shared__ int red[kPlanThreads / 64], slabs[kSlabs];
   int32_t* const children = smem;
   int32_t* const first = children + p.B;
   int32_t* const length = first + p.B;
@@ -286,12 +301,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
   }
   count_holders(p, children, length, change, lo, n);
   __syncthreads();
-  int count, total;
-  const uint32_t gone = settle_counts(p, change, lo, n, count);
-  int at = sum_before(count, red, total);
-#pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    if (gone >> j & 1) p.released[lo + at++] = lo + threadIdx.x * kEach + j;
+  const int total = settle_counts(p, change, lo, n, slabs, [&](int rank, int, int page) { p.released[lo + rank] = page; });
   if (threadIdx.x == 0) p.released_count[blockIdx.x] = total;
 }
 
@@ -520,9 +530,10 @@ int carry_out(Kernel kern, const Params& p, const TpaPool* pools, int num_pools,
 }
 
 // workgroups of one launch that does all: two on a compute unit, fewer where there are fewer chunks (four at a time) and numbers
+constexpr int kMostBlocks = 512;
 int blocks_for(int64_t chunks, int64_t numbers) {
   const int64_t want = std::max((chunks + 3) / 4, (numbers + kPlanThreads - 1) / kPlanThreads);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, 512));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, kMostBlocks));
 }
 
 template <typename Args>
@@ -569,7 +580,7 @@ extern "C" int tpa_pages_fork(const TpaPagesForkArgs* a, void* stream) {
     const size_t lds = 4 * ((size_t)3 * a->B + std::max(a->num_pages, 5 * a->M));
     static bool configured[kMaxDevices] = {};
     if (int rc = raise_lds_limit(configured, reinterpret_cast<const void*>(fork_small_kernel), 4 * (3 * TPA_PAGE_TABLES_MAX_REQUESTS + std::max(kRange, 5 * kSmall))); rc != TPA_OK) return rc;
-    const int groups = blocks_for((int64_t)a->M * pools.n * pools.chunks, a->M * P);
+    const int groups = std::min(blocks_for((int64_t)a->M * pools.n * pools.chunks, a->M * P), 255);
     hipLaunchKernelGGL(fork_small_kernel, dim3(1 + groups), dim3(kPlanThreads), lds, static_cast<hipStream_t>(stream), p, pools);
     return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
   }
