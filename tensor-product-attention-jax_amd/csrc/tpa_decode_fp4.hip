@@ -77,15 +77,15 @@ __device__ __forceinline__ int wave_prefix_sum(int x) {  // lane i: sum of lanes
 enum { kRowsApart, kFewHeads, kWholeSets };  // LAYOUT of the kernel
 
 // LDS: the tiles of the waves, the parts of Q that are not held in registers.  (Those that are held are made where the tiles will be.)
-template <int D, int NC, int QS, int LAYOUT>
+template <int D, int QS, int LAYOUT>
 struct Fp4Lds {
   static constexpr int kV = kRows * D;                            // elements of V's tile
   static constexpr int kA = kRows * 32;                           // of the head factors of 32 columns
-  static constexpr int kPerWave = kV + 2 * NC * kA;               // bf16 elements
+  static constexpr int kPerWave = kV + 2 * kA;                    // bf16 elements
   static constexpr int kHalf = D / 2, kRowStride = kHalf + 4;     // the waves are joined in two halves of D
   static_assert(4 * (32 * kRowStride + 64) <= 2 * kPerWave, "the join takes the room of the tiles");
-  static constexpr int kPart = NC * (D / 16) * 64;                // 16-byte words of a part of Q
-  static constexpr int kHeld = QS > 2 || (NC == 2 && D == 64) ? 0 : NC == 1 && (D == 64 || LAYOUT == kFewHeads) ? QS : 1;  // parts in registers: as far as they go there
+  static constexpr int kPart = D / 16 * 64;                      // 16-byte words of a part of Q
+  static constexpr int kHeld = QS > 2 ? 0 : D == 64 || LAYOUT == kFewHeads ? QS : 1;  // parts in registers: as far as they go there
   static_assert(16 * kHeld * kPart <= 2 * kPerWave * kWaves, "the held parts of Q take the room of the tiles");
   static constexpr size_t kBytes = 2 * (size_t)kPerWave * kWaves + 16 * (size_t)(QS - kHeld) * kPart;
 };
@@ -149,16 +149,15 @@ struct Eight {
 // (24 heads with one address a block and all else as for kRowsApart: 41.9 against 42.6, which is not worth a variant.)
 // Where there are few blocks, what is done once counts: 9 us with a block for every wave, 0.8 of them to find the share, 1.5 until the block is asked for,
 // 1.1 for Q, 2.1 for the block and 1.8 to join the waves.
-template <typename T, int D, int RK, int NC, int QS, int PS, int LAYOUT>
-__global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 : 1) void decode_fp4_kernel(Fp4Params p) {
-  using Lds = Fp4Lds<D, NC, QS, LAYOUT>;
+template <typename T, int D, int RK, int QS, int PS, int LAYOUT>
+__global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
+  using Lds = Fp4Lds<D, QS, LAYOUT>;
   constexpr int NKS = D / 16, NDB = D / 32, NW = D / 64;  // NW: 16-byte words of half a row's codes
   constexpr int NTOK = RK <= 4 ? 16 / RK : 32 / RK;       // tokens whose rows this lane has logits of
   constexpr int NV = RK <= 4 ? RK : RK / 2;               // rows of a token in this half of the wave
-  constexpr int NA = LAYOUT == kFewHeads ? 1 : NC;        // different sets of head factors
   extern __shared__ __attribute__((aligned(16))) uint16_t smem_fp4[];
   const int tid = threadIdx.x, w = scalar(tid >> 6), l = tid & 63, i = l & 31, g = l >> 5;
-  const int c0 = blockIdx.y * 32 * NC;
+  const int c0 = blockIdx.y * 32;
 
   // ---- this workgroup's share of the rounds, which every wave finds for itself: a lane has neighbouring sequences
   const int each = (p.B + 63) / 64, e0 = min(l * each, p.B), e1 = min(e0 + each, p.B);
@@ -192,36 +191,30 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
   first_round = __builtin_amdgcn_readlane(first_round, there);
 
   uint16_t* const lds_v = smem_fp4 + w * Lds::kPerWave;
-  uint16_t* const lds_a = lds_v + Lds::kV;  // [set][K, V][32 rows][32 columns]
+  uint16_t* const lds_a = lds_v + Lds::kV;  // [K, V][32 rows][32 columns]
   u32x4* const lds_q = reinterpret_cast<u32x4*>(smem_fp4);  // parts in registers later
   u32x4* const lds_q_rest = reinterpret_cast<u32x4*>(smem_fp4 + kWaves * Lds::kPerWave);
   constexpr int kHeld = Lds::kHeld;
 
   const Fp4Row parts(p.H, D);
-  // where the head factors of this lane's columns lie in a row: two chunks of 8 for every set
-  int a_at[NA][2], a_scale_at[NA][2];  // (kWholeSets: 32 heads from a_at[s][0] on, their scale's place among the scales of a in a_scale_at[s][0])
+  // where the head factors of this lane's columns lie in a row: two chunks of 8
+  int a_at[2], a_scale_at[2];  // (kWholeSets: 32 heads from a_at[0] on, their scale's place among the scales of a in a_scale_at[0])
 #pragma unroll
-  for (int s = 0; s < NA; ++s)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      int h;
-      small_quotient(c0 + 32 * s + 16 * g + 8 * q, p.H, p.inv_h, h);
-      a_at[s][q] = parts.a_codes + h / 2;
-      a_scale_at[s][q] = parts.a_scales + h / 32;
-      if constexpr (LAYOUT == kWholeSets) {
-        a_at[s][q] -= 8 * g;
-        a_scale_at[s][q] = h / 32;
-      }
+  for (int q = 0; q < 2; ++q) {
+    int h;
+    small_quotient(c0 + 16 * g + 8 * q, p.H, p.inv_h, h);
+    a_at[q] = parts.a_codes + h / 2;
+    a_scale_at[q] = parts.a_scales + h / 32;
+    if constexpr (LAYOUT == kWholeSets) {
+      a_at[q] -= 8 * g;
+      a_scale_at[q] = h / 32;
     }
+  }
   // this lane's row of a block: always the same rank
   const uint8_t* const k_base = static_cast<const uint8_t*>(p.kc.ptr) + (i % RK) * p.kc.stride_r;
   const uint8_t* const v_base = static_cast<const uint8_t*>(p.vc.ptr) + (i % RK) * p.vc.stride_r;
-  int row_of_col[NC];  // query row of this lane's column in every set (past the last: the last)
-#pragma unroll
-  for (int s = 0; s < NC; ++s) {
-    int h;
-    row_of_col[s] = small_quotient(min(c0 + 32 * s + i, p.cols - 1), p.H, p.inv_h, h);
-  }
+  int head;
+  const int row_of_col = small_quotient(min(c0 + i, p.cols - 1), p.H, p.inv_h, head);  // query row of this lane's column (past the last: the last)
 
   while (r0 < r1) {
     const int rounds = rounds_of<RK>(p, b);
@@ -234,12 +227,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     r0 = stop;
     if (end <= begin) continue;  // nothing but a share of its start
     const int len = length_of(p, b);
-    int last_of[NC], least_last[NC];
-#pragma unroll
-    for (int s = 0; s < NC; ++s) {
-      last_of[s] = keys_seen(p, len, row_of_col[s]) * RK - 1;
-      least_last[s] = scalar(__builtin_amdgcn_readfirstlane(last_of[s]));  // of the first column, whose row sees the fewest keys
-    }
+    const int last_of = keys_seen(p, len, row_of_col) * RK - 1, least_last = scalar(last_of);  // (the first column's row sees the fewest keys)
     const int last_row = keys_seen(p, len, p.lq - 1) * RK - 1;  // not below 0 here
     const int blk_begin = begin * kWaves + w, blk_end = min(end * kWaves, last_row / kRows + 1);
 
@@ -249,9 +237,9 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     struct Raw {
       u32x4 k[NW], v[NW];
       uint32_t k_scales, v_scales;           // kFewHeads: of b and of a, k_scales and v_scales the first and second word of K's row (g = 0) or V's
-      u32x2 ka[NA], va[NA];                  // kFewHeads: heads of the first 16 columns and of the others of K's row (g = 0) or V's
-      uint8_t ka_scale[NA][2], va_scale[NA][2];  // (not kFewHeads)
-      u32x4 a[NA];                               // kWholeSets: heads of every set, of K's row (g = 0) or V's, whose scale words are as for kFewHeads
+      uint32_t ka[2], va[2];                 // kRowsApart: 8 heads of K and of V twice; kFewHeads: ka the first 16 heads, va the others, of K's row (g = 0) or V's
+      uint8_t ka_scale[2], va_scale[2];      // (kRowsApart)
+      u32x4 a;                               // kWholeSets: 32 heads of K's row (g = 0) or V's, whose scale words are as for kFewHeads
     } raw;
     // this lane's half of K's row and of V's, and their ends
     auto take = [&](const uint8_t* k, const uint8_t* v) __attribute__((always_inline)) {
@@ -263,14 +251,12 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       raw.k_scales = *reinterpret_cast<const uint32_t*>(k + parts.b_scales);
       raw.v_scales = *reinterpret_cast<const uint32_t*>(v + parts.b_scales);
 #pragma unroll
-      for (int s = 0; s < NA; ++s)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          raw.ka[s][q] = *reinterpret_cast<const uint32_t*>(k + a_at[s][q]);
-          raw.va[s][q] = *reinterpret_cast<const uint32_t*>(v + a_at[s][q]);
-          raw.ka_scale[s][q] = k[a_scale_at[s][q]];
-          raw.va_scale[s][q] = v[a_scale_at[s][q]];
-        }
+      for (int q = 0; q < 2; ++q) {
+        raw.ka[q] = *reinterpret_cast<const uint32_t*>(k + a_at[q]);
+        raw.va[q] = *reinterpret_cast<const uint32_t*>(v + a_at[q]);
+        raw.ka_scale[q] = k[a_scale_at[q]];
+        raw.va_scale[q] = v[a_scale_at[q]];
+      }
     };
     // the same with the whole end of K's row in one half of the wave and of V's in the other: three loads instead of six (8 heads: what is read behind
     // them is not used)
@@ -282,11 +268,11 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       }
       const uint8_t* const mine = g ? v + at_v : k + at_k;
       if constexpr (LAYOUT == kWholeSets) {
-#pragma unroll
-        for (int s = 0; s < NA; ++s) raw.a[s] = *reinterpret_cast<const Word*>(mine + a_at[s][0]);
+        raw.a = *reinterpret_cast<const Word*>(mine + a_at[0]);
       } else {
-        raw.ka[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes);
-        raw.va[0] = *reinterpret_cast<const Pair*>(mine + parts.a_codes + (p.H == 32 ? 8 : 0));
+        const u32x2 first = *reinterpret_cast<const Pair*>(mine + parts.a_codes), others = *reinterpret_cast<const Pair*>(mine + parts.a_codes + (p.H == 32 ? 8 : 0));
+        raw.ka[0] = first[0]; raw.ka[1] = first[1];
+        raw.va[0] = others[0]; raw.va[1] = others[1];
       }
       if constexpr (D == 128) {
         const u32x2 x = *reinterpret_cast<const Pair*>(mine + parts.b_scales);
@@ -324,18 +310,15 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     auto part_q = [&](int q) __attribute__((always_inline)) { return q < kHeld ? lds_q + q * Lds::kPart : lds_q_rest + (q - kHeld) * Lds::kPart; };
     auto place_q = [&](int col, int d) __attribute__((always_inline)) {  // of number d of a column in a part of Q
       const int half = d / (D / 2), ks = d % (D / 2) / 8;
-      return ((col >> 5) * NKS + ks) * 64 + 32 * half + (col & 31);
+      return ks * 64 + 32 * half + col;
     };
     if constexpr (sizeof(T) == 2) {
       // by the matrix cores, 32 numbers of 32 columns a wave: rows d, columns c, contraction over the ranks, whose loads are all on their way at once.
       // (On the vector units, eight numbers a thread, the loads waited for four times: 6100 of the 18 800 cycles of the shortest call.)
-      for (int item = w; item < NC * NDB; item += kWaves) {
-        const int set = item / NDB, db = item % NDB;
-        int h;
-        const int qi = small_quotient(min(c0 + 32 * set + i, p.cols - 1), p.H, p.inv_h, h);
-        const uint16_t* const qa = static_cast<const uint16_t*>(p.qa.ptr) + b * p.qa.stride_b + qi * p.qa.stride_l + h;
-        // (columns of one set are of several query rows: their b rows differ, so a product for each of these rows, of which a column takes its own)
-        const int first_row = small_quotient(min(c0 + 32 * set, p.cols - 1), p.H, p.inv_h, h), last = small_quotient(min(c0 + 32 * set + 31, p.cols - 1), p.H, p.inv_h, h);
+      for (int db = w; db < NDB; db += kWaves) {
+        const uint16_t* const qa = static_cast<const uint16_t*>(p.qa.ptr) + b * p.qa.stride_b + row_of_col * p.qa.stride_l + head;
+        // (the columns may be of several query rows: their b rows differ, so a product for each of these rows, of which a column takes its own)
+        const int first_row = __builtin_amdgcn_readlane(row_of_col, 0), last = __builtin_amdgcn_readlane(row_of_col, 31);
         f32x16 x;
         for (int row = first_row; row <= last; ++row) {
           const uint16_t* const qb = static_cast<const uint16_t*>(p.qb.ptr) + b * p.qb.stride_b + row * p.qb.stride_l + 32 * db + i;
@@ -360,7 +343,7 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
             acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bw), __builtin_bit_cast(bf16x8, aw), acc, 0, 0, 0);
           }
 #pragma unroll
-          for (int v = 0; v < 16; ++v) x[v] = row == first_row || row == qi ? acc[v] : x[v];
+          for (int v = 0; v < 16; ++v) x[v] = row == first_row || row == row_of_col ? acc[v] : x[v];
         }
 #pragma unroll
         for (int n = 0; n < 4; ++n) {  // numbers 32 db + 8 n + 4 g + 0..3
@@ -369,11 +352,11 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
           split_pair<QS>(x[4 * n + 2] * p.scale, x[4 * n + 3] * p.scale, hi);
 #pragma unroll
           for (int q = 0; q < QS; ++q)
-            reinterpret_cast<u32x2*>(part_q(q))[2 * place_q(32 * set + i, 32 * db + 8 * n) + g] = u32x2{lo[q], hi[q]};
+            reinterpret_cast<u32x2*>(part_q(q))[2 * place_q(i, 32 * db + 8 * n) + g] = u32x2{lo[q], hi[q]};
         }
       }
     } else {
-      for (int item = tid; item < 32 * NC * (D / 8); item += kThreads) {
+      for (int item = tid; item < 32 * (D / 8); item += kThreads) {
         const int col = item / (D / 8), chunk = item % (D / 8);
         int h;
         const int qi = small_quotient(min(c0 + col, p.cols - 1), p.H, p.inv_h, h);
@@ -404,27 +387,22 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
       }
     }
     __syncthreads();
-    bf16x8 qf[kHeld ? kHeld * NC * NKS : 1];
+    bf16x8 qf[kHeld ? kHeld * NKS : 1];
     if constexpr (kHeld > 0) {
 #pragma unroll
-      for (int n = 0; n < kHeld * NC * NKS; ++n) qf[n] = __builtin_bit_cast(bf16x8, lds_q[n * 64 + l]);
+      for (int n = 0; n < kHeld * NKS; ++n) qf[n] = __builtin_bit_cast(bf16x8, lds_q[n * 64 + l]);
       __syncthreads();  // the tiles take their place
     }
 
-    f32x16 o[NC][NDB];
-    float m[NC], sum[NC];
+    f32x16 o[NDB];
+    float m = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int s = 0; s < NC; ++s) {
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[s][db][v] = 0.f;
-      m[s] = -INFINITY;
-      sum[s] = 0.f;
-    }
+      for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
 
     // products of the rows of K with Q; numbers of V and of the head factors to LDS
-    auto unpack = [&](int blk, f32x16 (&sp)[NC]) __attribute__((always_inline)) {
+    auto unpack = [&](int blk, f32x16& sp) __attribute__((always_inline)) {
       uint32_t k_scales = raw.k_scales, v_scales = raw.v_scales;
       uint32_t a_scales = D == 128 ? raw.v_scales : raw.k_scales >> 16;  // kWholeSets: of this half's matrix
       float ka_scale = 1.f, va_scale = 1.f;
@@ -459,142 +437,124 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
         }
       }
 #pragma unroll
-      for (int s = 0; s < NC; ++s)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) sp[s][v] = 0.f;
+      for (int v = 0; v < 16; ++v) sp[v] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) {
         const bf16x8 kf = fp4_bf16x8(raw.k[ks / 4][ks % 4], scale[0][ks / 4]);
 #pragma unroll
-        for (int s = 0; s < NC; ++s)
-#pragma unroll
-          for (int q = 0; q < QS; ++q) {
-            const bf16x8 qv = q < kHeld ? qf[q < kHeld ? (q * NC + s) * NKS + ks : 0] : __builtin_bit_cast(bf16x8, part_q(q)[(s * NKS + ks) * 64 + l]);
-            sp[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qv, sp[s], 0, 0, 0);
-          }
+        for (int q = 0; q < QS; ++q) {
+          const bf16x8 qv = q < kHeld ? qf[q < kHeld ? q * NKS + ks : 0] : __builtin_bit_cast(bf16x8, part_q(q)[ks * 64 + l]);
+          sp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qv, sp, 0, 0, 0);
+        }
         *reinterpret_cast<bf16x8*>(lds_v + tile_write_at<D>(i, NKS * g + ks)) = fp4_bf16x8(raw.v[ks / 4][ks % 4], scale[1][ks / 4]);
       }
       if constexpr (LAYOUT == kFewHeads) {
-        if (p.H == 8) { raw.ka[0][1] = raw.ka[0][0]; raw.va[0][1] = raw.va[0][0]; }
-        reinterpret_cast<u32x4*>(lds_a)[l] = u32x4{raw.ka[0][0], raw.ka[0][1], raw.va[0][0], raw.va[0][1]};  // [K, V][32 rows][32 codes]
+        if (p.H == 8) { raw.ka[1] = raw.ka[0]; raw.va[1] = raw.va[0]; }
+        reinterpret_cast<u32x4*>(lds_a)[l] = u32x4{raw.ka[0], raw.ka[1], raw.va[0], raw.va[1]};  // [K, V][32 rows][32 codes]
       } else if constexpr (LAYOUT == kWholeSets) {
+        const float scale_of_set = fp4_scale(a_scales >> 8 * a_scale_at[0] & 255);
 #pragma unroll
-        for (int s = 0; s < NA; ++s) {
-          const float scale_of_set = fp4_scale(a_scales >> 8 * a_scale_at[s][0] & 255);
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<bf16x8*>(lds_a + g * Lds::kA + a_write_at(i, q)) = fp4_bf16x8(raw.a[q], scale_of_set);
+      } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<bf16x8*>(lds_a + (2 * s + g) * Lds::kA + a_write_at(i, q)) = fp4_bf16x8(raw.a[s][q], scale_of_set);
+        for (int q = 0; q < 2; ++q) {
+          uint16_t* const at = lds_a + a_write_at(i, 2 * g + q);
+          *reinterpret_cast<bf16x8*>(at) = fp4_bf16x8(raw.ka[q], fp4_scale(raw.ka_scale[q]));
+          *reinterpret_cast<bf16x8*>(at + Lds::kA) = fp4_bf16x8(raw.va[q], fp4_scale(raw.va_scale[q]));
+        }
+      }
+    };
+    auto consume = [&](int blk, const f32x16& sp) __attribute__((always_inline)) {
+      const int lp = l & 15, dhalf = (l >> 4) & 1, row0 = blk * kRows;
+      float ak[16], av[16];  // of this lane's column, rows 8q + 4g + 0..3
+      if constexpr (LAYOUT == kFewHeads) {
+        // lane lp of 16 names row 8 (lp / 4) + 4 g + lp % 4, and gets its own column's codes of the sixteen rows
+        typedef int s32x2 __attribute__((ext_vector_type(2)));
+        const int at = 8 * (2 * (8 * (lp >> 2) + 4 * g + (lp & 3)) + dhalf);
+        const s32x2 tk = __builtin_amdgcn_ds_read_tr4_b64_v2i32((s32x2 __attribute__((address_space(3)))*)(reinterpret_cast<uint8_t*>(lds_a) + at));
+        const s32x2 tv = __builtin_amdgcn_ds_read_tr4_b64_v2i32((s32x2 __attribute__((address_space(3)))*)(reinterpret_cast<uint8_t*>(lds_a) + 512 + at));
+        float x[8];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          fp4_f32x8((uint32_t)tk[n], 1.f, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ak[8 * n + j] = x[j];
+          fp4_f32x8((uint32_t)tv[n], 1.f, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) av[8 * n + j] = x[j];
         }
       } else {
 #pragma unroll
-        for (int s = 0; s < NA; ++s)
+        for (int q = 0; q < 4; ++q) {
+          const int at = a_write_at(8 * q + 4 * g + (lp >> 2), 2 * dhalf + ((lp & 3) >> 1)) + 4 * (lp & 1);
+          const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + at));
+          const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + Lds::kA + at));
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint16_t* const at = lds_a + 2 * s * Lds::kA + a_write_at(i, 2 * g + q);
-            *reinterpret_cast<bf16x8*>(at) = fp4_bf16x8(raw.ka[s][q], fp4_scale(raw.ka_scale[s][q]));
-            *reinterpret_cast<bf16x8*>(at + Lds::kA) = fp4_bf16x8(raw.va[s][q], fp4_scale(raw.va_scale[s][q]));
+          for (int j = 0; j < 4; ++j) {
+            ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
+            av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
           }
+        }
       }
-    };
-    auto consume = [&](int blk, const f32x16 (&products)[NC]) __attribute__((always_inline)) {
-      const int lp = l & 15, dhalf = (l >> 4) & 1, row0 = blk * kRows;
-      float ak[16], av[16];  // of this lane's column, rows 8q + 4g + 0..3
-      auto head_factors = [&](int s) __attribute__((always_inline)) {
-        if constexpr (LAYOUT == kFewHeads) {
-          // lane lp of 16 names row 8 (lp / 4) + 4 g + lp % 4, and gets its own column's codes of the sixteen rows
-          typedef int s32x2 __attribute__((ext_vector_type(2)));
-          const int at = 8 * (2 * (8 * (lp >> 2) + 4 * g + (lp & 3)) + dhalf);
-          const s32x2 tk = __builtin_amdgcn_ds_read_tr4_b64_v2i32((s32x2 __attribute__((address_space(3)))*)(reinterpret_cast<uint8_t*>(lds_a) + at));
-          const s32x2 tv = __builtin_amdgcn_ds_read_tr4_b64_v2i32((s32x2 __attribute__((address_space(3)))*)(reinterpret_cast<uint8_t*>(lds_a) + 512 + at));
-          float x[8];
+      // ---- logits per token (log2 domain); from rank 8 on a token's rows span both halves of the wave
+      float st[NTOK], most = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            fp4_f32x8((uint32_t)tk[n], 1.f, x);
+      for (int t = 0; t < NTOK; ++t) {
+        const int v0 = t * NV;
+        float acc = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ak[8 * n + j] = x[j];
-            fp4_f32x8((uint32_t)tv[n], 1.f, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) av[8 * n + j] = x[j];
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int at = 2 * s * Lds::kA + a_write_at(8 * q + 4 * g + (lp >> 2), 2 * dhalf + ((lp & 3) >> 1)) + 4 * (lp & 1);
-            const s16x4 tk = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + at));
-            const s16x4 tv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(lds_a + Lds::kA + at));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              ak[4 * q + j] = bf16bits_to_f32((uint16_t)tk[j]);
-              av[4 * q + j] = bf16bits_to_f32((uint16_t)tv[j]);
-            }
-          }
-        }
-      };
-#pragma unroll
-      for (int s = 0; s < NC; ++s) {
-        if constexpr (NC > 1) __builtin_amdgcn_sched_barrier(0);
-        if (LAYOUT != kFewHeads || s == 0) head_factors(s);
-        const f32x16& sp = products[s];
-        // ---- logits per token (log2 domain); from rank 8 on a token's rows span both halves of the wave
-        float st[NTOK], most = -INFINITY;
+        for (int j = 0; j < NV; ++j) acc = fmaf(ak[v0 + j], sp[v0 + j], acc);
+        if constexpr (RK >= 8) acc = halves_sum(acc);
+        st[t] = acc;
+      }
+      if (row0 + kRows - 1 > least_last) {  // (the same in all lanes)
+        asm volatile("");                      // a branch: it is taken for the last keys alone
 #pragma unroll
         for (int t = 0; t < NTOK; ++t) {
-          const int v0 = t * NV;
-          float acc = 0.f;
-#pragma unroll
-          for (int j = 0; j < NV; ++j) acc = fmaf(ak[v0 + j], sp[v0 + j], acc);
-          if constexpr (RK >= 8) acc = halves_sum(acc);
-          st[t] = acc;
+          const int v0 = t * NV, row = RK >= 8 ? row0 + RK * t : row0 + 8 * (v0 >> 2) + 4 * g + (v0 & 3);  // the token's first row
+          if (row > last_of) st[t] = -INFINITY;
         }
-        if (row0 + kRows - 1 > least_last[s]) {  // (the same in all lanes)
-          asm volatile("");                      // a branch: it is taken for the last keys alone
+      }
 #pragma unroll
-          for (int t = 0; t < NTOK; ++t) {
-            const int v0 = t * NV, row = RK >= 8 ? row0 + RK * t : row0 + 8 * (v0 >> 2) + 4 * g + (v0 & 3);  // the token's first row
-            if (row > last_of[s]) st[t] = -INFINITY;
-          }
-        }
+      for (int t = 0; t < NTOK; ++t) most = fmaxf(most, st[t]);
+      most = halves_max(most);
+      // the reference is a whole number: a weight then has the same significand, and is rounded the same way, however the keys are dealt to
+      // waves and workgroups, and every factor that joins them is a power of two
+      const float m_new = fmaxf(m, __builtin_ceilf(most)), m_use = m_new == -INFINITY ? 0.f : m_new;
+      if (__any(m_new > m)) {
+        const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+        sum *= alpha;
 #pragma unroll
-        for (int t = 0; t < NTOK; ++t) most = fmaxf(most, st[t]);
-        most = halves_max(most);
-        // the reference is a whole number: a weight then has the same significand, and is rounded the same way, however the keys are dealt to
-        // waves and workgroups, and every factor that joins them is a power of two
-        const float m_new = fmaxf(m[s], __builtin_ceilf(most)), m_use = m_new == -INFINITY ? 0.f : m_new;
-        if (__any(m_new > m[s])) {
-          const float alpha = __builtin_amdgcn_exp2f(m[s] - m_use);
-          sum[s] *= alpha;
+        for (int db = 0; db < NDB; ++db)
 #pragma unroll
-          for (int db = 0; db < NDB; ++db)
+          for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+        m = m_new;
+      }
+      float pp[16];
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[s][db][v] *= alpha;
-          m[s] = m_new;
-        }
-        float pp[16];
+      for (int t = 0; t < NTOK; ++t) {
+        const float pt = __builtin_amdgcn_exp2f(st[t] - m_use);
+        sum += RK >= 8 ? 0.5f * pt : pt;  // both halves hold the token: each adds half of it
 #pragma unroll
-        for (int t = 0; t < NTOK; ++t) {
-          const float pt = __builtin_amdgcn_exp2f(st[t] - m_use);
-          sum[s] += RK >= 8 ? 0.5f * pt : pt;  // both halves hold the token: each adds half of it
+        for (int j = 0; j < NV; ++j) pp[t * NV + j] = pt * av[t * NV + j];
+      }
+      // ---- O^T[d, column] += sum over the rows of V[row, d] P'[row, column]; slot (g, j) = row 16 kk + 8 (j / 4) + 4 g + j % 4
 #pragma unroll
-          for (int j = 0; j < NV; ++j) pp[t * NV + j] = pt * av[t * NV + j];
-        }
-        // ---- O^T[d, column] += sum over the rows of V[row, d] P'[row, column]; slot (g, j) = row 16 kk + 8 (j / 4) + 4 g + j % 4
+      for (int kk = 0; kk < 2; ++kk) {
+        uint32_t words[4][PS];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          uint32_t words[4][PS];
+        for (int j = 0; j < 4; ++j) split_pair<PS>(pp[8 * kk + 2 * j], pp[8 * kk + 2 * j + 1], words[j]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) split_pair<PS>(pp[8 * kk + 2 * j], pp[8 * kk + 2 * j + 1], words[j]);
+        for (int db = 0; db < NDB; ++db) {
+          const bf16x8 vf = tile_tr<D>(lds_v, l, kk, db);
 #pragma unroll
-          for (int db = 0; db < NDB; ++db) {
-            const bf16x8 vf = tile_tr<D>(lds_v, l, kk, db);
-#pragma unroll
-            for (int q = 0; q < PS; ++q)
-              o[s][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(bf16x8, u32x4{words[0][q], words[1][q], words[2][q], words[3][q]}), o[s][db], 0, 0, 0);
-          }
+          for (int q = 0; q < PS; ++q)
+            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(bf16x8, u32x4{words[0][q], words[1][q], words[2][q], words[3][q]}), o[db], 0, 0, 0);
         }
       }
     };
     for (int blk = blk_begin; blk < blk_end; blk += kWaves) {
-      f32x16 sp[NC];
+      f32x16 sp;
       unpack(blk, sp);
       issue(blk + kWaves);
       consume(blk, sp);
@@ -604,51 +564,47 @@ __global__ __launch_bounds__(kThreads, QS <= 2 && NC <= (D == 128 ? 1 : 2) ? 2 :
     const int64_t slot = (int64_t)share + b;
     float* const red_o = reinterpret_cast<float*>(lds_v);
     constexpr int RS = Lds::kRowStride, HB = NDB / 2;
+    const int n_cols = min(32, p.cols - c0);
+    const float all = halves_sum(sum);
 #pragma unroll
-    for (int s = 0; s < NC; ++s) {
-      const int n_cols = min(32, p.cols - c0 - 32 * s);
-      if (n_cols <= 0) break;
-      const float all = halves_sum(sum[s]);
+    for (int half = 0; half < 2; ++half) {
+      __syncthreads();
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        __syncthreads();
+      for (int db = 0; db < HB; ++db)
 #pragma unroll
-        for (int db = 0; db < HB; ++db)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x16& x = o[s][half * HB + db];
-            *reinterpret_cast<f32x4*>(red_o + i * RS + 32 * db + 8 * q + 4 * g) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-          }
-        if (g == 0) {
-          red_o[32 * RS + i] = m[s];
-          red_o[32 * RS + 32 + i] = all;
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& x = o[half * HB + db];
+          *reinterpret_cast<f32x4*>(red_o + i * RS + 32 * db + 8 * q + 4 * g) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
         }
-        __syncthreads();
-        const int64_t base = slot * p.cols + c0 + 32 * s;
-        for (int idx = tid; idx < n_cols * (D / 8); idx += kThreads) {
-          const int c = idx / (D / 8), d = 4 * (idx % (D / 8));
-          float mw[kWaves], lw[kWaves], most = -INFINITY;
+      if (g == 0) {
+        red_o[32 * RS + i] = m;
+        red_o[32 * RS + 32 + i] = all;
+      }
+      __syncthreads();
+      const int64_t base = slot * p.cols + c0;
+      for (int idx = tid; idx < n_cols * (D / 8); idx += kThreads) {
+        const int c = idx / (D / 8), d = 4 * (idx % (D / 8));
+        float mw[kWaves], lw[kWaves], most = -INFINITY;
 #pragma unroll
-          for (int ww = 0; ww < kWaves; ++ww) {
-            const float* const from = reinterpret_cast<const float*>(smem_fp4 + ww * Lds::kPerWave);
-            mw[ww] = from[32 * RS + c];
-            lw[ww] = from[32 * RS + 32 + c];
-            most = fmaxf(most, mw[ww]);
-          }
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-          float lacc = 0.f;
+        for (int ww = 0; ww < kWaves; ++ww) {
+          const float* const from = reinterpret_cast<const float*>(smem_fp4 + ww * Lds::kPerWave);
+          mw[ww] = from[32 * RS + c];
+          lw[ww] = from[32 * RS + 32 + c];
+          most = fmaxf(most, mw[ww]);
+        }
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        float lacc = 0.f;
 #pragma unroll
-          for (int ww = 0; ww < kWaves; ++ww) {
-            const float* const from = reinterpret_cast<const float*>(smem_fp4 + ww * Lds::kPerWave);
-            const float f = lw[ww] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mw[ww] - most);  // 0: no key of this wave
-            acc += f * *reinterpret_cast<const f32x4*>(from + c * RS + d);
-            lacc += f * lw[ww];
-          }
-          *reinterpret_cast<f32x4*>(p.part_o + (base + c) * D + half * (D / 2) + d) = acc;
-          if (half == 0 && d == 0) {
-            p.part_m[base + c] = most;
-            p.part_l[base + c] = lacc;
-          }
+        for (int ww = 0; ww < kWaves; ++ww) {
+          const float* const from = reinterpret_cast<const float*>(smem_fp4 + ww * Lds::kPerWave);
+          const float f = lw[ww] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mw[ww] - most);  // 0: no key of this wave
+          acc += f * *reinterpret_cast<const f32x4*>(from + c * RS + d);
+          lacc += f * lw[ww];
+        }
+        *reinterpret_cast<f32x4*>(p.part_o + (base + c) * D + half * (D / 2) + d) = acc;
+        if (half == 0 && d == 0) {
+          p.part_m[base + c] = most;
+          p.part_l[base + c] = lacc;
         }
       }
     }
@@ -815,7 +771,7 @@ __global__ __launch_bounds__(kThreads) void decode_fp4_any_kernel(Fp4Params p) {
 bool mfma_takes(const TpaDecodeFp4Args* a) {
   if (a->dk != a->dv || (a->dk != 64 && a->dk != 128) || a->H % 8 || (a->rk != 1 && a->rk != 2 && a->rk != 4 && a->rk != 8)) return false;
   if ((int64_t)a->B * ((int64_t)a->lk * a->rk / (kRows * kWaves) + 1 + kStart) > INT32_MAX) return false;  // rounds
-  if ((int64_t)a->lq * a->H > 64 * 65535) return false;  // sets of columns are the second dimension of the grid
+  if ((int64_t)a->lq * a->H > 32 * 65535) return false;  // sets of columns are the second dimension of the grid
   for (const TpaFactor* f : {&a->k_cache, &a->v_cache})
     if (reinterpret_cast<uintptr_t>(f->ptr) % 4 || f->stride_b % 4 || f->stride_l % 4 || f->stride_r % 4) return false;
   return true;
@@ -828,12 +784,11 @@ bool dense_rows(const TpaDecodeFp4Args* a) {
   return (a->page_table ? (int64_t)a->page_size * a->rk : (int64_t)a->lk * a->rk) % kRows == 0;
 }
 
-struct Plan { int sets, col_groups, groups; bool dense; int64_t slots; size_t plan_bytes, bytes; };
+struct Plan { int col_groups, groups; bool dense; int64_t slots; size_t plan_bytes, bytes; };
 Plan plan_of(const TpaDecodeFp4Args* a) {
   Plan p;
   const int64_t cols = (int64_t)a->lq * a->H;
-  p.sets = cols > 32 ? 2 : 1;
-  p.col_groups = (int)((cols + 32 * p.sets - 1) / (32 * p.sets));
+  p.col_groups = (int)((cols + 31) / 32);
   const int64_t rounds = a->B * (((int64_t)a->lk * a->rk + kRows * kWaves - 1) / (kRows * kWaves) + kStart);
   p.groups = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, kMostGroups / p.col_groups));
   p.dense = dense_rows(a);
@@ -857,10 +812,10 @@ int check_args(const TpaDecodeFp4Args* a) {
   return TPA_OK;
 }
 
-template <typename T, int D, int RK, int NC, int QS, int PS, int LAYOUT>
+template <typename T, int D, int RK, int QS, int PS, int LAYOUT>
 int launch(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
-  auto kern = decode_fp4_kernel<T, D, RK, NC, QS, PS, LAYOUT>;
-  constexpr size_t lds = Fp4Lds<D, NC, QS, LAYOUT>::kBytes;
+  auto kern = decode_fp4_kernel<T, D, RK, QS, PS, LAYOUT>;
+  constexpr size_t lds = Fp4Lds<D, QS, LAYOUT>::kBytes;
   static bool configured[kMaxDevices] = {};
   if (int rc = raise_lds_limit(configured, reinterpret_cast<const void*>(kern), lds); rc != TPA_OK) return rc;
   hipLaunchKernelGGL(kern, dim3(p.groups, plan.col_groups), dim3(kThreads), lds, stream, p);
@@ -872,28 +827,25 @@ int launch_join(const Fp4Params& p, hipStream_t stream) {
   hipLaunchKernelGGL((join_kernel<T, D, SLICES>), dim3((unsigned)(((int64_t)p.B * p.cols + cols - 1) / cols)), dim3(kThreads), 0, stream, p);
   return hipGetLastError() == hipSuccess ? TPA_OK : TPA_ERR_LAUNCH;
 }
-template <typename T, int D, int RK, int NC>
-int launch_layout(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
-  constexpr int QS = sizeof(T) == 2 ? 2 : 3, PS = sizeof(T) == 2 ? 1 : 3;
-  if (!plan.dense) return launch<T, D, RK, NC, QS, PS, kRowsApart>(p, plan, stream);
-  if (p.H == 8 || p.H == 16 || p.H == 32) return launch<T, D, RK, NC, QS, PS, kFewHeads>(p, plan, stream);
-  if (p.H % 32 == 0 && D / 32 + p.H / 32 <= D / 16) return launch<T, D, RK, NC, QS, PS, kWholeSets>(p, plan, stream);
-  return launch<T, D, RK, NC, QS, PS, kRowsApart>(p, plan, stream);
-}
 template <typename T, int D, int RK>
-int launch_sets(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
-  const int rc = plan.sets == 1 ? launch_layout<T, D, RK, 1>(p, plan, stream) : launch_layout<T, D, RK, 2>(p, plan, stream);
-  if (rc != TPA_OK) return rc;
-  return p.groups > 8 * (int64_t)p.B ? launch_join<T, D, 8>(p, stream) : launch_join<T, D, 1>(p, stream);
+int launch_layout(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+  constexpr int QS = sizeof(T) == 2 ? 2 : 3, PS = QS;
+  if (!plan.dense) return launch<T, D, RK, QS, PS, kRowsApart>(p, plan, stream);
+  if (p.H == 8 || p.H == 16 || p.H == 32) return launch<T, D, RK, QS, PS, kFewHeads>(p, plan, stream);
+  if (p.H % 32 == 0 && D / 32 + p.H / 32 <= D / 16) return launch<T, D, RK, QS, PS, kWholeSets>(p, plan, stream);
+  return launch<T, D, RK, QS, PS, kRowsApart>(p, plan, stream);
 }
 template <typename T, int D>
-int launch_rank(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+int launch_both(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
+  int rc;
   switch (p.rk) {
-    case 1: return launch_sets<T, D, 1>(p, plan, stream);
-    case 2: return launch_sets<T, D, 2>(p, plan, stream);
-    case 4: return launch_sets<T, D, 4>(p, plan, stream);
-    default: return launch_sets<T, D, 8>(p, plan, stream);
+    case 1: rc = launch_layout<T, D, 1>(p, plan, stream); break;
+    case 2: rc = launch_layout<T, D, 2>(p, plan, stream); break;
+    case 4: rc = launch_layout<T, D, 4>(p, plan, stream); break;
+    default: rc = launch_layout<T, D, 8>(p, plan, stream);
   }
+  if (rc != TPA_OK) return rc;
+  return p.groups > 8 * (int64_t)p.B ? launch_join<T, D, 8>(p, stream) : launch_join<T, D, 1>(p, stream);
 }
 
 }  // namespace
@@ -938,6 +890,6 @@ extern "C" int tpa_decode_fp4(const TpaDecodeFp4Args* a, void* stream) {
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.plan_bytes);
   p.part_m = p.part_o + plan.slots * p.cols * p.dv;
   p.part_l = p.part_m + plan.slots * p.cols;
-  if (a->dtype == TPA_DTYPE_BF16) return a->dk == 128 ? launch_rank<uint16_t, 128>(p, plan, on) : launch_rank<uint16_t, 64>(p, plan, on);
-  return a->dk == 128 ? launch_rank<float, 128>(p, plan, on) : launch_rank<float, 64>(p, plan, on);
+  if (a->dtype == TPA_DTYPE_BF16) return a->dk == 128 ? launch_both<uint16_t, 128>(p, plan, on) : launch_both<uint16_t, 64>(p, plan, on);
+  return a->dk == 128 ? launch_both<float, 128>(p, plan, on) : launch_both<float, 64>(p, plan, on);
 }

@@ -108,7 +108,7 @@ def test_decode_workspace():
     need = decode(True)
     assert decode(workspace_bytes=need - 1) == WORKSPACE
     # more columns than a grid has sets of: the vector units, which need no workspace
-    assert decode(size=True, B=1, lq=524280, kernel=2) > 0 and decode(size=True, B=1, lq=524281) == 0 and decode(B=1, lq=524281, kernel=2) == UNSUPPORTED
+    assert decode(size=True, B=1, lq=262140, kernel=2) > 0 and decode(size=True, B=1, lq=262141) == 0 and decode(B=1, lq=262141, kernel=2) == UNSUPPORTED
 
 
 def beams(**changed):
