@@ -136,18 +136,22 @@ struct Eight {
   __device__ __forceinline__ float get(int j) const { return w[j >> 2][j & 3]; }
 };
 
-// T: of the queries and the output.  NC: sets of 32 columns of a workgroup.  QS, PS: bf16 numbers that stand for one of Q and of the weighted probabilities.
+// T: of the queries and the output.  QS, PS: bf16 numbers that stand for one of Q and of the weights p a_v: two for bf16 queries (with one, logits were off by up to 6e-3,
+// and outputs by half as much again as their own rounding, up to 0.0026 of their norm where that is 0.0016; the second number of a weight makes
+// 101 us of 94 for 128 sequences of 12 000 keys, in calls one behind the other, which the power limit slows down, 113 of 101), three for fp32.
 // LAYOUT: kRowsApart: every lane finds its row by itself and loads 8 heads and a scale at a time.
 // The others take blocks whose 32 rows lie one behind the other, all of them in memory (pages of whole blocks): a block has one address, a lane's place in it
 // never changes, and the ends of K's rows come in one half of the wave, those of V's in the other.
-// kFewHeads: 8, 16 or 32 heads: all columns of a set have their head factors in one block of 32, so its scale goes into those of K's and V's numbers, and the
+// kFewHeads: 8, 16 or 32 heads: all columns have their head factors in one block of 32, so its scale goes into those of K's and V's numbers, and the
 // codes themselves are transposed, to fp32 right from there.
-// kWholeSets: 64 heads, or 96 or 128 of 128 numbers: a set has a whole block of 32 heads, which is one load, and all scales of a row are in its last words.
-// What bounds the kernel is the issue of vector instructions and the first-level cache, which had work in 69 % of its cycles, none in waiting for memory:
-//   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 94 us, kRowsApart 104; 64 of 8192: 37, kRowsApart 42 (vector instructions of a block 228 and 308)
-//   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 42, kRowsApart 46; 48 of 8192, one row, 64 heads of 128, rank 2: 88, kRowsApart 107
+// kWholeSets: 64 heads, or 96 or 128 of 128 numbers: the columns have a whole block of 32 heads, which is one load, and all scales of a row are in its last words.
+// A workgroup has 32 columns.  (With two sets of them a block is unpacked once for 64, but one wave fits a SIMD with 128 numbers and no more with 64: from 46.8 us
+// for one set's 45 with 64 heads of 64 to 98 for 56 with 64 heads of 128.)
+// What bounds the kernel is the issue of instructions, vector and matrix ones half and half, by two waves a SIMD (three, of 168 registers, gain nothing):
+//   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 101 us, kRowsApart 115; 64 of 8192: 40, kRowsApart 46
+//   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 45, kRowsApart 50; 48 of 8192, one row, 64 heads of 128, rank 2: 56, kRowsApart 62
 // (24 heads with one address a block and all else as for kRowsApart: 41.9 against 42.6, which is not worth a variant.)
-// Where there are few blocks, what is done once counts: 9 us with a block for every wave, 0.8 of them to find the share, 1.5 until the block is asked for,
+// Where there are few blocks, what is done once counts: 8 us with a block for every wave, 0.8 of them to find the share, 1.5 until the block is asked for,
 // 1.1 for Q, 2.1 for the block and 1.8 to join the waves.
 template <typename T, int D, int RK, int QS, int PS, int LAYOUT>
 __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {

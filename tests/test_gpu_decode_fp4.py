@@ -1,7 +1,7 @@
 """tpa_decode_fp4 against softmax attention in 64 bits over the numbers that the rows stand for.
 
-Tolerances, before the first run.  With L the largest sum of the magnitudes in a logit and A the output's sum of the magnitudes p |V|: bf16 queries stand as two bf16
-numbers (off by 2^-17 of themselves) and a weight p a_v is rounded once (2^-8 of itself), fp32 ones are held to 2^-24 in both; fp32 sums of n
+Tolerances, before the first run.  With L the largest sum of the magnitudes in a logit and A the output's sum of the magnitudes p |V|: for bf16 queries both Q and a
+weight p a_v stand as two bf16 numbers (off by 2^-17 of themselves), for fp32 ones they are held to 2^-24; fp32 sums of n
 terms are off by n 2^-24 of the magnitudes, an exponential by 2^-22 and the 2^-23 of its argument.  So a logit is off by
   delta = (2^-17 or 2^-24, and (D + 2 rk + rq + 8) 2^-24) L + 2^-22
   |lse - exact| <= 2 delta + 2^-20 (|lse| + 1);  |o - exact| <= (2 delta + weight + (keys + 64) 2^-24) A + |o| half a step of its type + keys 2^-126 max |V|:
@@ -78,7 +78,7 @@ def compare(got, want, d, rq, rk, dtype):
     delta = ((2.0**-17 if bf16 else 2.0**-24) + (d + 2 * rk + rq + 8) * 2.0**-24) * big + 2.0**-22
     with np.errstate(invalid="ignore"):
         assert not (abs(gl - lse) > 2 * delta + 2.0**-20 * (abs(lse) + 1)).any()
-        t = (2 * delta.transpose(0, 2, 1)[..., None] + (2.0**-8 if bf16 else 2.0**-24) + (keys + 64) * 2.0**-24) * a + abs(o) * torch.finfo(dtype).eps / 2 + lost
+        t = (2 * delta.transpose(0, 2, 1)[..., None] + (2.0**-17 if bf16 else 2.0**-24) + (keys + 64) * 2.0**-24) * a + abs(o) * torch.finfo(dtype).eps / 2 + lost
         assert not (abs(go - o) > t).any(), np.nanmax(abs(go - o) / t)
 
 
