@@ -148,8 +148,8 @@ struct Eight {
 // A workgroup has 32 columns.  (With two sets of them a block is unpacked once for 64, but one wave fits a SIMD with 128 numbers and no more with 64: from 46.8 us
 // for one set's 45 with 64 heads of 64 to 98 for 56 with 64 heads of 128.)
 // What bounds the kernel is the issue of instructions, vector and matrix ones half and half, by two waves a SIMD (three, of 168 registers, gain nothing):
-//   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 101 us, kRowsApart 115; 64 of 8192: 40, kRowsApart 46
-//   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 45, kRowsApart 50; 48 of 8192, one row, 64 heads of 128, rank 2: 56, kRowsApart 62
+//   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 98 us, kRowsApart 115; 64 of 8192: 39, kRowsApart 46
+//   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 43, kRowsApart 50; 48 of 8192, one row, 64 heads of 128, rank 2: 56, kRowsApart 62
 // (24 heads with one address a block and all else as for kRowsApart: 41.9 against 42.6, which is not worth a variant.)
 // Where there are few blocks, what is done once counts: 8 us with a block for every wave, 0.8 of them to find the share, 1.5 until the block is asked for,
 // 1.1 for Q, 2.1 for the block and 1.8 to join the waves.
@@ -557,7 +557,12 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
         }
       }
     };
+    // The two waves of a SIMD come first block by block in turn: the older one, always first, ended its share at 25 us where the younger one took 42, half of it
+    // alone (12 sequences of 4500 keys, 4 query rows, 64 heads of 64; the kernel 1 to 3 us shorter)
+    int first = (blockIdx.x + blockIdx.y * gridDim.x) / (kMostGroups / 2);
     for (int blk = blk_begin; blk < blk_end; blk += kWaves) {
+      if (first++ & 1) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
       f32x16 sp;
       unpack(blk, sp);
       issue(blk + kWaves);
