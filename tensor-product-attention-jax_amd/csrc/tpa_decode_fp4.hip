@@ -85,7 +85,7 @@ struct Fp4Lds {
   static constexpr int kHalf = D / 2, kRowStride = kHalf + 4;     // the waves are joined in two halves of D
   static_assert(4 * (32 * kRowStride + 64) <= 2 * kPerWave, "the join takes the room of the tiles");
   static constexpr int kPart = D / 16 * 64;                      // 16-byte words of a part of Q
-  static constexpr int kHeld = QS > 2 ? 0 : D == 64 || LAYOUT == kFewHeads ? QS : 1;  // parts in registers: as far as they go there
+  static constexpr int kHeld = QS > 2 ? 0 : D == 64 || LAYOUT != kRowsApart ? QS : 1;  // parts in registers: as far as they go there
   static_assert(16 * kHeld * kPart <= 2 * kPerWave * kWaves, "the held parts of Q take the room of the tiles");
   static constexpr size_t kBytes = 2 * (size_t)kPerWave * kWaves + 16 * (size_t)(QS - kHeld) * kPart;
 };
@@ -142,14 +142,14 @@ struct Eight {
 // LAYOUT: kRowsApart: every lane finds its row by itself and loads 8 heads and a scale at a time.
 // The others take blocks whose 32 rows lie one behind the other, all of them in memory (pages of whole blocks): a block has one address, a lane's place in it
 // never changes, and the ends of K's rows come in one half of the wave, those of V's in the other.
-// kFewHeads: 8, 16 or 32 heads: all columns have their head factors in one block of 32, so its scale goes into those of K's and V's numbers, and the
-// codes themselves are transposed, to fp32 right from there.
-// kWholeSets: 64 heads, or 96 or 128 of 128 numbers: the columns have a whole block of 32 heads, which is one load, and all scales of a row are in its last words.
+// All columns have their head factors in one block of 32, so its scale goes into those of K's and V's numbers, and the codes themselves are transposed, to fp32 right from
+// there (with scales of their own in the tile, as kRowsApart has them, 43.7 us for 41 with 64 heads of 64).
+// kFewHeads: 8, 16 or 32 heads.  kWholeSets: 64 heads, or 96 or 128 of 128 numbers, whose scales are all in the last words of a row.
 // A workgroup has 32 columns.  (With two sets of them a block is unpacked once for 64, but one wave fits a SIMD with 128 numbers and no more with 64: from 46.8 us
 // for one set's 45 with 64 heads of 64 to 98 for 56 with 64 heads of 128.)
 // What bounds the kernel is the issue of instructions, vector and matrix ones half and half, by two waves a SIMD (three, of 168 registers, gain nothing):
 //   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 98 us, kRowsApart 115; 64 of 8192: 39, kRowsApart 46
-//   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 43, kRowsApart 50; 48 of 8192, one row, 64 heads of 128, rank 2: 56, kRowsApart 62
+//   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 41, kRowsApart 50; 48 of 8192, one row, 64 heads of 128, rank 2: 51, kRowsApart 62
 // (24 heads with one address a block and all else as for kRowsApart: 41.9 against 42.6, which is not worth a variant.)
 // Where there are few blocks, what is done once counts: 8 us with a block for every wave, 0.8 of them to find the share, 1.5 until the block is asked for,
 // 1.1 for Q, 2.1 for the block and 1.8 to join the waves.
@@ -240,10 +240,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
     typedef u32x2 __attribute__((aligned(4))) Pair;
     struct Raw {
       u32x4 k[NW], v[NW];
-      uint32_t k_scales, v_scales;           // kFewHeads: of b and of a, k_scales and v_scales the first and second word of K's row (g = 0) or V's
+      uint32_t k_scales, v_scales;           // not kRowsApart: of b and of a, k_scales and v_scales the first and second word of K's row (g = 0) or V's
       uint32_t ka[2], va[2];                 // kRowsApart: 8 heads of K and of V twice; kFewHeads: ka the first 16 heads, va the others, of K's row (g = 0) or V's
       uint8_t ka_scale[2], va_scale[2];      // (kRowsApart)
-      u32x4 a;                               // kWholeSets: 32 heads of K's row (g = 0) or V's, whose scale words are as for kFewHeads
+      u32x4 a;                               // kWholeSets: the 32 heads of K's row (g = 0) or V's, whose scale words are as for kFewHeads
     } raw;
     // this lane's half of K's row and of V's, and their ends
     auto take = [&](const uint8_t* k, const uint8_t* v) __attribute__((always_inline)) {
@@ -408,7 +408,6 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
     // products of the rows of K with Q; numbers of V and of the head factors to LDS
     auto unpack = [&](int blk, f32x16& sp) __attribute__((always_inline)) {
       uint32_t k_scales = raw.k_scales, v_scales = raw.v_scales;
-      uint32_t a_scales = D == 128 ? raw.v_scales : raw.k_scales >> 16;  // kWholeSets: of this half's matrix
       float ka_scale = 1.f, va_scale = 1.f;
       if constexpr (LAYOUT != kRowsApart) {
         const auto first = __builtin_amdgcn_permlane32_swap(raw.k_scales, raw.k_scales, false, false);
@@ -422,12 +421,16 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
       } else if constexpr (LAYOUT == kFewHeads) {
         ka_scale = fp4_scale(k_scales >> 16 & 255);
         va_scale = fp4_scale(v_scales >> 16 & 255);
+      } else if constexpr (LAYOUT == kWholeSets) {
+        const uint32_t of_half = (D == 128 ? raw.v_scales : raw.k_scales >> 16) >> 8 * a_scale_at[0] & 255;
+        const auto both = __builtin_amdgcn_permlane32_swap(of_half, of_half, false, false);
+        ka_scale = fp4_scale(both[0]);
+        va_scale = fp4_scale(both[1]);
       }
       if (LAYOUT != kRowsApart && blk * kRows + kRows - 1 > last_row && blk * kRows + i > last_row) {
         // behind the last token: whatever is there, numbers that a weight of 0 leaves at 0
         v_scales = 0;
         va_scale = 1.f;
-        a_scales = 0;
       }
       float scale[2][NW];
 #pragma unroll
@@ -435,7 +438,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
         const int shift = 8 * (NW * g + n);
         scale[0][n] = fp4_scale((k_scales >> shift) & 255);
         scale[1][n] = fp4_scale((v_scales >> shift) & 255);
-        if constexpr (LAYOUT == kFewHeads) {  // (a product past 2^127 is infinity, which the conversions make NaN of; one below 2^-127 counts as that)
+        if constexpr (LAYOUT != kRowsApart) {  // (a product past 2^127 is infinity, which the conversions make NaN of; one below 2^-127 counts as that)
           scale[0][n] *= ka_scale;
           scale[1][n] *= va_scale;
         }
@@ -456,9 +459,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
         if (p.H == 8) { raw.ka[1] = raw.ka[0]; raw.va[1] = raw.va[0]; }
         reinterpret_cast<u32x4*>(lds_a)[l] = u32x4{raw.ka[0], raw.ka[1], raw.va[0], raw.va[1]};  // [K, V][32 rows][32 codes]
       } else if constexpr (LAYOUT == kWholeSets) {
-        const float scale_of_set = fp4_scale(a_scales >> 8 * a_scale_at[0] & 255);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<bf16x8*>(lds_a + g * Lds::kA + a_write_at(i, q)) = fp4_bf16x8(raw.a[q], scale_of_set);
+        reinterpret_cast<u32x4*>(lds_a)[l] = raw.a;
       } else {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -471,7 +472,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
     auto consume = [&](int blk, const f32x16& sp) __attribute__((always_inline)) {
       const int lp = l & 15, dhalf = (l >> 4) & 1, row0 = blk * kRows;
       float ak[16], av[16];  // of this lane's column, rows 8q + 4g + 0..3
-      if constexpr (LAYOUT == kFewHeads) {
+      if constexpr (LAYOUT != kRowsApart) {
         // lane lp of 16 names row 8 (lp / 4) + 4 g + lp % 4, and gets its own column's codes of the sixteen rows
         typedef int s32x2 __attribute__((ext_vector_type(2)));
         const int at = 8 * (2 * (8 * (lp >> 2) + 4 * g + (lp & 3)) + dhalf);
