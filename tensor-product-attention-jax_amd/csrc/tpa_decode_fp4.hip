@@ -144,11 +144,11 @@ struct Eight {
 // never changes, and the ends of K's rows come in one half of the wave, those of V's in the other.
 // All columns have their head factors in one block of 32, so its scale goes into those of K's and V's numbers, and the codes themselves are transposed, to fp32 right from
 // there (with scales of their own in the tile, as kRowsApart has them, 43.7 us for 41 with 64 heads of 64).
-// kFewHeads: 8, 16 or 32 heads.  kWholeSets: 64 heads, or 96 or 128 of 128 numbers, whose scales are all in the last words of a row.
+// kFewHeads: 8 or 16 heads.  kWholeSets: 32 or 64 heads, or 96 or 128 of 128 numbers, whose scales are all in the last words of a row.
 // A workgroup has 32 columns.  (With two sets of them a block is unpacked once for 64, but one wave fits a SIMD with 128 numbers and no more with 64: from 46.8 us
 // for one set's 45 with 64 heads of 64 to 98 for 56 with 64 heads of 128.)
 // What bounds the kernel is the issue of instructions, vector and matrix ones half and half, by two waves a SIMD (three, of 168 registers, gain nothing):
-//   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 98 us, kRowsApart 115; 64 of 8192: 39, kRowsApart 46
+//   128 sequences of 12 000 keys, 32 heads of 128, rank 2: 96 us, kRowsApart 115; 64 of 8192: 39, kRowsApart 46
 //   12 sequences of 4500 keys, 4 query rows, 64 heads of 64, rank 4: 41, kRowsApart 50; 48 of 8192, one row, 64 heads of 128, rank 2: 51, kRowsApart 62
 // (24 heads with one address a block and all else as for kRowsApart: 41.9 against 42.6, which is not worth a variant.)
 // Where there are few blocks, what is done once counts: 8 us with a block for every wave, 0.8 of them to find the share, 1.5 until the block is asked for,
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
     struct Raw {
       u32x4 k[NW], v[NW];
       uint32_t k_scales, v_scales;           // not kRowsApart: of b and of a, k_scales and v_scales the first and second word of K's row (g = 0) or V's
-      uint32_t ka[2], va[2];                 // kRowsApart: 8 heads of K and of V twice; kFewHeads: ka the first 16 heads, va the others, of K's row (g = 0) or V's
+      uint32_t ka[2], va[2];                 // kRowsApart: 8 heads of K and of V twice; kFewHeads: ka the heads of K's row (g = 0) or V's
       uint8_t ka_scale[2], va_scale[2];      // (kRowsApart)
       u32x4 a;                               // kWholeSets: the 32 heads of K's row (g = 0) or V's, whose scale words are as for kFewHeads
     } raw;
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
         raw.va_scale[q] = v[a_scale_at[q]];
       }
     };
-    // the same with the whole end of K's row in one half of the wave and of V's in the other: three loads instead of six (8 heads: what is read behind
+    // the same with the whole end of K's row in one half of the wave and of V's in the other (8 heads: what is read behind
     // them is not used)
     auto take_ends = [&](const uint8_t* k, const uint8_t* v, uint32_t at_k, uint32_t at_v) __attribute__((always_inline)) {
 #pragma unroll
@@ -274,9 +274,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
       if constexpr (LAYOUT == kWholeSets) {
         raw.a = *reinterpret_cast<const Word*>(mine + a_at[0]);
       } else {
-        const u32x2 first = *reinterpret_cast<const Pair*>(mine + parts.a_codes), others = *reinterpret_cast<const Pair*>(mine + parts.a_codes + (p.H == 32 ? 8 : 0));
-        raw.ka[0] = first[0]; raw.ka[1] = first[1];
-        raw.va[0] = others[0]; raw.va[1] = others[1];
+        const u32x2 codes = *reinterpret_cast<const Pair*>(mine + parts.a_codes);
+        raw.ka[0] = codes[0]; raw.ka[1] = codes[1];
       }
       if constexpr (D == 128) {
         const u32x2 x = *reinterpret_cast<const Pair*>(mine + parts.b_scales);
@@ -456,8 +455,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(Fp4Params p) {
         *reinterpret_cast<bf16x8*>(lds_v + tile_write_at<D>(i, NKS * g + ks)) = fp4_bf16x8(raw.v[ks / 4][ks % 4], scale[1][ks / 4]);
       }
       if constexpr (LAYOUT == kFewHeads) {
-        if (p.H == 8) { raw.ka[1] = raw.ka[0]; raw.va[1] = raw.va[0]; }
-        reinterpret_cast<u32x4*>(lds_a)[l] = u32x4{raw.ka[0], raw.ka[1], raw.va[0], raw.va[1]};  // [K, V][32 rows][32 codes]
+        const uint32_t odd = p.H == 8 ? raw.ka[0] : raw.ka[1];
+        reinterpret_cast<u32x4*>(lds_a)[l] = u32x4{raw.ka[0], odd, raw.ka[0], odd};  // [K, V][32 rows][32 codes]
       } else if constexpr (LAYOUT == kWholeSets) {
         reinterpret_cast<u32x4*>(lds_a)[l] = raw.a;
       } else {
@@ -841,7 +840,7 @@ template <typename T, int D, int RK>
 int launch_layout(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
   constexpr int QS = sizeof(T) == 2 ? 2 : 3, PS = QS;
   if (!plan.dense) return launch<T, D, RK, QS, PS, kRowsApart>(p, plan, stream);
-  if (p.H == 8 || p.H == 16 || p.H == 32) return launch<T, D, RK, QS, PS, kFewHeads>(p, plan, stream);
+  if (p.H == 8 || p.H == 16) return launch<T, D, RK, QS, PS, kFewHeads>(p, plan, stream);
   if (p.H % 32 == 0 && D / 32 + p.H / 32 <= D / 16) return launch<T, D, RK, QS, PS, kWholeSets>(p, plan, stream);
   return launch<T, D, RK, QS, PS, kRowsApart>(p, plan, stream);
 }
