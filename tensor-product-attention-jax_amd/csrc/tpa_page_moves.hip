@@ -231,7 +231,7 @@ __device__ __forceinline__ int settle_counts(const ForkParams& p, const int32_t*
 }
 
 // ---- one launch, for pages of one range and no more than kSmall sequences: the first workgroup counts holders and makes the list, every other one makes the plan for
-// itself and carries out its share (a second launch costs the host 3.5 us; with it, 256 sequences over 4170 pages and 15 MB of copies took 16.4 + 5.4 us, with one
+// itself and carries out its share (a second launch costs the host 3.5 us; with it, 256 sequences over 4170 pages and 14 MB read and written took 16.4 + 5.4 us, with one
 // 17.8; 12.3 since the first workgroup, which is the last to end, reads the last pages, the counts and the table's rows in as few rounds of waiting as there
 // are).  One of these workgroups fits a compute unit (76 registers; at 64, for two, 60 bytes go to scratch memory: 15.9 us).
 constexpr int kSmall = 2048;
