@@ -221,6 +221,17 @@ def test_rows_with_room_between_them(gpu, h, d, rk, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("seed", range(24))
+def test_shapes_that_nobody_picked(gpu, seed, dtype):
+    rng = np.random.default_rng(1000 + seed)
+    pick = lambda *x: x[int(rng.integers(len(x)))]
+    h, d, rk, rq, lq, b = pick(8, 16, 24, 32, 40, 48, 56, 64, 96, 128, 7), pick(64, 128, 128, 64, 80), pick(1, 2, 2, 4, 8, 3), pick(1, 2, 6, 17), pick(1, 1, 2, 3, 6), int(rng.integers(1, 9))
+    tokens, page = int(np.exp(rng.uniform(0, np.log(600)))), pick(None, 1, 3, 8, 16, 32, 64, 100)
+    causal, offset = pick((NONE, 0), (TOP_LEFT, 40), (BOTTOM_RIGHT, 0), (BOTTOM_RIGHT, 2))
+    check(gpu, seed, b, lq, h, d, rq, rk, tokens, dtype, page=page, lengths=rng.integers(-1, tokens + 2, b).tolist(), causal=causal, offset=offset, scale=float(rng.uniform(0.02, 0.3)))
+
+
+@BOTH
 def test_tables_with_pages_outside_the_pools(gpu, dtype):
     """They are read as the nearest page, and other sequences are not touched by them."""
     h, d, rk, page = 16, 64, 2, 8
