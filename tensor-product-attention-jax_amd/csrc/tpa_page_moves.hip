@@ -57,6 +57,7 @@ struct Pools {
 };
 
 constexpr int kCopyThreads = 256;  // that copy a chunk: four loads each in flight
+// Past the caches, which hold none of it when it is read next: 500 MB read and written take 100.5 us (5.0 TB/s), through them 109.7.
 template <typename T>
 __device__ __forceinline__ void copy_chunk(char* to, const char* from, int64_t bytes, int thread) {
   T* const t = reinterpret_cast<T*>(to);
@@ -66,10 +67,10 @@ __device__ __forceinline__ void copy_chunk(char* to, const char* from, int64_t b
     T x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i + u * kCopyThreads < n) x[u] = f[i + u * kCopyThreads];
+      if (i + u * kCopyThreads < n) x[u] = __builtin_nontemporal_load(f + i + u * kCopyThreads);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i + u * kCopyThreads < n) t[i + u * kCopyThreads] = x[u];
+      if (i + u * kCopyThreads < n) __builtin_nontemporal_store(x[u], t + i + u * kCopyThreads);
   }
 }
 // `group` of `groups` groups of threads that share out the moves' chunks
