@@ -22,10 +22,13 @@ constexpr int kMostThreads = 1024;  // of the second launch, where a request has
 constexpr int kBatch = 512;      // logits that a wave looks at together, eight a lane
 constexpr int kHeld = 4096;      // candidates that the second launch holds in LDS
 constexpr int kListed = 512;     // candidates that it ranks among each other
-// log2(e) in two parts: one alone is off by 1.3e-8 of itself, which a logit of 12 makes 2e-7 of every term
+// log2(e) in two parts: one alone is off by 1.3e-8 of itself, which a distance of 12 makes 2e-7 of a term
 constexpr float kLog2eHigh = 1.44269502f, kLog2eLow = 1.92596299e-8f;
+// exp(d) of a distance d <= 0 from a maximum.  The maximum itself is a logit: its own term is then 1, and no term more, however large the logits are.  (A maximum
+// times log2(e) is rounded, and from logits of 3e9 on what it is off by makes infinities and zeros of the terms that stand at it.)
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(fmaf(d, kLog2eHigh, d * kLog2eLow)); }
 
-struct Sum { double s; float r; int unused; };  // sum of exp2(x log2 e - r)
+struct Sum { double s; float most; int unused; };  // sum of exp(x - most), most = the largest x; 0 and -inf: nothing but -inf
 struct Candidate { float logit; int token; };    // token < 0: none
 
 struct alignas(16) Ranked { double v; int flat, unused; };
@@ -120,20 +123,19 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(BeamParams p) {
     for (int n = 0; n < NB; ++n) held[n].load_part(logits + begin + n * kBatch + 8 * lane, end - begin - n * kBatch - 8 * lane);
   }
 
-  float r = -INFINITY, s = 0.f;  // this lane's logits: sum of exp2(x log2 e - r)
-  float most[NB], top = -INFINITY;
+  float top = -INFINITY, s = 0.f;  // this lane's logits: the largest, sum of exp(x - top)
+  float most[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     float x[8];
     held[n].get(x);
     most[n] = max8(x);
-    top = fmaxf(top, most[n]);
-    const float rn = fmaxf(r, most[n] * kLog2eHigh), ru = rn == -INFINITY ? 0.f : rn;
+    const float now = fmaxf(top, most[n]), use = now == -INFINITY ? 0.f : now;
     float terms[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) terms[j] = __builtin_amdgcn_exp2f(fmaf(x[j], kLog2eLow, fmaf(x[j], kLog2eHigh, -ru)));
-    s = fmaf(s, __builtin_amdgcn_exp2f(r - ru), ((terms[0] + terms[1]) + (terms[2] + terms[3])) + ((terms[4] + terms[5]) + (terms[6] + terms[7])));
-    r = rn;
+    for (int j = 0; j < 8; ++j) terms[j] = exp_of(x[j] - use);
+    s = fmaf(s, exp_of(top - use), ((terms[0] + terms[1]) + (terms[2] + terms[3])) + ((terms[4] + terms[5]) + (terms[6] + terms[7])));
+    top = now;
   }
 
   // the k-th largest of the lanes' maxima: at least k logits are no smaller
@@ -173,11 +175,11 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(BeamParams p) {
     } while (lanes);
   }
 
-  const float rw = from_ordered(wave_max(ordered(r))), ru = rw == -INFINITY ? 0.f : rw;
-  double sum = (double)s * (double)__builtin_amdgcn_exp2f(r - ru);
+  const float all = from_ordered(wave_max(ordered(top))), use = all == -INFINITY ? 0.f : all;
+  double sum = (double)s * (double)exp_of(top - use);
 #pragma unroll
   for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-  if (lane == 0) p.sums[id] = Sum{sum, rw, 0};
+  if (lane == 0) p.sums[id] = Sum{sum, all, 0};
   if (lane < p.k) p.candidates[id * p.k + lane] = Candidate{best, token};
 }
 
@@ -186,7 +188,9 @@ __host__ __device__ inline int held_of_each(int lists, int k) { return (int64_t)
 
 __global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
   extern __shared__ __attribute__((aligned(8))) char smem_beam[];
-  __shared__ double base[TPA_BEAM_MAX];  // of a beam: what is added to its logits
+  // of a beam: the value of logit x is score + ((x - most) - log_sum)  (one number for all three would lose the small ones beside a large `most`)
+  __shared__ double score[TPA_BEAM_MAX], log_sum[TPA_BEAM_MAX];
+  __shared__ float most_of[TPA_BEAM_MAX];
   __shared__ double red_value[kMostThreads / 64];
   __shared__ int red_flat[kMostThreads / 64];
   __shared__ double won_value[TPA_BEAM_MAX];
@@ -205,21 +209,25 @@ __global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
 
   for (int j = w; j < p.n; j += waves) {
     const int row = b * p.n + j;
-    double value = NAN;  // a finished beam's chunks have no candidates: nothing was written there
+    double log_of = NAN;  // a finished beam's chunks have no candidates: nothing was written there
+    float most = -INFINITY;
     if (!(p.finished && p.finished[row])) {
-      float r = -INFINITY;
-      for (int c = lane; c < p.chunks; c += 64) r = fmaxf(r, p.sums[(int64_t)row * p.chunks + c].r);
-      r = from_ordered(wave_max(ordered(r)));
+      for (int c = lane; c < p.chunks; c += 64) most = fmaxf(most, p.sums[(int64_t)row * p.chunks + c].most);
+      most = from_ordered(wave_max(ordered(most)));
       double s = 0;
       for (int c = lane; c < p.chunks; c += 64) {
         const Sum x = p.sums[(int64_t)row * p.chunks + c];
-        if (x.s != 0) s += x.s * exp2((double)x.r - (double)r);  // (0: nothing but logits of -inf)
+        if (x.s != 0) s += x.s * exp((double)x.most - (double)most);  // (0: nothing but logits of -inf)
       }
 #pragma unroll
       for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
-      value = (double)p.scores[row] - ((double)r + log2(s)) * 0.693147180559945309417;
+      log_of = log(s);
     }
-    if (lane == 0) base[j] = value;
+    if (lane == 0) {
+      score[j] = (double)p.scores[row];
+      log_sum[j] = log_of;
+      most_of[j] = most;
+    }
   }
   __syncthreads();
 
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
       const int j = i / p.chunks;
       for (int r = 0; r < p.k; ++r) {
         const Candidate c = r < hold ? held[i * hold + r] : all[i * p.k + r];
-        const double v = base[j] + (double)c.logit;
+        const double v = score[j] + (((double)c.logit - (double)most_of[j]) - log_sum[j]);
         if (c.token < 0 || !(fabs(v) < INFINITY) || !visit(v, j * p.vocab + c.token)) break;
       }
     }
