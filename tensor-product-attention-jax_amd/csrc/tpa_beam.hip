@@ -32,6 +32,11 @@ struct Sum { double s; float most; int unused; };  // sum of exp(x - most), most
 struct Candidate { float logit; int token; };    // token < 0: none
 
 struct alignas(16) Ranked { double v; int flat, unused; };
+// of a beam, `most` = its largest logit (one number for all three would lose the small ones beside a large `most`)
+struct alignas(32) Beam {
+  double score, most, log_sum, unused;
+  __device__ __forceinline__ double value(float logit) const { return score + (((double)logit - most) - log_sum); }
+};
 
 struct BeamParams {
   const void* logits;
@@ -44,6 +49,8 @@ struct BeamParams {
   Sum* sums;              // [B, beams, chunks]
   Candidate* candidates;  // [B, beams, chunks, k]
   int B, n, vocab, k, eos, chunks;
+  int chunk;              // logits of a chunk
+  bool bf16;
 };
 
 __device__ __forceinline__ float max8(const float (&x)[8]) {
@@ -188,9 +195,7 @@ __host__ __device__ inline int held_of_each(int lists, int k) { return (int64_t)
 
 __global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
   extern __shared__ __attribute__((aligned(8))) char smem_beam[];
-  // of a beam: the value of logit x is score + ((x - most) - log_sum)  (one number for all three would lose the small ones beside a large `most`)
-  __shared__ double score[TPA_BEAM_MAX], log_sum[TPA_BEAM_MAX];
-  __shared__ float most_of[TPA_BEAM_MAX];
+  __shared__ Beam beams[TPA_BEAM_MAX];
   __shared__ double red_value[kMostThreads / 64];
   __shared__ int red_flat[kMostThreads / 64];
   __shared__ double won_value[TPA_BEAM_MAX];
@@ -223,11 +228,7 @@ __global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
       for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
       log_of = log(s);
     }
-    if (lane == 0) {
-      score[j] = (double)p.scores[row];
-      log_sum[j] = log_of;
-      most_of[j] = most;
-    }
+    if (lane == 0) beams[j] = Beam{(double)p.scores[row], (double)most, log_of, 0};
   }
   __syncthreads();
 
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
       const int j = i / p.chunks;
       for (int r = 0; r < p.k; ++r) {
         const Candidate c = r < hold ? held[i * hold + r] : all[i * p.k + r];
-        const double v = score[j] + (((double)c.logit - (double)most_of[j]) - log_sum[j]);
+        const double v = beams[j].value(c.logit);
         if (c.token < 0 || !(fabs(v) < INFINITY) || !visit(v, j * p.vocab + c.token)) break;
       }
     }
@@ -325,18 +326,73 @@ __global__ __launch_bounds__(kMostThreads) void select_kernel(BeamParams p) {
     }
   }
   __syncthreads();
-  // places without a candidate: values of -inf, the lowest indices that have not won
-  if (tid == 0) {
-    int next = 0;
-    for (int i = found; i < p.k; ++next) {
-      bool taken = false;
-      for (int j = 0; j < found; ++j) taken = taken || won[j] == next;
-      if (taken) continue;
-      won_value[i] = -INFINITY;
-      won[i++] = next;
+  // Logits that differ can have the same value: beside one of 1e30 all others are -1e30.  The lists go by logits, so of those with the last place's value they may lack some, and lower
+  // indices than they hold.  Fp32 numbers are 2^-24 of themselves apart or more, the steps of the value's sums are 2^-51 of its largest number or less: such logits are no more than
+  // 2^-27 of that one (2^-26: x is off by as little).  Then the logits with this value are looked for again, in the chunks that have one of them in their lists.
+  if (found == p.k) {
+    const double last = won_value[p.k - 1];
+    bool alike = false;
+    if (lane < p.n) {  // every wave all beams (x is no number, or infinite, for a beam that is finished or without candidates)
+      const Beam of = beams[lane];
+      const double x = ((last - of.score) + of.log_sum) + of.most;
+      alike = fabs(x) < INFINITY && fabs(x) <= 0x1p-26 * fmax(fmax(fabs(last), fabs(of.score)), fmax(fabs(of.log_sum), fabs(of.most)));
     }
+    if (__any(alike)) {
+      int count = 0;  // places before, then those given again
+      while (won_value[count] > last) ++count;
+      for (int l0 = 0; l0 < lists && count < p.k; l0 += 64) {  // every wave the same lists
+        const int mine = l0 + lane, j_of_mine = mine / p.chunks;
+        bool has = false;
+        if (mine < lists) {
+          for (int r = 0; r < p.k && !has; ++r) {
+            const Candidate c = all[(int64_t)mine * p.k + r];
+            const double v = beams[j_of_mine].value(c.logit);
+            if (c.token < 0 || !(v >= last)) break;
+            has = v == last;
+          }
+          if (mine % p.chunks == 0 && p.finished && p.finished[b * p.n + j_of_mine]) has = beams[j_of_mine].score == last;
+        }
+        for (uint64_t those = __ballot(has); those && count < p.k; those &= those - 1) {
+          const int i = l0 + __builtin_ctzll(those), j = i / p.chunks, begin = (i - j * p.chunks) * p.chunk, end = begin + min(p.chunk, p.vocab - begin);
+          if (p.finished && p.finished[b * p.n + j]) {
+            if (tid == 0) won[count] = j * p.vocab + p.eos;
+            ++count;
+            continue;
+          }
+          const int64_t row = b * p.stride_b + j * p.stride_n;
+          for (int t0 = begin; t0 < end && count < p.k; t0 += threads) {
+            const int t = t0 + tid;
+            float x = -INFINITY;
+            if (t < end) x = p.bf16 ? bf16bits_to_f32(static_cast<const uint16_t*>(p.logits)[row + t]) : static_cast<const float*>(p.logits)[row + t];
+            const uint64_t here = __ballot(t < end && beams[j].value(x) == last);
+            if (lane == 0) red_flat[w] = __popcll(here);
+            __syncthreads();
+            int place = count + __popcll(here & ((1ull << lane) - 1));
+            for (int v = 0; v < waves; ++v) {
+              if (v < w) place += red_flat[v];
+              count += red_flat[v];
+            }
+            if ((here >> lane & 1) && place < p.k) won[place] = j * p.vocab + t;
+            __syncthreads();
+          }
+        }
+      }
+      __syncthreads();
+    }
+  } else {
+    // places without a candidate: values of -inf, the lowest indices that have not won
+    if (tid == 0) {
+      int next = 0;
+      for (int i = found; i < p.k; ++next) {
+        bool taken = false;
+        for (int j = 0; j < found; ++j) taken = taken || won[j] == next;
+        if (taken) continue;
+        won_value[i] = -INFINITY;
+        won[i++] = next;
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (tid < p.k) {
     const int64_t to = (int64_t)b * p.k + tid;
     const int beam = won[tid] / p.vocab, token = won[tid] - beam * p.vocab, row = b * p.n + beam;
@@ -390,13 +446,13 @@ extern "C" int tpa_beam_select(const TpaBeamSelectArgs* a, void* stream) {
   p.sums = static_cast<Sum*>(a->workspace);
   p.candidates = reinterpret_cast<Candidate*>(p.sums + parts);
   p.B = a->B; p.n = a->beams; p.vocab = a->vocab; p.k = a->num_out; p.eos = a->eos_token;
+  p.chunk = batches_of(a->B, a->beams, a->vocab, a->dtype) * kBatch; p.bf16 = a->dtype == TPA_DTYPE_BF16;
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  const bool bf16 = a->dtype == TPA_DTYPE_BF16;
   void (*kern)(BeamParams) = nullptr;
   switch (batches_of(a->B, a->beams, a->vocab, a->dtype)) {
-    case 2: kern = bf16 ? chunk_kernel<uint16_t, 2> : chunk_kernel<float, 2>; break;
-    case 4: kern = bf16 ? chunk_kernel<uint16_t, 4> : chunk_kernel<float, 4>; break;
-    case 8: kern = bf16 ? chunk_kernel<uint16_t, 8> : chunk_kernel<float, 8>; break;
+    case 2: kern = p.bf16 ? chunk_kernel<uint16_t, 2> : chunk_kernel<float, 2>; break;
+    case 4: kern = p.bf16 ? chunk_kernel<uint16_t, 4> : chunk_kernel<float, 4>; break;
+    case 8: kern = p.bf16 ? chunk_kernel<uint16_t, 8> : chunk_kernel<float, 8>; break;
     default: kern = chunk_kernel<uint16_t, 16>;
   }
   hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(kThreads), 0, on, p);
