@@ -415,7 +415,7 @@ typedef struct TpaDecodeFp4Args {
   TpaFactor k_cache, v_cache;   /* [B, lk, rk, bytes], or with page_table pools [page, token_in_page, rk, bytes]; strides in bytes */
   void* o;                      /* [B, lq, H, dv] contiguous, element type = dtype */
   float* lse;                   /* [B, H, lq] or NULL */
-  int32_t B, lq, lk, H, dk, dv, rq, rk;
+  int32_t B, lq, lk, H, dk, dv, rq, rk; /* dk and dv at most 256, B * lq * H at most 2^24, on the vector units below it, lk * rk below 2^30 */
   int32_t dtype;
   float sm_scale;
   int32_t causal, causal_offset; /* as in TpaFwdArgs */

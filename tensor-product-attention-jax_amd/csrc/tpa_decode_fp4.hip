@@ -807,6 +807,8 @@ Plan plan_of(const TpaDecodeFp4Args* a) {
   return p;
 }
 
+bool on_vector_units(const TpaDecodeFp4Args* a) { return a->kernel == TPA_KERNEL_GENERIC || !mfma_takes(a); }
+
 int check_args(const TpaDecodeFp4Args* a) {
   if (!a) return TPA_ERR_NULL;
   if (a->dtype != TPA_DTYPE_F32 && a->dtype != TPA_DTYPE_BF16) return TPA_ERR_DTYPE;
@@ -818,6 +820,8 @@ int check_args(const TpaDecodeFp4Args* a) {
     if (!f->ptr) return TPA_ERR_NULL;
   if (a->page_table && (a->page_size <= 0 || a->pages_per_seq <= 0 || a->num_pages <= 0 || (int64_t)a->page_size * a->pages_per_seq < a->lk)) return TPA_ERR_SHAPE;
   if (a->kernel == TPA_KERNEL_MFMA && !mfma_takes(a)) return TPA_ERR_UNSUPPORTED;
+  // the vector-unit kernel's workgroups of 256 threads: a launch takes fewer than 2^32
+  if (on_vector_units(a) && (int64_t)a->B * a->lq * a->H == 1 << 24) return TPA_ERR_SHAPE;
   return TPA_OK;
 }
 
@@ -862,7 +866,7 @@ int launch_both(const Fp4Params& p, const Plan& plan, hipStream_t stream) {
 
 extern "C" size_t tpa_decode_fp4_workspace_bytes(const TpaDecodeFp4Args* a) {
   using namespace tpa;
-  if (check_args(a) != TPA_OK || a->kernel == TPA_KERNEL_GENERIC || !mfma_takes(a)) return 0;
+  if (check_args(a) != TPA_OK || on_vector_units(a)) return 0;
   return plan_of(a).bytes;
 }
 
@@ -882,7 +886,7 @@ extern "C" int tpa_decode_fp4(const TpaDecodeFp4Args* a, void* stream) {
     p.coff = clamp_causal_offset(a->causal_offset, a->causal == TPA_CAUSAL_BOTTOM_RIGHT ? -far : -a->lq, far);
   }
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (a->kernel == TPA_KERNEL_GENERIC || !mfma_takes(a)) {
+  if (on_vector_units(a)) {
     p.scale = a->sm_scale;
     const dim3 grid((unsigned)(p.B * p.cols));
     if (a->dtype == TPA_DTYPE_BF16) hipLaunchKernelGGL(decode_fp4_any_kernel<uint16_t>, grid, dim3(kThreads), 0, on, p);

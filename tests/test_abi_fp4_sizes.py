@@ -1,0 +1,10 @@
+"""Sizes that a launch or 64 bits do not hold, which the operators over a cache in 4 bits and the beam selection refuse before any launch."""
+
+from test_abi_fp4 import SHAPE, WORKSPACE, decode
+
+
+def test_decode_one_row_more_than_a_launch_takes():
+    for columns in (dict(B=1 << 20, lq=2), dict(B=1 << 21, lq=1), dict(B=2, lq=1 << 20)):
+        assert decode(**columns, kernel=1) == SHAPE and decode(True, **columns, kernel=1) == 0
+    assert decode(B=2, lq=1 << 20) == SHAPE  # (too many columns for the matrix-core kernel)
+    assert decode(True, B=1 << 21, lq=1) > 0 and decode(B=1 << 21, lq=1, workspace_bytes=8) == WORKSPACE
