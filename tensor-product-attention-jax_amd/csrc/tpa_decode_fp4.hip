@@ -813,7 +813,7 @@ int check_args(const TpaDecodeFp4Args* a) {
   if (!a) return TPA_ERR_NULL;
   if (a->dtype != TPA_DTYPE_F32 && a->dtype != TPA_DTYPE_BF16) return TPA_ERR_DTYPE;
   if (a->B <= 0 || a->lq <= 0 || a->lk <= 0 || a->H <= 0 || a->dk <= 0 || a->dv <= 0 || a->rq <= 0 || a->rk <= 0) return TPA_ERR_SHAPE;
-  if (a->dk > 256 || a->dv > 256 || (int64_t)a->B * a->lq * a->H > 1 << 24 || (int64_t)a->lk * a->rk > INT32_MAX / 2) return TPA_ERR_SHAPE;
+  if (a->dk > 256 || a->dv > 256 || (int64_t)a->B * a->lq > 1 << 24 || (int64_t)a->B * a->lq * a->H > 1 << 24 || (int64_t)a->lk * a->rk > INT32_MAX / 2) return TPA_ERR_SHAPE;
   if (a->causal < TPA_CAUSAL_NONE || a->causal > TPA_CAUSAL_BOTTOM_RIGHT) return TPA_ERR_UNSUPPORTED;
   if (a->kernel != TPA_KERNEL_AUTO && a->kernel != TPA_KERNEL_GENERIC && a->kernel != TPA_KERNEL_MFMA) return TPA_ERR_UNSUPPORTED;
   for (const TpaFactor* f : {&a->qa, &a->qb, &a->k_cache, &a->v_cache})

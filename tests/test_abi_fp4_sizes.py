@@ -8,3 +8,10 @@ def test_decode_one_row_more_than_a_launch_takes():
         assert decode(**columns, kernel=1) == SHAPE and decode(True, **columns, kernel=1) == 0
     assert decode(B=2, lq=1 << 20) == SHAPE  # (too many columns for the matrix-core kernel)
     assert decode(True, B=1 << 21, lq=1) > 0 and decode(B=1 << 21, lq=1, workspace_bytes=8) == WORKSPACE
+
+
+def test_decode_sizes_whose_product_passes_64_bits():
+    """2^64 and 2^65: zero in 64 bits."""
+    for columns in (dict(B=1 << 22, lq=1 << 21, H=1 << 21), dict(B=1 << 22, lq=1 << 21, H=1 << 22), dict(B=1 << 30, lq=1 << 30, H=1 << 4)):
+        for kernel in (0, 1):
+            assert decode(**columns, kernel=kernel) == SHAPE and decode(True, **columns, kernel=kernel) == 0
