@@ -446,7 +446,8 @@ typedef struct TpaBeamSelectArgs {
   int32_t* parents;          /* [B, num_out] */
   int32_t* tokens;           /* [B, num_out] */
   uint8_t* new_finished;     /* [B, num_out] */
-  int32_t B, beams, vocab, num_out; /* beams and num_out at most TPA_BEAM_MAX, vocab at most 2^30, beams * vocab below 2^31, num_out <= beams * vocab */
+  int32_t B, beams, vocab, num_out; /* beams and num_out at most TPA_BEAM_MAX, vocab at most 2^30, beams * vocab below 2^31, num_out <= beams * vocab;
+                                           B below 2^24, fewer than 2^26 chunks (of 1024 to 8192 logits) in all beams */
   int32_t eos_token;         /* -1: none (then `finished` must be NULL) */
   int32_t dtype;
   void* workspace;           /* tpa_beam_select_workspace_bytes(...), 16-byte aligned */

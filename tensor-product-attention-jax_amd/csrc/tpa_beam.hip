@@ -414,13 +414,21 @@ int64_t chunks_of(int64_t B, int64_t n, int64_t vocab, int dtype) {
   const int64_t chunk = (int64_t)batches_of(B, n, vocab, dtype) * kBatch;
   return (vocab + chunk - 1) / chunk;
 }
+// Workgroups of the first launch for sizes that a call takes, otherwise 0.  A launch takes fewer than 2^32 work-items.
+int64_t groups_of(int64_t B, int64_t n, int64_t vocab, int64_t k, int dtype) {
+  if (dtype != TPA_DTYPE_F32 && dtype != TPA_DTYPE_BF16) return 0;
+  if (B <= 0 || n <= 0 || vocab <= 0 || k <= 0 || n > TPA_BEAM_MAX || k > TPA_BEAM_MAX || vocab > 1 << 30 || n * vocab > INT32_MAX || k > n * vocab || B * n > INT32_MAX) return 0;
+  const int64_t chunks = chunks_of(B, n, vocab, dtype), groups = (B * n * chunks + kThreads / 64 - 1) / (kThreads / 64);
+  // (the second launch has 1024 threads for more than 512 lists, of which the first has a wave for each: B is below 2^17 there)
+  return std::max(groups, B) * kThreads > UINT32_MAX || n * chunks * k > INT32_MAX ? 0 : groups;
+}
 
 }  // namespace
 }  // namespace tpa
 
 extern "C" size_t tpa_beam_select_workspace_bytes(int32_t B, int32_t beams, int32_t vocab, int32_t num_out, int32_t dtype) {
   using namespace tpa;
-  if (B <= 0 || beams <= 0 || vocab <= 0 || num_out <= 0 || beams > TPA_BEAM_MAX || num_out > TPA_BEAM_MAX) return 0;
+  if (!groups_of(B, beams, vocab, num_out, dtype)) return 0;
   const size_t parts = (size_t)B * beams * chunks_of(B, beams, vocab, dtype);
   return parts * (sizeof(Sum) + num_out * sizeof(Candidate));
 }
@@ -429,16 +437,14 @@ extern "C" int tpa_beam_select(const TpaBeamSelectArgs* a, void* stream) {
   using namespace tpa;
   if (!a) return TPA_ERR_NULL;
   if (a->dtype != TPA_DTYPE_F32 && a->dtype != TPA_DTYPE_BF16) return TPA_ERR_DTYPE;
-  if (a->B <= 0 || a->beams <= 0 || a->vocab <= 0 || a->num_out <= 0 || a->beams > TPA_BEAM_MAX || a->num_out > TPA_BEAM_MAX || a->vocab > 1 << 30)
-    return TPA_ERR_SHAPE;
-  if ((int64_t)a->beams * a->vocab > INT32_MAX || a->num_out > (int64_t)a->beams * a->vocab || (int64_t)a->B * a->beams > INT32_MAX) return TPA_ERR_SHAPE;
+  const int64_t groups = groups_of(a->B, a->beams, a->vocab, a->num_out, a->dtype);
+  if (!groups) return TPA_ERR_SHAPE;
   if (a->eos_token < -1 || a->eos_token >= a->vocab) return TPA_ERR_SHAPE;
   if (!a->logits || !a->scores || !a->new_scores || !a->parents || !a->tokens || !a->new_finished) return TPA_ERR_NULL;
   if (a->finished && a->eos_token < 0) return TPA_ERR_UNSUPPORTED;
   BeamParams p{};
   p.chunks = (int)chunks_of(a->B, a->beams, a->vocab, a->dtype);
-  const int64_t parts = (int64_t)a->B * a->beams * p.chunks, groups = (parts + kThreads / 64 - 1) / (kThreads / 64);
-  if (groups > INT32_MAX || (int64_t)a->beams * p.chunks * a->num_out > INT32_MAX) return TPA_ERR_SHAPE;
+  const int64_t parts = (int64_t)a->B * a->beams * p.chunks;
   if (!a->workspace || a->workspace_bytes < tpa_beam_select_workspace_bytes(a->B, a->beams, a->vocab, a->num_out, a->dtype)) return TPA_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return TPA_ERR_ALIGN;
   p.logits = a->logits; p.stride_b = a->stride_b; p.stride_n = a->stride_n; p.scores = a->scores; p.finished = a->finished;
