@@ -102,6 +102,7 @@ bool gpu_tensors(PyObject* const* args, int n) {
 }
 bool none_or_gpu(PyObject* arg) { return arg == Py_None || gpu_tensors(&arg, 1); }
 Tensor tensor_or_none(PyObject* arg) { return arg == Py_None ? Tensor() : THPVariable_Unpack(arg); }
+constexpr int64_t kNotGiven = INT64_MIN;  // a size that has a default
 int64_t integer(PyObject* arg) {
   const long long v = PyLong_AsLongLong(arg);
   if (v == -1 && PyErr_Occurred()) throw python_error();
@@ -1165,7 +1166,7 @@ PyObject* decode_fp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   static const char* const names[2] = {"qa", "qb"};
   check_dtypes(two, names, 2);
   a.dtype = dtype_code(qa.scalar_type());
-  const int64_t h = qa.size(3), dk = qb.size(3), dv = given_dv < 0 ? dk : given_dv;
+  const int64_t h = qa.size(3), dk = qb.size(3), dv = given_dv == kNotGiven ? dk : given_dv;
   if (h <= 0 || dk <= 0 || dv <= 0 || qa.size(2) <= 0) throw CallFailed{"tpa_decode_fp4", TPA_ERR_SHAPE};
   if (kc.dim() != 4) throw Raise{PyExc_ValueError, "k_cache must be [pages, page_size, rk, bytes], got " + sizes_of(kc)};
   check_fp4_cache(kc, "k_cache", kc.size(2), h, dk);
@@ -1232,7 +1233,7 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t given = integer(args[3]), eos = integer(args[4]);
   one_device({logits, scores, finished});
   if (logits.dim() != 3) throw Raise{PyExc_ValueError, "logits must be [b, beams, vocab], got " + sizes_of(logits)};
-  const int64_t b = logits.size(0), beams = logits.size(1), vocab = logits.size(2), k = given < 0 ? beams : given;
+  const int64_t b = logits.size(0), beams = logits.size(1), vocab = logits.size(2), k = given == kNotGiven ? beams : given;
   const int dtype = dtype_code(logits.scalar_type());
   for (const Tensor* t : {&scores, &finished})
     if (t->defined() && !is_shape(*t, {b, beams}))

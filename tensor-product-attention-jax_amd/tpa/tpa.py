@@ -132,6 +132,9 @@ def _lengths(kv_lengths, batch: int, device) -> torch.Tensor | None:
     return t
 
 
+_NOT_GIVEN = -(1 << 63)  # to the native calls: a size that has a default
+
+
 def _call(native, arrays, *rest):
     """One native call per operator (csrc/host_calls.cc); operands that are not GPU tensors yet are copied there first."""
     out = native(*arrays, *rest)
@@ -385,7 +388,7 @@ def tpa_decode_fp4(
     """
     return _call(
         _d.host_calls().decode_fp4, (qa, qb, k_cache, v_cache, kv_lengths, page_table, workspace),
-        sm_scale, int(kernel), _causal_code(causal), int(causal_offset), -1 if v_head_dim is None else int(v_head_dim),
+        sm_scale, int(kernel), _causal_code(causal), int(causal_offset), _NOT_GIVEN if v_head_dim is None else int(v_head_dim),
     )
 
 
@@ -417,7 +420,7 @@ def tpa_beam_select(logits, scores, *, num_out: int | None = None, finished=None
         new_finished[b, num_out] bool: the beam was finished, or the token is `eos_token`
     """
     return _call(
-        _d.host_calls().beam_select, (logits, scores, finished), -1 if num_out is None else int(num_out), -1 if eos_token is None else int(eos_token)
+        _d.host_calls().beam_select, (logits, scores, finished), _NOT_GIVEN if num_out is None else int(num_out), -1 if eos_token is None else int(eos_token)
     )
 
 
