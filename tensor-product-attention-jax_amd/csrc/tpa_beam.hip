@@ -1,15 +1,17 @@
 // The continuations of a step of beam search: the largest values of score + logit - log sum exp over a request's beams and vocabulary.
 //
-// First launch: a wave holds a chunk of a beam's logits in its registers.  Every lane sums exponentials against a maximum of its own; the k-th largest of
+// First launch: a wave holds a chunk of a beam's logits in its registers.  Every lane sums exponentials against a maximum of its own, a logit; the k-th largest of
 // the lanes' maxima bounds the chunk's k largest logits from below, and what is above it is put into a list sorted over the lanes (lane r: the r-th).
-// (Inside a beam the order of the values is that of the logits.)
+// (Inside a beam the order of the values is that of the logits, where these differ enough for 64 bits.)
 // Second launch: a workgroup for each request joins the sums and ranks the chunks' candidates, in 64 bits, behind a bound found in the same way.  It has
 // 1024 threads where there are many lists: each sum's and each list's reading is a wait of about 1 us (16 beams, 16 continuations, 160 000 fp32 logits, one
-// request: 15.3 us, with 256 threads 23.3; all candidates read in place of each list's first ones: 54), and 256 elsewhere (its barriers are cheaper).
-// Equal values go to the lower index: logits are put in by rising index, behind their equals, and the last step compares value and index.
+// request: 15.8 us; when it took 15.3, 23.3 with 256 threads and 54 with all candidates read in place of each list's first ones), and 256 elsewhere (its barriers are
+// cheaper).
+// Equal values go to the lower index: logits are put in by rising index, behind their equals, the last step compares value and index, and where different logits can have the last
+// place's value they are looked for once more.
 //
-// HBM bounds it where there are many beams (64 requests, 4 beams, 131 072 bf16 logits: 18.7 + 5.4 us, 67 MB at 3.6 TB/s in the first), the latency of two
-// launches where there are few (one request, 4 beams, 50 021 fp32 logits: 5.2 + 5.6 us).
+// HBM bounds it where there are many beams (64 requests, 4 beams, 131 072 bf16 logits: 19.2 + 6.8 us, 67 MB at 3.5 TB/s in the first), the latency of two
+// launches where there are few (one request, 4 beams, 50 021 fp32 logits: 5.3 + 6.6 us).
 #include <algorithm>
 
 #include "tpa_common.h"
